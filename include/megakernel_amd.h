@@ -198,6 +198,29 @@ hipError_t mk_decode_batch(const mk_model_dims* dims, int batch, const int32_t* 
                            size_t workspace_bytes, hipStream_t stream);
 
 /*
+ * Causal attention of packed sequences: num_seqs sequences of lengths[0], lengths[1], ... tokens (HOST
+ * array, read before the call returns; a length may be 0), their rows one after the other. Token t of a
+ * sequence attends to its tokens 0 .. t:
+ *   out[t][h] = sum over j <= t of softmax_j(q[t][h] . k[j][h / G] / sqrt(128)) v[j][h / G],
+ * G = q_heads / kv_heads (a whole number), heads of 128.
+ *   q        bf16, or fp32 with q_fp32 != 0; head h of row r at q + r * q_row_stride + h * q_head_stride
+ *            (strides in elements, >= 0; multiples of 8, of 4 for fp32), so that q, k and v may be
+ *            slices of one projection's rows
+ *   k, v     bf16, laid out likewise (strides multiples of 8, at most 2^24 elements between rows)
+ *   out      q's type, [rows][q_heads][128], written for the rows of the sequences alone
+ * All pointers 16-byte aligned. bf16 queries: products of bf16 operands (the softmax's weights rounded
+ * to bf16 for the product with v), everything else fp32. fp32 queries: products at fp32 accuracy. A value
+ * row that a token may not see does not reach it, whatever it holds. Asynchronous on `stream`, no
+ * workspace, results independent of what else is in the batch. Argument errors (also more than 2^31 - 256
+ * (row, head) pairs) return hipErrorInvalidValue before any launch. No reference counterpart: the
+ * reference's attention takes one token's queries (/root/reference/megakernel.cu:228-370).
+ */
+hipError_t mk_attention_packed(int q_heads, int kv_heads, const void* q, int64_t q_row_stride, int64_t q_head_stride,
+                               const void* k, int64_t k_row_stride, int64_t k_head_stride, const void* v,
+                               int64_t v_row_stride, int64_t v_head_stride, const int32_t* lengths, int num_seqs,
+                               int q_fp32, void* out, hipStream_t stream);
+
+/*
  * Several decode steps in one call, with no host synchronization between them: the device-side
  * multi-token loop. Step i (0 <= i < n) runs at position + i and reads its input token from device
  * memory, tokens[i] (int32, device array of n + 1 entries, tokens[0] set by the caller).

@@ -396,6 +396,75 @@ std::tuple<torch::Tensor, torch::Tensor> decode_batch(torch::Tensor tokens, torc
   return {logits, toks};
 }
 
+// Element strides of a [rows, heads, 128] operand of attention_packed, the heads' 128 elements contiguous.
+struct HeadRows {
+  int64_t row, head;
+};
+HeadRows check_heads(const torch::Tensor& t, const char* name, int64_t rows, torch::ScalarType type,
+                     const torch::Device& dev) {
+  TORCH_CHECK(t.defined() && t.dim() == 3 && t.size(2) == kHeadDim && t.size(1) >= 1, "megakernel: ", name,
+              " must be [rows, heads, 128]");
+  TORCH_CHECK(t.device() == dev, "megakernel: ", name, " must be on ", dev, ", got ", t.device());
+  TORCH_CHECK(t.scalar_type() == type, "megakernel: ", name, " must be ", type, ", got ", t.scalar_type());
+  TORCH_CHECK(t.size(0) == rows, "megakernel: ", name, " must have ", rows, " rows, got ", t.size(0));
+  TORCH_CHECK(t.stride(2) == 1, "megakernel: ", name, " must be contiguous in its last dimension");
+  const HeadRows s{t.size(0) > 1 ? t.stride(0) : 0, t.size(1) > 1 ? t.stride(1) : 0};
+  const int64_t unit = 16 / t.element_size();
+  TORCH_CHECK(s.row % unit == 0 && s.head % unit == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
+              "megakernel: ", name, "'s rows and heads must start on 16-byte boundaries");
+  TORCH_CHECK(s.row <= 1 << 24, "megakernel: ", name, "'s rows must be at most 2^24 elements apart");
+  return s;
+}
+
+struct PackedChecked {
+  HeadRows q, k, v;
+  std::vector<int32_t> lengths;
+};
+PackedChecked validate_packed(const torch::Tensor& q, const torch::Tensor& k, const torch::Tensor& v,
+                              const std::vector<int64_t>& lengths) {
+  TORCH_CHECK(q.defined() && q.dim() == 3, "megakernel: q must be [rows, heads, 128]");
+  TORCH_CHECK(q.scalar_type() == torch::kBFloat16 || q.scalar_type() == torch::kFloat32,
+              "megakernel: q must be bfloat16 or float32, got ", q.scalar_type());
+  const int64_t rows = q.size(0);
+  PackedChecked c;
+  c.q = check_heads(q, "q", rows, q.scalar_type(), q.device());
+  c.k = check_heads(k, "k", rows, torch::kBFloat16, q.device());
+  c.v = check_heads(v, "v", rows, torch::kBFloat16, q.device());
+  TORCH_CHECK(v.size(1) == k.size(1), "megakernel: k and v must have the same number of heads");
+  TORCH_CHECK(q.size(1) % k.size(1) == 0, "megakernel: q's heads (", q.size(1), ") must be a multiple of k's (",
+              k.size(1), ")");
+  TORCH_CHECK(rows * q.size(1) <= INT32_MAX - 255, "megakernel: more than 2^31 - 256 (row, head) pairs in one call");
+  int64_t total = 0;
+  for (int64_t n : lengths) {
+    TORCH_CHECK(n >= 0 && n <= rows, "megakernel: a sequence's length must be between 0 and the rows (", rows,
+                "), got ", n);
+    total += n;
+    c.lengths.push_back((int32_t)n);
+  }
+  TORCH_CHECK(total == rows, "megakernel: the lengths add up to ", total, " and q has ", rows, " rows");
+  return c;
+}
+
+// Causal attention of packed sequences (mk_attention_packed): q [rows, heads, 128] bf16 or fp32, k and v
+// [rows, K/V heads, 128] bf16 (any 16-byte aligned row and head strides), the sequences' lengths on the
+// host; returns [rows, heads, 128] in q's type.
+torch::Tensor attention_packed(torch::Tensor q, torch::Tensor k, torch::Tensor v, std::vector<int64_t> lengths) {
+  const PackedChecked c = validate_packed(q, k, v, lengths);
+  TORCH_CHECK(q.is_cuda(), "megakernel: q must be a GPU tensor");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(q.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(q.device().index()).stream();
+  auto out = torch::empty({q.size(0), q.size(1), kHeadDim}, q.options());
+  MK_HIP_CHECK(mk_attention_packed((int)q.size(1), (int)k.size(1), q.data_ptr(), c.q.row, c.q.head, k.data_ptr(),
+                                   c.k.row, c.k.head, v.data_ptr(), c.v.row, c.v.head, c.lengths.data(),
+                                   (int)c.lengths.size(), q.scalar_type() == torch::kFloat32, out.data_ptr(), stream));
+  return out;
+}
+
+// attention_packed's argument validation only (tensors on any one device, nothing is launched).
+void check_attention_packed(torch::Tensor q, torch::Tensor k, torch::Tensor v, std::vector<int64_t> lengths) {
+  validate_packed(q, k, v, lengths);
+}
+
 int64_t status() {
   uint32_t s = 0;
   MK_HIP_CHECK(mk_status(&s));
@@ -450,6 +519,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_batch", &decode_batch,
         "batched decode of B <= 64 sequences (int32 tokens [B], positions [B], caches [B, L, 8, max_seq, 128]); "
         "returns (fp32 logits [B, V], int32 greedy tokens [B] on device)");
+  m.def("attention_packed", &attention_packed,
+        "causal attention of packed sequences: q [rows, heads, 128] bf16 or fp32, k and v [rows, K/V heads, 128] "
+        "bf16, lengths a list that adds up to the rows; returns [rows, heads, 128] in q's type");
+  m.def("check_attention_packed", &check_attention_packed,
+        "validate attention_packed's arguments without launching");
   m.def("set_batch_engine", &set_batch_engine,
         "engine of decode_batch: 0 automatic (the persistent kernel for <= 16 sequences of the 0.6B shape), "
         "1 layer by layer, 2 persistent where it applies");
