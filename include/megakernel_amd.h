@@ -221,6 +221,46 @@ hipError_t mk_attention_packed(int q_heads, int kv_heads, const void* q, int64_t
                                int q_fp32, void* out, hipStream_t stream);
 
 /*
+ * Beam search's selection, on the logits of a batched decode. Rows are (group, beam) in order, `beams`
+ * (1..16) of them to a group; in each group the best `beams` of the candidates
+ *   (row r, token v) with scores[r] + logits[r][v] - log(sum over u of exp(logits[r][u]))
+ * go on, best first; among equal scores the lower row, within a row the larger logit, then the lower token.
+ * A row with finished[r] != 0 has the one candidate (eos, scores[r]). With eos = -1 nothing ends:
+ * `finished` is not read and out_finished is 0.
+ *   logits       fp32, row r at logits + r * row_stride (elements, >= 0), vocab (1..2^20) of them
+ *   scores, finished               [rows] fp32 / bytes, the rows' sums of log-probabilities so far
+ *   tokens, parents                [rows] int32: the token that beam i goes on with, and the row it goes on from
+ *   out_scores, out_finished       [rows]: its score, and whether it has ended (its token is eos, or its
+ *                                  parent had); none of the outputs may overlap an input
+ *   workspace    mk_beam_select_workspace_bytes(rows, vocab, beams) bytes of device memory, 256-byte aligned,
+ *                owned by the caller, not used after the call's work completes on `stream`
+ * A logit of -infinity is a candidate that only fills up (score -infinity), as is every candidate of a row
+ * whose score is -infinity. A NaN or +infinity among a group's scores or the logits of its rows (a failed
+ * decode's are NaN) shows in the whole group: tokens -1, scores NaN, every row its own parent.
+ * Ranking is in 64 bits. Asynchronous on `stream`; argument errors (rows not a multiple of beams or over
+ * 65,535, eos outside [-1, vocab)) return hipErrorInvalidValue before any launch. No reference counterpart:
+ * the reference takes the argmax (/root/reference/model.py:97).
+ */
+size_t mk_beam_select_workspace_bytes(int rows, int vocab, int beams);
+hipError_t mk_beam_select(int rows, int vocab, int beams, const float* logits, int64_t row_stride,
+                          const float* scores, const uint8_t* finished, int eos, int32_t* tokens, int32_t* parents,
+                          float* out_scores, uint8_t* out_finished, void* workspace, size_t workspace_bytes,
+                          hipStream_t stream);
+
+/*
+ * Reorders the caches of a batched decode (mk_decode_batch's: bf16 [rows][num_layers][8][max_seq_len][128])
+ * after a selection, in place: row b's positions [begin[b], end[b]) become what row parents[b] held there
+ * before the call, in every layer of both caches. All three are int32 device arrays of `rows` entries.
+ * parents[b] is a row of b's group of `beams` (1..16) consecutive rows (mk_beam_select's output); an entry
+ * outside its group leaves row b as it is. begin and end are cut to [0, max_seq_len]; positions that a
+ * prompt's beams share need not be moved (begin: the prompt's length). With parents naming the group's first
+ * row it spreads a prefilled prompt over its group. Asynchronous on `stream`, no workspace. Argument errors
+ * return hipErrorInvalidValue before any launch. No reference counterpart.
+ */
+hipError_t mk_beam_reorder(int num_layers, int rows, int beams, int max_seq_len, void* k_cache, void* v_cache,
+                           const int32_t* parents, const int32_t* begin, const int32_t* end, hipStream_t stream);
+
+/*
  * Several decode steps in one call, with no host synchronization between them: the device-side
  * multi-token loop. Step i (0 <= i < n) runs at position + i and reads its input token from device
  * memory, tokens[i] (int32, device array of n + 1 entries, tokens[0] set by the caller).

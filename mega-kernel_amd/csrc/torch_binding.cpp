@@ -460,9 +460,73 @@ torch::Tensor attention_packed(torch::Tensor q, torch::Tensor k, torch::Tensor v
   return out;
 }
 
-// attention_packed's argument validation only (tensors on any one device, nothing is launched).
-void check_attention_packed(torch::Tensor q, torch::Tensor k, torch::Tensor v, std::vector<int64_t> lengths) {
-  validate_packed(q, k, v, lengths);
+void check_row_vector(const torch::Tensor& t, const char* name, int64_t rows, torch::ScalarType type,
+                      const torch::Device& dev) {
+  TORCH_CHECK(t.defined() && t.device() == dev && t.scalar_type() == type && t.is_contiguous() && t.dim() == 1 &&
+                  t.size(0) == rows,
+              "megakernel: ", name, " must be a contiguous ", type, " [", rows, "] tensor on ", dev);
+}
+
+void check_beams(int64_t rows, int64_t beams) {
+  TORCH_CHECK(beams >= 1 && beams <= 16, "megakernel: beams must be between 1 and 16, got ", beams);
+  TORCH_CHECK(rows >= 1 && rows <= 65535 && rows % beams == 0,
+              "megakernel: the rows must be a multiple of beams (", beams, ") and at most 65535, got ", rows);
+}
+
+// Beam search's selection (mk_beam_select) on decode_batch's logits: rows are (group, beam) in order.
+// Returns (tokens int32 [rows], parents int32 [rows], scores fp32 [rows], finished bool [rows]).
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor> beam_select(torch::Tensor logits,
+                                                                                   torch::Tensor scores,
+                                                                                   torch::Tensor finished,
+                                                                                   int64_t beams, int64_t eos) {
+  TORCH_CHECK(logits.defined() && logits.dim() == 2 && logits.scalar_type() == torch::kFloat32 &&
+                  logits.size(1) >= 1 && logits.size(1) <= 1 << 20 && logits.stride(1) == 1,
+              "megakernel: logits must be float32 [rows, vocab], contiguous in their last dimension, of a vocabulary "
+              "of 1 to 2^20");
+  const int64_t rows = logits.size(0), V = logits.size(1);
+  check_beams(rows, beams);
+  check_row_vector(scores, "scores", rows, torch::kFloat32, logits.device());
+  check_row_vector(finished, "finished", rows, torch::kBool, logits.device());
+  TORCH_CHECK(eos >= -1 && eos < V, "megakernel: eos must be -1 or a token in [0, ", V, "), got ", eos);
+  TORCH_CHECK(logits.is_cuda(), "megakernel: logits must be a GPU tensor");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(logits.device().index()).stream();
+  const size_t bytes = mk_beam_select_workspace_bytes((int)rows, (int)V, (int)beams);
+  auto ws = torch::empty({(int64_t)bytes}, logits.options().dtype(torch::kUInt8));
+  auto toks = torch::empty({rows}, logits.options().dtype(torch::kInt32));
+  auto parents = torch::empty_like(toks);
+  auto out_scores = torch::empty_like(scores);
+  auto out_finished = torch::empty_like(finished);
+  MK_HIP_CHECK(mk_beam_select((int)rows, (int)V, (int)beams, logits.data_ptr<float>(), logits.stride(0),
+                              scores.data_ptr<float>(), reinterpret_cast<const uint8_t*>(finished.data_ptr<bool>()),
+                              (int)eos, toks.data_ptr<int32_t>(), parents.data_ptr<int32_t>(),
+                              out_scores.data_ptr<float>(), reinterpret_cast<uint8_t*>(out_finished.data_ptr<bool>()),
+                              ws.data_ptr(), bytes, stream));
+  return {toks, parents, out_scores, out_finished};
+}
+
+// Reorders decode_batch's caches in place (mk_beam_reorder): row b's positions [begin[b], end[b]) become
+// those of row parents[b].
+void beam_reorder(torch::Tensor kc, torch::Tensor vc, torch::Tensor parents, torch::Tensor begin, torch::Tensor end,
+                  int64_t beams) {
+  TORCH_CHECK(kc.defined() && kc.dim() == 5, "megakernel: k_cache must be [rows, layers, 8, max_seq, 128]");
+  const int64_t rows = kc.size(0), L = kc.size(1), S = kc.size(3);
+  check_beams(rows, beams);
+  TORCH_CHECK(L >= 1 && S >= 1 && L * kKVHeads * 2 * ((S + 15) / 16) <= INT32_MAX,
+              "megakernel: the caches have no positions, or too many");
+  check_bf16(kc, "k_cache", {rows, L, kKVHeads, S, kHeadDim}, kc.device());
+  check_bf16(vc, "v_cache", {rows, L, kKVHeads, S, kHeadDim}, kc.device());
+  TORCH_CHECK(kc.data_ptr() != vc.data_ptr(), "megakernel: k_cache and v_cache must be distinct");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(kc.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(vc.data_ptr()) % 16 == 0,
+              "megakernel: k_cache and v_cache must start on 16-byte boundaries");
+  check_row_vector(parents, "parents", rows, torch::kInt32, kc.device());
+  check_row_vector(begin, "begin", rows, torch::kInt32, kc.device());
+  check_row_vector(end, "end", rows, torch::kInt32, kc.device());
+  TORCH_CHECK(kc.is_cuda(), "megakernel: k_cache must be a GPU tensor");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(kc.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(kc.device().index()).stream();
+  MK_HIP_CHECK(mk_beam_reorder((int)L, (int)rows, (int)beams, (int)S, kc.data_ptr(), vc.data_ptr(),
+                               parents.data_ptr<int32_t>(), begin.data_ptr<int32_t>(), end.data_ptr<int32_t>(), stream));
 }
 
 int64_t status() {
@@ -522,8 +586,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attention_packed", &attention_packed,
         "causal attention of packed sequences: q [rows, heads, 128] bf16 or fp32, k and v [rows, K/V heads, 128] "
         "bf16, lengths a list that adds up to the rows; returns [rows, heads, 128] in q's type");
-  m.def("check_attention_packed", &check_attention_packed,
-        "validate attention_packed's arguments without launching");
+  m.def("beam_select", &beam_select,
+        "beam search's selection: logits fp32 [rows, vocab], scores fp32 [rows], finished bool [rows], beams, eos (or "
+        "-1); returns (int32 tokens, int32 parents, fp32 scores, bool finished), [rows] each, on device");
+  m.def("beam_reorder", &beam_reorder,
+        "reorder decode_batch's caches in place: row b's positions [begin[b], end[b]) become those of row parents[b] "
+        "(int32 [rows] on device, parents inside the row's group of beams)");
   m.def("set_batch_engine", &set_batch_engine,
         "engine of decode_batch: 0 automatic (the persistent kernel for <= 16 sequences of the 0.6B shape), "
         "1 layer by layer, 2 persistent where it applies");
