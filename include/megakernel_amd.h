@@ -168,6 +168,28 @@ hipError_t mk_prefill_paged(const mk_model_dims* dims, const int32_t* tokens, in
                             hipStream_t stream);
 
 /*
+ * Prefill of several prompts in one call, into the caches of a batched decode: num_seqs (1..64) prompts of
+ * lengths[0], lengths[1], ... tokens (HOST array, read before the call returns; each 1..max_seq_len, at most
+ * MK_PREFILL_BATCH_TOKENS in all), their tokens one after the other in `tokens` (int32 device array). All
+ * their rows go through each layer's products together, attention per prompt (as mk_attention_packed).
+ * Prompt s is written to positions 0 .. lengths[s] - 1 of its cache, which starts at k_cache + s * seq_stride
+ * elements ([num_layers][8][max_seq_len][128] bf16; seq_stride a multiple of 8 and at least that size: for
+ * mk_decode_batch's caches exactly that, or a multiple for every n-th of them). Writes each prompt's last
+ * logits, fp32 [num_seqs][vocab], and, when out_tokens is not NULL, its greedy token. Numerics, weights,
+ * workspace rules and asynchrony as mk_prefill (mk_prefill_batch_workspace_bytes(dims, all tokens)); the
+ * vocabulary size must be a multiple of 16. A token outside [0, vocab) makes the call report NaN logits and
+ * token -1 for every prompt. Argument errors return hipErrorInvalidValue before any launch. Replaces one
+ * Transformers prefill and cache copy per prompt (/root/reference/model.py:72-87).
+ */
+#define MK_PREFILL_BATCH_TOKENS 262144
+size_t mk_prefill_batch_workspace_bytes(const mk_model_dims* dims, int num_tokens);
+hipError_t mk_prefill_batch(const mk_model_dims* dims, const int32_t* tokens, const int32_t* lengths, int num_seqs,
+                            const void* embed_weight, const void* lm_head_weight, const void* final_norm_weight,
+                            const void* layer_weights, const void* cos_table, const void* sin_table, void* k_cache,
+                            void* v_cache, int64_t seq_stride, int max_seq_len, float* logits, int32_t* out_tokens,
+                            void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/*
  * Batched decode: `batch` (1..64) independent sequences advance by one token each in one call.
  * Two engines: up to 16 sequences of the Qwen3-0.6B shape run as one persistent kernel (256
  * workgroups exchanging data through epoch-tagged words, the batch as the columns of the matrix-core

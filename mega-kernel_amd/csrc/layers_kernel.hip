@@ -43,6 +43,7 @@
 #include "mk_device.h"
 #include "mk_batch.h"
 #include "mk_layers.h"
+#include "mk_packed.h"
 #include "../../include/megakernel_amd.h"
 
 namespace mkp {
@@ -71,6 +72,19 @@ __device__ __forceinline__ size_t kv_row(const KvMap& m, int layer, int head, in
   return (((((size_t)layer * m.num_pages + page) * HKV + head) << m.shift) + (p & ((1 << m.shift) - 1))) * D;
 }
 
+// Rows of several prompts packed one after the other (mk_prefill_batch): row m is position rows[m].y of
+// sequence rows[m].x, whose cache starts seq_stride elements after that of the one before. Without a
+// table the rows are one sequence's, at position + m.
+struct PackedRows {
+  const int2* rows;
+  int64_t seq_stride;
+};
+__device__ __forceinline__ int row_pos(const PackedRows& pk, int position, int m) {
+  return pk.rows ? pk.rows[m].y : position + m;
+}
+__device__ __forceinline__ size_t row_cache(const PackedRows& pk, int m) {
+  return pk.rows ? (size_t)pk.rows[m].x * pk.seq_stride : 0;
+}
 
 // ------------------------------------------------------------------------------------------------
 // GEMM C[M][N] = A[M][K] . W[N][K]^T on the matrix cores, A given as a bf16 hi/lo pair in the
@@ -88,35 +102,8 @@ __device__ __forceinline__ size_t kv_row(const KvMap& m, int layer, int head, in
 constexpr int MT = 128, NT = 128, KT = 64, KP = KT + 16;
 constexpr int CP = NT + 4;                              // padded fp32 row of the epilogue tile
 
-// Fragment-major layout of a bf16 activation matrix with K columns (K a multiple of 32), the A
-// operand of gemm_kernel: 16-row x 32-column blocks of 1 KB, block (m / 16, k / 32) at KB offset
-// (m / 16) * (K / 32) + k / 32; inside a block, MFMA lane l = (m % 16) + 16 * ((k % 32) / 8) holds
-// the 16 bytes of columns [8 ((k % 32) / 8), +8). A wave reads one operand fragment as 1 KB of
-// consecutive bytes. Buffers in this layout hold whole row tiles (operand_rows); rows past M are never
-// written, and the sums they produce are never stored.
-__device__ __forceinline__ size_t frag_off(int m, int k, int K) {
-  return ((((size_t)(m >> 4) * (K >> 5) + (k >> 5)) * 64 + ((k >> 3) & 3) * 16 + (m & 15)) << 3) + (k & 7);
-}
 static size_t frag_rows(int M) { return (size_t)(M + MT - 1) / MT * MT; }
 
-// Activation operand of the skinny products in fragment order ("skinny fragments", used by the
-// batched decode): for column block cb (sequences 8 cb .. 8 cb + 7) and K block kb (32 inputs), one
-// 1 KB fragment holding, at lane l, MFMA column li = l % 16 (sequence 8 cb + li / 2, bf16 hi part for
-// even li, lo for odd) and inputs 32 kb + 8 (l / 16) .. + 8. A wave then loads a whole B operand as
-// 1 KB of consecutive bytes. In row order (B rows of ldx elements, hi and lo in two arrays) each lane
-// of such a load reads 16 bytes of a different row, and the vector cache takes one access per lane:
-// at 64 sequences that was the skinny products' bound (rocprof at 64 sequences: ~64 L1 accesses per
-// load instruction, TA address stalls). Rows past the batch are never written; their columns of the
-// products are never read.
-// Column-block major: the K blocks of one column block are adjacent. (K-block major, the column blocks of
-// one K block adjacent, measured on MI355X from 9 to 64 sequences and 16 to 256 prompt tokens at both
-// widths: within 0.4% either way, but 131 tokens 1,612 -> 1,634 us, 40 at 1.7B 1,740 -> 1,754.)
-__host__ __device__ inline int skf_blocks(int B) { return (B + 7) / 8; }
-__host__ __device__ inline size_t skf_frag(int cb, int kb, int K) { return (size_t)cb * (K >> 5) + kb; }
-__host__ __device__ inline size_t skf_off(int b, int k, int part, int K) {
-  const int cb = b >> 3, li = 2 * (b & 7) + part, kb = k >> 5, lg = (k & 31) >> 3;
-  return ((skf_frag(cb, kb, K) * 64 + lg * 16 + li) << 3) + (k & 7);
-}
 // Elements of the skinny fragments of B rows, hi and lo. A product's last column blocks may lie past
 // skf_blocks(B) (its workgroups take equal numbers of blocks, at most 12): those are inside the buffer,
 // and their columns of the product are never read.
@@ -155,6 +142,7 @@ struct GemmArgs {
   KvMap kv;
   int32_t* bad;
   int layer, position;
+  PackedRows pk;
 };
 
 // first element of weight row r (0..127) of N-tile t
@@ -418,7 +406,8 @@ __global__ void __launch_bounds__(64 * NW * KS, PF == 4 ? 1 : 2) gemm_kernel(con
     for (int pass = 0; pass < 8; ++pass) {
       const int r = 32 * wave + 4 * pass + rq, m = m0 + r;
       if (m >= g.M) continue;
-      const int pos = g.position + m;
+      const int pos = row_pos(g.pk, g.position, m);
+      const size_t seq = row_cache(g.pk, m);
       const int page = tn >= HQ && g.kv.bt ? kv_page(g.kv, pos, g.bad) : 0;
       float v[8];
       ld8(r, 8 * tt, v);
@@ -427,7 +416,7 @@ __global__ void __launch_bounds__(64 * NW * KS, PF == 4 ? 1 : 2) gemm_kernel(con
           uint32_t p[4];
 #pragma unroll
           for (int q = 0; q < 4; ++q) p[q] = pack_bf16x2(v[2 * q], v[2 * q + 1]);
-          *reinterpret_cast<uint4*>(g.v_cache + kv_row(g.kv, g.layer, tn - HQ - HKV, pos, page) + 8 * tt) =
+          *reinterpret_cast<uint4*>(g.v_cache + seq + kv_row(g.kv, g.layer, tn - HQ - HKV, pos, page) + 8 * tt) =
               make_uint4(p[0], p[1], p[2], p[3]);
         }
         continue;
@@ -448,7 +437,7 @@ __global__ void __launch_bounds__(64 * NW * KS, PF == 4 ? 1 : 2) gemm_kernel(con
         uint32_t p[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) p[q] = pack_bf16x2(v[2 * q], v[2 * q + 1]);
-        *reinterpret_cast<uint4*>(g.k_cache + kv_row(g.kv, g.layer, tn - HQ, pos, page) + 8 * tt) =
+        *reinterpret_cast<uint4*>(g.k_cache + seq + kv_row(g.kv, g.layer, tn - HQ, pos, page) + 8 * tt) =
             make_uint4(p[0], p[1], p[2], p[3]);
       }
     }
@@ -1427,21 +1416,22 @@ __global__ void __launch_bounds__(256) bnorm_kernel(float* x, const int32_t* tok
   }
 }
 
-// The raw Q/K/V sums of M consecutive prompt tokens of one sequence (fp32 [M][4096], or S such arrays
-// of K-range sums added in order; row m at position pos0 + m): per-head RMSNorm + RoPE on q and k,
+// The raw Q/K/V sums of M prompt tokens (fp32 [M][4096], or S such arrays of K-range sums added in order;
+// row m at position pos0 + m of one sequence, or where pk says): per-head RMSNorm + RoPE on q and k,
 // q kept as a bf16 hi/lo pair [M][2048], k and v rounded to bf16 into the cache [L][8][max_seq][128].
 __global__ void __launch_bounds__(64) qkv_post_kernel(const float* raw, int S, int M, int pos0, const uint16_t* q_norm,
                                                        const uint16_t* k_norm, const uint16_t* cos_tab,
                                                        const uint16_t* sin_tab, uint16_t* qh, uint16_t* ql,
                                                        uint16_t* k_cache, uint16_t* v_cache, int layer, KvMap kv,
-                                                       int32_t* bad) {
+                                                       int32_t* bad, PackedRows pk) {
   // one item (row b, head hd) per 16-lane group, lane t holding dims 8 t .. +7 (head_norm_rope's
   // layout): 16-byte loads and stores
   const int t = threadIdx.x & 15;
   const int item = blockIdx.x * 4 + (threadIdx.x >> 4);  // single-wave workgroups: the items spread over the CUs
   if (item >= M * (HQ + 2 * HKV)) return;  // uniform in the 16-lane group
   const int b = item / (HQ + 2 * HKV), hd = item % (HQ + 2 * HKV);
-  const int pos = pos0 + b;
+  const int pos = row_pos(pk, pos0, b);
+  const size_t seq = row_cache(pk, b);
   // the sums of S K ranges (EPI_QKV_PART), added in order
   const size_t rstride = (size_t)M * (HQ + 2 * HKV) * D;
   const float* r = raw + (size_t)b * (HQ + 2 * HKV) * D + hd * D + 8 * t;
@@ -1462,7 +1452,7 @@ __global__ void __launch_bounds__(64) qkv_post_kernel(const float* raw, int S, i
   };
   if (hd >= HQ + HKV) {  // v
     if (page >= 0)
-      *reinterpret_cast<uint4*>(v_cache + kv_row(kv, layer, hd - HQ - HKV, pos, page) + 8 * t) = pack();
+      *reinterpret_cast<uint4*>(v_cache + seq + kv_row(kv, layer, hd - HQ - HKV, pos, page) + 8 * t) = pack();
     return;
   }
   // per-head RMSNorm and rotate-half RoPE (/root/reference/megakernel.cu:490-630, 548-555)
@@ -1478,7 +1468,7 @@ __global__ void __launch_bounds__(64) qkv_post_kernel(const float* raw, int S, i
     *reinterpret_cast<uint4*>(qh + o) = hi;
     *reinterpret_cast<uint4*>(ql + o) = lo;
   } else if (page >= 0) {
-    *reinterpret_cast<uint4*>(k_cache + kv_row(kv, layer, hd - HQ, pos, page) + 8 * t) = pack();
+    *reinterpret_cast<uint4*>(k_cache + seq + kv_row(kv, layer, hd - HQ, pos, page) + 8 * t) = pack();
   }
 }
 
@@ -2115,6 +2105,8 @@ struct Work {
   float* ssq;   // short prompts: sums of squares per row and 16 columns of x [H / 16][M]
   u64* keys;
   int32_t* bad;
+  int2* rows;   // packed prompts: where each row belongs (PackedRows)
+  float* last;  // packed prompts: the residual of each sequence's last token [sequences][H]
 };
 
 // Whether a prompt runs its products on the skinny kernels (weights as the MFMA A operand, the tokens as
@@ -2195,9 +2187,9 @@ static size_t operand_rows(int I, int M) {
 // operand_rows rows); q (hi, lo) bf16 [M][2048]; for a prompt on the skinny kernels the raw Q/K/V sums; the split-K partials of
 // the residual products; the argmax keys. Offsets in bytes, each 256-byte aligned.
 struct Layout {
-  size_t x, ah, al, bh, bl, qh, ql, raw, part, qpart, apart, ssq, keys, bad, bytes;
+  size_t x, ah, al, bh, bl, qh, ql, raw, part, qpart, apart, ssq, keys, bad, rows, last, bytes;
 };
-static Layout layout(int H, int I, int M, bool small) {
+static Layout layout(int H, int I, int M, bool small, bool packed = false) {
   const size_t A = H > HQ * D ? H : HQ * D;
   Layout L;
   size_t o = 0;
@@ -2218,27 +2210,31 @@ static Layout layout(int H, int I, int M, bool small) {
   size_t qp = sq > 1 ? (size_t)sq * M * (HQ + 2 * HKV) * D : 0;
   if (su > 1 && (size_t)su * M * 2 * I > qp) qp = (size_t)su * M * 2 * I;
   L.qpart = take(qp * 4);
-  L.apart = take(attn_part_slots(M) * 2 * attn_part_rows(M) * APS * 4);
+  L.apart = take(packed ? 0 : attn_part_slots(M) * 2 * attn_part_rows(M) * APS * 4);
   L.ssq = take(small ? (size_t)M * (H / 16) * 4 : 0);
-  L.keys = take(8);
+  L.keys = take(packed ? BMAX * 8 : 8);
   L.bad = take(4);
+  L.rows = take(packed ? (size_t)M * sizeof(int2) : 0);
+  L.last = take(packed ? (size_t)BMAX * H * 4 : 0);
   L.bytes = o;
   return L;
 }
-// Workspace that a call of M tokens needs, at whichever position.
-static size_t call_bytes(int H, int I, int M) {
-  return std::max(layout(H, I, M, small_prompt(H, M, 0)).bytes, layout(H, I, M, small_prompt(H, M, 1)).bytes);
+// Workspace that a call of M tokens needs, at whichever position (packed prompts: small_prompt's choice for
+// later positions, their attention being a kernel of its own).
+static size_t call_bytes(int H, int I, int M, bool packed = false) {
+  return std::max(layout(H, I, M, small_prompt(H, M, packed), packed).bytes,
+                  layout(H, I, M, small_prompt(H, M, 1), packed).bytes);
 }
 // Workspace for calls of up to M tokens. A layout of more tokens can be the smaller one: it has fewer K
 // splits, or is of the other path. Between such steps (a path's longest prompt, a full row tile while a
 // residual product still splits) a layout grows with M, so the largest is the one of M or of the last size
 // before a step.
-static size_t prefill_bytes(int H, int I, int M) {
-  size_t n = call_bytes(H, I, M);
+static size_t prefill_bytes(int H, int I, int M, bool packed = false) {
+  size_t n = call_bytes(H, I, M, packed);
   for (int position = 0; position < 2; ++position)
-    if (small_m(H, position) < M) n = std::max(n, call_bytes(H, I, small_m(H, position)));
+    if (small_m(H, position) < M) n = std::max(n, call_bytes(H, I, small_m(H, position), packed));
   const int last = 192 / std::max(H / NT, 1);  // row tiles from which no product splits (resid_splits)
-  for (int t = 1; t <= last && t * MT < M; ++t) n = std::max(n, call_bytes(H, I, t * MT));
+  for (int t = 1; t <= last && t * MT < M; ++t) n = std::max(n, call_bytes(H, I, t * MT, packed));
   return n;
 }
 static Work carve(void* base, const Layout& L) {
@@ -2258,6 +2254,8 @@ static Work carve(void* base, const Layout& L) {
   w.ssq = reinterpret_cast<float*>(p + L.ssq);
   w.keys = reinterpret_cast<u64*>(p + L.keys);
   w.bad = reinterpret_cast<int32_t*>(p + L.bad);
+  w.rows = reinterpret_cast<int2*>(p + L.rows);
+  w.last = reinterpret_cast<float*>(p + L.last);
   return w;
 }
 
@@ -2300,11 +2298,79 @@ static hipError_t launch_gemm(dim3 grid, const GemmArgs& g, hipStream_t st) {
   return hipGetLastError();
 }
 
+// The final norm of B <= 64 rows of x, the tied LM head and the greedy tokens (keys cleared before). af: skinny
+// fragments of B rows; ah, al: fragment-major, whole row tiles (af may be ah: one or the other is used).
+template <int H>
+static hipError_t lm_head_rows(const mk_model_dims& dims, int B, float* x, const uint16_t* final_norm,
+                               const uint16_t* lm_head, uint16_t* af, uint16_t* ah, uint16_t* al, float* logits,
+                               int32_t* out_tokens, u64* keys, int32_t* bad, hipStream_t st) {
+  hipError_t e;
+#define MKB_LAUNCH(...)                                   \
+  do {                                                    \
+    hipLaunchKernelGGL(__VA_ARGS__);                      \
+    if ((e = hipGetLastError()) != hipSuccess) return e;  \
+  } while (0)
+  const dim3 rows(B), nthr(64);  // the norm: one row per single-wave workgroup
+  // the final norm, then the tied LM head as one more skinny
+  // product (vocabulary rows x the B normalised rows: each table byte read once, on the matrix
+  // cores) and the greedy keys
+  const bool lm_tiles = B > 8 && dims.vocab % NT == 0;
+  if (lm_tiles)
+    MKB_LAUNCH((bnorm_kernel<H, 1>), rows, nthr, 0, st, x, nullptr, nullptr, dims.vocab, bad, nullptr, 0,
+               final_norm, ah, al, B);
+  else
+    MKB_LAUNCH((bnorm_kernel<H, 2>), rows, nthr, 0, st, x, nullptr, nullptr, dims.vocab, bad, nullptr, 0,
+               final_norm, af, nullptr, B);
+  if (!lm_tiles) {
+    SkArgs lmh{};
+    lmh.xh = af; lmh.B = B; lmh.N = dims.vocab; lmh.K = H;
+    lmh.w0 = lm_head; lmh.n1 = dims.vocab; lmh.n2 = dims.vocab; lmh.out = logits;
+    if ((e = launch_skinny<SK_RAW>(lmh, st)) != hipSuccess) return e;
+  } else {
+    // beyond one column block the skinny product re-reads every row's activations per 16 table
+    // rows; a 128-row tile of the table reads them once per 128 (the B rows are one row tile)
+    GemmArgs gl{};
+    gl.ah = ah; gl.al = al; gl.M = B; gl.N = dims.vocab; gl.K = H;
+    gl.w0 = lm_head; gl.part = logits;  // logits[b][v], no residual
+    if ((e = launch_gemm<EPI_RESID>(dim3(dims.vocab / NT, 1, 1), gl, st)) != hipSuccess) return e;
+  }
+  MKB_LAUNCH(logits_argmax_kernel, dim3((dims.vocab + 4095) / 4096, B), dim3(256), 0, st, logits, dims.vocab, keys, bad);
+  if (out_tokens) MKB_LAUNCH(keys_to_tokens_kernel, dim3(1), dim3(64), 0, st, keys, B, bad, out_tokens);
+#undef MKB_LAUNCH
+  return hipSuccess;
+}
+
+// Several prompts in one call (mk_prefill_batch): n of them (0: one prompt), their rows' table and lengths
+// (HOST), and the row after each one's last.
+struct PackedEnds {
+  int32_t end[BMAX];
+};
+struct PackedRun {
+  int n = 0;
+  PackedRows rows{};
+  const int32_t* lengths = nullptr;
+  PackedEnds ends{};
+};
+__global__ void __launch_bounds__(256) packed_rows_kernel(PackedEnds ends, int n, int M, int2* rows) {
+  const int m = blockIdx.x * 256 + threadIdx.x;
+  if (m >= M) return;
+  int s = 0, first = 0;
+  while (s < n - 1 && m >= ends.end[s]) first = ends.end[s++];
+  rows[m] = make_int2(s, m - first);
+}
+template <int H>
+__global__ void __launch_bounds__(H / 4) last_rows_kernel(const float* x, PackedEnds ends, float* last) {
+  const int s = blockIdx.x, c = 4 * threadIdx.x;
+  *reinterpret_cast<float4*>(last + (size_t)s * H + c) =
+      *reinterpret_cast<const float4*>(x + (size_t)(ends.end[s] - 1) * H + c);
+}
+
 template <int H, int I>
 static hipError_t run(const mk_model_dims& dims, const int32_t* tokens, int M, int position, const uint16_t* embed,
                       const uint16_t* lm_head, const uint16_t* final_norm, const mk_layer_weights* layers,
                       const uint16_t* cos_tab, const uint16_t* sin_tab, uint16_t* k_cache, uint16_t* v_cache,
-                      const KvMap& kv, float* logits, int32_t* out_token, const Work& wk, hipStream_t st) {
+                      const KvMap& kv, float* logits, int32_t* out_token, const Work& wk, hipStream_t st,
+                      const PackedRun& pk = {}) {
   const int mtiles = (M + MT - 1) / MT;
   hipError_t e;
 #define MKP_LAUNCH(...)                                   \
@@ -2312,13 +2378,23 @@ static hipError_t run(const mk_model_dims& dims, const int32_t* tokens, int M, i
     hipLaunchKernelGGL(__VA_ARGS__);                      \
     if ((e = hipGetLastError()) != hipSuccess) return e;  \
   } while (0)
-  MKP_LAUNCH(keys_init_kernel, dim3(1), dim3(64), 0, st, wk.keys, 1, wk.bad);
-  const AttnPlan ap = attn_plan(M, position);
+  MKP_LAUNCH(keys_init_kernel, dim3(1), dim3(64), 0, st, wk.keys, pk.n ? pk.n : 1, wk.bad);
+  const AttnPlan ap = pk.n ? AttnPlan{} : attn_plan(M, position);
   if ((size_t)ap.wgs > attn_part_slots(M)) return hipErrorInvalidValue;  // cannot happen (see attn_plan)
-  const bool small = small_prompt(H, M, position);
+  const bool small = small_prompt(H, M, pk.n ? 1 : position);
+  if (pk.n) MKP_LAUNCH(packed_rows_kernel, dim3((M + 255) / 256), dim3(256), 0, st, pk.ends, pk.n, M, wk.rows);
+  // layer l's attention, of the one prompt or of the packed ones, into the O product's operand
+  auto attend = [&](const AttnArgs& at) -> hipError_t {
+    if (pk.n) {
+      return mkp_attention_prefill({at.qh, at.ql, at.k_cache, at.v_cache, at.oh, at.ol, at.frag, at.layer, kv.max_seq,
+                                    pk.rows.seq_stride, pk.lengths, pk.n}, st);
+    }
+    MKP_LAUNCH(attn_kernel, dim3(ap.wgs), dim3(512), 0, st, at);
+    if (ap.merge) MKP_LAUNCH(attn_merge_kernel, dim3(ap.merge), dim3(256), 0, st, at);
+    return hipSuccess;
+  };
   const AttnArgs at0{wk.qh, wk.ql, k_cache, v_cache, wk.ah, wk.al, small ? 2 : 1, M, 0, position, kv, wk.bad,
                      wk.apart, ap.chunk, attn_part_rows(M)};
-  const dim3 attn_grid(ap.wgs);
   if (small) {
     // Short prompts: the products are weight-bandwidth bound, so they run on the skinny kernels, the
     // norms folded into them (SK_RESID).
@@ -2332,18 +2408,17 @@ static hipError_t run(const mk_model_dims& dims, const int32_t* tokens, int M, i
       q.w0 = (const uint16_t*)lw.q_weight; q.w1 = (const uint16_t*)lw.k_weight; q.w2 = (const uint16_t*)lw.v_weight;
       q.n1 = HQ * D; q.n2 = (HQ + HKV) * D; q.out = wk.raw;
       if ((e = launch_skinny<SK_RAW>(q, st)) != hipSuccess) return e;
-      if (position == 0) {
+      if (position == 0 && !pk.n) {
         const ShortAttnArgs sa{wk.raw, M, l, (const uint16_t*)lw.q_norm_weight, (const uint16_t*)lw.k_norm_weight,
                                cos_tab, sin_tab, k_cache, v_cache, kv, wk.bad, wk.ah};
         if ((e = launch_short_attn(sa, st)) != hipSuccess) return e;
       } else {
         MKP_LAUNCH(qkv_post_kernel, dim3((M * (HQ + 2 * HKV) + 3) / 4), dim3(64), 0, st, wk.raw, 1, M, position,
                    (const uint16_t*)lw.q_norm_weight, (const uint16_t*)lw.k_norm_weight, cos_tab, sin_tab, wk.qh,
-                   wk.ql, k_cache, v_cache, l, kv, wk.bad);
+                   wk.ql, k_cache, v_cache, l, kv, wk.bad, pk.rows);
         AttnArgs at = at0;
         at.layer = l;
-        MKP_LAUNCH(attn_kernel, attn_grid, dim3(512), 0, st, at);
-        if (ap.merge) MKP_LAUNCH(attn_merge_kernel, dim3(ap.merge), dim3(256), 0, st, at);
+        if ((e = attend(at)) != hipSuccess) return e;
       }
       if ((e = skinny_mlp<H, I>(lw, l + 1 < dims.num_layers ? (const uint16_t*)layers[l + 1].norm_weight : nullptr,
                                 M, wk.ah, wk.al, wk.bh, wk.x, wk.ssq, st)) != hipSuccess)
@@ -2370,21 +2445,20 @@ static hipError_t run(const mk_model_dims& dims, const int32_t* tokens, int M, i
     g.N = (HQ + 2 * HKV) * D;
     g.q_norm = (const uint16_t*)lw.q_norm_weight; g.k_norm = (const uint16_t*)lw.k_norm_weight;
     g.cos_tab = cos_tab; g.sin_tab = sin_tab; g.qh = wk.qh; g.ql = wk.ql; g.k_cache = k_cache; g.v_cache = v_cache;
-    g.layer = l; g.position = position; g.kv = kv; g.bad = wk.bad;
+    g.layer = l; g.position = position; g.kv = kv; g.bad = wk.bad; g.pk = pk.rows;
     if (sq > 1) {
       GemmArgs gq = g;
       gq.part = wk.qpart;
       if ((e = launch_gemm<EPI_QKV_PART>(dim3(g.N / NT, mtiles, sq), gq, st)) != hipSuccess) return e;
       MKP_LAUNCH(qkv_post_kernel, dim3((M * (HQ + 2 * HKV) + 3) / 4), dim3(64), 0, st, wk.qpart, sq, M, position,
                  (const uint16_t*)lw.q_norm_weight, (const uint16_t*)lw.k_norm_weight, cos_tab, sin_tab, wk.qh, wk.ql,
-                 k_cache, v_cache, l, kv, wk.bad);
+                 k_cache, v_cache, l, kv, wk.bad, pk.rows);
     } else if ((e = launch_gemm<EPI_QKV>(dim3(g.N / NT, mtiles), g, st)) != hipSuccess) {
       return e;
     }
     AttnArgs at = at0;
     at.layer = l;
-    MKP_LAUNCH(attn_kernel, attn_grid, dim3(512), 0, st, at);
-    if (ap.merge) MKP_LAUNCH(attn_merge_kernel, dim3(ap.merge), dim3(256), 0, st, at);
+    if ((e = attend(at)) != hipSuccess) return e;
     GemmArgs go{};
     go.ah = wk.ah; go.al = wk.al; go.M = M; go.N = H; go.K = HQ * D;
     go.w0 = (const uint16_t*)lw.o_proj_weight; go.x = wk.x; go.ldx = H; go.part = so > 1 ? wk.part : nullptr;
@@ -2411,6 +2485,11 @@ static hipError_t run(const mk_model_dims& dims, const int32_t* tokens, int M, i
   if (!small && sd > 1)  // the last layer's down partials into the residual
     MKP_LAUNCH((bnorm_kernel<H, 0>), dim3((M + 3) / 4), dim3(256), 0, st, wk.x, nullptr, embed, dims.vocab, wk.bad,
                wk.part, sd, nullptr, nullptr, nullptr, M);
+  if (pk.n) {  // each sequence's last row's
+    MKP_LAUNCH(last_rows_kernel<H>, dim3(pk.n), dim3(H / 4), 0, st, wk.x, pk.ends, wk.last);
+    return lm_head_rows<H>(dims, pk.n, wk.last, final_norm, lm_head, wk.ah, wk.ah, wk.al, logits, out_token, wk.keys,
+                           wk.bad, st);
+  }
   // the last row's logits and greedy token
   MKP_LAUNCH(lm_head_kernel<H>, dim3(256), dim3(512), 0, st, wk.x, M - 1, final_norm, lm_head, dims.vocab, logits,
              wk.keys, wk.bad);
@@ -2485,6 +2564,50 @@ extern "C" hipError_t mk_prefill_paged(const mk_model_dims* dims, const int32_t*
   return prefill_impl(dims, tokens, num_tokens, position, embed_weight, lm_head_weight, final_norm_weight,
                       layer_weights, cos_table, sin_table, k_pages, v_pages, kv, max_seq_len, logits, out_token,
                       workspace, workspace_bytes, stream);
+}
+
+extern "C" size_t mk_prefill_batch_workspace_bytes(const mk_model_dims* dims, int num_tokens) {
+  if (!dims || num_tokens < 1 || num_tokens > MK_PREFILL_BATCH_TOKENS) return 0;
+  return prefill_bytes(dims->hidden, dims->intermediate, num_tokens, true);
+}
+
+extern "C" hipError_t mk_prefill_batch(const mk_model_dims* dims, const int32_t* tokens, const int32_t* lengths,
+                                       int num_seqs, const void* embed_weight, const void* lm_head_weight,
+                                       const void* final_norm_weight, const void* layer_weights, const void* cos_table,
+                                       const void* sin_table, void* k_cache, void* v_cache, int64_t seq_stride,
+                                       int max_seq_len, float* logits, int32_t* out_tokens, void* workspace,
+                                       size_t workspace_bytes, hipStream_t stream) {
+  if (!dims || !tokens || !lengths || !embed_weight || !lm_head_weight || !final_norm_weight || !layer_weights ||
+      !cos_table || !sin_table || !k_cache || !v_cache || !logits || !workspace)
+    return hipErrorInvalidValue;
+  const bool s06 = dims->hidden == 1024 && dims->intermediate == 3072;
+  const bool s17 = dims->hidden == 2048 && dims->intermediate == 6144;
+  if (!(s06 || s17) || dims->num_layers < 1 || dims->vocab < 1 || dims->vocab % 16 != 0) return hipErrorInvalidValue;
+  if (num_seqs < 1 || num_seqs > BMAX || max_seq_len < 1) return hipErrorInvalidValue;
+  // a sequence's cache may be followed by others of the same batch: at least its own size apart
+  if (num_seqs > 1 && seq_stride < (int64_t)dims->num_layers * HKV * max_seq_len * D) return hipErrorInvalidValue;
+  if (seq_stride % 8 != 0) return hipErrorInvalidValue;
+  PackedRun pk;
+  int64_t total = 0;
+  for (int i = 0; i < num_seqs; ++i) {
+    if (lengths[i] < 1 || lengths[i] > max_seq_len) return hipErrorInvalidValue;
+    total += lengths[i];
+    if (total > MK_PREFILL_BATCH_TOKENS) return hipErrorInvalidValue;
+    pk.ends.end[i] = (int32_t)total;
+  }
+  const int M = (int)total;
+  const Layout L = layout(dims->hidden, dims->intermediate, M, small_prompt(dims->hidden, M, 1), true);
+  if (workspace_bytes < L.bytes || reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return hipErrorInvalidValue;
+  const Work wk = carve(workspace, L);
+  pk.n = num_seqs;
+  pk.lengths = lengths;
+  pk.rows = {wk.rows, seq_stride};
+  const KvMap kv{nullptr, 0, 0, max_seq_len};
+  const mk_layer_weights* lw = static_cast<const mk_layer_weights*>(layer_weights);  // host array
+  auto* go = s06 ? &run<1024, 3072> : &run<2048, 6144>;
+  return go(*dims, tokens, M, 0, (const uint16_t*)embed_weight, (const uint16_t*)lm_head_weight,
+            (const uint16_t*)final_norm_weight, lw, (const uint16_t*)cos_table, (const uint16_t*)sin_table,
+            (uint16_t*)k_cache, (uint16_t*)v_cache, kv, logits, out_tokens, wk, stream, pk);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -2567,33 +2690,8 @@ static hipError_t run_batch(const mk_model_dims& dims, int B, const int32_t* tok
                               st)) != hipSuccess)
       return e;
   }
-  // the final norm, then the tied LM head as one more skinny
-  // product (vocabulary rows x the B normalised rows: each table byte read once, on the matrix
-  // cores) and the greedy keys
-  const bool lm_tiles = B > 8 && dims.vocab % NT == 0;
-  if (lm_tiles)
-    MKB_LAUNCH((bnorm_kernel<H, 1>), rows, nthr, 0, st, x, nullptr, embed, dims.vocab, bad, nullptr, 0,
-               final_norm, ah, al, B);
-  else
-    MKB_LAUNCH((bnorm_kernel<H, 2>), rows, nthr, 0, st, x, nullptr, embed, dims.vocab, bad, nullptr, 0,
-               final_norm, af, nullptr, B);
-  if (!lm_tiles) {
-    SkArgs lmh{};
-    lmh.xh = af; lmh.B = B; lmh.N = dims.vocab; lmh.K = H;
-    lmh.w0 = lm_head; lmh.n1 = dims.vocab; lmh.n2 = dims.vocab; lmh.out = logits;
-    if ((e = launch_skinny<SK_RAW>(lmh, st)) != hipSuccess) return e;
-  } else {
-    // beyond one column block the skinny product re-reads every row's activations per 16 table
-    // rows; a 128-row tile of the table reads them once per 128 (the B rows are one row tile)
-    GemmArgs gl{};
-    gl.ah = ah; gl.al = al; gl.M = B; gl.N = dims.vocab; gl.K = H;
-    gl.w0 = lm_head; gl.part = logits;  // logits[b][v], no residual
-    if ((e = launch_gemm<EPI_RESID>(dim3(dims.vocab / NT, 1, 1), gl, st)) != hipSuccess) return e;
-  }
-  MKB_LAUNCH(logits_argmax_kernel, dim3((dims.vocab + 4095) / 4096, B), dim3(256), 0, st, logits, dims.vocab, keys, bad);
-  if (out_tokens) MKB_LAUNCH(keys_to_tokens_kernel, dim3(1), dim3(64), 0, st, keys, B, bad, out_tokens);
+  return lm_head_rows<H>(dims, B, x, final_norm, lm_head, af, ah, al, logits, out_tokens, keys, bad, st);
 #undef MKB_LAUNCH
-  return hipSuccess;
 }
 
 }  // namespace mkp

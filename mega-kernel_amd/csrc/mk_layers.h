@@ -72,4 +72,33 @@ __device__ __forceinline__ void head_norm_rope(float (&v)[8], const float (&wn)[
   }
 }
 
+// Fragment-major layout of a bf16 activation matrix with K columns (K a multiple of 32), the A
+// operand of gemm_kernel: 16-row x 32-column blocks of 1 KB, block (m / 16, k / 32) at KB offset
+// (m / 16) * (K / 32) + k / 32; inside a block, MFMA lane l = (m % 16) + 16 * ((k % 32) / 8) holds
+// the 16 bytes of columns [8 ((k % 32) / 8), +8). A wave reads one operand fragment as 1 KB of
+// consecutive bytes. Buffers in this layout hold whole row tiles (operand_rows); rows past M are never
+// written, and the sums they produce are never stored.
+__device__ __forceinline__ size_t frag_off(int m, int k, int K) {
+  return ((((size_t)(m >> 4) * (K >> 5) + (k >> 5)) * 64 + ((k >> 3) & 3) * 16 + (m & 15)) << 3) + (k & 7);
+}
+
+// Activation operand of the skinny products in fragment order ("skinny fragments", used by the
+// batched decode): for column block cb (sequences 8 cb .. 8 cb + 7) and K block kb (32 inputs), one
+// 1 KB fragment holding, at lane l, MFMA column li = l % 16 (sequence 8 cb + li / 2, bf16 hi part for
+// even li, lo for odd) and inputs 32 kb + 8 (l / 16) .. + 8. A wave then loads a whole B operand as
+// 1 KB of consecutive bytes. In row order (B rows of ldx elements, hi and lo in two arrays) each lane
+// of such a load reads 16 bytes of a different row, and the vector cache takes one access per lane:
+// at 64 sequences that was the skinny products' bound (rocprof at 64 sequences: ~64 L1 accesses per
+// load instruction, TA address stalls). Rows past the batch are never written; their columns of the
+// products are never read.
+// Column-block major: the K blocks of one column block are adjacent. (K-block major, the column blocks of
+// one K block adjacent, measured on MI355X from 9 to 64 sequences and 16 to 256 prompt tokens at both
+// widths: within 0.4% either way, but 131 tokens 1,612 -> 1,634 us, 40 at 1.7B 1,740 -> 1,754.)
+__host__ __device__ inline int skf_blocks(int B) { return (B + 7) / 8; }
+__host__ __device__ inline size_t skf_frag(int cb, int kb, int K) { return (size_t)cb * (K >> 5) + kb; }
+__host__ __device__ inline size_t skf_off(int b, int k, int part, int K) {
+  const int cb = b >> 3, li = 2 * (b & 7) + part, kb = k >> 5, lg = (k & 31) >> 3;
+  return ((skf_frag(cb, kb, K) * 64 + lg * 16 + li) << 3) + (k & 7);
+}
+
 }  // namespace mkp

@@ -57,7 +57,7 @@ struct PackedArgs {
   void* out;           // PARTS 1: bf16 [rows][heads][128], 2: fragments, 3: fp32 [rows][heads][128]
   uint16_t* out_lo;    // PARTS 2: attn_out's `ol`
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // elements
-  int64_t kv_seq;      // elements between the sequences' caches; 0: their K/V rows are packed as the queries are
+  int64_t kv_seq;      // PARTS 2: elements between the sequences' caches
   int hkv, g, nseq, frag;
   // the launch's sequences, longest first: query blocks before them, first row, length, number
   int32_t first[PSEQ], row[PSEQ], len[PSEQ], seq[PSEQ];
@@ -126,9 +126,9 @@ __global__ void __launch_bounds__(64 * PW, 2) packed_attention_kernel(const Pack
   const int last = (min(rows, (qb + 1) * PR) - 1) / a.g;  // the block's last token
   const int wlast = r0 < rows ? (min(rows, r0 + 32) - 1) / a.g : -1;
   const int ntile = last / PK + 1;
-  const int64_t kv0 = a.kv_seq ? a.seq[si] * a.kv_seq : 0;
-  const uint16_t* kbase = a.k + (a.kv_seq ? kv0 : row0 * a.k_row) + kh * a.k_head;
-  const uint16_t* vbase = a.v + (a.kv_seq ? kv0 : row0 * a.v_row) + kh * a.v_head;
+  // its first key and value row: in the sequence's cache, or packed as the queries are
+  const uint16_t* kbase = a.k + (PARTS == 2 ? a.seq[si] * a.kv_seq : row0 * a.k_row) + kh * a.k_head;
+  const uint16_t* vbase = a.v + (PARTS == 2 ? a.seq[si] * a.kv_seq : row0 * a.v_row) + kh * a.v_head;
 
   // wave w stages rows 16 w .. 16 w + 15 of a tile, four to an instruction (lane l: chunk l % 16 of row
   // l / 16), through registers, where the next tile waits while this one is multiplied. Keys past the
@@ -191,7 +191,9 @@ __global__ void __launch_bounds__(64 * PW, 2) packed_attention_kernel(const Pack
   f32x16 acc[4];  // dims 32 b + 8 (j / 4) + 4 g + j % 4 of query `col`
 #pragma unroll
   for (int b = 0; b < 4; ++b) acc[b] = f32x16{};
-  float mrun = -INFINITY, lrun = 0.f;  // maximum of the raw scores; this lane's half of the sum
+  // running maximum of the raw scores, the same in the exponents' scale (rounded once: the weights and the
+  // later rescaling refer to one number), this lane's half of the sum
+  float mrun = -INFINITY, mscaled = 0.f, lrun = 0.f;
   constexpr float C = ATT_SCALE * 1.4426950408889634f;
 
   // one tile into the running softmax and the output. MASKED: some query of the block sees it in part
@@ -229,8 +231,9 @@ __global__ void __launch_bounds__(64 * PW, 2) packed_attention_kernel(const Pack
       for (int j = 0; j < 16; ++j) m = fmaxf(m, st[h][j]);
     m = xmax32(m);
     const float mc = m == -INFINITY ? 0.f : m * C;  // a query that has seen no key of weight so far
-    const float alpha = __builtin_amdgcn_exp2f(mrun * C - mc);
+    const float alpha = __builtin_amdgcn_exp2f(mscaled - mc);  // exactly 1 when the maximum holds
     mrun = m;
+    mscaled = mc;
     float sum = 0.f;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -328,7 +331,15 @@ __global__ void __launch_bounds__(64 * PW, 2) packed_attention_kernel(const Pack
         *reinterpret_cast<uint4*>((uint16_t*)a.out + (m * (a.hkv * a.g) + hq) * D + d) =
             make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]),
                        pack_bf16x2(o[6], o[7]));
-      } else if constexpr (PARTS == 3) {
+      } else if constexpr (PARTS == 2) {  // attn_out's two fragment orders (layers_kernel.hip)
+        uint4 p[PARTS];
+        split_parts<PARTS>(o, p);
+        const int64_t kk = hq * D + d;
+        uint16_t* out = (uint16_t*)a.out;
+        *reinterpret_cast<uint4*>(out + (a.frag == 2 ? skf_off(m, kk, 0, HQ * D) : frag_off(m, kk, HQ * D))) = p[0];
+        *reinterpret_cast<uint4*>(a.frag == 2 ? out + skf_off(m, kk, 1, HQ * D)
+                                              : a.out_lo + frag_off(m, kk, HQ * D)) = p[1];
+      } else {
         float4* p = reinterpret_cast<float4*>((float*)a.out + (m * (a.hkv * a.g) + hq) * D + d);
         p[0] = make_float4(o[0], o[1], o[2], o[3]);
         p[1] = make_float4(o[4], o[5], o[6], o[7]);
@@ -368,6 +379,26 @@ static hipError_t launch_packed(PackedArgs& a, const int32_t* lengths, int num_s
     return hipErrorOutOfMemory;
   }
   return hipSuccess;
+}
+
+hipError_t mkp_attention_prefill(const MkPackedPrefill& p, hipStream_t stream) {
+  PackedArgs a{};
+  a.q = p.qh;
+  a.ql = p.ql;
+  const int64_t layer = (int64_t)p.layer * HKV * p.max_seq * D;
+  a.k = p.k_cache + layer;
+  a.v = p.v_cache + layer;
+  a.out = p.oh;
+  a.out_lo = p.ol;
+  a.q_row = HQ * D;
+  a.q_head = D;
+  a.k_row = a.v_row = D;
+  a.k_head = a.v_head = (int64_t)p.max_seq * D;
+  a.kv_seq = p.seq_stride;
+  a.hkv = HKV;
+  a.g = HQ / HKV;
+  a.frag = p.frag;
+  return launch_packed<2>(a, p.lengths, p.num_seqs, stream);
 }
 
 extern "C" hipError_t mk_attention_packed(int q_heads, int kv_heads, const void* q, int64_t q_row_stride,

@@ -396,6 +396,60 @@ std::tuple<torch::Tensor, torch::Tensor> decode_batch(torch::Tensor tokens, torc
   return {logits, toks};
 }
 
+// Prefill of several prompts (mk_prefill_batch) into decode_batch's caches: tokens int32 [all tokens] on the
+// weights' device, the prompts' lengths on the host, caches bf16 [prompts, L, 8, max_seq, 128] whose first
+// dimension may have any larger stride (k_caches[::n]: every n-th sequence's). Returns (fp32 logits
+// [prompts, V], int32 greedy tokens [prompts] on the device).
+std::tuple<torch::Tensor, torch::Tensor> prefill_batch(torch::Tensor tokens, std::vector<int64_t> lengths,
+                                                       torch::Tensor embed, torch::Tensor lm_head,
+                                                       torch::Tensor final_norm, std::vector<torch::Tensor> lw,
+                                                       torch::Tensor cos, torch::Tensor sin, torch::Tensor kc,
+                                                       torch::Tensor vc, int64_t max_seq_len) {
+  Checked c = validate(0, embed, lm_head, final_norm, lw, cos, sin, kc, vc, 0, max_seq_len, false, true);
+  const int64_t S = (int64_t)lengths.size(), L = c.dims.num_layers;
+  TORCH_CHECK(S >= 1 && S <= 64, "megakernel: lengths must name 1 to 64 prompts, got ", S);
+  int64_t total = 0;
+  std::vector<int32_t> len;
+  for (int64_t n : lengths) {
+    TORCH_CHECK(n >= 1 && n <= max_seq_len, "megakernel: a prompt's length must be between 1 and max_seq_len (",
+                max_seq_len, "), got ", n);
+    total += n;
+    len.push_back((int32_t)n);
+  }
+  TORCH_CHECK(total <= MK_PREFILL_BATCH_TOKENS, "megakernel: at most ", MK_PREFILL_BATCH_TOKENS, " tokens in one call");
+  TORCH_CHECK(tokens.defined() && tokens.device() == c.dev && tokens.scalar_type() == torch::kInt32 &&
+                  tokens.is_contiguous() && tokens.dim() == 1 && tokens.size(0) == total,
+              "megakernel: tokens must be a contiguous int32 tensor of the lengths' sum (", total, ") on ", c.dev);
+  TORCH_CHECK(c.dims.vocab % 16 == 0, "megakernel: the vocabulary size must be a multiple of 16");
+  for (const torch::Tensor* t : {&kc, &vc}) {
+    const char* name = t == &kc ? "k_cache" : "v_cache";
+    TORCH_CHECK(t->defined() && t->dim() == 5 && t->size(0) == S, "megakernel: ", name,
+                " must be [prompts, layers, 8, max_seq, 128] for ", S, " prompts");
+    check_bf16((*t)[0], name, {L, kKVHeads, max_seq_len, kHeadDim}, c.dev);
+    TORCH_CHECK(S == 1 || (t->stride(0) % 8 == 0 && t->stride(0) >= L * kKVHeads * max_seq_len * kHeadDim),
+                "megakernel: ", name, "'s sequences must not overlap and start on 16-byte boundaries");
+  }
+  TORCH_CHECK(S == 1 || kc.stride(0) == vc.stride(0), "megakernel: k_cache and v_cache must have the same strides");
+  TORCH_CHECK(embed.is_cuda(), "megakernel: embed_weight must be a GPU tensor");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(c.dev);
+  hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(c.dev.index()).stream();
+  std::vector<mk_layer_weights> table(L);
+  for (int64_t l = 0; l < L; ++l) {
+    const torch::Tensor* t = &lw[l * kPerLayer];
+    table[l] = {t[0].data_ptr(), t[1].data_ptr(), t[2].data_ptr(), t[3].data_ptr(), t[4].data_ptr(), t[5].data_ptr(),
+                t[6].data_ptr(), t[7].data_ptr(), t[8].data_ptr(), t[9].data_ptr(), t[10].data_ptr()};
+  }
+  const size_t bytes = mk_prefill_batch_workspace_bytes(&c.dims, (int)total);
+  auto ws = torch::empty({(int64_t)bytes}, embed.options().dtype(torch::kUInt8));
+  auto logits = torch::empty({S, c.dims.vocab}, embed.options().dtype(torch::kFloat32));
+  auto toks = torch::empty({S}, embed.options().dtype(torch::kInt32));
+  MK_HIP_CHECK(mk_prefill_batch(&c.dims, tokens.data_ptr<int32_t>(), len.data(), (int)S, embed.data_ptr(),
+                                lm_head.data_ptr(), final_norm.data_ptr(), table.data(), cos.data_ptr(), sin.data_ptr(),
+                                kc.data_ptr(), vc.data_ptr(), S == 1 ? 0 : kc.stride(0), (int)max_seq_len,
+                                logits.data_ptr<float>(), toks.data_ptr<int32_t>(), ws.data_ptr(), bytes, stream));
+  return {logits, toks};
+}
+
 // Element strides of a [rows, heads, 128] operand of attention_packed, the heads' 128 elements contiguous.
 struct HeadRows {
   int64_t row, head;
@@ -583,6 +637,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("decode_batch", &decode_batch,
         "batched decode of B <= 64 sequences (int32 tokens [B], positions [B], caches [B, L, 8, max_seq, 128]); "
         "returns (fp32 logits [B, V], int32 greedy tokens [B] on device)");
+  m.def("prefill_batch", &prefill_batch,
+        "prefill of 1 to 64 prompts (int32 tokens one after the other, lengths a list) into decode_batch's caches "
+        "[prompts, L, 8, max_seq, 128]; returns (fp32 logits [prompts, V], int32 greedy tokens [prompts] on device)");
   m.def("attention_packed", &attention_packed,
         "causal attention of packed sequences: q [rows, heads, 128] bf16 or fp32, k and v [rows, K/V heads, 128] "
         "bf16, lengths a list that adds up to the rows; returns [rows, heads, 128] in q's type");
