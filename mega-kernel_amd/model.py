@@ -18,9 +18,14 @@ Mirrors ``/root/reference/model.py`` step for step:
   * ``--native-prefill``: the prompt goes through the batched prefill kernel (``prefill``: all
     prompt tokens at once on the matrix cores, writing the ``[L, 8, max_seq, 128]`` cache
     directly) instead of the Transformers prefill and cache copy.
+  * ``--beams W`` (and ``--prompts S``): beam search instead of the greedy loop, S prompts of different
+    lengths with W beams each (S * W <= 64). ``prefill_batch`` fills the first beam's cache of every
+    prompt in one call and ``beam_reorder`` spreads it over the others; each step is ``beam_select``,
+    ``beam_reorder`` of the rows generated so far, and ``decode_batch`` of all beams. Nothing is read
+    back until the last step.
 
     python mega-kernel_amd/model.py [--shape qwen3-0.6b] [--prompt 32] [--max-seq 512] [--new 64]
-                                    [--device-loop] [--native-prefill]
+                                    [--device-loop] [--native-prefill] [--beams 4 [--prompts 2] [--eos ID]]
 """
 import argparse
 import os
@@ -49,6 +54,49 @@ def build_model(shape, max_positions, seed=0):
     return Qwen3ForCausalLM(cfg).to(torch.bfloat16).eval()
 
 
+def beam_search(kernel, prompts, beams, new, eos, embed, final_norm, layer_weights, cos, sin, max_seq):
+    """The best ``beams`` continuations of up to ``new`` tokens of each prompt (lists of token ids), best first, as
+    (tokens, score) with the score the sum of their log-probabilities; a continuation ends with ``eos`` (-1: none
+    does). All calls are queued without reading anything back, so ``new`` steps are always made."""
+    import torch
+    dev, rows = embed.device, len(prompts) * beams
+    lengths = [len(p) for p in prompts]
+    shape = (rows, len(layer_weights) // 11, 8, max_seq, 128)
+    k, v = (torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    packed = torch.tensor([t for p in prompts for t in p], dtype=torch.int32, device=dev)
+    weights = (embed, embed, final_norm, layer_weights, cos, sin)
+    first, _ = kernel.prefill_batch(packed, lengths, *weights, k[::beams], v[::beams], max_seq)
+    begin = torch.tensor(lengths, dtype=torch.int32, device=dev).repeat_interleave(beams)
+    heads = torch.arange(rows, dtype=torch.int32, device=dev) // beams * beams
+    kernel.beam_reorder(k, v, heads, torch.zeros_like(begin), begin, beams)
+    logits = first.repeat_interleave(beams, 0)
+    scores = torch.full((rows,), -float("inf"), device=dev)
+    scores[::beams] = 0  # a prompt's beams are one until the first selection
+    finished = torch.zeros(rows, dtype=torch.bool, device=dev)
+    position, steps = begin.clone(), []
+    for i in range(new):
+        tokens, parents, scores, finished = kernel.beam_select(logits, scores, finished, beams, eos)
+        steps.append((tokens, parents, finished))
+        if i + 1 < new:
+            kernel.beam_reorder(k, v, parents, begin, position, beams)
+            logits, _ = kernel.decode_batch(tokens, position, *weights, k, v, max_seq)
+            position = position + 1
+    steps, scores = [tuple(t.tolist() for t in s) for s in steps], scores.tolist()
+    found = []
+    for s in range(len(prompts)):
+        group = []
+        for row in range(s * beams, (s + 1) * beams):
+            path, at = [], row
+            for i in reversed(range(new)):
+                tokens, parents, _ = steps[i]
+                if i == 0 or not steps[i - 1][2][parents[at]]:  # not the repeated end of a finished one
+                    path.append(tokens[at])
+                at = parents[at]
+            group.append((path[::-1], scores[row]))
+        found.append(group)
+    return found
+
+
 def run(argv=None, keep_prefill_cache=False):
     """Runs the driver and returns what it did: the generated tokens (the prefill's greedy token
     first), the prompt length, the device status after the loop, ms per token, and, with
@@ -63,7 +111,12 @@ def run(argv=None, keep_prefill_cache=False):
     ap.add_argument("--native-prefill", action="store_true",
                     help="fill the cache with the batched prefill kernel (prefill) instead of the Transformers "
                          "prefill and cache copy")
+    ap.add_argument("--beams", type=int, default=0, help="beam search with this many beams per prompt (1 to 16)")
+    ap.add_argument("--prompts", type=int, default=1, help="with --beams: prompts searched together")
+    ap.add_argument("--eos", type=int, default=-1, help="with --beams: the token that ends a continuation")
     a = ap.parse_args(argv)
+    if a.beams and (a.beams > 16 or a.beams < 0 or a.prompts < 1 or a.beams * a.prompts > 64):
+        ap.error("--beams takes 1 to 16 beams per prompt, and at most 64 in all")
     import torch
     import megakernel
 
@@ -75,6 +128,23 @@ def run(argv=None, keep_prefill_cache=False):
     embed = model.model.embed_tokens.weight.detach().to(dev)
     final_norm = model.model.norm.weight.detach().to(dev)
     cos, sin = megakernel.rope_tables(model, a.max_seq, dev)
+
+    if a.beams:
+        # prompts of different lengths, the longest of --prompt tokens: pieces of the same random ids
+        prompts = [ids[0, :max(1, a.prompt - 5 * i)].tolist() for i in range(a.prompts)]
+        new = min(a.new, a.max_seq - a.prompt)
+        t0 = time.perf_counter()
+        found = beam_search(kernel, prompts, a.beams, new, a.eos, embed, final_norm, layer_weights, cos, sin, a.max_seq)
+        wall = time.perf_counter() - t0
+        for i, group in enumerate(found):
+            print(f"prompt {i} ({len(prompts[i])} tokens): " + "; ".join(
+                f"{score:.3f} {tokens[:8]}{' ...' if len(tokens) > 8 else ''}" for tokens, score in group))
+        print(f"beam search: {a.prompts} x {a.beams} beams, {new} steps in {wall * 1e3:.1f} ms, device status "
+              f"{kernel.status()}")
+        return {"prompt": a.prompt, "prompts": prompts, "beams": found, "status": kernel.status(),
+                "generated": [t for group in found for tokens, _ in group for t in tokens],
+                "inputs": {"embed": embed, "final_norm": final_norm, "layer_weights": layer_weights, "cos": cos,
+                           "sin": sin, "max_seq": a.max_seq}}
 
     k_cache, v_cache = megakernel.empty_cache(len(model.model.layers), a.max_seq, dev)
     if a.native_prefill:
