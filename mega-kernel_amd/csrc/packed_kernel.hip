@@ -45,10 +45,24 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
 
-constexpr int PK = 64;         // keys per tile
 constexpr int PW = 4;          // waves per workgroup
 constexpr int PR = 32 * PW;    // rows per workgroup
 constexpr int PSEQ = 128;      // sequences per launch (their places travel as kernel arguments)
+
+// Division by a number that the host knows: q = n / d for 0 <= n < 2^31 by a multiplication (the rounded-up
+// reciprocal of d at 32 + ceil(log2 d) bits is off by less than 2^-31 of n / d).
+struct DivBy {
+  uint32_t d, mul, shift;
+};
+static DivBy div_by(uint32_t d) {
+  uint32_t l = 0;
+  while ((1u << l) < d) ++l;
+  return {d, (uint32_t)(((1ull << (32 + l)) + d - 1) / d - (1ull << 32)), l};  // the multiplier's low 32 of 33 bits
+}
+__device__ __forceinline__ int div(uint32_t n, const DivBy& b) {
+  return (int)((uint32_t)(((uint64_t)__umulhi(n, b.mul) + n) >> b.shift));
+}
+__device__ __forceinline__ int mod(uint32_t n, const DivBy& b) { return (int)(n - div(n, b) * b.d); }
 
 struct PackedArgs {
   const void* q;       // PARTS 1: bf16, 2: the hi parts, 3: fp32
@@ -58,8 +72,9 @@ struct PackedArgs {
   uint16_t* out_lo;    // PARTS 2: attn_out's `ol`
   int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // elements
   int64_t kv_seq;      // PARTS 2: elements between the sequences' caches
+  DivBy by_hkv, by_g;
   int hkv, g, nseq, frag;
-  // the launch's sequences, longest first: query blocks before them, first row, length, number
+  // the launch's sequences, longest first: see the kernel's order of blocks; first row, length, number
   int32_t first[PSEQ], row[PSEQ], len[PSEQ], seq[PSEQ];
 };
 
@@ -101,73 +116,125 @@ __device__ __forceinline__ uint32_t finite_or_0(uint32_t w) {
 // transposed read takes 64 bytes of each of 4 rows).
 constexpr int PKS = 2 * D + 16, PVS = 2 * D + 64;
 
+template <int PK, int KS>
 struct PackedSmem {
-  unsigned char k[2][PK * PKS];
-  unsigned char v[2][PK * PVS];
-  int bad[PW];  // per staging wave: an infinity or NaN in a value row of a tile seen in part
+  struct Tiles {
+    unsigned char k[2][PK * PKS];
+    unsigned char v[2][PK * PVS];
+  };
+  union {
+    Tiles tiles[KS];
+    struct {  // the second wave group's output columns, maximum and sum, lane by lane
+      float acc[KS > 1 ? PW : 1][64][64], m[PW][64], l[PW][64];
+    } join;
+  };
+  int bad[KS * PW];  // per staging wave: an infinity or NaN in a value row of a tile seen in part
 };
 
-template <int PARTS>
-__global__ void __launch_bounds__(64 * PW, 2) packed_attention_kernel(const PackedArgs a) {
-  __shared__ __attribute__((aligned(16))) PackedSmem sm;
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+template <int PARTS, int PK, int KS>
+__global__ void __launch_bounds__(64 * PW * KS, 2) packed_attention_kernel(const PackedArgs a) {
+  constexpr int PH = PK / 32, NX = PK / (4 * PW);  // 32-key halves of a tile, chunks of K that a lane stages
+  __shared__ __attribute__((aligned(16))) PackedSmem<PK, KS> sm;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int w = wave % PW, ks = wave / PW;   // a group of PW waves takes every KS-th tile: tile ks, KS + ks, ...
   const int col = lane & 31, g = lane >> 5;  // this lane's query and half of the K slots
+  auto& tiles = sm.tiles[ks];
   // workgroup b: K/V head b % hkv (with 8 heads, a head's keys stay in one XCD's L2), query block b / hkv of
-  // the launch, a sequence's last block (the most keys) first
-  const int kh = blockIdx.x % a.hkv, item = blockIdx.x / a.hkv;
-  int si = -1;
+  // the launch's. The blocks go by their number in their sequence, the highest (the most keys) first: with the
+  // sequences' block counts n_0 >= n_1 >= ..., those above n_1 are sequence 0's, the next down to n_2 sequence
+  // 0's and 1's in turn, and so on; first[i] blocks come before those of i + 1 sequences in turn.
+  // The tables are read whole, a lane an entry, and picked from with lane reads: arguments are far away, and
+  // one round trip there costs as much as a tile.
+  int tf[PSEQ / 64], tl[PSEQ / 64], tr[PSEQ / 64], ts[PSEQ / 64];
 #pragma unroll
-  for (int o = 0; o < PSEQ; o += 64)
-    si += __popcll(__builtin_amdgcn_ballot_w64(o + lane < a.nseq && a.first[o + lane] <= item));
-  const int len = a.len[si], row0 = a.row[si], rows = len * a.g;
-  const int qb = (rows + PR - 1) / PR - 1 - (item - a.first[si]);
+  for (int o = 0; o < PSEQ / 64; ++o) {
+    tf[o] = a.first[64 * o + lane];
+    tl[o] = a.len[64 * o + lane];
+    tr[o] = a.row[64 * o + lane];
+    ts[o] = PARTS == 2 ? a.seq[64 * o + lane] : 0;
+  }
+  auto pick = [&](const int (&t)[PSEQ / 64], int n) {
+    int v = __builtin_amdgcn_readlane(t[0], n & 63);
+#pragma unroll
+    for (int o = 1; o < PSEQ / 64; ++o) v = n >= 64 * o ? __builtin_amdgcn_readlane(t[o], n & 63) : v;
+    return v;
+  };
+  const int kh = mod(blockIdx.x, a.by_hkv), item = div(blockIdx.x, a.by_hkv);
+  int pi = -1;
+#pragma unroll
+  for (int o = 0; o < PSEQ / 64; ++o)
+    pi += __popcll(__builtin_amdgcn_ballot_w64(64 * o + lane < a.nseq && tf[o] <= item));
+  const int at = item - pick(tf, pi), turn = at / (pi + 1), si = at - turn * (pi + 1);
+  const int qb = (pick(tl, pi) * a.g + PR - 1) / PR - 1 - turn;
+  const int len = pick(tl, si), row0 = pick(tr, si), rows = len * a.g;
   const int r0 = qb * PR + 32 * w, r = r0 + col;          // this wave's first row, this lane's row
-  const int rc = min(r, rows - 1), tok = rc / a.g, hq = kh * a.g + rc % a.g;
-  const int last = (min(rows, (qb + 1) * PR) - 1) / a.g;  // the block's last token
-  const int wlast = r0 < rows ? (min(rows, r0 + 32) - 1) / a.g : -1;
-  const int ntile = last / PK + 1;
+  const int rc = min(r, rows - 1), tok = div(rc, a.by_g), hq = kh * a.g + (rc - tok * a.g);
+  const int first = div(qb * PR, a.by_g), last = div(min(rows, (qb + 1) * PR) - 1, a.by_g);  // the block's tokens
+  const int wfirst = div(r0, a.by_g), wlast = r0 < rows ? div(min(rows, r0 + 32) - 1, a.by_g) : -1;  // the wave's
+  const int ntile = last / PK + 1, niter = (ntile + KS - 1) / KS;
+  auto tile = [&](int i) { return KS * i + ks; };
   // its first key and value row: in the sequence's cache, or packed as the queries are
-  const uint16_t* kbase = a.k + (PARTS == 2 ? a.seq[si] * a.kv_seq : row0 * a.k_row) + kh * a.k_head;
-  const uint16_t* vbase = a.v + (PARTS == 2 ? a.seq[si] * a.kv_seq : row0 * a.v_row) + kh * a.v_head;
+  const char* kbase = (const char*)(a.k + (PARTS == 2 ? pick(ts, si) * a.kv_seq : row0 * a.k_row) + kh * a.k_head);
+  const char* vbase = (const char*)(a.v + (PARTS == 2 ? pick(ts, si) * a.kv_seq : row0 * a.v_row) + kh * a.v_head);
 
-  // wave w stages rows 16 w .. 16 w + 15 of a tile, four to an instruction (lane l: chunk l % 16 of row
-  // l / 16), through registers, where the next tile waits while this one is multiplied. Keys past the
+  // a group's wave w stages rows PK / 4 w .. of its tile, four to an instruction (lane l: chunk l % 16 of row
+  // l / 16), through registers, where a later tile waits while this one is multiplied. Keys past the
   // block's last one are that one again (masked).
-  const int srow = 16 * w + (lane >> 4), chunk = lane & 15;
+  const int srow = PK / PW * w + (lane >> 4), chunk = lane & 15;
   struct Tile {
-    uint4 k[4], v[4];
+    uint4 x[NX];
   };
-  auto load = [&](Tile& x, int t) __attribute__((always_inline)) {
+  auto load = [&](Tile& d, const char* base, int64_t row, int i, bool whole = false) __attribute__((always_inline)) {
+    const int key = tile(i) * PK;
+    const uint32_t rb = 2 * (uint32_t)row;
+    if (whole || key + PK - 1 <= last) {  // the tile's rows as uniform bases, the lane's on them as 32 bits
+      const uint32_t o = srow * rb + 16 * chunk;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      // the tile's first row as a uniform base, the lane's as 32 bits on it
-      const uint32_t key = min(srow + 4 * i, last - t * PK);
-      x.k[i] = ld_global16(reinterpret_cast<const uint4*>(
-          reinterpret_cast<const char*>(kbase + (int64_t)(t * PK) * a.k_row) + (key * (2 * (uint32_t)a.k_row) + 16 * chunk)));
-      x.v[i] = ld_global16(reinterpret_cast<const uint4*>(
-          reinterpret_cast<const char*>(vbase + (int64_t)(t * PK) * a.v_row) + (key * (2 * (uint32_t)a.v_row) + 16 * chunk)));
+      for (int n = 0; n < NX; ++n)
+        d.x[n] = ld_global16(reinterpret_cast<const uint4*>(base + (key + 4 * n) * (2 * row) + o));
+    } else {
+#pragma unroll
+      for (int n = 0; n < NX; ++n)
+        d.x[n] = ld_global16(reinterpret_cast<const uint4*>(base + key * (2 * row) +
+                                                            (min(srow + 4 * n, last - key) * rb + 16 * chunk)));
     }
   };
-  const int first = qb * PR / a.g;  // the block's first token
-  auto store = [&](const Tile& x, int t) __attribute__((always_inline)) {
-    const int buf = t & 1;
+  auto store_k = [&](const Tile& d, int i) __attribute__((always_inline)) {
+    unsigned char* p = tiles.k[i & 1] + srow * PKS + 16 * chunk;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int rr = srow + 4 * i;
-      *reinterpret_cast<uint4*>(sm.k[buf] + rr * PKS + 16 * chunk) = x.k[i];
-      *reinterpret_cast<uint4*>(sm.v[buf] + rr * PVS + 16 * chunk) = x.v[i];
-    }
-    if (t * PK + PK - 1 > first) {  // a tile that some query of the block sees in part
-      uint32_t n = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        n |= nonfinite2(x.v[i].x) | nonfinite2(x.v[i].y) | nonfinite2(x.v[i].z) | nonfinite2(x.v[i].w);
-      if (n) sm.bad[w] = 1;
-    }
+    for (int n = 0; n < NX; ++n) *reinterpret_cast<uint4*>(p + 4 * n * PKS) = d.x[n];
   };
-  if (lane == 0) sm.bad[w] = 0;
-  Tile x;
-  load(x, 0);
+  auto store_v = [&](Tile& d, int i, bool whole = false) __attribute__((always_inline)) {
+    if (!whole && tile(i) * PK + PK - 1 > first) {  // a tile that some query of the block sees in part: finite rows only
+      uint32_t bad = 0;
+#pragma unroll
+      for (int n = 0; n < NX; ++n)
+        bad |= nonfinite2(d.x[n].x) | nonfinite2(d.x[n].y) | nonfinite2(d.x[n].z) | nonfinite2(d.x[n].w);
+      if (bad) {
+        sm.bad[wave] = 1;
+#pragma unroll
+        for (int n = 0; n < NX; ++n)
+          d.x[n] = make_uint4(finite_or_0(d.x[n].x), finite_or_0(d.x[n].y), finite_or_0(d.x[n].z), finite_or_0(d.x[n].w));
+      }
+    }
+    unsigned char* p = tiles.v[i & 1] + srow * PVS + 16 * chunk;
+#pragma unroll
+    for (int n = 0; n < NX; ++n) *reinterpret_cast<uint4*>(p + 4 * n * PVS) = d.x[n];
+  };
+  Tile x;  // on the way to LDS: V of the next tile, then K of the one after it
+  if (lane == 0) sm.bad[wave] = 0;
+  if (tile(0) < ntile) {
+    Tile k0, k1, v0;
+    load(k0, kbase, a.k_row, 0);
+    load(v0, vbase, a.v_row, 0);
+    if (tile(1) < ntile) {
+      load(k1, kbase, a.k_row, 1);
+      load(x, vbase, a.v_row, 1);
+    }
+    store_k(k0, 0);
+    store_v(v0, 0);
+    if (tile(1) < ntile) store_k(k1, 1);
+  }
 
   // the queries as the B operand: dims 16 s + 8 g .. +7 of row `col`
   uint4 fq[PARTS][8];
@@ -196,122 +263,200 @@ __global__ void __launch_bounds__(64 * PW, 2) packed_attention_kernel(const Pack
   float mrun = -INFINITY, mscaled = 0.f, lrun = 0.f;
   constexpr float C = ATT_SCALE * 1.4426950408889634f;
 
-  // one tile into the running softmax and the output. MASKED: some query of the block sees it in part
-  auto consume = [&](int t, auto MASKED) __attribute__((always_inline)) {
-    constexpr bool masked = decltype(MASKED)::value;
-    const int k0 = t * PK, buf = t & 1;
-    // this lane's places in the tile: K row `col` at dims 8 g, V row 4 g + l % 16 / 4 at dims 16 (l / 16 % 2) + 4 (l % 4)
-    const unsigned char* kt = sm.k[buf] + col * PKS + 16 * g;
-    const unsigned char* vt = sm.v[buf] + (4 * g + ((lane & 15) >> 2)) * PVS + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-    f32x16 st[2];
-    st[0] = f32x16{};
-    st[1] = f32x16{};
+  // raw scores of the group's tile i
+  typedef f32x16 Scores[PH];
+  auto scores = [&](Scores& st, int i) __attribute__((always_inline)) {
+    const unsigned char* kt = tiles.k[i & 1] + col * PKS + 16 * g;  // K row `col` at dims 8 g
+#pragma unroll
+    for (int h = 0; h < PH; ++h) st[h] = f32x16{};
 #pragma unroll
     for (int s = 0; s < 8; ++s) {
-      uint4 fk[2];
+      uint4 fk[PH];
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        fk[h] = *reinterpret_cast<const uint4*>(kt + 32 * h * PKS + 32 * s);
+      for (int h = 0; h < PH; ++h) fk[h] = *reinterpret_cast<const uint4*>(kt + 32 * h * PKS + 32 * s);
 #pragma unroll
       for (int p = 0; p < PARTS; ++p)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) st[h] = mfma32(fk[h], fq[p][s], st[h]);
+        for (int h = 0; h < PH; ++h) st[h] = mfma32(fk[h], fq[p][s], st[h]);
     }
-    if constexpr (masked) {
+  };
+  // its mask, if some query of the wave sees it in part
+  auto mask = [&](Scores& st, int i) __attribute__((always_inline)) {
+    const int key = tile(i) * PK;
+    if (key + PK - 1 > wfirst) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int h = 0; h < PH; ++h)
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-          if (k0 + 32 * h + 8 * (j >> 2) + 4 * g + (j & 3) > tok) st[h][j] = -INFINITY;
+          if (key + 32 * h + 8 * (j >> 2) + 4 * g + (j & 3) > tok) st[h][j] = -INFINITY;
     }
-    float m = mrun;
+  };
+  // the running maximum with it
+  float mnew = -INFINITY;
+  auto maximum = [&](const Scores& st) __attribute__((always_inline)) {
+    mnew = mrun;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < PH; ++h)
 #pragma unroll
-      for (int j = 0; j < 16; ++j) m = fmaxf(m, st[h][j]);
-    m = xmax32(m);
-    const float mc = m == -INFINITY ? 0.f : m * C;  // a query that has seen no key of weight so far
+      for (int j = 0; j < 16; ++j) mnew = fmaxf(mnew, st[h][j]);
+    mnew = xmax32(mnew);
+  };
+  // the output and the sum to that maximum
+  auto rescale = [&]() __attribute__((always_inline)) {
+    const float mc = mnew == -INFINITY ? 0.f : mnew * C;  // a query that has seen no key of weight so far
     const float alpha = __builtin_amdgcn_exp2f(mscaled - mc);  // exactly 1 when the maximum holds
-    mrun = m;
+    mrun = mnew;
     mscaled = mc;
-    float sum = 0.f;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        st[h][j] = __builtin_amdgcn_exp2f(fmaf(st[h][j], C, -mc));
-        sum += st[h][j];
-      }
-    lrun = fmaf(lrun, alpha, sum);
+    lrun *= alpha;
     if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0) {
 #pragma unroll
       for (int b = 0; b < 4; ++b) acc[b] *= alpha;
     }
-    auto weigh = [&](auto BAD) __attribute__((always_inline)) {
+  };
+  // half a tile's weights, in place of its scores, and their sum (of the rounded ones, where they are)
+  auto weights = [&](f32x16& st) __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        float pw[8];
+    for (int j = 0; j < 16; ++j) st[j] = __builtin_amdgcn_exp2f(fmaf(st[j], C, -mscaled));
+    float sum = 0.f;
+    if constexpr (PARTS == 1) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) pw[j] = st[u >> 1][8 * (u & 1) + j];
-        uint4 fp[PARTS];
-        split_parts<PARTS>(pw, fp);
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          uint2 h[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            h[e] = __builtin_bit_cast(
-                uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
-                           vt + (16 * u + 8 * e) * PVS + 64 * b)));
-          }
-          uint4 fv = make_uint4(h[0].x, h[0].y, h[1].x, h[1].y);
-          if constexpr (decltype(BAD)::value)
-            fv = make_uint4(finite_or_0(fv.x), finite_or_0(fv.y), finite_or_0(fv.z), finite_or_0(fv.w));
-#pragma unroll
-          for (int p = 0; p < PARTS; ++p) acc[b] = mfma32(fv, fp[p], acc[b]);
-        }
+      for (int j = 0; j < 16; j += 2) {
+        const bf16x2_t p = {(__bf16)st[j], (__bf16)st[j + 1]}, one = {(__bf16)1.f, (__bf16)1.f};
+        sum = __builtin_amdgcn_fdot2_f32_bf16(p, one, sum, false);
       }
-    };
-    if (!masked || !(sm.bad[0] | sm.bad[1] | sm.bad[2] | sm.bad[3])) {  // the same for every lane
-      weigh(std::false_type{});
     } else {
-      weigh(std::true_type{});
-      for (int key = 0; key < PK; ++key) {
-        if (k0 + key > tok) break;
 #pragma unroll
-        for (int b = 0; b < 4; ++b)
+      for (int j = 0; j < 16; ++j) sum += st[j];
+    }
+    lrun += sum;
+  };
+  // O^T += V^T . P^T over keys 32 h .. 32 h + 31 of the tile
+  auto output = [&](const f32x16& st, int i, int h) __attribute__((always_inline)) {
+    // this lane's places: V row 4 g + l % 16 / 4 at dims 16 (l / 16 % 2) + 4 (l % 4)
+    const unsigned char* vt = tiles.v[i & 1] + (4 * g + ((lane & 15) >> 2)) * PVS + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint2 x = *reinterpret_cast<const uint2*>(sm.v[buf] + key * PVS + 64 * b + 16 * q + 8 * g);
-            const float f[4] = {bf16_lo(x.x), bf16_hi(x.x), bf16_lo(x.y), bf16_hi(x.y)};
+    for (int u = 0; u < 2; ++u) {
+      float pw[8];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              if (!(fabsf(f[j]) < INFINITY)) acc[b][4 * q + j] += f[j];
-          }
+      for (int j = 0; j < 8; ++j) pw[j] = st[8 * u + j];
+      uint4 fp[PARTS];
+      split_parts<PARTS>(pw, fp);
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        uint2 x[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          x[e] = __builtin_bit_cast(
+              uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(
+                         vt + (32 * h + 16 * u + 8 * e) * PVS + 64 * b)));
+        const uint4 fv = make_uint4(x[0].x, x[0].y, x[1].x, x[1].y);
+#pragma unroll
+        for (int p = 0; p < PARTS; ++p) acc[b] = mfma32(fv, fp[p], acc[b]);
       }
     }
   };
 
-  store(x, 0);
+  // Tile i's weights are taken while the matrix cores make tile i + 1's scores. A place in LDS is written in
+  // the step after the one that read it last (tile i + 1's V takes tile i - 1's, tile i + 2's K tile i's), so
+  // one barrier a step is enough.
+  Scores st, sn;
   __syncthreads();
-  // the tiles that every query of the block sees whole, then the others
-  const int nfull = min((first + 1) / PK, ntile - 1);
-  for (int t = 0; t < nfull; ++t) {
-    load(x, t + 1);
-    consume(t, std::false_type{});
-    store(x, t + 1);
-    __syncthreads();  // tile t consumed by every wave, tile t + 1 staged
+  if (tile(0) * PK <= wlast) {
+    scores(st, 0);
+    mask(st, 0);
+    maximum(st);
   }
-  for (int t = nfull; t < ntile; ++t) {
-    if (t + 1 < ntile) load(x, t + 1);
-    if (t * PK <= wlast) consume(t, std::true_type{});
-    if (t + 1 < ntile) store(x, t + 1);
+  __syncthreads();  // tile 0's scores made by every wave: tile 2's K takes its place in the first step
+  int i = 0;
+  // tiles whose next one the whole block sees, two before the last: no masks, no ends
+  auto step = [&](Scores& st, Scores& sn, int i) __attribute__((always_inline)) {
+    store_v(x, i + 1, true);
+    load(x, kbase, a.k_row, i + 2, true);
+    rescale();
+    scores(sn, i + 1);
+#pragma unroll
+    for (int h = 0; h < PH; ++h) weights(st[h]);
+#pragma unroll
+    for (int h = 0; h < PH; ++h) output(st[h], i, h);
+    maximum(sn);
+    store_k(x, i + 2);
+    load(x, vbase, a.v_row, i + 2, true);
+    __syncthreads();
+  };
+  for (const int nfast = min((first + 1) / (PK * KS) - 1, (last + 1) / (PK * KS) - 2); i + 1 < nfast; i += 2) {
+    step(st, sn, i);
+    step(sn, st, i + 1);
+  }
+  for (; i < niter; ++i) {
+    const bool next = tile(i + 1) < ntile, after = tile(i + 2) < ntile, seen = tile(i) * PK <= wlast;
+    if (next) store_v(x, i + 1);
+    if (after) load(x, kbase, a.k_row, i + 2);
+    if (seen) {
+      rescale();
+      if (next) scores(sn, i + 1);
+#pragma unroll
+      for (int h = 0; h < PH; ++h) weights(st[h]);
+    }
+    if (after) {
+      store_k(x, i + 2);
+      load(x, vbase, a.v_row, i + 2);
+    }
+    if (seen) {
+#pragma unroll
+      for (int h = 0; h < PH; ++h) output(st[h], i, h);
+    }
+    if (seen && next) {
+      mask(sn, i + 1);
+      maximum(sn);
+#pragma unroll
+      for (int h = 0; h < PH; ++h) st[h] = sn[h];
+    }
     __syncthreads();
   }
+  if constexpr (KS > 1) {  // the second group's sums to the first's
+    if (ks == 1) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) sm.join.acc[w][16 * b + j][lane] = acc[b][j];
+      sm.join.m[w][lane] = mrun;
+      sm.join.l[w][lane] = lrun;
+    }
+    __syncthreads();
+    if (ks == 1) return;
+    const float mo = sm.join.m[w][lane];
+    mnew = fmaxf(mrun, mo);
+    rescale();
+    const float f = mo == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mo * C - mscaled);  // no tile: nothing, whatever its place holds
+    lrun = fmaf(f, sm.join.l[w][lane], lrun);
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) acc[b][j] = fmaf(f, sm.join.acc[w][16 * b + j][lane], acc[b][j]);
+  }
   if (r0 >= rows) return;
+  int bad = 0;
+#pragma unroll
+  for (int n = 0; n < KS * PW; ++n) bad |= sm.bad[n];
+  if (bad) {
+    // what was left out of the tiles seen in part, to the queries that see it
+    for (int key = (max(first - PK + 2, 0) + PK - 1) / PK * PK; key <= tok; ++key) {
+      const uint16_t* vr = reinterpret_cast<const uint16_t*>(vbase + key * (2 * a.v_row)) + 4 * g;
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float f = bf16_to_f32(vr[32 * b + 8 * q + j]);
+            if (!(fabsf(f) < INFINITY)) acc[b][4 * q + j] += f;
+          }
+    }
+  }
 
   // the output's columns are queries: 8 dims of one query per lane after a swap between the wave's halves
   const float inv = 1.f / xsum32(lrun);
+  const int64_t m = row0 + tok;
 #pragma unroll
   for (int b = 0; b < 4; ++b)
 #pragma unroll
@@ -326,7 +471,6 @@ __global__ void __launch_bounds__(64 * PW, 2) packed_attention_kernel(const Pack
       }
       if (r >= rows) continue;
       const int d = 32 * b + 8 * (q + g);
-      const int64_t m = row0 + tok;
       if constexpr (PARTS == 1) {
         *reinterpret_cast<uint4*>((uint16_t*)a.out + (m * (a.hkv * a.g) + hq) * D + d) =
             make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]),
@@ -334,7 +478,7 @@ __global__ void __launch_bounds__(64 * PW, 2) packed_attention_kernel(const Pack
       } else if constexpr (PARTS == 2) {  // attn_out's two fragment orders (layers_kernel.hip)
         uint4 p[PARTS];
         split_parts<PARTS>(o, p);
-        const int64_t kk = hq * D + d;
+        const int kk = hq * D + d;
         uint16_t* out = (uint16_t*)a.out;
         *reinterpret_cast<uint4*>(out + (a.frag == 2 ? skf_off(m, kk, 0, HQ * D) : frag_off(m, kk, HQ * D))) = p[0];
         *reinterpret_cast<uint4*>(a.frag == 2 ? out + skf_off(m, kk, 1, HQ * D)
@@ -351,27 +495,37 @@ __global__ void __launch_bounds__(64 * PW, 2) packed_attention_kernel(const Pack
 
 using namespace mkp;
 
-// The launches of a call: the sequences longest first (a block costs its keys, so the long chains start
-// first and short ones fill the CUs that finish), at most PSEQ of them to a launch.
-template <int PARTS>
+// The launches of a call: the sequences longest first, at most PSEQ of them to a launch (a block costs its
+// keys, so the long chains start first and short ones fill the CUs that finish).
+template <int PARTS, int PK>
 static hipError_t launch_packed(PackedArgs& a, const int32_t* lengths, int num_seqs, hipStream_t stream) {
+  a.by_hkv = div_by(a.hkv);
+  a.by_g = div_by(a.g);
   try {
     std::vector<int32_t> order(num_seqs), row(num_seqs);
     std::iota(order.begin(), order.end(), 0);
     for (int i = 0, at = 0; i < num_seqs; at += lengths[i++]) row[i] = at;
     std::stable_sort(order.begin(), order.end(), [&](int32_t x, int32_t y) { return lengths[x] > lengths[y]; });
     for (int s = 0; s < num_seqs && lengths[order[s]] > 0;) {
-      int blocks = 0, n = 0;
+      int n = 0;
+      int64_t blocks = 0;
       for (; n < PSEQ && s < num_seqs && lengths[order[s]] > 0; ++n, ++s) {
         const int i = order[s];
-        a.first[n] = blocks;
         a.row[n] = row[i];
         a.len[n] = lengths[i];
         a.seq[n] = i;
-        blocks += (int)(((int64_t)lengths[i] * a.g + PR - 1) / PR);
+      }
+      auto count = [&](int i) { return i < n ? ((int64_t)a.len[i] * a.g + PR - 1) / PR : 0; };
+      for (int i = 0; i < n; ++i) {
+        a.first[i] = (int32_t)blocks;
+        blocks += (count(i) - count(i + 1)) * (i + 1);
       }
       a.nseq = n;
-      hipLaunchKernelGGL((packed_attention_kernel<PARTS>), dim3((unsigned)blocks * a.hkv), dim3(64 * PW), 0, stream, a);
+      const dim3 grid((unsigned)(blocks * a.hkv));
+      if (grid.x <= 512)
+        hipLaunchKernelGGL((packed_attention_kernel<PARTS, PK, 2>), grid, dim3(2 * 64 * PW), 0, stream, a);
+      else
+        hipLaunchKernelGGL((packed_attention_kernel<PARTS, PK, 1>), grid, dim3(64 * PW), 0, stream, a);
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
     }
@@ -398,7 +552,7 @@ hipError_t mkp_attention_prefill(const MkPackedPrefill& p, hipStream_t stream) {
   a.hkv = HKV;
   a.g = HQ / HKV;
   a.frag = p.frag;
-  return launch_packed<2>(a, p.lengths, p.num_seqs, stream);
+  return launch_packed<2, 32>(a, p.lengths, p.num_seqs, stream);
 }
 
 extern "C" hipError_t mk_attention_packed(int q_heads, int kv_heads, const void* q, int64_t q_row_stride,
@@ -414,7 +568,7 @@ extern "C" hipError_t mk_attention_packed(int q_heads, int kv_heads, const void*
     total += lengths[i];
   }
   // rows of a K/V head and workgroups are counted in 32 bits
-  if (total * q_heads > INT32_MAX - 2 * PR + 1) return hipErrorInvalidValue;
+  if (total * q_heads > INT32_MAX - 255) return hipErrorInvalidValue;
   if (total == 0) return hipSuccess;
   if (!q || !k || !v || !out) return hipErrorInvalidValue;
   for (const void* p : {q, k, v, (const void*)out})
@@ -438,5 +592,5 @@ extern "C" hipError_t mk_attention_packed(int q_heads, int kv_heads, const void*
   a.v_head = v_head_stride;
   a.hkv = kv_heads;
   a.g = q_heads / kv_heads;
-  return q_fp32 ? launch_packed<3>(a, lengths, num_seqs, stream) : launch_packed<1>(a, lengths, num_seqs, stream);
+  return q_fp32 ? launch_packed<3, 32>(a, lengths, num_seqs, stream) : launch_packed<1, 64>(a, lengths, num_seqs, stream);
 }
