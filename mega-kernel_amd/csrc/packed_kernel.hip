@@ -23,7 +23,8 @@
 //
 // A masked key weighs nothing, whatever its value row holds: a tile that some query sees in part is looked
 // over for infinities and NaN, and where it has any they are added outside the matrix product to the
-// queries that see them (0 times infinity would reach the others).
+// queries that see them (0 times infinity would reach the others). Where weights are multiplied by parts,
+// every tile is (a part may be 0 or negative where the weight is not).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -45,8 +46,6 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
 
-constexpr int PW = 4;          // waves per workgroup
-constexpr int PR = 32 * PW;    // rows per workgroup
 constexpr int PSEQ = 128;      // sequences per launch (their places travel as kernel arguments)
 
 // Division by a number that the host knows: q = n / d for 0 <= n < 2^31 by a multiplication (the rounded-up
@@ -116,7 +115,7 @@ __device__ __forceinline__ uint32_t finite_or_0(uint32_t w) {
 // transposed read takes 64 bytes of each of 4 rows).
 constexpr int PKS = 2 * D + 16, PVS = 2 * D + 64;
 
-template <int PK, int KS>
+template <int PK, int RG, int KS>
 struct PackedSmem {
   struct Tiles {
     unsigned char k[2][PK * PKS];
@@ -124,19 +123,21 @@ struct PackedSmem {
   };
   union {
     Tiles tiles[KS];
-    struct {  // the second wave group's output columns, maximum and sum, lane by lane
-      float acc[KS > 1 ? PW : 1][64][64], m[PW][64], l[PW][64];
+    struct {  // the output blocks that a key group leaves to another, the maxima and sums, lane by lane
+      float acc[KS > 1 ? KS : 1][KS > 1 ? RG : 1][KS > 1 ? 64 - 64 / KS : 1][64], m[KS][RG][64], l[KS][RG][64];
     } join;
   };
-  int bad[KS * PW];  // per staging wave: an infinity or NaN in a value row of a tile seen in part
+  int bad[KS * RG];  // per staging wave: an infinity or NaN taken out of a tile's values
 };
 
-template <int PARTS, int PK, int KS>
-__global__ void __launch_bounds__(64 * PW * KS, 2) packed_attention_kernel(const PackedArgs a) {
-  constexpr int PH = PK / 32, NX = PK / (4 * PW);  // 32-key halves of a tile, chunks of K that a lane stages
-  __shared__ __attribute__((aligned(16))) PackedSmem<PK, KS> sm;
+// PK: keys per tile; RG: waves on different rows, 32 each; KS: groups of RG waves on different tiles
+template <int PARTS, int PK, int RG, int KS>
+__global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attention_kernel(const PackedArgs a) {
+  constexpr int PR = 32 * RG;                      // rows per workgroup
+  constexpr int PH = PK / 32, NX = PK / (4 * RG);  // 32-key halves of a tile, chunks of K that a lane stages
+  __shared__ __attribute__((aligned(16))) PackedSmem<PK, RG, KS> sm;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int w = wave % PW, ks = wave / PW;   // a group of PW waves takes every KS-th tile: tile ks, KS + ks, ...
+  const int w = wave % RG, ks = wave / RG;   // key group ks takes tiles ks, KS + ks, ...
   const int col = lane & 31, g = lane >> 5;  // this lane's query and half of the K slots
   auto& tiles = sm.tiles[ks];
   // workgroup b: K/V head b % hkv (with 8 heads, a head's keys stay in one XCD's L2), query block b / hkv of
@@ -177,10 +178,10 @@ __global__ void __launch_bounds__(64 * PW * KS, 2) packed_attention_kernel(const
   const char* kbase = (const char*)(a.k + (PARTS == 2 ? pick(ts, si) * a.kv_seq : row0 * a.k_row) + kh * a.k_head);
   const char* vbase = (const char*)(a.v + (PARTS == 2 ? pick(ts, si) * a.kv_seq : row0 * a.v_row) + kh * a.v_head);
 
-  // a group's wave w stages rows PK / 4 w .. of its tile, four to an instruction (lane l: chunk l % 16 of row
+  // a key group's wave w stages rows PK / RG w .. of its tile, four to an instruction (lane l: chunk l % 16 of row
   // l / 16), through registers, where a later tile waits while this one is multiplied. Keys past the
   // block's last one are that one again (masked).
-  const int srow = PK / PW * w + (lane >> 4), chunk = lane & 15;
+  const int srow = PK / RG * w + (lane >> 4), chunk = lane & 15;
   struct Tile {
     uint4 x[NX];
   };
@@ -205,7 +206,8 @@ __global__ void __launch_bounds__(64 * PW * KS, 2) packed_attention_kernel(const
     for (int n = 0; n < NX; ++n) *reinterpret_cast<uint4*>(p + 4 * n * PKS) = d.x[n];
   };
   auto store_v = [&](Tile& d, int i, bool whole = false) __attribute__((always_inline)) {
-    if (!whole && tile(i) * PK + PK - 1 > first) {  // a tile that some query of the block sees in part: finite rows only
+    // a tile that some query of the block sees in part, or that is multiplied by parts: finite values only
+    if (PARTS > 1 || (!whole && tile(i) * PK + PK - 1 > first)) {
       uint32_t bad = 0;
 #pragma unroll
       for (int n = 0; n < NX; ++n)
@@ -413,43 +415,68 @@ __global__ void __launch_bounds__(64 * PW * KS, 2) packed_attention_kernel(const
     }
     __syncthreads();
   }
-  if constexpr (KS > 1) {  // the second group's sums to the first's
-    if (ks == 1) {
+  // Each key group finishes 4 / KS of the four output blocks: it leaves its sums of the others in LDS, and
+  // takes the other groups' of its own.
+  constexpr int NB = 4 / KS;
+  const int b0 = NB * ks;
+  f32x16 out[NB];
+  if constexpr (KS > 1) {
+    int n = 0;
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
+    for (int b = 0; b < 4; ++b) {
+      if (b / NB == ks) continue;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) sm.join.acc[w][16 * b + j][lane] = acc[b][j];
-      sm.join.m[w][lane] = mrun;
-      sm.join.l[w][lane] = lrun;
+      for (int j = 0; j < 16; ++j) sm.join.acc[ks][w][n + j][lane] = acc[b][j];
+      n += 16;
     }
+    const float me = mrun == -INFINITY ? -INFINITY : mscaled;  // the exponents' scale that the sums refer to
+    sm.join.m[ks][w][lane] = me;
+    sm.join.l[ks][w][lane] = lrun;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int o = 0; o < KS; ++o)
+        if (o == ks) out[b] = acc[NB * o + b];
     __syncthreads();
-    if (ks == 1) return;
-    const float mo = sm.join.m[w][lane];
-    mnew = fmaxf(mrun, mo);
-    rescale();
-    const float f = mo == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mo * C - mscaled);  // no tile: nothing, whatever its place holds
-    lrun = fmaf(f, sm.join.l[w][lane], lrun);
+    float mc = me;
 #pragma unroll
-    for (int b = 0; b < 4; ++b)
+    for (int o = 0; o < KS; ++o) mc = fmaxf(mc, sm.join.m[o][w][lane]);
+    if (mc == -INFINITY) mc = 0.f;
+    const float own = __builtin_amdgcn_exp2f(me - mc);  // 0 for a group that saw no key
+    lrun *= own;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) acc[b][j] = fmaf(f, sm.join.acc[w][16 * b + j][lane], acc[b][j]);
+    for (int b = 0; b < NB; ++b) out[b] *= own;
+#pragma unroll
+    for (int o = 0; o < KS; ++o) {
+      if (o == ks) continue;
+      const float f = __builtin_amdgcn_exp2f(sm.join.m[o][w][lane] - mc);
+      lrun = fmaf(f, sm.join.l[o][w][lane], lrun);
+      const int n = 16 * (b0 - (ks > o ? NB : 0));  // this group's first block among those that group o left
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) out[b][j] = fmaf(f, sm.join.acc[o][w][n + 16 * b + j][lane], out[b][j]);
+    }
+  } else {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) out[b] = acc[b];
   }
   if (r0 >= rows) return;
   int bad = 0;
 #pragma unroll
-  for (int n = 0; n < KS * PW; ++n) bad |= sm.bad[n];
+  for (int n = 0; n < KS * RG; ++n) bad |= sm.bad[n];
   if (bad) {
-    // what was left out of the tiles seen in part, to the queries that see it
-    for (int key = (max(first - PK + 2, 0) + PK - 1) / PK * PK; key <= tok; ++key) {
-      const uint16_t* vr = reinterpret_cast<const uint16_t*>(vbase + key * (2 * a.v_row)) + 4 * g;
+    // what was left out of the tiles, to the queries that see it
+    for (int key = PARTS > 1 ? 0 : (max(first - PK + 2, 0) + PK - 1) / PK * PK; key <= tok; ++key) {
+      const uint16_t* vr = reinterpret_cast<const uint16_t*>(vbase + key * (2 * a.v_row)) + 32 * b0 + 4 * g;
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float f = bf16_to_f32(vr[32 * b + 8 * q + j]);
-            if (!(fabsf(f) < INFINITY)) acc[b][4 * q + j] += f;
+            if (!(fabsf(f) < INFINITY)) out[b][4 * q + j] += f;
           }
     }
   }
@@ -458,19 +485,19 @@ __global__ void __launch_bounds__(64 * PW * KS, 2) packed_attention_kernel(const
   const float inv = 1.f / xsum32(lrun);
   const int64_t m = row0 + tok;
 #pragma unroll
-  for (int b = 0; b < 4; ++b)
+  for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int q = 0; q < 4; q += 2) {
       float o[8];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[b][4 * q + j] * inv),
-                                                        __float_as_uint(acc[b][4 * q + 4 + j] * inv), false, false);
+        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(out[b][4 * q + j] * inv),
+                                                        __float_as_uint(out[b][4 * q + 4 + j] * inv), false, false);
         o[j] = __uint_as_float(x[0]);
         o[4 + j] = __uint_as_float(x[1]);
       }
       if (r >= rows) continue;
-      const int d = 32 * b + 8 * (q + g);
+      const int d = 32 * (b0 + b) + 8 * (q + g);
       if constexpr (PARTS == 1) {
         *reinterpret_cast<uint4*>((uint16_t*)a.out + (m * (a.hkv * a.g) + hq) * D + d) =
             make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]),
@@ -479,9 +506,9 @@ __global__ void __launch_bounds__(64 * PW * KS, 2) packed_attention_kernel(const
         uint4 p[PARTS];
         split_parts<PARTS>(o, p);
         const int kk = hq * D + d;
-        uint16_t* out = (uint16_t*)a.out;
-        *reinterpret_cast<uint4*>(out + (a.frag == 2 ? skf_off(m, kk, 0, HQ * D) : frag_off(m, kk, HQ * D))) = p[0];
-        *reinterpret_cast<uint4*>(a.frag == 2 ? out + skf_off(m, kk, 1, HQ * D)
+        uint16_t* hi = (uint16_t*)a.out;
+        *reinterpret_cast<uint4*>(hi + (a.frag == 2 ? skf_off(m, kk, 0, HQ * D) : frag_off(m, kk, HQ * D))) = p[0];
+        *reinterpret_cast<uint4*>(a.frag == 2 ? hi + skf_off(m, kk, 1, HQ * D)
                                               : a.out_lo + frag_off(m, kk, HQ * D)) = p[1];
       } else {
         float4* p = reinterpret_cast<float4*>((float*)a.out + (m * (a.hkv * a.g) + hq) * D + d);
@@ -508,24 +535,39 @@ static hipError_t launch_packed(PackedArgs& a, const int32_t* lengths, int num_s
     std::stable_sort(order.begin(), order.end(), [&](int32_t x, int32_t y) { return lengths[x] > lengths[y]; });
     for (int s = 0; s < num_seqs && lengths[order[s]] > 0;) {
       int n = 0;
-      int64_t blocks = 0;
       for (; n < PSEQ && s < num_seqs && lengths[order[s]] > 0; ++n, ++s) {
         const int i = order[s];
         a.row[n] = row[i];
         a.len[n] = lengths[i];
         a.seq[n] = i;
       }
-      auto count = [&](int i) { return i < n ? ((int64_t)a.len[i] * a.g + PR - 1) / PR : 0; };
-      for (int i = 0; i < n; ++i) {
-        a.first[i] = (int32_t)blocks;
-        blocks += (count(i) - count(i + 1)) * (i + 1);
-      }
       a.nseq = n;
-      const dim3 grid((unsigned)(blocks * a.hkv));
-      if (grid.x <= 512)
-        hipLaunchKernelGGL((packed_attention_kernel<PARTS, PK, 2>), grid, dim3(2 * 64 * PW), 0, stream, a);
-      else
-        hipLaunchKernelGGL((packed_attention_kernel<PARTS, PK, 1>), grid, dim3(64 * PW), 0, stream, a);
+      // the workgroups of blocks of pr rows, and each sequence's place among them
+      auto places = [&](int pr) {
+        auto count = [&](int i) { return i < n ? ((int64_t)a.len[i] * a.g + pr - 1) / pr : 0; };
+        int64_t blocks = 0;
+        for (int i = 0; i < n; ++i) {
+          a.first[i] = (int32_t)blocks;
+          blocks += (count(i) - count(i + 1)) * (i + 1);
+        }
+        return dim3((unsigned)(blocks * a.hkv));
+      };
+      // Few rows: 32 to a workgroup and its four waves on different keys, so that the work spreads over the
+      // CUs; up to two workgroups of 128 rows per CU: two key groups of four waves, one workgroup to a CU (the
+      // longest chain decides, and its keys are shared out); else 128 rows and one key group, two workgroups
+      // to a CU. Measured on MI355X (16 query heads on 8), us with 128 rows / 32 rows: bf16 128 tokens
+      // 9.2 / 8.0, 512 (256 workgroups of 32 rows) 15.5 / 14.2, 1,024 (512) 23.5 / 27.2; fp32 128 15.2 / 9.8,
+      // 512 28.5 / 17.9, 1,024 46.1 / 34.9, 2,048 over that. With one / two key groups: 3,584 tokens (448
+      // workgroups of 128 rows) bf16 82.2 / 70.0, fp32 182 / 148, 2,048 bf16 43.2 / 40.2; 200 prompts of 48
+      // (1,600) 36.5 / 56.7.
+      dim3 grid = places(32);
+      if (grid.x <= (PARTS == 1 ? 256 : 512)) {
+        hipLaunchKernelGGL((packed_attention_kernel<PARTS, 32, 1, 4>), grid, dim3(256), 0, stream, a);
+      } else if ((grid = places(128)).x <= 512) {
+        hipLaunchKernelGGL((packed_attention_kernel<PARTS, PK, 4, 2>), grid, dim3(512), 0, stream, a);
+      } else {
+        hipLaunchKernelGGL((packed_attention_kernel<PARTS, PK, 4, 1>), grid, dim3(256), 0, stream, a);
+      }
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
     }

@@ -70,3 +70,137 @@ def test_head_layouts(kernel, heads, dtype):
     """Query heads per K/V head that divide a tile's rows, that do not, and more than it has rows."""
     lengths = [67, 1, 130]
     check(kernel, *inputs(sum(lengths), *heads, dtype, seed=heads[0]), lengths)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("lengths", [[2048], [3000, 17], [900] * 5, [1 + 13 * i for i in range(60)],
+                                     [3 + i % 61 for i in range(150)], [40] * 300], ids=lambda v: f"{len(v)}x{v[0]}")
+def test_every_split_of_the_work(kernel, lengths, dtype):
+    """32 rows to a workgroup (the lengths above), two key groups (up to 512 workgroups of 128 rows), one, and
+    more sequences than one launch takes."""
+    check(kernel, *inputs(sum(lengths), 16, 8, dtype, seed=7), lengths)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_random_lengths_again_and_again(kernel, dtype):
+    """Waves of a workgroup run apart by different amounts; a place in LDS that is written too early shows as a
+    wrong row in some of these."""
+    gen = torch.Generator().manual_seed(11)
+    for _ in range(30):
+        lengths = torch.randint(1, 420, (int(torch.randint(1, 6, (1,), generator=gen)),), generator=gen).tolist()
+        check(kernel, *inputs(sum(lengths), 16, 8, dtype, seed=sum(lengths)), lengths)
+
+
+def test_strided_operands(kernel):
+    """q, k and v as slices of one projection's rows, in another order, and keys shared by expansion."""
+    lengths = [70, 200, 1]
+    n = sum(lengths)
+    rows = torch.randn(n, 40, D, device=DEV).to(torch.bfloat16)
+    check(kernel, rows[:, 24:], rows[:, 8:16], rows[:, :8], lengths)
+    heads_first = torch.randn(16, n, D, device=DEV).to(torch.bfloat16).transpose(0, 1)
+    check(kernel, heads_first, rows[:, 8:16], rows[:, :8], lengths)
+    check(kernel, heads_first.float()[:, ::2], rows[:, 8:12], rows[:, ::10], lengths)
+    one = torch.randn(n, 1, D, device=DEV).to(torch.bfloat16).expand(n, 8, D)
+    check(kernel, heads_first, one, rows[:, :8], lengths)
+
+
+def test_key_rows_far_apart(kernel):
+    """Rows 2^18 elements apart: offsets inside the operands pass 2^31 bytes."""
+    n = 4500
+    big = torch.zeros(n * (1 << 18) + 2 * D, dtype=torch.bfloat16, device=DEV)
+    k, v = (big.as_strided((n, 1, D), (1 << 18, D, 1), o) for o in (0, D))
+    q, kk, vv = inputs(n, 2, 1, torch.bfloat16, seed=3)
+    k.copy_(kk)
+    v.copy_(vv)
+    check(kernel, q, k, v, [n - 100, 100])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_one_sharp_key_and_large_scores(kernel, dtype):
+    """Scores in the hundreds: the running maximum grows tile by tile, and all weight ends on one key."""
+    lengths = [300, 90]
+    q, k, v = inputs(390, 4, 2, dtype, seed=5)
+    k *= torch.linspace(0.1, 6, 390, device=DEV).to(torch.bfloat16)[:, None, None]
+    check(kernel, q * 4, k, v, lengths)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("lengths", [[200], [40, 130, 64], [700, 500]], ids=str)
+def test_values_that_a_token_may_not_see_do_not_reach_it(kernel, lengths, dtype):
+    """Infinities and NaN in some value rows: tokens before them, and other sequences, are as without them;
+    tokens from them on get the infinity or NaN that the formula gives, in those dimensions alone."""
+    n = sum(lengths)
+    q, k, v = inputs(n, 6, 2, dtype, seed=9)
+    want = check(kernel, q, k, v, lengths)
+    bad = v.clone()
+    starts = [sum(lengths[:i]) for i in range(len(lengths))]
+    marks = []  # (sequence, its first marked token, K/V head, dim, value)
+    for s, (at, length) in enumerate(zip(starts, lengths)):
+        for j, (t, value) in enumerate(((length // 3, math.inf), (length - 1, math.nan), (length // 2, -math.inf))):
+            head, dim = j % 2, 5 + 40 * j + s
+            bad[at + t, head, dim] = value
+            marks.append((s, t, head, dim, value))
+    got = kernel.attention_packed(q, k, bad, lengths)
+    expect = want.clone()
+    for s, t, head, dim, value in marks:
+        r = slice(starts[s] + t, starts[s] + lengths[s])
+        expect[r, 3 * head:3 * head + 3, dim] = value
+    fine = torch.isfinite(expect)
+    assert torch.equal(got[fine], want[fine])
+    assert torch.equal(torch.isnan(got), torch.isnan(expect))
+    assert torch.equal(got[~fine & ~torch.isnan(expect)], expect[~fine & ~torch.isnan(expect)])
+
+
+def test_a_nan_key_or_query_stays_with_the_rows_that_see_it(kernel):
+    lengths = [100, 150]
+    q, k, v = inputs(250, 2, 1, torch.bfloat16, seed=10)
+    want = kernel.attention_packed(q, k, v, lengths)
+    k[170] = math.nan
+    q[20, 1] = math.nan
+    got = kernel.attention_packed(q, k, v, lengths)
+    nan = torch.zeros_like(got, dtype=torch.bool)
+    nan[170:] = True
+    nan[20, 1] = True
+    assert torch.equal(torch.isnan(got), nan) and torch.equal(got[~nan], want[~nan])
+
+
+def test_a_sequence_does_not_depend_on_its_batch(kernel):
+    """Rows of a sequence alone, at another place and among others, in launches of the same kind: bit for bit."""
+    lengths = [130, 77, 64]
+    q, k, v = inputs(sum(lengths), 16, 8, torch.bfloat16, seed=12)
+    whole = kernel.attention_packed(q, k, v, lengths)
+    at = 0
+    for n in lengths:
+        r = slice(at, at + n)
+        assert torch.equal(kernel.attention_packed(q[r], k[r], v[r], [n]), whole[r])
+        at += n
+
+
+def test_empty_call(kernel):
+    q, k, v = inputs(0, 16, 8, torch.bfloat16)
+    assert kernel.attention_packed(q, k, v, []).shape == (0, 16, 128)
+    assert kernel.attention_packed(q, k, v, [0, 0]).shape == (0, 16, 128)
+
+
+def test_on_another_stream_and_in_a_graph(kernel):
+    lengths = [300, 20, 129]
+    q, k, v = inputs(sum(lengths), 16, 8, torch.bfloat16, seed=13)
+    want = kernel.attention_packed(q, k, v, lengths)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = kernel.attention_packed(q, k, v, lengths)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = kernel.attention_packed(q, k, v, lengths)
+    for seed in (14, 15, 16):
+        for old, new in zip((q, k, v), inputs(sum(lengths), 16, 8, torch.bfloat16, seed=seed)):
+            old.copy_(new)
+        held.zero_()
+        eager = kernel.attention_packed(q, k, v, lengths)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, eager)
