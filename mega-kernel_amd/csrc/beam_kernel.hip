@@ -5,8 +5,8 @@
 //   score[r] + logit[r][v] - log(sum over u of exp(logit[r][u])),
 // a finished row the one candidate (eos, score[r]), and the group's `beams` best go on. Within a row the
 // order of the candidates is that of the logits, so it needs no arithmetic:
-//   beam_chunk_kernel  a wave takes 2,048 logits of a row, all in registers: their maximum, the sum of
-//                      exp(logit - maximum), and their `beams` best (logit, token) as 64-bit keys, best first;
+//   beam_chunk_kernel  a workgroup takes 8,192 logits of a row, a wave 2,048, all in registers: their maximum,
+//                      the sum of exp(logit - maximum), and their `beams` best (logit, token) as 64-bit keys;
 //   beam_pick_kernel   a workgroup per group: a wave joins a row's sums (64 bits) and keys, then the group's
 //                      beams^2 row bests are ranked by their scores in 64 bits, which tell apart any two
 //                      candidates of one row and, between rows, what the fp32 sums resolve.
@@ -27,20 +27,24 @@
 namespace mkp {
 
 constexpr int BEAMS_MAX = 16;
-constexpr int BC = 2048;                 // logits per wave
+constexpr int BL = 2048;                 // logits per wave of the first kernel
+constexpr int BC = 4 * BL;               // and per workgroup: a chunk
 constexpr int BV_MAX = 1 << 20;          // vocabulary: BV_MAX / BC heads per row in LDS
 constexpr int PICK_WAVES = 8;
 
 // Key of (logit, token): larger for the larger logit, then the lower token; 0 is no candidate (a NaN's
 // key is never used: its row's sum is NaN too).
-__device__ __forceinline__ u64 beam_key(float x, int v) {
+__device__ __forceinline__ uint32_t order_bits(float x) {  // unsigned order is the numbers'
   const uint32_t u = __float_as_uint(x + 0.f);  // -0 as 0
-  return ((u64)((u & 0x80000000u) ? ~u : (u | 0x80000000u)) << 32) | (0xffffffffu - (uint32_t)v);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
-__device__ __forceinline__ float key_logit(u64 k) {
-  const uint32_t u = (uint32_t)(k >> 32);
+__device__ __forceinline__ float from_order_bits(uint32_t u) {
   return __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
 }
+__device__ __forceinline__ u64 beam_key(float x, int v) {
+  return ((u64)order_bits(x) << 32) | (0xffffffffu - (uint32_t)v);
+}
+__device__ __forceinline__ float key_logit(u64 k) { return from_order_bits((uint32_t)(k >> 32)); }
 __device__ __forceinline__ int key_token(u64 k) { return (int)(0xffffffffu - (uint32_t)k); }
 
 __device__ __forceinline__ float wave_max(float v) {
@@ -81,98 +85,132 @@ struct BeamArgs {
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));  // rows may start at any element
 
-__global__ void __launch_bounds__(256) beam_chunk_kernel(const BeamArgs a) {
+__global__ void __launch_bounds__(256, 5) beam_chunk_kernel(const BeamArgs a) {
   __shared__ u64 list[4][64];
+  __shared__ float smax[4], ssum[4];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int chunk = blockIdx.x * 4 + w, row = blockIdx.y;
-  if (chunk >= a.chunks) return;
-  if (a.eos >= 0 && a.finished[row]) return;  // its one candidate needs no logits
+  const int row = blockIdx.y, W = a.beams;
+  const int v0 = blockIdx.x * BC + w * BL + 4 * lane;  // this lane's logits: v0 + 256 j + q
   const float* x = a.logits + row * a.row_stride;
-  const int v0 = chunk * BC + 4 * lane;  // this lane's logits: v0 + 256 j + q
-  float f[BC / 64];
-  if ((chunk + 1) * BC <= a.vocab) {
+  float f[BL / 64];
+  // all loads at once; whether the row has ended is known by the time they arrive
+  const bool ended = a.eos >= 0 && a.finished[row];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const f4u t = *reinterpret_cast<const f4u*>(x + v0 + 256 * j);
+  for (int j = 0; j < BL / 256; ++j) {
+    const int v = v0 + 256 * j;
+    if (v + 3 < a.vocab) {
+      const f4u t = *reinterpret_cast<const f4u*>(x + v);
 #pragma unroll
       for (int q = 0; q < 4; ++q) f[4 * j + q] = t[q];
-    }
-  } else {
+    } else {
 #pragma unroll
-    for (int i = 0; i < BC / 64; ++i) {
-      const int v = v0 + 256 * (i >> 2) + (i & 3);
-      f[i] = v < a.vocab ? x[v] : -INFINITY;
+      for (int q = 0; q < 4; ++q) f[4 * j + q] = v + q < a.vocab ? x[v + q] : -INFINITY;
     }
   }
+  if (ended) return;  // its one candidate needs no logits
   float lmax = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < BC / 64; ++i) lmax = fmaxf(lmax, f[i]);
+  for (int i = 0; i < BL / 64; ++i) lmax = fmaxf(lmax, f[i]);
   const float m = wave_max(lmax), mc = m == -INFINITY ? 0.f : m;
   float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < BC / 64; ++i) sum += __builtin_amdgcn_exp2f((f[i] - mc) * 1.4426950408889634f);
+  for (int i = 0; i < BL / 64; ++i) sum += __builtin_amdgcn_exp2f((f[i] - mc) * 1.4426950408889634f);
   sum = wave_sum(sum);
-  const int64_t slot = (int64_t)row * a.chunks + chunk;
-  if (lane == 0) a.stat[slot] = make_float2(m, sum);
-
-  // The `beams`-th largest of the lanes' maxima: at least `beams` logits reach it, and few more.
-  float t = m, left = lmax;
-  for (int k = 0; k < a.beams; ++k) {
-    t = wave_max(left);
-    const u64 at = __builtin_amdgcn_ballot_w64(left == t);
-    if (lane == (at ? __ffsll((unsigned long long)at) - 1 : -1)) left = -INFINITY;  // one of the lanes that hold it
+  if (lane == 0) {
+    smax[w] = m;
+    ssum[w] = sum;
   }
-  int n = 0;
+
+  // A threshold that at least W lanes' maxima reach, and few others: the upper half of the W-th largest
+  // maximum's bits (in an order that is the numbers'), bit by bit.
+  const uint32_t u = order_bits(lmax);
+  uint32_t bits = 0;
 #pragma unroll
-  for (int i = 0; i < BC / 64; ++i) {
-    const int v = v0 + 256 * (i >> 2) + (i & 3);
-    const bool in = f[i] >= t && v < a.vocab;
-    const u64 all = __builtin_amdgcn_ballot_w64(in);
-    if (all) {
+  for (int b = 31; b >= 16; --b) {
+    const uint32_t more = bits | (1u << b);
+    if (__popcll(__builtin_amdgcn_ballot_w64(u >= more)) >= W) bits = more;
+  }
+  const float t = bits <= order_bits(-INFINITY) ? -INFINITY : from_order_bits(bits);
+  uint32_t mine = 0;  // this lane's logits that reach it
+#pragma unroll
+  for (int i = 0; i < BL / 64; ++i)
+    if (f[i] >= t) mine |= 1u << i;
+#pragma unroll
+  for (int i = 0; i < BL / 64; ++i)
+    if (v0 + 256 * (i >> 2) + (i & 3) >= a.vocab) mine &= ~(1u << i);
+  int n = 0;
+  for (u64 all; (all = __builtin_amdgcn_ballot_w64(mine != 0)) != 0; n += __popcll(all)) {
+    if (n > 64) break;
+    if (mine) {
+      const int i = __ffs(mine) - 1;
+      mine &= mine - 1;
+      float x = f[0];
+#pragma unroll
+      for (int o = 1; o < BL / 64; ++o) x = i == o ? f[o] : x;
       const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
-      if (in && at < 64) list[w][at] = beam_key(f[i], v);
-      n += __popcll(all);
+      if (at < 64) list[w][at] = beam_key(x, v0 + 256 * (i >> 2) + (i & 3));
     }
   }
-  wave_sync();
-  u64* out = a.cand + slot * a.beams;
-  if (n <= 64) {  // the lane's place among them is how many are larger
-    const u64 key = lane < n ? list[w][lane] : 0;
-    int rank = 0;
-    for (int i = 0; i < n; ++i) rank += list[w][i] > key;
-    if (lane < n && rank < a.beams) out[rank] = key;
-    if (lane >= n && lane < a.beams) out[lane] = 0;
-  } else {  // many equal logits: the largest key below the last one, `beams` times
-    u64 last = ~(u64)0;
-    for (int k = 0; k < a.beams; ++k) {
+  if (n <= 64) {
+    if (lane >= n) list[w][lane] = 0;
+  } else {  // many equal logits: the largest key below the last one, W times
+    u64 last = ~(u64)0, kept = 0;
+    for (int k = 0; k < W; ++k) {
       u64 best = 0;
 #pragma unroll
-      for (int i = 0; i < BC / 64; ++i) {
+      for (int i = 0; i < BL / 64; ++i) {
         const int v = v0 + 256 * (i >> 2) + (i & 3);
         const u64 key = v < a.vocab ? beam_key(f[i], v) : 0;
         if (key < last && key > best) best = key;
       }
       last = wave_max_key(best);
-      if (lane == 0) out[k] = last;
+      if (lane == k) kept = last;
+    }
+    list[w][lane] = kept;
+  }
+  __syncthreads();
+  // the workgroup's W best: a key's place is how many are larger (keys differ, but for the empty ones)
+  const u64 key = list[w][lane];
+  int rank = 0;
+  for (int o = 0; o < 4; ++o)
+    for (int i = 0; i < 64 && list[o][i] != 0; i += 8) {  // filled from the front
+#pragma unroll
+      for (int q = 0; q < 8; ++q) rank += list[o][i + q] > key;
+    }
+  const int64_t slot = (int64_t)row * a.chunks + blockIdx.x;
+  if (key != 0 && rank < W) a.cand[slot * W + rank] = key;
+  if (w == 0) {
+    // where the chunk has fewer than W logits, no candidate
+    const int have = min(BC, a.vocab - (int)blockIdx.x * BC);
+    if (lane >= have && lane < W) a.cand[slot * W + lane] = 0;
+    if (lane == 0) {
+      const float M = fmaxf(fmaxf(smax[0], smax[1]), fmaxf(smax[2], smax[3]));
+      float s = 0.f;
+#pragma unroll
+      for (int o = 0; o < 4; ++o)
+        s += smax[o] == -INFINITY ? ssum[o] : ssum[o] * __builtin_amdgcn_exp2f((smax[o] - M) * 1.4426950408889634f);
+      a.stat[slot] = make_float2(M, s);
     }
   }
 }
 
 __global__ void __launch_bounds__(64 * PICK_WAVES) beam_pick_kernel(const BeamArgs a) {
-  __shared__ u64 heads[PICK_WAVES][BV_MAX / BC];
-  __shared__ u64 near[PICK_WAVES][BEAMS_MAX * BEAMS_MAX];
-  __shared__ int sel[PICK_WAVES][BEAMS_MAX];
-  __shared__ double score[BEAMS_MAX * BEAMS_MAX];
-  __shared__ int token[BEAMS_MAX * BEAMS_MAX];  // -1: no candidate
+  constexpr int NL = BV_MAX / BC / 64, NK = BEAMS_MAX * BEAMS_MAX / 64;  // chunks, and a group's candidates, per lane
+  __shared__ __attribute__((aligned(16))) uint32_t heads[PICK_WAVES][64 * NL];
+  __shared__ __attribute__((aligned(16))) u64 near[PICK_WAVES][64 * NK];
+  __shared__ u64 least[PICK_WAVES];
+  __shared__ double score[64 * NK];
+  __shared__ int token[64 * NK];  // -1: no candidate
   __shared__ int failed[BEAMS_MAX];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int W = a.beams, first = blockIdx.x * W;
+  const int W = a.beams, W2 = W * W, first = blockIdx.x * W;
   for (int r = w; r < W; r += PICK_WAVES) {
     const int row = first + r;
+    const int64_t s0 = (int64_t)row * a.chunks;
     const double base = a.scores[row];
-    const bool bad = !(base < INFINITY);  // NaN or +infinity
+    const bool bad = !(base < INFINITY), ended = a.eos >= 0 && a.finished[row];  // bad: NaN or +infinity
     if (lane < W) token[r * W + lane] = -1;
-    if (a.eos >= 0 && a.finished[row]) {
+    if (ended) {
       if (lane == 0) {
         score[r * W] = base;
         token[r * W] = a.eos;
@@ -180,45 +218,76 @@ __global__ void __launch_bounds__(64 * PICK_WAVES) beam_pick_kernel(const BeamAr
       }
       continue;
     }
-    const int64_t s0 = (int64_t)row * a.chunks;
-    // log of the row's sum, in 64 bits over the chunks' sums
+    // the chunks' sums and best keys, NL to a lane
+    float2 st[NL];
+    u64 head[NL];
     float m = -INFINITY;
-    for (int i = lane; i < a.chunks; i += 64) {
-      m = fmaxf(m, a.stat[s0 + i].x);
-      heads[w][i] = a.cand[(s0 + i) * W];
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      const int i = 64 * n + lane;
+      st[n] = make_float2(-INFINITY, 0.f);
+      head[n] = 0;
+      if (i < a.chunks) {
+        st[n] = a.stat[s0 + i];
+        head[n] = a.cand[(s0 + i) * W];
+      }
+      m = fmaxf(m, st[n].x);
+      heads[w][i] = (uint32_t)(head[n] >> 32);
     }
-    if (lane < W) sel[w][lane] = 0;  // a failed row may have fewer chunks with a key
+    if (lane == 0) least[w] = 0;
     wave_sync();
+    // The W-th best of the chunks' best keys: none but keys that reach it are among the row's W best. (Of equal
+    // logits the earlier chunk's is the lower token. A failed row's keys may be anything.)
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
+      const int i = 64 * n + lane;
+      if (64 * n >= a.chunks) break;
+      const uint32_t h = heads[w][i];
+      int rank = 0;
+      for (int j = 0; j < a.chunks; j += 8) {  // places past the last chunk hold 0
+        const uint4 x = *reinterpret_cast<const uint4*>(&heads[w][j]), y = *reinterpret_cast<const uint4*>(&heads[w][j + 4]);
+        const uint32_t o[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int q = 0; q < 8; ++q) rank += o[q] > h || (o[q] == h && j + q < i);
+      }
+      if (i < a.chunks && rank == W - 1) least[w] = head[n];
+    }
+    // log of the row's sum: the chunks' sums in fp32, joined in 64 bits
     m = wave_max(m);
     double sum = 0;
-    for (int i = lane; i < a.chunks; i += 64) {
-      const float2 s = a.stat[s0 + i];
-      sum += s.x == -INFINITY ? (double)s.y : (double)s.y * exp((double)s.x - (double)m);  // s.y: 0, or NaN
-    }
+#pragma unroll
+    for (int n = 0; n < NL; ++n)
+      sum += st[n].x == -INFINITY ? st[n].y  // 0, or NaN
+                                  : st[n].y * __builtin_amdgcn_exp2f((st[n].x - m) * 1.4426950408889634f);
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
     const double lse = (double)m + log(sum);
     if (lane == 0) failed[r] = bad || sum != sum;
-    // the W chunks with the best first keys hold the row's W best keys
-    for (int i = lane; i < a.chunks; i += 64) {
-      const u64 key = heads[w][i];
-      int rank = 0;
-      for (int j = 0; j < a.chunks; ++j) rank += heads[w][j] > key;
-      if (rank < W) sel[w][rank] = i;  // keys differ, but for the empty ones: a chunk always has a candidate
+    wave_sync();
+    // the keys that reach it: W at least (if there are as many), W a chunk of W chunks at most
+    const u64 low = least[w];
+    const int keys = a.chunks * W;
+    int n = 0;
+    for (int e = lane; e - lane < keys; e += 64) {
+      const u64 key = e < keys ? a.cand[s0 * W + e] : 0;
+      const u64 all = __builtin_amdgcn_ballot_w64(key != 0 && key >= low);
+      const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
+      if (key != 0 && key >= low && at < 64 * NK) near[w][at] = key;
+      n += __popcll(all);
     }
+    n = min(n, 64 * NK);
+    if (lane < 8 && n + lane < 64 * NK) near[w][n + lane] = 0;
     wave_sync();
-    const int nsel = min(W, a.chunks);
-    for (int e = lane; e < nsel * W; e += 64) near[w][e] = a.cand[(s0 + sel[w][e / W]) * W + e % W];
-    wave_sync();
-    for (int e = lane; e < nsel * W; e += 64) {
+    for (int e = lane; e < n; e += 64) {
       const u64 key = near[w][e];
-      if (key == 0) continue;
-      int rank = 0;
-      for (int j = 0; j < nsel * W; ++j) rank += near[w][j] > key;
-      if (rank < W) {
+      int place = 0;
+      for (int j = 0; j < n; j += 8)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) place += near[w][j + q] > key;
+      if (place < W) {
         const float x = key_logit(key);
-        score[r * W + rank] = x == -INFINITY ? -INFINITY : base + ((double)x - lse);
-        token[r * W + rank] = key_token(key);
+        score[r * W + place] = x == -INFINITY ? -INFINITY : base + ((double)x - lse);
+        token[r * W + place] = key_token(key);
       }
     }
     wave_sync();  // the next row's keys take the same places
@@ -226,26 +295,38 @@ __global__ void __launch_bounds__(64 * PICK_WAVES) beam_pick_kernel(const BeamAr
   __syncthreads();
   bool fail = false;
   for (int r = 0; r < W; ++r) fail |= failed[r] != 0;
-  if (tid >= W * W) return;
-  const int r = tid / W;
   if (fail) {  // every beam of the group shows it
-    if (tid % W == 0) {
-      a.tokens[first + r] = -1;
-      a.parents[first + r] = first + r;
-      a.out_scores[first + r] = __builtin_nanf("");
-      a.out_finished[first + r] = a.eos >= 0 ? a.finished[first + r] : 0;
+    if (tid < W) {
+      a.tokens[first + tid] = -1;
+      a.parents[first + tid] = first + tid;
+      a.out_scores[first + tid] = __builtin_nanf("");
+      a.out_finished[first + tid] = a.eos >= 0 ? a.finished[first + tid] : 0;
     }
     return;
   }
-  if (token[tid] < 0) return;
-  const double s = score[tid];
-  int rank = 0;
-  for (int j = 0; j < W * W; ++j) rank += token[j] >= 0 && (score[j] > s || (score[j] == s && j < tid));
-  if (rank < W) {
-    a.tokens[first + rank] = token[tid];
-    a.parents[first + rank] = first + r;
-    a.out_scores[first + rank] = (float)s;
-    a.out_finished[first + rank] = a.eos >= 0 && (token[tid] == a.eos || a.finished[first + r]);
+  // The group's candidates by score, equal ones by row and place: a wave counts for one candidate at a time
+  // how many come before it.
+  double sc[NK];
+#pragma unroll
+  for (int n = 0; n < NK; ++n) {
+    const int e = 64 * n + lane;
+    sc[n] = e < W2 && token[e] >= 0 ? score[e] : __builtin_nan("");  // comes before none
+  }
+#pragma unroll 4
+  for (int c = w; c < W2; c += PICK_WAVES) {
+    const int t = token[c];
+    const double s = score[c];
+    int before = 0;
+#pragma unroll
+    for (int n = 0; n < NK; ++n)
+      if (64 * n < W2) before += __popcll(__builtin_amdgcn_ballot_w64(sc[n] > s || (sc[n] == s && 64 * n + lane < c)));
+    if (t >= 0 && before < W && lane == 0) {
+      const int at = first + before, r = first + c / W;
+      a.tokens[at] = t;
+      a.parents[at] = r;
+      a.out_scores[at] = (float)s;
+      a.out_finished[at] = a.eos >= 0 && (t == a.eos || a.finished[r]);
+    }
   }
 }
 
@@ -337,7 +418,7 @@ extern "C" hipError_t mk_beam_select(int rows, int vocab, int beams, const float
   a.parents = parents;
   a.out_scores = out_scores;
   a.out_finished = out_finished;
-  hipLaunchKernelGGL(beam_chunk_kernel, dim3((a.chunks + 3) / 4, rows), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL(beam_chunk_kernel, dim3(a.chunks, rows), dim3(256), 0, stream, a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(beam_pick_kernel, dim3(rows / beams), dim3(64 * PICK_WAVES), 0, stream, a);
