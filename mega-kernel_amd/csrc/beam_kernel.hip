@@ -85,10 +85,13 @@ struct BeamArgs {
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));  // rows may start at any element
 
-__global__ void __launch_bounds__(256, 5) beam_chunk_kernel(const BeamArgs a) {
-  __shared__ u64 list[4][64];
+__global__ void __launch_bounds__(256) beam_chunk_kernel(const BeamArgs a) {
+  __shared__ u64 list[64];
   __shared__ float smax[4], ssum[4];
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ uint32_t sbits[4];
+  __shared__ u64 sbest[4];
+  __shared__ int count;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int row = blockIdx.y, W = a.beams;
   const int v0 = blockIdx.x * BC + w * BL + 4 * lane;  // this lane's logits: v0 + 256 j + q
   const float* x = a.logits + row * a.row_stride;
@@ -108,9 +111,19 @@ __global__ void __launch_bounds__(256, 5) beam_chunk_kernel(const BeamArgs a) {
     }
   }
   if (ended) return;  // its one candidate needs no logits
+  auto token = [&](int i) { return v0 + 256 * (i >> 2) + (i & 3); };
   float lmax = -INFINITY;
 #pragma unroll
   for (int i = 0; i < BL / 64; ++i) lmax = fmaxf(lmax, f[i]);
+  // A threshold that at least W lanes' maxima reach, and few others: the upper half of the W-th largest
+  // maximum's bits (in an order that is the numbers'), bit by bit. The highest of the four waves' serves all.
+  const uint32_t u = order_bits(lmax);
+  uint32_t bits = 0;
+#pragma unroll
+  for (int b = 31; b >= 16; --b) {
+    const uint32_t more = bits | (1u << b);
+    if (__popcll(__builtin_amdgcn_ballot_w64(u >= more)) >= W) bits = more;
+  }
   const float m = wave_max(lmax), mc = m == -INFINITY ? 0.f : m;
   float sum = 0.f;
 #pragma unroll
@@ -119,78 +132,63 @@ __global__ void __launch_bounds__(256, 5) beam_chunk_kernel(const BeamArgs a) {
   if (lane == 0) {
     smax[w] = m;
     ssum[w] = sum;
+    sbits[w] = bits;
   }
-
-  // A threshold that at least W lanes' maxima reach, and few others: the upper half of the W-th largest
-  // maximum's bits (in an order that is the numbers'), bit by bit.
-  const uint32_t u = order_bits(lmax);
-  uint32_t bits = 0;
-#pragma unroll
-  for (int b = 31; b >= 16; --b) {
-    const uint32_t more = bits | (1u << b);
-    if (__popcll(__builtin_amdgcn_ballot_w64(u >= more)) >= W) bits = more;
-  }
+  if (tid == 0) count = 0;
+  __syncthreads();
+  bits = max(max(sbits[0], sbits[1]), max(sbits[2], sbits[3]));
   const float t = bits <= order_bits(-INFINITY) ? -INFINITY : from_order_bits(bits);
   uint32_t mine = 0;  // this lane's logits that reach it
 #pragma unroll
   for (int i = 0; i < BL / 64; ++i)
     if (f[i] >= t) mine |= 1u << i;
+  if (blockIdx.x * BC + (w + 1) * BL > a.vocab)
 #pragma unroll
-  for (int i = 0; i < BL / 64; ++i)
-    if (v0 + 256 * (i >> 2) + (i & 3) >= a.vocab) mine &= ~(1u << i);
-  int n = 0;
-  for (u64 all; (all = __builtin_amdgcn_ballot_w64(mine != 0)) != 0; n += __popcll(all)) {
-    if (n > 64) break;
-    if (mine) {
-      const int i = __ffs(mine) - 1;
-      mine &= mine - 1;
-      float x = f[0];
-#pragma unroll
-      for (int o = 1; o < BL / 64; ++o) x = i == o ? f[o] : x;
-      const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
-      if (at < 64) list[w][at] = beam_key(x, v0 + 256 * (i >> 2) + (i & 3));
-    }
-  }
-  if (n <= 64) {
-    if (lane >= n) list[w][lane] = 0;
-  } else {  // many equal logits: the largest key below the last one, W times
-    u64 last = ~(u64)0, kept = 0;
-    for (int k = 0; k < W; ++k) {
-      u64 best = 0;
-#pragma unroll
-      for (int i = 0; i < BL / 64; ++i) {
-        const int v = v0 + 256 * (i >> 2) + (i & 3);
-        const u64 key = v < a.vocab ? beam_key(f[i], v) : 0;
-        if (key < last && key > best) best = key;
-      }
-      last = wave_max_key(best);
-      if (lane == k) kept = last;
-    }
-    list[w][lane] = kept;
+    for (int i = 0; i < BL / 64; ++i)
+      if (token(i) >= a.vocab) mine &= ~(1u << i);
+  while (mine) {
+    const int v = token(__ffs(mine) - 1);
+    mine &= mine - 1;
+    const int at = atomicAdd(&count, 1);
+    if (at >= 64) break;
+    list[at] = beam_key(x[v], v);  // the logit again: cheaper than finding it among the registers
   }
   __syncthreads();
-  // the workgroup's W best: a key's place is how many are larger (keys differ, but for the empty ones)
-  const u64 key = list[w][lane];
-  int rank = 0;
-  for (int o = 0; o < 4; ++o)
-    for (int i = 0; i < 64 && list[o][i] != 0; i += 8) {  // filled from the front
-#pragma unroll
-      for (int q = 0; q < 8; ++q) rank += list[o][i + q] > key;
-    }
   const int64_t slot = (int64_t)row * a.chunks + blockIdx.x;
-  if (key != 0 && rank < W) a.cand[slot * W + rank] = key;
-  if (w == 0) {
-    // where the chunk has fewer than W logits, no candidate
-    const int have = min(BC, a.vocab - (int)blockIdx.x * BC);
-    if (lane >= have && lane < W) a.cand[slot * W + lane] = 0;
-    if (lane == 0) {
-      const float M = fmaxf(fmaxf(smax[0], smax[1]), fmaxf(smax[2], smax[3]));
-      float s = 0.f;
-#pragma unroll
-      for (int o = 0; o < 4; ++o)
-        s += smax[o] == -INFINITY ? ssum[o] : ssum[o] * __builtin_amdgcn_exp2f((smax[o] - M) * 1.4426950408889634f);
-      a.stat[slot] = make_float2(M, s);
+  u64* out = a.cand + slot * W;
+  const int n = count;
+  if (n <= 64) {  // a key's place is how many are larger
+    if (w == 0) {
+      const u64 key = lane < n ? list[lane] : 0;
+      int place = 0;
+      for (int i = 0; i < n; ++i) place += list[i] > key;
+      if (lane < n && place < W) out[place] = key;
+      if (lane >= n && lane < W) out[lane] = 0;  // fewer than W logits
     }
+  } else {  // many equal logits: the largest key below the last one, W times
+    u64 last = ~(u64)0;
+    for (int k = 0; k < W; ++k) {
+      u64 best = 0;
+#pragma unroll 1
+      for (int i = 0; i < BL / 64; ++i) {  // from memory: kept in registers, their keys would cost the others theirs
+        const u64 key = token(i) < a.vocab ? beam_key(x[token(i)], token(i)) : 0;
+        if (key < last && key > best) best = key;
+      }
+      best = wave_max_key(best);
+      __syncthreads();
+      if (lane == 0) sbest[w] = best;
+      __syncthreads();
+      last = max(max(sbest[0], sbest[1]), max(sbest[2], sbest[3]));
+      if (tid == 0) out[k] = last;
+    }
+  }
+  if (tid == 0) {
+    const float M = fmaxf(fmaxf(smax[0], smax[1]), fmaxf(smax[2], smax[3]));
+    float s = 0.f;
+#pragma unroll
+    for (int o = 0; o < 4; ++o)
+      s += smax[o] == -INFINITY ? ssum[o] : ssum[o] * __builtin_amdgcn_exp2f((smax[o] - M) * 1.4426950408889634f);
+    a.stat[slot] = make_float2(M, s);
   }
 }
 
