@@ -112,7 +112,8 @@ __host__ __device__ inline size_t skf_elems(int B, int K) { return (size_t)(skf_
 // EPI_QKV_PART / EPI_SILU_PART: the QKV / gate-up products split over K on small grids, each K range's
 // raw sums into part[blockIdx.z][M][N] (N = 4096 / 2 I, a tile's columns as in EPI_QKV / EPI_SILU);
 // qkv_post_kernel / silu_post_kernel add the ranges in order and finish the epilogue.
-enum Epi { EPI_QKV = 0, EPI_RESID = 1, EPI_SILU = 2, EPI_QKV_PART = 3, EPI_SILU_PART = 4 };
+// EPI_QKV_ROWS: EPI_QKV for rows of several prompts (GemmArgs::pk says where each belongs).
+enum Epi { EPI_QKV = 0, EPI_RESID = 1, EPI_SILU = 2, EPI_QKV_PART = 3, EPI_SILU_PART = 4, EPI_QKV_ROWS = 5 };
 
 struct GemmArgs {
   const uint16_t* ah;  // fragment-major, K columns
@@ -148,7 +149,7 @@ struct GemmArgs {
 // first element of weight row r (0..127) of N-tile t
 template <int EPI>
 __device__ __forceinline__ const uint16_t* weight_row(const GemmArgs& g, int t, int r) {
-  if constexpr (EPI == EPI_QKV || EPI == EPI_QKV_PART) {
+  if constexpr (EPI == EPI_QKV || EPI == EPI_QKV_PART || EPI == EPI_QKV_ROWS) {
     if (t < HQ) return g.w0 + (size_t)(t * D + r) * g.K;
     if (t < HQ + HKV) return g.w1 + (size_t)((t - HQ) * D + r) * g.K;
     return g.w2 + (size_t)((t - HQ - HKV) * D + r) * g.K;
@@ -396,7 +397,7 @@ __global__ void __launch_bounds__(64 * NW * KS, PF == 4 ? 1 : 2) gemm_kernel(con
     return;
   }
 
-  if constexpr (EPI == EPI_QKV) {
+  if constexpr (EPI == EPI_QKV || EPI == EPI_QKV_ROWS) {
     // tile tn is one head: q head tn (< 16), k head tn - 16 (< 24) or v head tn - 24. 16 lanes per
     // row (lane t: dims 8t .. 8t + 7), 4 rows per wave and pass, 8 passes
     const int tt = lane & 15, rq = lane >> 4;  // tt: the lane's 8 dims; rq: its row of the pass
@@ -406,8 +407,8 @@ __global__ void __launch_bounds__(64 * NW * KS, PF == 4 ? 1 : 2) gemm_kernel(con
     for (int pass = 0; pass < 8; ++pass) {
       const int r = 32 * wave + 4 * pass + rq, m = m0 + r;
       if (m >= g.M) continue;
-      const int pos = row_pos(g.pk, g.position, m);
-      const size_t seq = row_cache(g.pk, m);
+      const int pos = EPI == EPI_QKV ? g.position + m : row_pos(g.pk, g.position, m);
+      const size_t seq = EPI == EPI_QKV ? 0 : row_cache(g.pk, m);
       const int page = tn >= HQ && g.kv.bt ? kv_page(g.kv, pos, g.bad) : 0;
       float v[8];
       ld8(r, 8 * tt, v);
@@ -2272,7 +2273,7 @@ static int gemm_pf(dim3 grid, int K) {
 }
 template <int EPI>
 static hipError_t launch_gemm(dim3 grid, const GemmArgs& g, hipStream_t st) {
-  if constexpr (EPI == EPI_QKV || EPI == EPI_SILU) {
+  if constexpr (EPI == EPI_QKV || EPI == EPI_SILU || EPI == EPI_QKV_ROWS) {
     if (grid.z == 1 && tall_tiles((int)grid.x, g.M) && g.K / KT % 2 == 0) {
       hipLaunchKernelGGL((gemm_kernel<EPI, 2, 8>), dim3(grid.x, (grid.y + 1) / 2), dim3(512), 0, st, g);
       return hipGetLastError();
@@ -2453,7 +2454,8 @@ static hipError_t run(const mk_model_dims& dims, const int32_t* tokens, int M, i
       MKP_LAUNCH(qkv_post_kernel, dim3((M * (HQ + 2 * HKV) + 3) / 4), dim3(64), 0, st, wk.qpart, sq, M, position,
                  (const uint16_t*)lw.q_norm_weight, (const uint16_t*)lw.k_norm_weight, cos_tab, sin_tab, wk.qh, wk.ql,
                  k_cache, v_cache, l, kv, wk.bad, pk.rows);
-    } else if ((e = launch_gemm<EPI_QKV>(dim3(g.N / NT, mtiles), g, st)) != hipSuccess) {
+    } else if ((e = pk.n ? launch_gemm<EPI_QKV_ROWS>(dim3(g.N / NT, mtiles), g, st)
+                         : launch_gemm<EPI_QKV>(dim3(g.N / NT, mtiles), g, st)) != hipSuccess) {
       return e;
     }
     AttnArgs at = at0;
@@ -2487,6 +2489,8 @@ static hipError_t run(const mk_model_dims& dims, const int32_t* tokens, int M, i
                wk.part, sd, nullptr, nullptr, nullptr, M);
   if (pk.n) {  // each sequence's last row's
     MKP_LAUNCH(last_rows_kernel<H>, dim3(pk.n), dim3(H / 4), 0, st, wk.x, pk.ends, wk.last);
+    // the operand areas of the layers are free: whole row tiles of at least H columns each, or the fragments of
+    // as many rows (the sequences are no more than the tokens)
     return lm_head_rows<H>(dims, pk.n, wk.last, final_norm, lm_head, wk.ah, wk.ah, wk.al, logits, out_token, wk.keys,
                            wk.bad, st);
   }
@@ -2586,7 +2590,9 @@ extern "C" hipError_t mk_prefill_batch(const mk_model_dims* dims, const int32_t*
   if (num_seqs < 1 || num_seqs > BMAX || max_seq_len < 1) return hipErrorInvalidValue;
   // a sequence's cache may be followed by others of the same batch: at least its own size apart
   if (num_seqs > 1 && seq_stride < (int64_t)dims->num_layers * HKV * max_seq_len * D) return hipErrorInvalidValue;
-  if (seq_stride % 8 != 0) return hipErrorInvalidValue;
+  if (seq_stride % 8 != 0 || reinterpret_cast<uintptr_t>(k_cache) % 16 != 0 ||
+      reinterpret_cast<uintptr_t>(v_cache) % 16 != 0)
+    return hipErrorInvalidValue;
   PackedRun pk;
   int64_t total = 0;
   for (int i = 0; i < num_seqs; ++i) {

@@ -426,6 +426,8 @@ std::tuple<torch::Tensor, torch::Tensor> prefill_batch(torch::Tensor tokens, std
     TORCH_CHECK(t->defined() && t->dim() == 5 && t->size(0) == S, "megakernel: ", name,
                 " must be [prompts, layers, 8, max_seq, 128] for ", S, " prompts");
     check_bf16((*t)[0], name, {L, kKVHeads, max_seq_len, kHeadDim}, c.dev);
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, "megakernel: ", name,
+                " must start on a 16-byte boundary");
     TORCH_CHECK(S == 1 || (t->stride(0) % 8 == 0 && t->stride(0) >= L * kKVHeads * max_seq_len * kHeadDim),
                 "megakernel: ", name, "'s sequences must not overlap and start on 16-byte boundaries");
   }
@@ -566,7 +568,7 @@ void beam_reorder(torch::Tensor kc, torch::Tensor vc, torch::Tensor parents, tor
   TORCH_CHECK(kc.defined() && kc.dim() == 5, "megakernel: k_cache must be [rows, layers, 8, max_seq, 128]");
   const int64_t rows = kc.size(0), L = kc.size(1), S = kc.size(3);
   check_beams(rows, beams);
-  TORCH_CHECK(L >= 1 && S >= 1 && L * kKVHeads * 2 * ((S + 15) / 16) <= INT32_MAX,
+  TORCH_CHECK(L >= 1 && S >= 1 && L * kKVHeads * 2 * ((S + 15) / 16) <= INT32_MAX - 8192,
               "megakernel: the caches have no positions, or too many");
   check_bf16(kc, "k_cache", {rows, L, kKVHeads, S, kHeadDim}, kc.device());
   check_bf16(vc, "v_cache", {rows, L, kKVHeads, S, kHeadDim}, kc.device());

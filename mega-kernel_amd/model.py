@@ -117,6 +117,8 @@ def run(argv=None, keep_prefill_cache=False):
     a = ap.parse_args(argv)
     if a.beams and (a.beams > 16 or a.beams < 0 or a.prompts < 1 or a.beams * a.prompts > 64):
         ap.error("--beams takes 1 to 16 beams per prompt, and at most 64 in all")
+    if a.beams and not 1 <= a.prompt < a.max_seq:
+        ap.error("--beams needs a prompt that leaves room in --max-seq")
     import torch
     import megakernel
 

@@ -185,3 +185,80 @@ def test_reorder_ranges(kernel):
 def test_reorder_leaves_rows_whose_parent_is_elsewhere(kernel):
     k, v = caches(6, 2, 33, seed=2)
     reorder_check(kernel, k, v, [-1, 0, 3, 2, 9, 2 ** 31 - 1], [0] * 6, [33] * 6, 3)
+
+
+# ---------------------------------------------------------------------------------------------------
+def test_calls_on_two_streams_at_once(kernel):
+    """Each call has a workspace of its own."""
+    sets = [inputs(32, 100003, seed=20 + i, done=5) for i in range(2)]
+    want = [kernel.beam_select(*s, 8, 77) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(8):
+        for i, (stream, s) in enumerate(zip(streams, sets)):
+            with torch.cuda.stream(stream):
+                got[i].append(kernel.beam_select(*s, 8, 77))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+
+
+def test_a_step_in_a_graph(kernel):
+    """Selection and reordering captured together and replayed on other logits and other caches."""
+    rows, beams, L, S = 8, 4, 2, 96
+    logits, scores, finished = inputs(rows, 20011, seed=30, done=1)
+    k, v = caches(rows, L, S, seed=31)
+    begin, end = i32([10] * 4 + [33] * 4), i32([60] * 4 + [90] * 4)
+
+    def step():
+        out = kernel.beam_select(logits, scores, finished, beams, 5)
+        kernel.beam_reorder(k, v, out[1], begin, end, beams)
+        return out
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for seed in (32, 33, 34):
+        for old, new in zip((logits, scores, finished), inputs(rows, 20011, seed=seed, done=2)):
+            old.copy_(new)
+        for old, new in zip((k, v), caches(rows, L, S, seed=seed)):
+            old.copy_(new)
+        k0, v0 = k.clone(), v.clone()
+        want = step()
+        want_k, want_v = k.clone(), v.clone()
+        k.copy_(k0)
+        v.copy_(v0)
+        for t in held:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(held, want))
+        assert torch.equal(k, want_k) and torch.equal(v, want_v)
+
+
+def test_offsets_past_32_bits(kernel):
+    """Caches whose elements, and logits whose bytes, pass 2^32."""
+    rows, L, S = 16, 28, 4096
+    k, v = (torch.zeros(rows, L, 8, S, 128, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    for t in (k, v):
+        for b in range(rows):
+            t[b, :, :, S - 40:] = torch.randn(L, 8, 40, 128, device=DEV, dtype=torch.bfloat16)
+    tail = [t[:, :, :, S - 40:].clone() for t in (k, v)]
+    parents = [15, 14, 13, 12, 0, 0, 0, 0, 8, 9, 1, 2, 3, 4, 5, 6]
+    kernel.beam_reorder(k, v, i32(parents), i32([S - 33] * rows), i32([S] * rows), 16)
+    for t, old in zip((k, v), tail):
+        now = t[:, :, :, S - 40:]
+        assert torch.equal(now[:, :, :, :7], old[:, :, :, :7])
+        for b, p in enumerate(parents):
+            assert torch.equal(now[b, :, :, 7:], old[p, :, :, 7:])
+        assert (t[:, :, :, :S - 40] == 0).all()
+    del k, v, tail
+    wide = torch.zeros(1 << 31, device=DEV).view(4, 1 << 29)
+    logits = wide[:, -50000:]
+    logits.copy_(torch.randn(4, 50000, device=DEV))
+    check(kernel, logits, torch.tensor([-1.0, -2.5, -1.25, -3.0], device=DEV),
+          torch.zeros(4, dtype=torch.bool, device=DEV), 4, 9)

@@ -187,3 +187,22 @@ def test_beam_search_of_several_prompts(mini):
         n = len(ids)
         _check_cache(kd[b], kw, n, f"beam {b} k")
         _check_cache(vd[b], vw, n, f"beam {b} v")
+
+
+def test_many_tokens(mini_2k):
+    """64 prompts of 1,000 tokens, 64,000 rows: each as alone, to summation order."""
+    s = mini_2k.shape
+    prompts = [hf.prompt_ids(1000, s.vocab, seed=100 + i)[0].tolist() for i in range(64)]
+    kd, vd = _caches(mini_2k, 64)
+    logits, toks = _prefill_batch(mini_2k, prompts, kd, vd)
+    for i in (0, 31, 63):
+        k1, v1 = (t[0] for t in _caches(mini_2k, 1))
+        tokens = torch.tensor(prompts[i], dtype=torch.int32, device=DEV)
+        want, tok = mini_2k.kernel.prefill(tokens, mini_2k.embed, mini_2k.lm_head, mini_2k.final_norm, mini_2k.layers,
+                                           mini_2k.cos, mini_2k.sin, k1, v1, 0, mini_2k.max_seq)
+        maxabs, _ = stats(logits[i].cpu(), want.cpu())
+        print(f"[prefill_batch] prompt {i} of 64,000 tokens: max|d| {maxabs:.3e}", flush=True)
+        assert maxabs < 5e-3
+        _check_cache(kd[i], k1.cpu(), 1000, "k")
+        _check_cache(vd[i], v1.cpu(), 1000, "v")
+    assert mini_2k.kernel.status() == 0

@@ -57,7 +57,7 @@ def test_attention_packed_c(lib):
 
 def test_beam_select_c(lib):
     need = lib.mk_beam_select_workspace_bytes
-    assert need(8, 151936, 4) >= 8 * 75 * (4 * 8 + 8) and need(8, 151936, 4) % 256 == 0
+    assert 0 < need(4, 151936, 4) < need(8, 151936, 4) < need(8, 1 << 20, 4) and need(8, 151936, 4) % 256 == 0
     assert need(0, 100, 1) == need(4, 0, 1) == need(4, (1 << 20) + 1, 1) == need(4, 100, 0) == need(34, 100, 17) == 0
 
     def call(rows=8, vocab=1000, beams=4, logits=P, stride=1000, scores=P, finished=P, eos=3, outs=(P, P, P, P), ws=P,
@@ -110,6 +110,8 @@ def test_prefill_batch_c(lib):
     assert call(dims=Dims(1024, 3072, 28, 1000)) == INVALID  # vocabulary no multiple of 16
     assert call(lengths=()) == call(lengths=(1,) * 65) == call(lengths=(5, 0)) == call(lengths=(-1,)) == INVALID
     assert call(lengths=(5, 513)) == call(lengths=(2 ** 31 - 1,), max_seq=2 ** 31 - 1) == INVALID
+    for i in (6, 7):  # the caches' alignment
+        assert call(ptrs=tuple(vp(4104) if j == i else P for j in range(8))) == INVALID
     assert call(stride=one - 8) == call(stride=one + 4) == call(max_seq=0) == INVALID
     assert call(nbytes=1000) == INVALID
 
@@ -226,5 +228,6 @@ def test_prefill_batch_op(ext):
     refuses("v_cache must be", v=z(1, L, 8, S, 128))
     refuses("must have shape", k=z(2, L, 8, S + 1, 128))
     refuses("must not overlap", k=z(1, L, 8, S, 128).expand(2, -1, -1, -1, -1))
+    refuses("16-byte boundary", k=z(2 * L * 8 * S * 128 + 4)[4:].view(2, L, 8, S, 128))
     refuses("same strides", k=wide[0])
     refuses("cos/sin tables", max_seq=S + 1)
