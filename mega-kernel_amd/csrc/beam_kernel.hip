@@ -63,12 +63,6 @@ __device__ __forceinline__ u64 wave_max_key(u64 k) {
   return k;
 }
 
-// LDS that one lane of a wave wrote and another reads
-__device__ __forceinline__ void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
 struct BeamArgs {
   const float* logits;  // [rows][row_stride]
   int64_t row_stride;

@@ -125,6 +125,12 @@ __device__ __forceinline__ float xmax32(float v) {
 // Full wave sum; every lane receives the result.
 __device__ __forceinline__ float wave_sum(float v) { return xsum32(xsum16(row16_sum(v))); }
 
+// LDS that one lane of a wave wrote and another reads
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 __device__ __forceinline__ unsigned xcc_id() {
   return __builtin_amdgcn_s_getreg((20) | (0 << 6) | ((4 - 1) << 11));  // HW_REG_XCC_ID[3:0]
 }

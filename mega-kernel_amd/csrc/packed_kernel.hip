@@ -43,6 +43,7 @@
 namespace mkp {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void lds_void;
 
@@ -73,6 +74,7 @@ struct PackedArgs {
   int64_t kv_seq;      // PARTS 2: elements between the sequences' caches
   DivBy by_hkv, by_g;
   int hkv, g, nseq, frag;
+  int alone;  // sequences whose blocks come one sequence after another, before the others' in turn
   // the launch's sequences, longest first: see the kernel's order of blocks; first row, length, number
   int32_t first[PSEQ], row[PSEQ], len[PSEQ], seq[PSEQ];
 };
@@ -141,9 +143,10 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
   const int col = lane & 31, g = lane >> 5;  // this lane's query and half of the K slots
   auto& tiles = sm.tiles[ks];
   // workgroup b: K/V head b % hkv (with 8 heads, a head's keys stay in one XCD's L2), query block b / hkv of
-  // the launch's. The blocks go by their number in their sequence, the highest (the most keys) first: with the
-  // sequences' block counts n_0 >= n_1 >= ..., those above n_1 are sequence 0's, the next down to n_2 sequence
-  // 0's and 1's in turn, and so on; first[i] blocks come before those of i + 1 sequences in turn.
+  // the launch's. The blocks of the first `alone` sequences come one sequence after another, the last block (the
+  // most keys) first. The others' go by their number in their sequence, the highest first: with the sequences'
+  // block counts n_0 >= n_1 >= ..., those above n_1 are sequence 0's, the next down to n_2 sequence 0's and 1's in
+  // turn, and so on. first[i] blocks come before sequence i's, or before those of it and the ones in turn with it.
   // The tables are read whole, a lane an entry, and picked from with lane reads: arguments are far away, and
   // one round trip there costs as much as a tile.
   int tf[PSEQ / 64], tl[PSEQ / 64], tr[PSEQ / 64], ts[PSEQ / 64];
@@ -165,7 +168,8 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
 #pragma unroll
   for (int o = 0; o < PSEQ / 64; ++o)
     pi += __popcll(__builtin_amdgcn_ballot_w64(64 * o + lane < a.nseq && tf[o] <= item));
-  const int at = item - pick(tf, pi), turn = at / (pi + 1), si = at - turn * (pi + 1);
+  const int at = item - pick(tf, pi), m = pi < a.alone ? 1 : pi - a.alone + 1;  // sequences in turn
+  const int turn = at / m, si = pi < a.alone ? pi : a.alone + at - turn * m;
   const int qb = (pick(tl, pi) * a.g + PR - 1) / PR - 1 - turn;
   const int len = pick(tl, si), row0 = pick(tr, si), rows = len * a.g;
   const int r0 = qb * PR + 32 * w, r = r0 + col;          // this wave's first row, this lane's row
@@ -216,7 +220,8 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
         sm.bad[wave] = 1;
 #pragma unroll
         for (int n = 0; n < NX; ++n)
-          d.x[n] = make_uint4(finite_or_0(d.x[n].x), finite_or_0(d.x[n].y), finite_or_0(d.x[n].z), finite_or_0(d.x[n].w));
+          d.x[n] = make_uint4(finite_or_0(d.x[n].x), finite_or_0(d.x[n].y), finite_or_0(d.x[n].z),
+                              finite_or_0(d.x[n].w));
       }
     }
     unsigned char* p = tiles.v[i & 1] + srow * PVS + 16 * chunk;
@@ -335,7 +340,8 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
   // O^T += V^T . P^T over keys 32 h .. 32 h + 31 of the tile
   auto output = [&](const f32x16& st, int i, int h) __attribute__((always_inline)) {
     // this lane's places: V row 4 g + l % 16 / 4 at dims 16 (l / 16 % 2) + 4 (l % 4)
-    const unsigned char* vt = tiles.v[i & 1] + (4 * g + ((lane & 15) >> 2)) * PVS + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+    const unsigned char* vt =
+        tiles.v[i & 1] + (4 * g + ((lane & 15) >> 2)) * PVS + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       float pw[8];
@@ -461,6 +467,7 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
 #pragma unroll
     for (int b = 0; b < NB; ++b) out[b] = acc[b];
   }
+  if constexpr (KS > 1) __syncthreads();  // what the groups left is read: its place takes the output rows
   if (r0 >= rows) return;
   int bad = 0;
 #pragma unroll
@@ -483,39 +490,72 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
 
   // the output's columns are queries: 8 dims of one query per lane after a swap between the wave's halves
   const float inv = 1.f / xsum32(lrun);
-  const int64_t m = row0 + tok;
+  auto dims8 = [&](int b, int q, float (&o)[8]) __attribute__((always_inline)) {
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
+    for (int j = 0; j < 4; ++j) {
+      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(out[b][4 * q + j] * inv),
+                                                      __float_as_uint(out[b][4 * q + 4 + j] * inv), false, false);
+      o[j] = __uint_as_float(x[0]);
+      o[4 + j] = __uint_as_float(x[1]);
+    }
+  };
+  if constexpr (PARTS == 2) {  // attn_out's two fragment orders (layers_kernel.hip)
+    const int64_t m = row0 + tok;
 #pragma unroll
-    for (int q = 0; q < 4; q += 2) {
-      float o[8];
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(out[b][4 * q + j] * inv),
-                                                        __float_as_uint(out[b][4 * q + 4 + j] * inv), false, false);
-        o[j] = __uint_as_float(x[0]);
-        o[4 + j] = __uint_as_float(x[1]);
-      }
-      if (r >= rows) continue;
-      const int d = 32 * (b0 + b) + 8 * (q + g);
-      if constexpr (PARTS == 1) {
-        *reinterpret_cast<uint4*>((uint16_t*)a.out + (m * (a.hkv * a.g) + hq) * D + d) =
-            make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]), pack_bf16x2(o[4], o[5]),
-                       pack_bf16x2(o[6], o[7]));
-      } else if constexpr (PARTS == 2) {  // attn_out's two fragment orders (layers_kernel.hip)
+      for (int q = 0; q < 4; q += 2) {
+        float o[8];
+        dims8(b, q, o);
+        if (r >= rows) continue;
         uint4 p[PARTS];
         split_parts<PARTS>(o, p);
-        const int kk = hq * D + d;
+        const int kk = hq * D + 32 * (b0 + b) + 8 * (q + g);
         uint16_t* hi = (uint16_t*)a.out;
         *reinterpret_cast<uint4*>(hi + (a.frag == 2 ? skf_off(m, kk, 0, HQ * D) : frag_off(m, kk, HQ * D))) = p[0];
         *reinterpret_cast<uint4*>(a.frag == 2 ? hi + skf_off(m, kk, 1, HQ * D)
                                               : a.out_lo + frag_off(m, kk, HQ * D)) = p[1];
-      } else {
-        float4* p = reinterpret_cast<float4*>((float*)a.out + (m * (a.hkv * a.g) + hq) * D + d);
-        p[0] = make_float4(o[0], o[1], o[2], o[3]);
-        p[1] = make_float4(o[4], o[5], o[6], o[7]);
       }
+  } else {
+    // Through the wave's own 32 padded rows of LDS, so that a store instruction writes whole lines, BB bytes of
+    // a row at a time, past the L2s: 64 prompts 168 -> 158 us, 3,584 fp32 tokens 151 -> 148 (whole lines into
+    // the L2s 168 and 149, 32 bytes of 32 rows past them 192).
+    constexpr int ES = PARTS == 1 ? 2 : 4, BB = 32 * NB * ES < 256 ? 32 * NB * ES : 256;
+    constexpr int NP = BB / (32 * ES), LR = BB / 16;  // output blocks at a time, lanes to a row
+    static_assert(sizeof(sm.tiles) >= KS * RG * 32 * (BB + 16));
+    unsigned char* ob = reinterpret_cast<unsigned char*>(&sm.tiles) + wave * 32 * (BB + 16);
+#pragma unroll
+    for (int pass = 0; pass < NB / NP; ++pass) {
+#pragma unroll
+      for (int b = 0; b < NP; ++b)
+#pragma unroll
+        for (int q = 0; q < 4; q += 2) {
+          float o[8];
+          dims8(NP * pass + b, q, o);
+          unsigned char* p = ob + col * (BB + 16) + ES * (32 * b + 8 * (q + g));
+          if constexpr (PARTS == 1) {
+            *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]),
+                                                      pack_bf16x2(o[4], o[5]), pack_bf16x2(o[6], o[7]));
+          } else {
+            *reinterpret_cast<float4*>(p) = make_float4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<float4*>(p + 16) = make_float4(o[4], o[5], o[6], o[7]);
+          }
+        }
+      wave_sync();
+#pragma unroll
+      for (int n = 0; n < LR / 2; ++n) {
+        const int orow = 64 / LR * n + lane / LR, ro = r0 + orow;
+        const u32x4 x = *reinterpret_cast<const u32x4*>(ob + orow * (BB + 16) + 16 * (lane % LR));
+        if (ro < rows) {
+          const int t = div(ro, a.by_g);
+          const int64_t at = (int64_t)(row0 + t) * (a.hkv * a.g) + kh * a.g + (ro - t * a.g);
+          unsigned char* p = (unsigned char*)a.out + ES * (at * D + 32 * (b0 + NP * pass)) + 16 * (lane % LR);
+          __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(p));
+        }
+      }
+      wave_sync();
     }
+  }
 }
 
 }  // namespace mkp
@@ -545,10 +585,20 @@ static hipError_t launch_packed(PackedArgs& a, const int32_t* lengths, int num_s
       // the workgroups of blocks of pr rows, and each sequence's place among them
       auto places = [&](int pr) {
         auto count = [&](int i) { return i < n ? ((int64_t)a.len[i] * a.g + pr - 1) / pr : 0; };
-        int64_t blocks = 0;
+        // Blocks of one sequence after another find its keys in the L2s; blocks in turn, the longest first, end
+        // together. So in turn are the last sequences, as many as keep the 512 workgroups that run at once busy
+        // for as long as the longest block before them lasts (in units of the keys of one block). Measured on
+        // MI355X, us with all in turn / so / none in turn: 64 prompts of 64 to 960 tokens 158 / 148 / 148, of 512
+        // 136 / 125 / 132, 24 of 1,024 151 / 145 / 153, 8 of 2,048 162 / 163 / 179 (16 query heads on 8, bf16).
+        int64_t blocks = 0, rest = 0;
+        a.alone = 0;
+        for (int i = n - 1; i > 0 && a.alone == 0 && pr == 128; --i) {
+          rest += count(i) * (count(i) + 1) / 2;
+          if (rest * a.hkv >= 512 * count(i - 1)) a.alone = i;
+        }
         for (int i = 0; i < n; ++i) {
           a.first[i] = (int32_t)blocks;
-          blocks += (count(i) - count(i + 1)) * (i + 1);
+          blocks += i < a.alone ? count(i) : (count(i) - count(i + 1)) * (i - a.alone + 1);
         }
         return dim3((unsigned)(blocks * a.hkv));
       };
@@ -634,5 +684,6 @@ extern "C" hipError_t mk_attention_packed(int q_heads, int kv_heads, const void*
   a.v_head = v_head_stride;
   a.hkv = kv_heads;
   a.g = q_heads / kv_heads;
-  return q_fp32 ? launch_packed<3, 32>(a, lengths, num_seqs, stream) : launch_packed<1, 64>(a, lengths, num_seqs, stream);
+  return q_fp32 ? launch_packed<3, 32>(a, lengths, num_seqs, stream)
+                : launch_packed<1, 64>(a, lengths, num_seqs, stream);
 }
