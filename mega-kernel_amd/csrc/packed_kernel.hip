@@ -126,7 +126,7 @@ struct PackedSmem {
   union {
     Tiles tiles[KS];
     struct {  // the output blocks that a key group leaves to another, the maxima and sums, lane by lane
-      float acc[KS > 1 ? KS : 1][KS > 1 ? RG : 1][KS > 1 ? 64 - 64 / KS : 1][64], m[KS][RG][64], l[KS][RG][64];
+      float acc[KS > 1 ? KS : 1][KS > 1 ? RG : 1][KS > 1 ? 16 - 16 / KS : 1][64][4], m[KS][RG][64], l[KS][RG][64];
     } join;
   };
   int bad[KS * RG];  // per staging wave: an infinity or NaN taken out of a tile's values
@@ -157,6 +157,10 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
     tr[o] = a.row[64 * o + lane];
     ts[o] = PARTS == 2 ? a.seq[64 * o + lane] : 0;
   }
+  asm volatile("" ::"s"(a.q), "s"(a.k), "s"(a.v), "s"(a.q_row), "s"(a.q_head), "s"(a.k_row), "s"(a.k_head),
+               "s"(a.v_row), "s"(a.v_head), "s"(a.by_hkv.d), "s"(a.by_hkv.mul),
+               "s"(a.by_hkv.shift), "s"(a.by_g.mul), "s"(a.by_g.shift), "s"(a.g), "s"(a.nseq),
+               "s"(a.alone));  // the other arguments, all in the same trip
   auto pick = [&](const int (&t)[PSEQ / 64], int n) {
     int v = __builtin_amdgcn_readlane(t[0], n & 63);
 #pragma unroll
@@ -189,20 +193,22 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
   struct Tile {
     uint4 x[NX];
   };
-  auto load = [&](Tile& d, const char* base, int64_t row, int i, bool whole = false) __attribute__((always_inline)) {
-    const int key = tile(i) * PK;
-    const uint32_t rb = 2 * (uint32_t)row;
-    if (whole || key + PK - 1 <= last) {  // the tile's rows as uniform bases, the lane's on them as 32 bits
-      const uint32_t o = srow * rb + 16 * chunk;
+  // Uniform bases, the lane's row on them as 32 bits. No branch, or the compiler waits for what is in flight where
+  // its two sides meet.
+  auto load = [&](Tile& d, const char* base, int64_t row, int i) __attribute__((always_inline)) {
+    const int key = min(tile(i) * PK, last);
+    const uint32_t rb = 2 * (uint32_t)row, o = srow * rb + 16 * chunk;
+    const uint32_t end = min(last - key, PK - 1) * rb + 16 * chunk;
 #pragma unroll
-      for (int n = 0; n < NX; ++n)
-        d.x[n] = ld_global16(reinterpret_cast<const uint4*>(base + (key + 4 * n) * (2 * row) + o));
-    } else {
+    for (int n = 0; n < NX; ++n)
+      d.x[n] = ld_global16(reinterpret_cast<const uint4*>(base + key * (2 * row) + min(o + 4 * n * rb, end)));
+  };
+  // the same where the block has all of the tile's keys
+  auto load_whole = [&](Tile& d, const char* base, int64_t row, int i) __attribute__((always_inline)) {
+    const uint32_t o = srow * (2 * (uint32_t)row) + 16 * chunk;
 #pragma unroll
-      for (int n = 0; n < NX; ++n)
-        d.x[n] = ld_global16(reinterpret_cast<const uint4*>(base + key * (2 * row) +
-                                                            (min(srow + 4 * n, last - key) * rb + 16 * chunk)));
-    }
+    for (int n = 0; n < NX; ++n)
+      d.x[n] = ld_global16(reinterpret_cast<const uint4*>(base + (tile(i) * PK + 4 * n) * (2 * row) + o));
   };
   auto store_k = [&](const Tile& d, int i) __attribute__((always_inline)) {
     unsigned char* p = tiles.k[i & 1] + srow * PKS + 16 * chunk;
@@ -228,38 +234,58 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
 #pragma unroll
     for (int n = 0; n < NX; ++n) *reinterpret_cast<uint4*>(p + 4 * n * PVS) = d.x[n];
   };
+  // The queries: a row's 256 bytes (or 2 times 256) by 16 lanes, and through LDS to the lanes whose B operand they
+  // are. (Read by those directly, 16 bytes of 32 rows to an instruction, their addresses took longer than a tile.)
+  // The key groups of a row group share the reading.
+  constexpr int QP = PARTS == 1 ? 1 : 2;  // 256-byte pieces: hi and lo, or half a row of fp32 each
+  const int qrow = 32 / KS * ks + (lane >> 4);  // among the wave's 32, and 4, 8 .. after it
+  uint4 qx[QP][8 / KS];
+  const int64_t qo = ((int64_t)(row0 + tok) * a.q_row + hq * a.q_head) * (PARTS == 3 ? 4 : 2);  // row `col`, bytes
+#pragma unroll
+  for (int n = 0; n < 8 / KS; ++n) {
+    const int64_t o = (int64_t)((uint64_t)(uint32_t)__shfl((int)(qo >> 32), qrow + 4 * n) << 32 |
+                                (uint32_t)__shfl((int)qo, qrow + 4 * n));
+#pragma unroll
+    for (int p = 0; p < QP; ++p)
+      qx[p][n] = ld_global16(reinterpret_cast<const uint4*>((const char*)(PARTS == 2 && p ? a.ql : a.q) + o +
+                                                            (PARTS == 3 ? 256 * p : 0) + 16 * chunk));
+  }
+  uint4 fq[PARTS][8];  // dims 16 s + 8 g .. +7 of row `col`
   Tile x;  // on the way to LDS: V of the next tile, then K of the one after it
-  if (lane == 0) sm.bad[wave] = 0;
-  if (tile(0) < ntile) {
-    Tile k0, k1, v0;
+  {
+    Tile k0, v0;  // (of a tile that the block does not have: its last key)
     load(k0, kbase, a.k_row, 0);
     load(v0, vbase, a.v_row, 0);
-    if (tile(1) < ntile) {
-      load(k1, kbase, a.k_row, 1);
-      load(x, vbase, a.v_row, 1);
+    if (lane == 0) sm.bad[wave] = 0;
+    unsigned char* qs = reinterpret_cast<unsigned char*>(&sm.tiles);
+    static_assert(sizeof(sm.tiles) >= PR * PKS);
+#pragma unroll
+    for (int p = 0; p < QP; ++p) {
+      if (p) __syncthreads();
+#pragma unroll
+      for (int n = 0; n < 8 / KS; ++n)
+        *reinterpret_cast<uint4*>(qs + (32 * w + qrow + 4 * n) * PKS + 16 * chunk) = qx[p][n];
+      __syncthreads();
+      const unsigned char* row = qs + (32 * w + col) * PKS;
+      if constexpr (PARTS == 3) {
+#pragma unroll
+        for (int s = 4 * p; s < 4 * p + 4; ++s) {
+          const float4 x = *reinterpret_cast<const float4*>(row + 64 * (s & 3) + 32 * g);
+          const float4 y = *reinterpret_cast<const float4*>(row + 64 * (s & 3) + 32 * g + 16);
+          const float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+          uint4 part[PARTS];
+          split_parts<PARTS>(f, part);
+#pragma unroll
+          for (int i = 0; i < PARTS; ++i) fq[i][s] = part[i];
+        }
+      } else {
+#pragma unroll
+        for (int s = 0; s < 8; ++s) fq[p][s] = *reinterpret_cast<const uint4*>(row + 32 * s + 16 * g);
+      }
     }
+    __syncthreads();
     store_k(k0, 0);
     store_v(v0, 0);
-    if (tile(1) < ntile) store_k(k1, 1);
-  }
-
-  // the queries as the B operand: dims 16 s + 8 g .. +7 of row `col`
-  uint4 fq[PARTS][8];
-#pragma unroll
-  for (int s = 0; s < 8; ++s) {
-    const int64_t o = (int64_t)(row0 + tok) * a.q_row + hq * a.q_head + 16 * s + 8 * g;
-    if constexpr (PARTS == 3) {
-      const float4 x = *reinterpret_cast<const float4*>((const float*)a.q + o);
-      const float4 y = *reinterpret_cast<const float4*>((const float*)a.q + o + 4);
-      const float f[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-      uint4 p[PARTS];
-      split_parts<PARTS>(f, p);
-#pragma unroll
-      for (int i = 0; i < PARTS; ++i) fq[i][s] = p[i];
-    } else {
-      fq[0][s] = *reinterpret_cast<const uint4*>((const uint16_t*)a.q + o);
-      if constexpr (PARTS == 2) fq[1][s] = *reinterpret_cast<const uint4*>(a.ql + o);
-    }
   }
 
   f32x16 acc[4];  // dims 32 b + 8 (j / 4) + 4 g + j % 4 of query `col`
@@ -368,18 +394,27 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
   // the step after the one that read it last (tile i + 1's V takes tile i - 1's, tile i + 2's K tile i's), so
   // one barrier a step is enough.
   Scores st, sn;
+  Tile k1;
+  const bool more = tile(1) < ntile;
+  if (more) {
+    load(k1, kbase, a.k_row, 1);
+    load(x, vbase, a.v_row, 1);
+  }
   __syncthreads();
   if (tile(0) * PK <= wlast) {
     scores(st, 0);
     mask(st, 0);
     maximum(st);
+    mrun = mnew;  // what the first tile's rescaling would come to
+    mscaled = mnew == -INFINITY ? 0.f : mnew * C;
   }
+  if (more) store_k(k1, 1);
   __syncthreads();  // tile 0's scores made by every wave: tile 2's K takes its place in the first step
   int i = 0;
   // tiles whose next one the whole block sees, two before the last: no masks, no ends
   auto step = [&](Scores& st, Scores& sn, int i) __attribute__((always_inline)) {
     store_v(x, i + 1, true);
-    load(x, kbase, a.k_row, i + 2, true);
+    load_whole(x, kbase, a.k_row, i + 2);
     rescale();
     scores(sn, i + 1);
 #pragma unroll
@@ -388,7 +423,7 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
     for (int h = 0; h < PH; ++h) output(st[h], i, h);
     maximum(sn);
     store_k(x, i + 2);
-    load(x, vbase, a.v_row, i + 2, true);
+    load_whole(x, vbase, a.v_row, i + 2);
     __syncthreads();
   };
   for (const int nfast = min((first + 1) / (PK * KS) - 1, (last + 1) / (PK * KS) - 2); i + 1 < nfast; i += 2) {
@@ -432,8 +467,10 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
     for (int b = 0; b < 4; ++b) {
       if (b / NB == ks) continue;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) sm.join.acc[ks][w][n + j][lane] = acc[b][j];
-      n += 16;
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<float4*>(sm.join.acc[ks][w][n + j][lane]) =
+            make_float4(acc[b][4 * j], acc[b][4 * j + 1], acc[b][4 * j + 2], acc[b][4 * j + 3]);
+      n += 4;
     }
     const float me = mrun == -INFINITY ? -INFINITY : mscaled;  // the exponents' scale that the sums refer to
     sm.join.m[ks][w][lane] = me;
@@ -457,11 +494,16 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
       if (o == ks) continue;
       const float f = __builtin_amdgcn_exp2f(sm.join.m[o][w][lane] - mc);
       lrun = fmaf(f, sm.join.l[o][w][lane], lrun);
-      const int n = 16 * (b0 - (ks > o ? NB : 0));  // this group's first block among those that group o left
+      const int n = 4 * (b0 - (ks > o ? NB : 0));  // this group's first block among those that group o left
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) out[b][j] = fmaf(f, sm.join.acc[o][w][n + 16 * b + j][lane], out[b][j]);
+        for (int j = 0; j < 4; ++j) {
+          const float4 x = *reinterpret_cast<const float4*>(sm.join.acc[o][w][n + 4 * b + j][lane]);
+          const float t[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) out[b][4 * j + e] = fmaf(f, t[e], out[b][4 * j + e]);
+        }
     }
   } else {
 #pragma unroll
@@ -602,18 +644,20 @@ static hipError_t launch_packed(PackedArgs& a, const int32_t* lengths, int num_s
         }
         return dim3((unsigned)(blocks * a.hkv));
       };
-      // Few rows: 32 to a workgroup and its four waves on different keys, so that the work spreads over the
-      // CUs; up to two workgroups of 128 rows per CU: two key groups of four waves, one workgroup to a CU (the
-      // longest chain decides, and its keys are shared out); else 128 rows and one key group, two workgroups
-      // to a CU. Measured on MI355X (16 query heads on 8), us with 128 rows / 32 rows: bf16 128 tokens
-      // 9.2 / 8.0, 512 (256 workgroups of 32 rows) 15.5 / 14.2, 1,024 (512) 23.5 / 27.2; fp32 128 15.2 / 9.8,
-      // 512 28.5 / 17.9, 1,024 46.1 / 34.9, 2,048 over that. With one / two key groups: 3,584 tokens (448
-      // workgroups of 128 rows) bf16 82.2 / 70.0, fp32 182 / 148, 2,048 bf16 43.2 / 40.2; 200 prompts of 48
-      // (1,600) 36.5 / 56.7.
+      // Few rows: 32 to a workgroup and its four waves on different keys, so that the work spreads over the CUs.
+      // Up to one workgroup of 128 rows per CU, or two where chains are long: two key groups of four waves, one
+      // workgroup to a CU (the longest chain decides, and its keys are shared out). Else 128 rows and one key
+      // group, two workgroups to a CU. Measured on MI355X (16 query heads on 8), us, first with 32 / 128 rows:
+      // bf16 128 tokens 7.4 / 8.4, 640 (320 workgroups of 32 rows) 13.9 / 16.4, 3 prompts of 200 (312) 11.9 /
+      // 10.3, 1,024 (512) 23.7 / 21.7; fp32 128 8.8 / 12.4, 1,024 32.4 / 43.8, 2,048 98 / 80. Then with two / one
+      // key groups: bf16 3 prompts of 600 (240 workgroups of 128 rows) 16.4 / 18.0, 3,584 tokens (448) 67.6 /
+      // 83.3, 4 of 1,024 (512) 30.2 / 29.6, 8 of 512 (512) 21.8 / 18.5, 32 of 128 (512) 17.8 / 11.6; fp32 3,584
+      // 155 / 190, 5 of 768 (480) 48.9 / 50.7, 6 of 600 (480) 42.5 / 40.8, 32 of 128 27.2 / 20.8.
+      const int longest = a.len[0];
       dim3 grid = places(32);
-      if (grid.x <= (PARTS == 1 ? 256 : 512)) {
+      if (grid.x <= (PARTS > 1 ? 512 : longest < 512 ? 256 : 384)) {
         hipLaunchKernelGGL((packed_attention_kernel<PARTS, 32, 1, 4>), grid, dim3(256), 0, stream, a);
-      } else if ((grid = places(128)).x <= 512) {
+      } else if ((grid = places(128)).x <= (longest < (PARTS > 1 ? 768 : 1024) ? 256 : 512)) {
         hipLaunchKernelGGL((packed_attention_kernel<PARTS, PK, 4, 2>), grid, dim3(512), 0, stream, a);
       } else {
         hipLaunchKernelGGL((packed_attention_kernel<PARTS, PK, 4, 1>), grid, dim3(256), 0, stream, a);
