@@ -63,6 +63,30 @@ __device__ __forceinline__ u64 wave_max_key(u64 k) {
   return k;
 }
 
+__device__ __forceinline__ double join64(uint32_t lo, uint32_t hi) {
+  return __builtin_bit_cast(double, (u64)hi << 32 | lo);
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp64(double v) {
+  const u64 u = __builtin_bit_cast(u64, v);
+  return join64(__float_as_uint(dpp<CTRL>(__uint_as_float((uint32_t)u))),
+                __float_as_uint(dpp<CTRL>(__uint_as_float((uint32_t)(u >> 32)))));
+}
+__device__ __forceinline__ double wave_sum64(double v) {
+  v += dpp64<0xB1>(v);
+  v += dpp64<0x4E>(v);
+  v += dpp64<0x141>(v);
+  v += dpp64<0x140>(v);
+  u64 u = __builtin_bit_cast(u64, v);
+  auto lo = __builtin_amdgcn_permlane16_swap((uint32_t)u, (uint32_t)u, false, false);
+  auto hi = __builtin_amdgcn_permlane16_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
+  v = join64(lo[0], hi[0]) + join64(lo[1], hi[1]);
+  u = __builtin_bit_cast(u64, v);
+  lo = __builtin_amdgcn_permlane32_swap((uint32_t)u, (uint32_t)u, false, false);
+  hi = __builtin_amdgcn_permlane32_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
+  return join64(lo[0], hi[0]) + join64(lo[1], hi[1]);
+}
+
 struct BeamArgs {
   const float* logits;  // [rows][row_stride]
   int64_t row_stride;
@@ -188,32 +212,23 @@ __global__ void __launch_bounds__(256) beam_chunk_kernel(const BeamArgs a) {
 
 __global__ void __launch_bounds__(64 * PICK_WAVES) beam_pick_kernel(const BeamArgs a) {
   constexpr int NL = BV_MAX / BC / 64, NK = BEAMS_MAX * BEAMS_MAX / 64;  // chunks, and a group's candidates, per lane
-  __shared__ __attribute__((aligned(16))) uint32_t heads[PICK_WAVES][64 * NL];
+  constexpr int KL = 4;
+  __shared__ __attribute__((aligned(16))) u64 heads[PICK_WAVES][64 * NL];
   __shared__ __attribute__((aligned(16))) u64 near[PICK_WAVES][64 * NK];
   __shared__ u64 least[PICK_WAVES];
-  __shared__ double score[64 * NK];
-  __shared__ int token[64 * NK];  // -1: no candidate
-  __shared__ int failed[BEAMS_MAX];
+  __shared__ double score[64 * NK];  // NaN: no candidate
+  __shared__ int token[64 * NK];
+  __shared__ int state[BEAMS_MAX];  // 1: the row has failed, 2: it had ended
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int W = a.beams, W2 = W * W, first = blockIdx.x * W;
   for (int r = w; r < W; r += PICK_WAVES) {
     const int row = first + r;
     const int64_t s0 = (int64_t)row * a.chunks;
-    const double base = a.scores[row];
-    const bool bad = !(base < INFINITY), ended = a.eos >= 0 && a.finished[row];  // bad: NaN or +infinity
-    if (lane < W) token[r * W + lane] = -1;
-    if (ended) {
-      if (lane == 0) {
-        score[r * W] = base;
-        token[r * W] = a.eos;
-        failed[r] = bad;
-      }
-      continue;
-    }
-    // the chunks' sums and best keys, NL to a lane
+    // what the row needs, in one trip: the chunks' sums and best keys, NL to a lane, and its keys, KL to a lane (of
+    // the few rows that have more, the others below); an ended row has none that mean anything
     float2 st[NL];
-    u64 head[NL];
-    float m = -INFINITY;
+    u64 head[NL], own[KL];
+    const int keys = a.chunks * W;
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
       const int i = 64 * n + lane;
@@ -223,26 +238,39 @@ __global__ void __launch_bounds__(64 * PICK_WAVES) beam_pick_kernel(const BeamAr
         st[n] = a.stat[s0 + i];
         head[n] = a.cand[(s0 + i) * W];
       }
+    }
+#pragma unroll
+    for (int n = 0; n < KL; ++n) own[n] = 64 * n + lane < keys ? a.cand[s0 * W + 64 * n + lane] : 0;
+    const double base = a.scores[row];
+    const bool bad = !(base < INFINITY), ended = a.eos >= 0 && a.finished[row];  // bad: NaN or +infinity
+    if (lane < W) score[r * W + lane] = __builtin_nan("");
+    if (ended) {
+      if (lane == 0) {
+        score[r * W] = base;
+        token[r * W] = a.eos;
+        state[r] = 2 + bad;
+      }
+      continue;
+    }
+    float m = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < NL; ++n) {
       m = fmaxf(m, st[n].x);
-      heads[w][i] = (uint32_t)(head[n] >> 32);
+      heads[w][64 * n + lane] = head[n];
     }
     if (lane == 0) least[w] = 0;
     wave_sync();
-    // The W-th best of the chunks' best keys: none but keys that reach it are among the row's W best. (Of equal
-    // logits the earlier chunk's is the lower token. A failed row's keys may be anything.)
+    // The W-th best of the chunks' best keys: none but keys that reach it are among the row's W best. (No two keys
+    // are the same but those of no logit, 0. A failed row's keys may be anything.)
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
-      const int i = 64 * n + lane;
       if (64 * n >= a.chunks) break;
-      const uint32_t h = heads[w][i];
       int rank = 0;
-      for (int j = 0; j < a.chunks; j += 8) {  // places past the last chunk hold 0
-        const uint4 x = *reinterpret_cast<const uint4*>(&heads[w][j]), y = *reinterpret_cast<const uint4*>(&heads[w][j + 4]);
-        const uint32_t o[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll 2
+      for (int j = 0; j < a.chunks; j += 4)  // places past the last chunk hold 0
 #pragma unroll
-        for (int q = 0; q < 8; ++q) rank += o[q] > h || (o[q] == h && j + q < i);
-      }
-      if (i < a.chunks && rank == W - 1) least[w] = head[n];
+        for (int q = 0; q < 4; ++q) rank += heads[w][j + q] > head[n];
+      if (head[n] != 0 && rank == W - 1) least[w] = head[n];
     }
     // log of the row's sum: the chunks' sums in fp32, joined in 64 bits
     m = wave_max(m);
@@ -251,22 +279,23 @@ __global__ void __launch_bounds__(64 * PICK_WAVES) beam_pick_kernel(const BeamAr
     for (int n = 0; n < NL; ++n)
       sum += st[n].x == -INFINITY ? st[n].y  // 0, or NaN
                                   : st[n].y * __builtin_amdgcn_exp2f((st[n].x - m) * 1.4426950408889634f);
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o);
+    sum = wave_sum64(sum);
     const double lse = (double)m + log(sum);
-    if (lane == 0) failed[r] = bad || sum != sum;
+    if (lane == 0) state[r] = bad || sum != sum;
     wave_sync();
     // the keys that reach it: W at least (if there are as many), W a chunk of W chunks at most
     const u64 low = least[w];
-    const int keys = a.chunks * W;
     int n = 0;
-    for (int e = lane; e - lane < keys; e += 64) {
-      const u64 key = e < keys ? a.cand[s0 * W + e] : 0;
+    auto keep = [&](u64 key) {
       const u64 all = __builtin_amdgcn_ballot_w64(key != 0 && key >= low);
       const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0));
       if (key != 0 && key >= low && at < 64 * NK) near[w][at] = key;
       n += __popcll(all);
-    }
+    };
+#pragma unroll
+    for (int i = 0; i < KL; ++i)
+      if (64 * i < keys) keep(own[i]);
+    for (int e = 64 * KL + lane; e - lane < keys; e += 64) keep(e < keys ? a.cand[s0 * W + e] : 0);
     n = min(n, 64 * NK);
     if (lane < 8 && n + lane < 64 * NK) near[w][n + lane] = 0;
     wave_sync();
@@ -285,39 +314,35 @@ __global__ void __launch_bounds__(64 * PICK_WAVES) beam_pick_kernel(const BeamAr
     wave_sync();  // the next row's keys take the same places
   }
   __syncthreads();
-  bool fail = false;
-  for (int r = 0; r < W; ++r) fail |= failed[r] != 0;
+  const int mine = lane < W ? state[lane] : 0;
+  const u64 over = __builtin_amdgcn_ballot_w64(mine & 2);
+  const bool fail = __builtin_amdgcn_ballot_w64(mine & 1) != 0;
   if (fail) {  // every beam of the group shows it
     if (tid < W) {
       a.tokens[first + tid] = -1;
       a.parents[first + tid] = first + tid;
       a.out_scores[first + tid] = __builtin_nanf("");
-      a.out_finished[first + tid] = a.eos >= 0 ? a.finished[first + tid] : 0;
+      a.out_finished[first + tid] = over >> tid & 1;
     }
     return;
   }
-  // The group's candidates by score, equal ones by row and place: a wave counts for one candidate at a time
-  // how many come before it.
-  double sc[NK];
-#pragma unroll
-  for (int n = 0; n < NK; ++n) {
-    const int e = 64 * n + lane;
-    sc[n] = e < W2 && token[e] >= 0 ? score[e] : __builtin_nan("");  // comes before none
-  }
-#pragma unroll 4
-  for (int c = w; c < W2; c += PICK_WAVES) {
-    const int t = token[c];
-    const double s = score[c];
+  // The group's candidates by score, equal ones by row and place: eight lanes count for one candidate how many
+  // come before it.
+  for (int c0 = 0; c0 < W2; c0 += 64 * PICK_WAVES / 8) {
+    const int c = c0 + tid / 8, cc = min(c, W2 - 1);
+    const double s = score[cc];
     int before = 0;
-#pragma unroll
-    for (int n = 0; n < NK; ++n)
-      if (64 * n < W2) before += __popcll(__builtin_amdgcn_ballot_w64(sc[n] > s || (sc[n] == s && 64 * n + lane < c)));
-    if (t >= 0 && before < W && lane == 0) {
-      const int at = first + before, r = first + c / W;
+#pragma unroll 4
+    for (int e = tid & 7; e < W2; e += 8) before += score[e] > s || (score[e] == s && e < cc);
+    before += __builtin_amdgcn_update_dpp(0, before, 0xB1, 0xf, 0xf, false);
+    before += __builtin_amdgcn_update_dpp(0, before, 0x4E, 0xf, 0xf, false);
+    before += __builtin_amdgcn_update_dpp(0, before, 0x141, 0xf, 0xf, false);
+    if (c < W2 && s == s && before < W && (tid & 7) == 0) {
+      const int at = first + before, r = c / W, t = token[c];
       a.tokens[at] = t;
-      a.parents[at] = r;
+      a.parents[at] = first + r;
       a.out_scores[at] = (float)s;
-      a.out_finished[at] = a.eos >= 0 && (t == a.eos || a.finished[r]);
+      a.out_finished[at] = a.eos >= 0 && (t == a.eos || (over >> r & 1));
     }
   }
 }
