@@ -18,6 +18,9 @@
 //               m = silu(a . Wg^T) * (a . Wu^T)        (gemm, EPI_SILU: gate and up rows in one tile)
 //               x += m . Wd^T                          (gemm, EPI_RESID)
 //   logits of the last row = RMSNorm(x) . E^T, greedy token (lm_head_kernel, fused argmax)
+// Several prompts at once (mk_prefill_batch): their rows one after the other through the same products, a table of
+// positions and caches per row, and the packed attention (packed_kernel.hip) per prompt. 8 prompts of 32 tokens
+// (0.6B) take 2.13 ms, a call each 7.40; 16 of 64 to 664 13.0 and 39.4.
 // When the residual products' tile grid is small (below 192 tiles) they are split over K into
 // partials that the next norm adds in a fixed order; on grids of at most 128 tiles QKV and gate/up
 // are split over K too, into raw sums that qkv_post_kernel / silu_post_kernel finish. The attention

@@ -7,7 +7,8 @@
 //
 // Tiles. The G query heads of a K/V head share its keys, so a sequence's queries of one K/V head are
 // taken as len * G rows, row r = (token r / G, head r % G), whatever G is. A workgroup takes 128
-// consecutive rows, a wave 32 of them, and runs over the keys 64 at a time up to its last token's:
+// consecutive rows (on small grids 32), a wave 32 of them, and runs over the keys 64 or 32 at a time up to its
+// last token's, where that pays with its waves in groups on different keys:
 //   S^T = K . Q^T   (v_mfma_f32_32x32x16_bf16, keys as rows): lane l holds the scores of its one query
 //                   l % 32 against keys 8 (j / 4) + 4 (l / 32) + j % 4, j = 0..15, of each 32-key half,
 //                   so the running maximum takes registers and one lane swap, the sum registers alone;
@@ -15,7 +16,14 @@
 //                   K slots of a 16-key step mean keys {4 g .. 4 g + 3, 8 + 4 g .. +3} (g = l / 32); the
 //                   A operand is V read transposed from LDS (ds_read_b64_tr_b16) in the same order. The
 //                   output's columns are the queries too: rescaling is one factor per lane.
-// K and V tiles are staged through LDS, two deep.
+// K and V tiles are staged through LDS, two deep. 32 rows to a wave rather than 64: the output and the scores of
+// two tiles then stay in the 256 registers of two waves per SIMD (64 rows: 628 us where this takes 372).
+//
+// Bound by the matrix cores and the exponentials beside them on long sequences: 8,192 + 4,096 + 1,801 tokens of 16
+// heads on 8 take 377 us, 948 TFLOP/s of useful products (a library product of 16,384 cubed: 1,351), MFMA busy 46%
+// and VALU issuing 46% of the time; 3,584 fp32 tokens 146 us, 1,080 TFLOP/s with the three products each. By
+// memory and the blocks' first loads on short ones: 64 prompts of 64 to 960 tokens 157 us (2.6 TB/s, 550 TFLOP/s).
+// By latency on few: 32 tokens 6.1 us, most of it the fetch of code and operands by one wave per SIMD.
 //
 // Rounding. Queries and weights are multiplied as PARTS bf16 numbers whose sum they are: 1 for bf16
 // queries (a weight is then off by at most 2^-8 of itself, as the output is by its own rounding), 2 for
