@@ -20,10 +20,10 @@
 // two tiles then stay in the 256 registers of two waves per SIMD (64 rows: 628 us where this takes 372).
 //
 // Bound by the matrix cores and the exponentials beside them on long sequences: 8,192 + 4,096 + 1,801 tokens of 16
-// heads on 8 take 377 us, 948 TFLOP/s of useful products (a library product of 16,384 cubed: 1,351), MFMA busy 46%
-// and VALU issuing 46% of the time; 3,584 fp32 tokens 146 us, 1,080 TFLOP/s with the three products each. By
-// memory and the blocks' first loads on short ones: 64 prompts of 64 to 960 tokens 157 us (2.6 TB/s, 550 TFLOP/s).
-// By latency on few: 32 tokens 6.1 us, most of it the fetch of code and operands by one wave per SIMD.
+// heads on 8 take 362 us, 987 TFLOP/s of useful products (a library product of 16,384 cubed: 1,351), MFMA busy 46%
+// and VALU issuing 46% of the time; 3,584 fp32 tokens 141 us, 1,120 TFLOP/s with the three products each. By
+// memory and the blocks' first loads on short ones: 64 prompts of 64 to 960 tokens 153 us (2.6 TB/s, 567 TFLOP/s).
+// By latency on few: 32 tokens 6.2 us, most of it the fetch of code and operands by one wave per SIMD.
 //
 // Rounding. Queries and weights are multiplied as PARTS bf16 numbers whose sum they are: 1 for bf16
 // queries (a weight is then off by at most 2^-8 of itself, as the output is by its own rounding), 2 for
@@ -299,8 +299,8 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
   f32x16 acc[4];  // dims 32 b + 8 (j / 4) + 4 g + j % 4 of query `col`
 #pragma unroll
   for (int b = 0; b < 4; ++b) acc[b] = f32x16{};
-  // running maximum of the raw scores, the same in the exponents' scale (rounded once: the weights and the
-  // later rescaling refer to one number), this lane's half of the sum
+  // running maximum of the raw scores, the number that the exponents refer to (in their scale), this lane's half of
+  // the sum
   float mrun = -INFINITY, mscaled = 0.f, lrun = 0.f;
   constexpr float C = ATT_SCALE * 1.4426950408889634f;
 
@@ -342,14 +342,19 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
       for (int j = 0; j < 16; ++j) mnew = fmaxf(mnew, st[h][j]);
     mnew = xmax32(mnew);
   };
-  // the output and the sum to that maximum
+  // The output and the sum to a new reference, where the maximum has left the old one 2^8 behind: until then the
+  // weights are up to 2^8 instead of 1, as exact in bf16 and fp32, and the 64 products (which some query of a wave
+  // asks for at most tiles if each new maximum does) are saved: 8,192 + 4,096 + 1,801 tokens 375 -> 362 us, 3,584
+  // fp32 tokens 148 -> 141.
   auto rescale = [&]() __attribute__((always_inline)) {
-    const float mc = mnew == -INFINITY ? 0.f : mnew * C;  // a query that has seen no key of weight so far
-    const float alpha = __builtin_amdgcn_exp2f(mscaled - mc);  // exactly 1 when the maximum holds
+    const float mc = mnew * C;
+    const bool first = mrun == -INFINITY;  // a query that has seen no key of weight so far
+    const float ref = first ? (mnew == -INFINITY ? 0.f : mc) : mc > mscaled + 8.f ? mc : mscaled;
     mrun = mnew;
-    mscaled = mc;
-    lrun *= alpha;
-    if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0) {
+    if (__builtin_amdgcn_ballot_w64(ref != mscaled) != 0) {
+      const float alpha = __builtin_amdgcn_exp2f(mscaled - ref);  // exactly 1 where it holds
+      mscaled = ref;
+      lrun *= alpha;
 #pragma unroll
       for (int b = 0; b < 4; ++b) acc[b] *= alpha;
     }

@@ -126,6 +126,21 @@ def test_one_sharp_key_and_large_scores(kernel, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("step", [0.02, 0.5, -0.02, -0.5], ids=str)
+def test_scores_that_rise_or_fall_along_the_keys(kernel, step, dtype):
+    """A maximum that grows a little with every tile, or by a lot, from very low scores or from high ones; queries
+    of one wave whose maxima move differently."""
+    for lengths in ([150], [1500], [500] * 20):
+        q, k, v = inputs(sum(lengths), 16, 8, dtype, seed=5, scale=0.1)
+        u = torch.zeros(D, device=DEV)
+        u[::4] = 1.0
+        at = torch.cat([torch.arange(n, device=DEV) for n in lengths]).float()
+        k = (k.float() * 0.1 + (step * (at - 300.0)).view(-1, 1, 1) * u).to(torch.bfloat16)
+        q = (q.float() + u * (torch.arange(len(at), device=DEV) % 5 - 1.0).view(-1, 1, 1) / 4).to(dtype)
+        check(kernel, q, k, v, lengths)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
 @pytest.mark.parametrize("lengths", [[200], [40, 130, 64], [700, 500]], ids=str)
 def test_values_that_a_token_may_not_see_do_not_reach_it(kernel, lengths, dtype):
     """Infinities and NaN in some value rows: tokens before them, and other sequences, are as without them;
