@@ -20,8 +20,8 @@
 // two tiles then stay in the 256 registers of two waves per SIMD (64 rows: 628 us where this takes 372).
 //
 // Bound by the matrix cores and the exponentials beside them on long sequences: 8,192 + 4,096 + 1,801 tokens of 16
-// heads on 8 take 362 us, 987 TFLOP/s of useful products (a library product of 16,384 cubed: 1,351), MFMA busy 46%
-// and VALU issuing 46% of the time; 3,584 fp32 tokens 141 us, 1,120 TFLOP/s with the three products each. By
+// heads on 8 take 362 us, 987 TFLOP/s of useful products (a library product of 16,384 cubed: 1,351), MFMA busy 47%
+// and VALU issuing 40% of the time; 3,584 fp32 tokens 141 us, 1,120 TFLOP/s with the three products each. By
 // memory and the blocks' first loads on short ones: 64 prompts of 64 to 960 tokens 153 us (2.6 TB/s, 567 TFLOP/s).
 // By latency on few: 32 tokens 6.2 us, most of it the fetch of code and operands by one wave per SIMD.
 //
