@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
   };
   // The output and the sum to a new reference, where the maximum has left the old one 2^8 behind: until then the
   // weights are up to 2^8 instead of 1, as exact in bf16 and fp32, and the 64 products (which some query of a wave
-  // asks for at most tiles if each new maximum does) are saved: 8,192 + 4,096 + 1,801 tokens 375 -> 362 us, 3,584
+  // asks for in most tiles if each new maximum does) are saved: 8,192 + 4,096 + 1,801 tokens 375 -> 362 us, 3,584
   // fp32 tokens 148 -> 141.
   auto rescale = [&]() __attribute__((always_inline)) {
     const float mc = mnew * C;
