@@ -260,8 +260,9 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
   }
   uint4 fq[PARTS][8];  // dims 16 s + 8 g .. +7 of row `col`
   Tile x;  // on the way to LDS: V of the next tile, then K of the one after it
+  Tile v0;
   {
-    Tile k0, v0;  // (of a tile that the block does not have: its last key)
+    Tile k0;  // (of a tile that the block does not have: its last key)
     load(k0, kbase, a.k_row, 0);
     load(v0, vbase, a.v_row, 0);
     if (lane == 0) sm.bad[wave] = 0;
@@ -293,7 +294,6 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
     }
     __syncthreads();
     store_k(k0, 0);
-    store_v(v0, 0);
   }
 
   f32x16 acc[4];  // dims 32 b + 8 (j / 4) + 4 g + j % 4 of query `col`
@@ -421,6 +421,7 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
     mrun = mnew;  // what the first tile's rescaling would come to
     mscaled = mnew == -INFINITY ? 0.f : mnew * C;
   }
+  store_v(v0, 0);
   if (more) store_k(k1, 1);
   __syncthreads();  // tile 0's scores made by every wave: tile 2's K takes its place in the first step
   int i = 0;
