@@ -23,7 +23,7 @@
 // heads on 8 take 362 us, 987 TFLOP/s of useful products (a library product of 16,384 cubed: 1,351), MFMA busy 47%
 // and VALU issuing 40% of the time; 3,584 fp32 tokens 141 us, 1,120 TFLOP/s with the three products each. By
 // memory and the blocks' first loads on short ones: 64 prompts of 64 to 960 tokens 153 us (2.6 TB/s, 567 TFLOP/s).
-// By latency on few: 32 tokens 6.2 us, most of it the fetch of code and operands by one wave per SIMD.
+// By latency on few: 32 tokens 5.8 us, most of it the fetch of code and operands by one wave per SIMD.
 //
 // Rounding. Queries and weights are multiplied as PARTS bf16 numbers whose sum they are: 1 for bf16
 // queries (a weight is then off by at most 2^-8 of itself, as the output is by its own rounding), 2 for
@@ -134,7 +134,7 @@ struct PackedSmem {
   union {
     Tiles tiles[KS];
     struct {  // the output blocks that a key group leaves to another, the maxima and sums, lane by lane
-      float acc[KS > 1 ? KS : 1][KS > 1 ? RG : 1][KS > 1 ? 16 - 16 / KS : 1][64][4], m[KS][RG][64], l[KS][RG][64];
+      float acc[KS > 1 ? KS : 1][KS > 1 ? RG : 1][KS == 4 ? 16 : 16 - 16 / KS + (KS == 1)][64][4], m[KS][RG][64], l[KS][RG][64];
     } join;
   };
   int bad[KS * RG];  // per staging wave: an infinity or NaN taken out of a tile's values
@@ -170,10 +170,10 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
                "s"(a.by_hkv.shift), "s"(a.by_g.mul), "s"(a.by_g.shift), "s"(a.g), "s"(a.nseq),
                "s"(a.alone));  // the other arguments, all in the same trip
   auto pick = [&](const int (&t)[PSEQ / 64], int n) {
-    int v = __builtin_amdgcn_readlane(t[0], n & 63);
+    int v = t[0];
 #pragma unroll
-    for (int o = 1; o < PSEQ / 64; ++o) v = n >= 64 * o ? __builtin_amdgcn_readlane(t[o], n & 63) : v;
-    return v;
+    for (int o = 1; o < PSEQ / 64; ++o) v = n >= 64 * o ? t[o] : v;
+    return __builtin_amdgcn_readlane(v, n & 63);
   };
   const int kh = mod(blockIdx.x, a.by_hkv), item = div(blockIdx.x, a.by_hkv);
   int pi = -1;
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
   for (int o = 0; o < PSEQ / 64; ++o)
     pi += __popcll(__builtin_amdgcn_ballot_w64(64 * o + lane < a.nseq && tf[o] <= item));
   const int at = item - pick(tf, pi), m = pi < a.alone ? 1 : pi - a.alone + 1;  // sequences in turn
-  const int turn = at / m, si = pi < a.alone ? pi : a.alone + at - turn * m;
+  const int turn = m == 1 ? at : at / m, si = pi < a.alone ? pi : a.alone + at - turn * m;
   const int qb = (pick(tl, pi) * a.g + PR - 1) / PR - 1 - turn;
   const int len = pick(tl, si), row0 = pick(tr, si), rows = len * a.g;
   const int r0 = qb * PR + 32 * w, r = r0 + col;          // this wave's first row, this lane's row
@@ -471,7 +471,8 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
     __syncthreads();
   }
   // Each key group finishes 4 / KS of the four output blocks: it leaves its sums of the others in LDS, and
-  // takes the other groups' of its own.
+  // takes the other groups' of its own. (Of four groups each leaves all: picking its own among the registers is
+  // more code, which a small grid's CUs fetch for the first time: 32 tokens 6.05 -> 5.80 us, 512 in fp32 16.3 -> 15.6.)
   constexpr int NB = 4 / KS;
   const int b0 = NB * ks;
   f32x16 out[NB];
@@ -479,7 +480,7 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
     int n = 0;
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      if (b / NB == ks) continue;
+      if (KS == 2 && b / NB == ks) continue;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         *reinterpret_cast<float4*>(sm.join.acc[ks][w][n + j][lane]) =
@@ -490,25 +491,25 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attentio
     sm.join.m[ks][w][lane] = me;
     sm.join.l[ks][w][lane] = lrun;
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int o = 0; o < KS; ++o)
-        if (o == ks) out[b] = acc[NB * o + b];
+    for (int b = 0; b < NB; ++b) {
+      if constexpr (KS == 2) out[b] = ks ? acc[NB + b] : acc[b];
+      else out[b] = f32x16{};
+    }
     __syncthreads();
     float mc = me;
 #pragma unroll
     for (int o = 0; o < KS; ++o) mc = fmaxf(mc, sm.join.m[o][w][lane]);
     if (mc == -INFINITY) mc = 0.f;
-    const float own = __builtin_amdgcn_exp2f(me - mc);  // 0 for a group that saw no key
+    const float own = KS == 2 ? __builtin_amdgcn_exp2f(me - mc) : 0.f;  // 0 for a group that saw no key
     lrun *= own;
 #pragma unroll
     for (int b = 0; b < NB; ++b) out[b] *= own;
 #pragma unroll
     for (int o = 0; o < KS; ++o) {
-      if (o == ks) continue;
+      if (KS == 2 && o == ks) continue;
       const float f = __builtin_amdgcn_exp2f(sm.join.m[o][w][lane] - mc);
       lrun = fmaf(f, sm.join.l[o][w][lane], lrun);
-      const int n = 4 * (b0 - (ks > o ? NB : 0));  // this group's first block among those that group o left
+      const int n = 4 * (b0 - (KS == 2 && ks > o ? NB : 0));  // this group's first block among those that group o left
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
