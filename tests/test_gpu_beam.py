@@ -67,6 +67,17 @@ def test_vocabularies_and_beams(kernel, vocab, groups, beams):
     check(kernel, logits, scores, finished, beams, eos=vocab // 2)
 
 
+@pytest.mark.parametrize("groups,beams", [(2, 3), (1, 16)])
+@pytest.mark.parametrize("vocab", [600001, 1 << 20])
+def test_largest_vocabularies(kernel, vocab, groups, beams):
+    """More chunks of a row than a wave has lanes, and more keys of them than its lanes read at once."""
+    logits, scores, finished = inputs(groups * beams, vocab, seed=beams, done=1)
+    check(kernel, logits, scores, finished, beams, eos=vocab - 1)
+    logits[:] = 0.5  # all equal: the lowest tokens
+    logits[:, vocab - 7:] = 2.0
+    check(kernel, logits, scores, finished, beams, eos=3)
+
+
 def test_first_step_from_one_live_beam(kernel):
     """Only the first beam of a group is live at the start: the others' scores are -infinity."""
     logits, scores, finished = inputs(8, 5000, seed=3)
