@@ -7,7 +7,7 @@
 //
 // Tiles. The G query heads of a K/V head share its keys, so a sequence's queries of one K/V head are
 // taken as len * G rows, row r = (token r / G, head r % G), whatever G is. A workgroup takes 128
-// consecutive rows (on small grids 32), a wave 32 of them, and runs over the keys 64 or 32 at a time up to its
+// consecutive rows (on small grids 64 or 32), a wave 32 of them, and runs over the keys 64 or 32 at a time up to its
 // last token's, where that pays with its waves in groups on different keys:
 //   S^T = K . Q^T   (v_mfma_f32_32x32x16_bf16, keys as rows): lane l holds the scores of its one query
 //                   l % 32 against keys 8 (j / 4) + 4 (l / 32) + j % 4, j = 0..15, of each 32-key half,
@@ -134,7 +134,8 @@ struct PackedSmem {
   union {
     Tiles tiles[KS];
     struct {  // the output blocks that a key group leaves to another, the maxima and sums, lane by lane
-      float acc[KS > 1 ? KS : 1][KS > 1 ? RG : 1][KS == 4 ? 16 : 16 - 16 / KS + (KS == 1)][64][4], m[KS][RG][64], l[KS][RG][64];
+      float acc[KS > 1 ? KS : 1][KS > 1 ? RG : 1][KS == 4 ? 16 : 16 - 16 / KS + (KS == 1)][64][4];
+      float m[KS][RG][64], l[KS][RG][64];
     } join;
   };
   int bad[KS * RG];  // per staging wave: an infinity or NaN taken out of a tile's values
@@ -142,7 +143,7 @@ struct PackedSmem {
 
 // PK: keys per tile; RG: waves on different rows, 32 each; KS: groups of RG waves on different tiles
 template <int PARTS, int PK, int RG, int KS>
-__global__ void __launch_bounds__(64 * RG * KS, RG == 4 ? 2 : 1) packed_attention_kernel(const PackedArgs a) {
+__global__ void __launch_bounds__(64 * RG * KS, RG == 1 ? 1 : 2) packed_attention_kernel(const PackedArgs a) {
   constexpr int PR = 32 * RG;                      // rows per workgroup
   constexpr int PH = PK / 32, NX = PK / (4 * RG);  // 32-key halves of a tile, chunks of K that a lane stages
   __shared__ __attribute__((aligned(16))) PackedSmem<PK, RG, KS> sm;
@@ -659,19 +660,24 @@ static hipError_t launch_packed(PackedArgs& a, const int32_t* lengths, int num_s
         }
         return dim3((unsigned)(blocks * a.hkv));
       };
-      // Few rows: 32 to a workgroup and its four waves on different keys, so that the work spreads over the CUs.
-      // Up to one workgroup of 128 rows per CU, or two where chains are long: two key groups of four waves, one
-      // workgroup to a CU (the longest chain decides, and its keys are shared out). Else 128 rows and one key
-      // group, two workgroups to a CU. Measured on MI355X (16 query heads on 8), us, first with 32 / 128 rows:
-      // bf16 128 tokens 7.4 / 8.4, 640 (320 workgroups of 32 rows) 13.9 / 16.4, 3 prompts of 200 (312) 11.9 /
-      // 10.3, 1,024 (512) 23.7 / 21.7; fp32 128 8.8 / 12.4, 1,024 32.4 / 43.8, 2,048 98 / 80. Then with two / one
-      // key groups: bf16 3 prompts of 600 (240 workgroups of 128 rows) 16.4 / 18.0, 3,584 tokens (448) 67.6 /
-      // 83.3, 4 of 1,024 (512) 30.2 / 29.6, 8 of 512 (512) 21.8 / 18.5, 32 of 128 (512) 17.8 / 11.6; fp32 3,584
-      // 155 / 190, 5 of 768 (480) 48.9 / 50.7, 6 of 600 (480) 42.5 / 40.8, 32 of 128 27.2 / 20.8.
+      // A causal grid lasts as long as its longest chain of keys, so where it leaves CUs idle the chains are shared
+      // out among more waves: 32 rows to a workgroup and four key groups of one wave; 64 rows and four groups of
+      // two, where one workgroup a CU takes all, or two in turn and chains are long; 128 rows and two groups of
+      // four likewise; else 128 rows and one group, two workgroups to a CU. Measured on MI355X (16 query heads on
+      // 8), us. With 32 / 64 rows: bf16 256 tokens (128 workgroups of 32 rows) 9.0 / -, 400 (200) 11.6 / 10.5;
+      // fp32 700 (352) 19.4 / 22.2, 800 (400) 23.7 / 24.0, 8 prompts of 100 (448) 15.0 / 11.2. With 64 rows / 128
+      // and two groups: bf16 800 tokens (200 workgroups of 64 rows) 13.9 / 18.3, 1,500 (376) 21.5 / 28.2, 2,048
+      // (512) 31.4 / 35.0, 2,500 (632) 48.5 / 43.5, 700 + 200 + 100 (264) 13.0 / 17.0, 3 of 600 (456) 16.8 / 16.0,
+      // 8 of 256 (512) 13.8 / 11.0; fp32 1,500 38.5 / 56.8, 2,048 60 / 75, 5 of 300 (400) 21.0 / 18.9. With two /
+      // one key groups of 128 rows: bf16 3,584 tokens (448 workgroups) 67.6 / 83.3, 4 of 1,024 (512) 30.2 / 29.6, 8
+      // of 512 (512) 21.8 / 18.5, 32 of 128 (512) 17.8 / 11.6; fp32 3,584 155 / 190, 5 of 768 (480) 48.9 / 50.7, 6
+      // of 600 (480) 42.5 / 40.8, 32 of 128 27.2 / 20.8.
       const int longest = a.len[0];
       dim3 grid = places(32);
-      if (grid.x <= (PARTS > 1 ? 512 : longest < 512 ? 256 : 384)) {
+      if (grid.x <= (PARTS > 1 ? 384 : 160)) {
         hipLaunchKernelGGL((packed_attention_kernel<PARTS, 32, 1, 4>), grid, dim3(256), 0, stream, a);
+      } else if ((grid = places(64)).x <= (longest < 640 ? 256 : 512)) {
+        hipLaunchKernelGGL((packed_attention_kernel<PARTS, 32, 2, 4>), grid, dim3(512), 0, stream, a);
       } else if ((grid = places(128)).x <= (longest < (PARTS > 1 ? 768 : 1024) ? 256 : 512)) {
         hipLaunchKernelGGL((packed_attention_kernel<PARTS, PK, 4, 2>), grid, dim3(512), 0, stream, a);
       } else {
