@@ -662,23 +662,27 @@ static hipError_t launch_packed(PackedArgs& a, const int32_t* lengths, int num_s
       };
       // A causal grid lasts as long as its longest chain of keys, so where it leaves CUs idle the chains are shared
       // out among more waves: 32 rows to a workgroup and four key groups of one wave; 64 rows and four groups of
-      // two, where one workgroup a CU takes all, or two in turn and chains are long; 128 rows and two groups of
-      // four likewise; else 128 rows and one group, two workgroups to a CU. Measured on MI355X (16 query heads on
+      // two, where one workgroup a CU takes all, or two in turn and chains are long; 64 rows and two groups, two
+      // workgroups to a CU; 128 rows and two groups of four, two in turn on long chains; else 128 rows and one
+      // group, two workgroups to a CU. Measured on MI355X (16 query heads on
       // 8), us. With 32 / 64 rows: bf16 256 tokens (128 workgroups of 32 rows) 9.0 / -, 400 (200) 11.6 / 10.5;
       // fp32 700 (352) 19.4 / 22.2, 800 (400) 23.7 / 24.0, 8 prompts of 100 (448) 15.0 / 11.2. With 64 rows / 128
       // and two groups: bf16 800 tokens (200 workgroups of 64 rows) 13.9 / 18.3, 1,500 (376) 21.5 / 28.2, 2,048
-      // (512) 31.4 / 35.0, 2,500 (632) 48.5 / 43.5, 700 + 200 + 100 (264) 13.0 / 17.0, 3 of 600 (456) 16.8 / 16.0,
-      // 8 of 256 (512) 13.8 / 11.0; fp32 1,500 38.5 / 56.8, 2,048 60 / 75, 5 of 300 (400) 21.0 / 18.9. With two /
-      // one key groups of 128 rows: bf16 3,584 tokens (448 workgroups) 67.6 / 83.3, 4 of 1,024 (512) 30.2 / 29.6, 8
-      // of 512 (512) 21.8 / 18.5, 32 of 128 (512) 17.8 / 11.6; fp32 3,584 155 / 190, 5 of 768 (480) 48.9 / 50.7, 6
-      // of 600 (480) 42.5 / 40.8, 32 of 128 27.2 / 20.8.
+      // (512) 31.4 / 35.0, 2,500 (632) 48.5 / 43.5, 700 + 200 + 100 (264) 13.0 / 17.0; fp32 1,500 38.5 / 56.8, 2,048
+      // 60 / 75. With 64 rows and four / two groups / 128 rows and two: bf16 3 of 600 (456) 16.8 / 14.4 / 15.8, 8 of
+      // 256 (512) 13.8 / 9.7 / 10.8, 6 of 600 (912) 31 / 22.5 / 19.5 (one group); fp32 5 of 300 (400) 21.0 / 17.0 /
+      // 18.8. With two / one key groups of 128 rows: bf16 3,584 tokens (448 workgroups) 67.6 / 83.3, 4 of 1,024
+      // (512) 30.2 / 29.6, 8 of 512 (512) 21.8 / 18.5, 32 of 128 (512) 17.8 / 11.6; fp32 3,584 155 / 190, 5 of 768
+      // (480) 48.9 / 50.7, 6 of 600 (480) 42.5 / 40.8, 32 of 128 27.2 / 20.8.
       const int longest = a.len[0];
       dim3 grid = places(32);
       if (grid.x <= (PARTS > 1 ? 384 : 160)) {
         hipLaunchKernelGGL((packed_attention_kernel<PARTS, 32, 1, 4>), grid, dim3(256), 0, stream, a);
       } else if ((grid = places(64)).x <= (longest < 640 ? 256 : 512)) {
         hipLaunchKernelGGL((packed_attention_kernel<PARTS, 32, 2, 4>), grid, dim3(512), 0, stream, a);
-      } else if ((grid = places(128)).x <= (longest < (PARTS > 1 ? 768 : 1024) ? 256 : 512)) {
+      } else if (grid.x <= 512) {
+        hipLaunchKernelGGL((packed_attention_kernel<PARTS, 32, 2, 2>), grid, dim3(256), 0, stream, a);
+      } else if ((grid = places(128)).x <= 512 && longest >= (PARTS > 1 ? 768 : 1024)) {
         hipLaunchKernelGGL((packed_attention_kernel<PARTS, PK, 4, 2>), grid, dim3(512), 0, stream, a);
       } else {
         hipLaunchKernelGGL((packed_attention_kernel<PARTS, PK, 4, 1>), grid, dim3(256), 0, stream, a);

@@ -76,11 +76,11 @@ def test_head_layouts(kernel, heads, dtype):
 @pytest.mark.parametrize("lengths", [[2048], [3000, 17], [900] * 5, [1 + 13 * i for i in range(60)],
                                      [3 + i % 61 for i in range(150)], [40] * 300, [301] * 40,
                                      [1900] + [64 + 9 * i for i in range(50)] + [5] * 70,
-                                     [450], [800, 3, 64, 65], [1500], [1000, 700], [300] * 5],
+                                     [450], [800, 3, 64, 65], [1500], [1000, 700], [300] * 5, [600, 599, 601]],
                          ids=lambda v: f"{len(v)}x{v[0]}")
 def test_every_split_of_the_work(kernel, lengths, dtype):
-    """32 rows to a workgroup (the lengths above), 64 (up to 512 workgroups of those), 128 and two key groups, one,
-    with all blocks in turn and with the first sequences' one after another, and more sequences than one launch
+    """32 rows to a workgroup (the lengths above), 64 (up to 512 workgroups of those) and four key groups or two,
+    128 and two or one, with all blocks in turn and with the first sequences' one after another, and more sequences than one launch
     takes."""
     check(kernel, *inputs(sum(lengths), 16, 8, dtype, seed=7), lengths)
 
