@@ -80,8 +80,8 @@ def test_head_layouts(kernel, heads, dtype):
                          ids=lambda v: f"{len(v)}x{v[0]}")
 def test_every_split_of_the_work(kernel, lengths, dtype):
     """32 rows to a workgroup (the lengths above), 64 (up to 512 workgroups of those) and four key groups or two,
-    128 and two or one, with all blocks in turn and with the first sequences' one after another, and more sequences than one launch
-    takes."""
+    128 and two or one, with all blocks in turn and with the first sequences' one after another, and more sequences
+    than one launch takes."""
     check(kernel, *inputs(sum(lengths), 16, 8, dtype, seed=7), lengths)
 
 
