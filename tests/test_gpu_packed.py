@@ -144,7 +144,8 @@ def test_scores_that_rise_or_fall_along_the_keys(kernel, step, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
-@pytest.mark.parametrize("lengths", [[200], [40, 130, 64], [700, 500]], ids=str)
+@pytest.mark.parametrize("lengths", [[200], [40, 130, 64], [700, 500], [300] * 5, [700] * 8, [1300, 1250, 900],
+                                     [250] * 30], ids=lambda v: f"{len(v)}x{v[0]}")
 def test_values_that_a_token_may_not_see_do_not_reach_it(kernel, lengths, dtype):
     """Infinities and NaN in some value rows: tokens before them, and other sequences, are as without them;
     tokens from them on get the infinity or NaN that the formula gives, in those dimensions alone."""
