@@ -33,6 +33,8 @@
 // over for infinities and NaN, and where it has any they are added outside the matrix product to the
 // queries that see them (0 times infinity would reach the others). Where weights are multiplied by parts,
 // every tile is (a part may be 0 or negative where the weight is not).
+// Keys stay as they are: an infinite one may give such queries a NaN where the formula has an infinity. The sum shows
+// it, and the row is made again from whole queries (fp32 and hi/lo queries alone; nothing of it is in the loop).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -527,6 +529,62 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 1 ? 1 : 2) packed_attentio
   }
   if constexpr (KS > 1) __syncthreads();  // what the groups left is read: its place takes the output rows
   if (r0 >= rows) return;
+  float sum = xsum32(lrun);
+  if constexpr (PARTS > 1) {
+    // A query's part may be 0, or of the other sign, where the query is not (or an infinity, for one beyond bf16's
+    // range), so on an infinite key component the parts' products are NaN where the query's is an infinity. Such a
+    // score has made its row's sum NaN: these rows are made again from whole queries, key after key in fp32.
+    const bool again = sum != sum;
+    if (__builtin_amdgcn_ballot_w64(again) != 0) {
+      int c = col;
+      asm volatile("" : "+v"(c));  // the query's place found again: kept, it would take registers of the loop above
+      const int rq = min(r0 + c, rows - 1), tq = div(rq, a.by_g);
+      const int64_t qo = ((int64_t)(row0 + tq) * a.q_row + (kh * a.g + (rq - tq * a.g)) * a.q_head) * (PARTS == 3 ? 4 : 2);
+      float m = -INFINITY, l = 0.f;
+      if (again)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) out[b] = f32x16{};
+#pragma unroll 1
+      for (int key = 0; key <= wlast; ++key) {
+        float dot[8] = {};  // by the lane's 64 dims of query and key, the other half's beside them
+#pragma unroll 1
+        for (int s = 0; s < 8; ++s) {
+          const char* qp = (const char*)a.q + qo + (PARTS == 3 ? 64 : 32) * s + (PARTS == 3 ? 32 : 16) * g;
+          const uint4 x = *reinterpret_cast<const uint4*>(qp);
+          const uint4 y = *reinterpret_cast<const uint4*>(PARTS == 3 ? qp + 16 : (const char*)a.ql + (qp - (const char*)a.q));
+          const uint4 k = *reinterpret_cast<const uint4*>(kbase + key * (2 * a.k_row) + 32 * s + 16 * g);
+          const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w}, kw[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float qe;
+            if constexpr (PARTS == 3) qe = __uint_as_float(e < 4 ? xw[e] : yw[e - 4]);
+            else qe = (e & 1 ? bf16_hi(xw[e / 2]) : bf16_lo(xw[e / 2])) + (e & 1 ? bf16_hi(yw[e / 2]) : bf16_lo(yw[e / 2]));
+            dot[e] = fmaf(qe, e & 1 ? bf16_hi(kw[e / 2]) : bf16_lo(kw[e / 2]), dot[e]);
+          }
+        }
+        const float score =
+            xsum32(((dot[0] + dot[1]) + (dot[2] + dot[3])) + ((dot[4] + dot[5]) + (dot[6] + dot[7]))) * C;
+        const bool seen = again && key <= tok;
+        const float mn = seen ? fmaxf(m, score) : m, ref = mn == -INFINITY ? 0.f : mn;
+        const float alpha = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - ref);
+        const float wt = seen ? __builtin_amdgcn_exp2f(score - ref) : 0.f;
+        m = mn;
+        l = fmaf(l, alpha, wt);
+        const char* vr = vbase + key * (2 * a.v_row) + 64 * b0 + 8 * g;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint2 v = *reinterpret_cast<const uint2*>(vr + 64 * b + 16 * q);
+            const uint32_t f[2] = {finite_or_0(v.x), finite_or_0(v.y)};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              out[b][4 * q + j] = fmaf(wt, j & 1 ? bf16_hi(f[j / 2]) : bf16_lo(f[j / 2]), out[b][4 * q + j] * alpha);
+          }
+      }
+      if (again) sum = l;
+    }
+  }
   int bad = 0;
 #pragma unroll
   for (int n = 0; n < KS * RG; ++n) bad |= sm.bad[n];
@@ -547,7 +605,7 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 1 ? 1 : 2) packed_attentio
   }
 
   // the output's columns are queries: 8 dims of one query per lane after a swap between the wave's halves
-  const float inv = 1.f / xsum32(lrun);
+  const float inv = 1.f / sum;
   auto dims8 = [&](int b, int q, float (&o)[8]) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {

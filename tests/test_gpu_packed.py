@@ -224,3 +224,105 @@ def test_on_another_stream_and_in_a_graph(kernel):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(held, eager)
+
+
+SPLITS = [[200], [40, 130, 64], [700, 500], [300] * 5, [700] * 8, [1300, 1250, 900], [250] * 30]
+
+
+def keys_with_infinities(lengths, dtype, seed):
+    """Inputs whose dimension 7 is positive in every query; some keys (never a sequence's first) hold -infinity
+    there, which leaves them no weight, and one sequence's last holds +infinity: NaN for the row that sees it."""
+    n = sum(lengths)
+    q, k, v = inputs(n, 6, 2, dtype, seed=seed)
+    q[:, :, 7] = q[:, :, 7].abs() + 0.25
+    starts = [sum(lengths[:i]) for i in range(len(lengths))]
+    for j, (at, length) in enumerate(zip(starts, lengths)):
+        for t in (1 + j % 3, length // 3, length // 2, length - 2):
+            k[at + t, j % 2, 7] = -math.inf
+    k[starts[-1] + lengths[-1] - 1, 1, 7] = math.inf
+    return q, k, v
+
+
+def check_where_finite(got, want, limit):
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    fine = ~torch.isnan(want)
+    err = (got.double() - want)[fine].abs().max().item()
+    assert err <= limit, err
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("lengths", SPLITS, ids=lambda v: f"{len(v)}x{v[0]}")
+def test_infinite_keys(kernel, lengths, dtype):
+    """A score of -infinity has no weight, one of +infinity or NaN (a query's 0 on an infinite key) makes its row
+    NaN, and no other row knows of it."""
+    q, k, v = keys_with_infinities(lengths, dtype, seed=21)
+    q[lengths[0] - 1, 0, 7] = 0.0  # a row that meets infinite keys with a 0
+    print(f"[packed] {dtype} infinite keys, lengths {lengths[:12]}", flush=True)
+    got = kernel.attention_packed(q, k, v, lengths)
+    limit = bound(q, k.masked_fill(torch.isinf(k), 0), v, dtype)
+    want = reference(q, k, v, lengths)
+    assert torch.isnan(want[lengths[0] - 1, 0]).all() and torch.isnan(want[-1, 3:]).all()
+    check_where_finite(got, want, limit)
+
+
+def test_fp32_queries_up_to_the_largest_number(kernel):
+    """fp32 holds numbers above bf16's largest, which a first bf16 part cannot: the formula's scores are ordinary,
+    on keys as small as bf16's."""
+    lengths = [90, 300]
+    q, k, v = inputs(390, 4, 2, torch.float32, seed=22)
+    q[::3, :, 9] = 3.4e38
+    q[1::3, 1, 9] = -3.402e38
+    k[:, :, 9] = (k[:, :, 9].sign() * 2.0 ** -126).to(torch.bfloat16)
+    got = kernel.attention_packed(q, k, v, lengths)
+    assert (got.double() - reference(q, k, v, lengths)).abs().max().item() <= bound(q, k, v, torch.float32)
+
+
+def fragments(rows, cols, hi, lo):
+    """A bf16 hi/lo pair of matrices out of 16 x 32 blocks of 1 KB: lane m % 16 + 16 (k % 32 / 8) of a block holds 8
+    consecutive columns."""
+    m, c = torch.arange(rows, device=DEV)[:, None], torch.arange(cols, device=DEV)[None]
+    at = (((m // 16) * (cols // 32) + c // 32) * 64 + (c // 8 % 4) * 16 + m % 16) * 8 + c % 8
+    return hi[at].double() + lo[at].double()
+
+
+@pytest.mark.parametrize("lengths", SPLITS, ids=lambda v: f"{len(v)}x{v[0]}")
+def test_infinite_keys_for_the_prefills_queries(lengths):
+    """The form that prefill_batch runs (bf16 hi/lo queries over the caches, by the library's internal entry). Weights
+    and output are held as two bf16 numbers, off by 2^-16 of the largest |v| together; the scores' fp32 sums of 16
+    products are off by at most 2^-20 of sum |q k| / sqrt(128), the output by twice that times the largest |v|."""
+    import ctypes
+    from megakernel import build as mkbuild
+
+    class Prefill(ctypes.Structure):
+        _fields_ = [(n, ctypes.c_void_p) for n in ("qh", "ql", "k_cache", "v_cache", "oh", "ol")] + [
+            ("frag", ctypes.c_int), ("layer", ctypes.c_int), ("max_seq", ctypes.c_int), ("seq_stride", ctypes.c_int64),
+            ("lengths", ctypes.c_void_p), ("num_seqs", ctypes.c_int)]
+
+    n, hq, hkv, T = sum(lengths), 16, 8, max(lengths)
+    q, k, v = inputs(n, hq, hkv, torch.float32, seed=23)
+    q[:, :, 7] = q[:, :, 7].abs() + 0.25
+    qh = q.to(torch.bfloat16)
+    ql = (q - qh.float()).to(torch.bfloat16)
+    caches = torch.full((2, len(lengths), hkv, T, D), math.nan, dtype=torch.bfloat16, device=DEV)
+    at = 0
+    for i, length in enumerate(lengths):
+        for t in (1 + i % 3, length // 3, length // 2, length - 2):
+            k[at + t, i % 8, 7] = -math.inf
+        for dst, src in zip(caches, (k, v)):
+            dst[i, :, :length] = src[at:at + length].transpose(0, 1)
+        at += length
+    oh, ol = (torch.zeros((n + 15) // 16 * 16 * hq * D, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    host = (ctypes.c_int32 * len(lengths))(*lengths)
+    call = Prefill(qh.data_ptr(), ql.data_ptr(), caches[0].data_ptr(), caches[1].data_ptr(), oh.data_ptr(), ol.data_ptr(),
+                   1, 0, T, hkv * T * D, ctypes.addressof(host), len(lengths))
+    lib = ctypes.CDLL(mkbuild.LIB)
+    run = lib["_Z21mkp_attention_prefillRK15MkPackedPrefillP12ihipStream_t"]
+    run.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+    print(f"[packed] hi/lo infinite keys, lengths {lengths[:12]}", flush=True)
+    assert run(ctypes.addressof(call), torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    want = reference(qh.float() + ql.float(), k, v, lengths)
+    finite = k.masked_fill(torch.isinf(k), 0)
+    smax = (q.double().abs().amax((0, 1)) * finite.double().abs().amax((0, 1))).sum().item() / math.sqrt(D)
+    limit = (2 * 2.0 ** -20 * smax + 2 * 2.0 ** -16) * v.float().abs().max().item()
+    check_where_finite(fragments(n, hq * D, oh, ol).view(n, hq, D), want, limit)
