@@ -355,7 +355,9 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 1 ? 1 : 2) packed_attentio
     const float ref = first ? (mnew == -INFINITY ? 0.f : mc) : mc > mscaled + 8.f ? mc : mscaled;
     mrun = mnew;
     if (__builtin_amdgcn_ballot_w64(ref != mscaled) != 0) {
-      const float alpha = __builtin_amdgcn_exp2f(mscaled - ref);  // exactly 1 where it holds
+      // exactly 1 where the reference holds; of what has no weight so far (and a first maximum far below 0 would
+      // make of 0 times infinity) too
+      const float alpha = first ? 1.f : __builtin_amdgcn_exp2f(mscaled - ref);
       mscaled = ref;
       lrun *= alpha;
 #pragma unroll

@@ -326,3 +326,23 @@ def test_infinite_keys_for_the_prefills_queries(lengths):
     smax = (q.double().abs().amax((0, 1)) * finite.double().abs().amax((0, 1))).sum().item() / math.sqrt(D)
     limit = (2 * 2.0 ** -20 * smax + 2 * 2.0 ** -16) * v.float().abs().max().item()
     check_where_finite(fragments(n, hq * D, oh, ol).view(n, hq, D), want, limit)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("lengths", SPLITS, ids=lambda v: f"{len(v)}x{v[0]}")
+def test_very_low_scores_behind_keys_without_weight(kernel, lengths, dtype):
+    """Every sequence begins with keys of score -infinity, up to more than a tile of them, and goes on with scores
+    around -150: the first finite maximum is far below 0. (fp32 queries: one term makes most of a score, and each of
+    the up to 24 products added to it rounds at its size: 6 times the bound's 2^-22.)"""
+    n = sum(lengths)
+    q, k, v = inputs(n, 6, 2, dtype, seed=24, scale=0.1)
+    q[:, :, 7], q[:, :, 8] = 1.0, 40.0
+    k[:, :, 8] = -42.0
+    at = 0
+    for j, length in enumerate(lengths):
+        k[at:at + min(1 + 47 * (j % 4), length - 1) if j else at + 130, :, 7] = -math.inf
+        at += length
+    print(f"[packed] {dtype} low scores, lengths {lengths[:12]}", flush=True)
+    got = kernel.attention_packed(q, k, v, lengths)
+    limit = (6 if dtype == torch.float32 else 1) * bound(q, k.masked_fill(torch.isinf(k), 0), v, dtype)
+    check_where_finite(got, reference(q, k, v, lengths), limit)
