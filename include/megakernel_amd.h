@@ -232,7 +232,8 @@ hipError_t mk_decode_batch(const mk_model_dims* dims, int batch, const int32_t* 
  *   out      q's type, [rows][q_heads][128], written for the rows of the sequences alone
  * All pointers 16-byte aligned. bf16 queries: products of bf16 operands (the softmax's weights rounded
  * to bf16 for the product with v), everything else fp32. fp32 queries: products at fp32 accuracy. A value
- * row that a token may not see does not reach it, whatever it holds. Asynchronous on `stream`, no
+ * row that a token may not see does not reach it, whatever it holds; an infinite or NaN value that it sees does,
+ * however small the weight; a row whose scores are all -infinity is NaN. Asynchronous on `stream`, no
  * workspace, results independent of what else is in the batch. Argument errors (also more than 2^31 - 256
  * (row, head) pairs) return hipErrorInvalidValue before any launch. No reference counterpart: the
  * reference's attention takes one token's queries (/root/reference/megakernel.cu:228-370).

@@ -30,9 +30,10 @@
 // the prefill's hi/lo pairs (2^-16), 3 for fp32 queries (2^-24). Scores, maximum, sum and output are fp32.
 //
 // A masked key weighs nothing, whatever its value row holds: a tile that some query sees in part is looked
-// over for infinities and NaN, and where it has any they are added outside the matrix product to the
-// queries that see them (0 times infinity would reach the others). Where weights are multiplied by parts,
-// every tile is (a part may be 0 or negative where the weight is not).
+// over for infinities and NaN, and where it has any they are left out of the matrix product (0 times infinity would
+// reach the others). Where weights are multiplied by parts, every tile is (a part may be 0 or negative where the
+// weight is not). Behind the loop a block that left some out, or whose outputs are not finite, looks for those that
+// each query sees: they are its output, also where fp32 holds their weight as 0.
 // Keys stay as they are: an infinite one may give such queries a NaN where the formula has an infinity. The sum shows
 // it, and the row is made again from whole queries (fp32 and hi/lo queries alone; nothing of it is in the loop).
 #include <hip/hip_runtime.h>
@@ -587,12 +588,26 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 1 ? 1 : 2) packed_attentio
       if (again) sum = l;
     }
   }
+  // Infinite and NaN values: those that a query sees are what it gets, however small their weights. They were left out
+  // of the tiles, or (one part, tiles that every query of the block sees) have gone through the products, from which
+  // an output that they enter never comes out finite.
   int bad = 0;
 #pragma unroll
   for (int n = 0; n < KS * RG; ++n) bad |= sm.bad[n];
-  if (bad) {
-    // what was left out of the tiles, to the queries that see it
-    for (int key = PARTS > 1 ? 0 : (max(first - PK + 2, 0) + PK - 1) / PK * PK; key <= tok; ++key) {
+  if constexpr (PARTS == 1) {
+    float zero = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) zero = fmaf(out[b][j], 0.f, zero);
+    bad |= zero != zero;
+  }
+  if (bad && sum == sum) {
+    f32x16 seen[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) seen[b] = f32x16{};
+#pragma unroll 1
+    for (int key = 0; key <= tok; ++key) {
       const uint16_t* vr = reinterpret_cast<const uint16_t*>(vbase + key * (2 * a.v_row)) + 32 * b0 + 4 * g;
 #pragma unroll
       for (int b = 0; b < NB; ++b)
@@ -601,13 +616,17 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 1 ? 1 : 2) packed_attentio
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float f = bf16_to_f32(vr[32 * b + 8 * q + j]);
-            if (!(fabsf(f) < INFINITY)) out[b][4 * q + j] += f;
+            if (!(fabsf(f) < INFINITY)) seen[b][4 * q + j] += f;
           }
     }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) out[b][j] = seen[b][j] != 0.f ? seen[b][j] : out[b][j];
   }
 
   // the output's columns are queries: 8 dims of one query per lane after a swap between the wave's halves
-  const float inv = 1.f / sum;
+  const float inv = sum > 0.f ? 1.f / sum : __builtin_nanf("");  // no key of weight: NaN, as 0 / 0
   auto dims8 = [&](int b, int q, float (&o)[8]) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {

@@ -346,3 +346,48 @@ def test_very_low_scores_behind_keys_without_weight(kernel, lengths, dtype):
     got = kernel.attention_packed(q, k, v, lengths)
     limit = (6 if dtype == torch.float32 else 1) * bound(q, k.masked_fill(torch.isinf(k), 0), v, dtype)
     check_where_finite(got, reference(q, k, v, lengths), limit)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("lengths", SPLITS, ids=lambda v: f"{len(v)}x{v[0]}")
+@pytest.mark.parametrize("rise", [600.0, 0.5], ids=["sharp key", "rising scores"])
+def test_an_infinite_value_with_a_weight_too_small_to_hold(kernel, lengths, dtype, rise):
+    """A weight is positive however small: an infinite value that a token sees reaches it, also where fp32 holds the
+    weight as 0 (scores behind it that are hundreds higher), wherever its key lies in the tiles. (fp32 queries: 6 times the bound's
+    2^-22, as one term makes most of a score and up to 24 products are added to it.)"""
+    n = sum(lengths)
+    q, k, v = inputs(n, 6, 2, dtype, seed=25)
+    starts = [sum(lengths[:i]) for i in range(len(lengths))]
+    q[:, :, 8] = 8.0
+    k[:, :, 8] = 0.0
+    marks = []
+    for s, (at, length) in enumerate(zip(starts, lengths)):
+        if rise > 100:
+            k[at + length // 2:at + length, :, 8] = rise
+        else:
+            k[at:at + length, :, 8] = (rise * torch.arange(length, device=DEV)).to(torch.bfloat16)[:, None]
+        for j, (t, value) in enumerate(((0, math.inf), (length // 4, -math.inf), (length // 3, math.nan))):
+            v[at + t, j % 2, 11 + 40 * j] = value
+            marks.append((slice(at + t, at + length), j % 2, 11 + 40 * j, value))
+    print(f"[packed] {dtype} infinite values of no weight, lengths {lengths[:12]}", flush=True)
+    got = kernel.attention_packed(q, k, v, lengths)
+    finite = v.masked_fill(~torch.isfinite(v), 0)
+    want = reference(q, k, finite, lengths)
+    for r, head, dim, value in marks:
+        want[r, 3 * head:3 * head + 3, dim] = value
+    inf = torch.isinf(want)
+    assert torch.equal(torch.isinf(got), inf) and torch.equal(got[inf].double(), want[inf])
+    limit = (6 if dtype == torch.float32 else 1) * bound(q, k, finite, dtype)
+    check_where_finite(got.masked_fill(inf, 0), want.masked_fill(inf, 0), limit)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_a_row_whose_keys_all_have_no_weight(kernel, dtype):
+    """Nothing but scores of -infinity: 0 / 0, in the dimensions of an infinite value too."""
+    q, k, v = inputs(300, 6, 2, dtype, seed=28)
+    q[:, :, 7] = 1.0
+    k[:70, :, 7] = -math.inf
+    v[3, :, 20] = math.inf
+    got = kernel.attention_packed(q, k, v, [300])
+    assert torch.isnan(got[:70]).all()
+    assert torch.isfinite(got[70:, :, :20]).all() and torch.isfinite(got[70:, :, 21:]).all()
