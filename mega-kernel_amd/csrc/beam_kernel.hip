@@ -5,13 +5,13 @@
 //   score[r] + logit[r][v] - log(sum over u of exp(logit[r][u])),
 // a finished row the one candidate (eos, score[r]), and the group's `beams` best go on. Within a row the
 // order of the candidates is that of the logits, so it needs no arithmetic:
-//   beam_chunk_kernel  a workgroup takes 8,192 logits of a row, a wave 2,048, all in registers: their maximum,
-//                      the sum of exp(logit - maximum), and their `beams` best (logit, token) as 64-bit keys;
+//   beam_chunk_kernel  a workgroup takes 8,192 logits of a row, a wave 2,048, all in registers: the sum of
+//                      exp(logit - reference) to 2^-22, and their `beams` best (logit, token) as 64-bit keys;
 //   beam_pick_kernel   a workgroup per group: a wave joins a row's sums (64 bits) and keys, then the group's
 //                      beams^2 row bests are ranked by their scores in 64 bits, which tell apart any two
-//                      candidates of one row and, between rows, what the fp32 sums resolve.
+//                      candidates of one row and, between rows, what the sums' 2^-22 resolve.
 // Bound by the read of the logits where there are many rows (8 x 8 beams of a vocabulary of 151,936, 38.9 MB in all:
-// 16.1 us, 12.3 and 4.3 of them in the two kernels), by launches and round trips where there are few (4 beams
+// 17.7 us; 16.1 with plain fp32 sums), by launches and round trips where there are few (4 beams
 // 9.4 us). 2,048 logits to a wave: 32 registers hold them, and 64 rows make 4,864 waves, one round on the chip.
 // Equal candidates: the lower row first, within a row the larger logit, then the lower token.
 //
@@ -90,6 +90,11 @@ __device__ __forceinline__ double wave_sum64(double v) {
   return join64(lo[0], hi[0]) + join64(lo[1], hi[1]);
 }
 
+// A sum that refers to R, for the higher reference M (mostly the same one); a sum without a reference is 0, or NaN.
+__device__ __forceinline__ double to_reference(double R, double sum, double M) {
+  return R == M || R == -INFINITY ? sum : sum * exp(R - M);
+}
+
 struct BeamArgs {
   const float* logits;  // [rows][row_stride]
   int64_t row_stride;
@@ -97,7 +102,7 @@ struct BeamArgs {
   const uint8_t* finished;
   int rows, vocab, beams, eos, chunks;
   u64* cand;     // [rows][chunks][beams]
-  float2* stat;  // [rows][chunks]: maximum, sum of exp(logit - maximum)
+  double2* stat;  // [rows][chunks]: a reference R and the sum of exp(logit - R); -infinity: no logit above that
   int32_t *tokens, *parents;
   float* out_scores;
   uint8_t* out_finished;
@@ -108,7 +113,7 @@ typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));  // rows may 
 
 __global__ void __launch_bounds__(256) beam_chunk_kernel(const BeamArgs a) {
   __shared__ u64 list[64];
-  __shared__ float smax[4], ssum[4];
+  __shared__ double sref[4], ssum[4];
   __shared__ uint32_t sbits[4];
   __shared__ u64 sbest[4];
   __shared__ int count;
@@ -145,13 +150,31 @@ __global__ void __launch_bounds__(256) beam_chunk_kernel(const BeamArgs a) {
     const uint32_t more = bits | (1u << b);
     if (__popcll(__builtin_amdgcn_ballot_w64(u >= more)) >= W) bits = more;
   }
-  const float m = wave_max(lmax), mc = m == -INFINITY ? 0.f : m;
-  float sum = 0.f;
+  // The sum of exp(logit - R) to 2^-22 of itself, also where all terms' roundings point one way (thousands of equal
+  // logits). R is the maximum's next multiple of 32 towards 0, so the difference is exact (a rounded one is of a term
+  // at least e^16 below the maximum). The product with log2 e keeps what its rounding leaves, c, for a sum of its own:
+  // exp(d) = exp2(p) (1 + c log 2). Terms are off by exp2's step, 2^-23, and by half a one where two are added in fp32;
+  // all else is in 64 bits. (With plain fp32 a floor of 151,936 equal logits under peaks was off by 2^-20.)
+  constexpr float L = 1.4426950408889634f, L2 = (float)(1.4426950408889634 - (double)L);  // log2 e
+  const float m = wave_max(lmax), ref = m == -INFINITY ? 0.f : 32.f * truncf(m * (1.f / 32));
+  double sum = 0;
+  float rest = 0.f;
 #pragma unroll
-  for (int i = 0; i < BL / 64; ++i) sum += __builtin_amdgcn_exp2f((f[i] - mc) * 1.4426950408889634f);
-  sum = wave_sum(sum);
+  for (int i = 0; i < BL / 64; i += 2) {
+    float e[2];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      // e^-136 is 0 in fp32; -infinity would make c NaN, NaN stays
+      const float d = __builtin_elementwise_maximum(f[i + q] - ref, -136.f), p = d * L;
+      const float c = fmaf(d, L2, fmaf(d, L, -p));
+      e[q] = __builtin_amdgcn_exp2f(p);
+      rest = fmaf(e[q], c, rest);
+    }
+    sum += e[0] + e[1];
+  }
+  sum = wave_sum64(fma((double)rest, 0.6931471805599453, sum));
   if (lane == 0) {
-    smax[w] = m;
+    sref[w] = m == -INFINITY ? -INFINITY : ref;
     ssum[w] = sum;
     sbits[w] = bits;
   }
@@ -204,12 +227,11 @@ __global__ void __launch_bounds__(256) beam_chunk_kernel(const BeamArgs a) {
     }
   }
   if (tid == 0) {
-    const float M = fmaxf(fmaxf(smax[0], smax[1]), fmaxf(smax[2], smax[3]));
-    float s = 0.f;
+    const double R = fmax(fmax(sref[0], sref[1]), fmax(sref[2], sref[3]));
+    double s = 0;
 #pragma unroll
-    for (int o = 0; o < 4; ++o)
-      s += smax[o] == -INFINITY ? ssum[o] : ssum[o] * __builtin_amdgcn_exp2f((smax[o] - M) * 1.4426950408889634f);
-    a.stat[slot] = make_float2(M, s);
+    for (int o = 0; o < 4; ++o) s += to_reference(sref[o], ssum[o], R);
+    a.stat[slot] = make_double2(R, s);
   }
 }
 
@@ -229,13 +251,13 @@ __global__ void __launch_bounds__(64 * PICK_WAVES) beam_pick_kernel(const BeamAr
     const int64_t s0 = (int64_t)row * a.chunks;
     // what the row needs, in one trip: the chunks' sums and best keys, NL to a lane, and its keys, KL to a lane (of
     // the few rows that have more, the others below); an ended row has none that mean anything
-    float2 st[NL];
+    double2 st[NL];
     u64 head[NL], own[KL];
     const int keys = a.chunks * W;
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
       const int i = 64 * n + lane;
-      st[n] = make_float2(-INFINITY, 0.f);
+      st[n] = make_double2(-INFINITY, 0);
       head[n] = 0;
       if (i < a.chunks) {
         st[n] = a.stat[s0 + i];
@@ -258,7 +280,7 @@ __global__ void __launch_bounds__(64 * PICK_WAVES) beam_pick_kernel(const BeamAr
     float m = -INFINITY;
 #pragma unroll
     for (int n = 0; n < NL; ++n) {
-      m = fmaxf(m, st[n].x);
+      m = fmaxf(m, (float)st[n].x);
       heads[w][64 * n + lane] = head[n];
     }
     if (lane == 0) least[w] = 0;
@@ -275,13 +297,11 @@ __global__ void __launch_bounds__(64 * PICK_WAVES) beam_pick_kernel(const BeamAr
         for (int q = 0; q < 4; ++q) rank += heads[w][j + q] > head[n];
       if (head[n] != 0 && rank == W - 1) least[w] = head[n];
     }
-    // log of the row's sum: the chunks' sums in fp32, joined in 64 bits
+    // log of the row's sum
     m = wave_max(m);
     double sum = 0;
 #pragma unroll
-    for (int n = 0; n < NL; ++n)
-      sum += st[n].x == -INFINITY ? st[n].y  // 0, or NaN
-                                  : st[n].y * __builtin_amdgcn_exp2f((st[n].x - m) * 1.4426950408889634f);
+    for (int n = 0; n < NL; ++n) sum += to_reference(st[n].x, st[n].y, m);
     sum = wave_sum64(sum);
     const double lse = (double)m + log(sum);
     if (lane == 0) state[r] = bad || sum != sum;
@@ -413,7 +433,7 @@ using namespace mkp;
 extern "C" size_t mk_beam_select_workspace_bytes(int rows, int vocab, int beams) {
   if (rows < 1 || vocab < 1 || vocab > BV_MAX || beams < 1 || beams > BEAMS_MAX) return 0;
   const size_t slots = (size_t)rows * ((vocab + BC - 1) / BC);
-  return align256(slots * beams * sizeof(u64)) + align256(slots * sizeof(float2));
+  return align256(slots * beams * sizeof(u64)) + align256(slots * sizeof(double2));
 }
 
 extern "C" hipError_t mk_beam_select(int rows, int vocab, int beams, const float* logits, int64_t row_stride,
@@ -437,7 +457,7 @@ extern "C" hipError_t mk_beam_select(int rows, int vocab, int beams, const float
   a.eos = eos;
   a.chunks = (vocab + BC - 1) / BC;
   a.cand = static_cast<u64*>(workspace);
-  a.stat = reinterpret_cast<float2*>(static_cast<char*>(workspace) +
+  a.stat = reinterpret_cast<double2*>(static_cast<char*>(workspace) +
                                      align256((size_t)rows * a.chunks * beams * sizeof(u64)));
   a.tokens = tokens;
   a.parents = parents;

@@ -273,3 +273,37 @@ def test_offsets_past_32_bits(kernel):
     logits.copy_(torch.randn(4, 50000, device=DEV))
     check(kernel, logits, torch.tensor([-1.0, -2.5, -1.25, -3.0], device=DEV),
           torch.zeros(4, dtype=torch.bool, device=DEV), 4, 9)
+
+
+@pytest.mark.parametrize("gap", [3.0, 5.5, 7.3, 8.0, 9.77, 11.2, 15.9, 20.0])
+@pytest.mark.parametrize("base", [0.0, -3.3, 40.7, -300.1], ids=str)
+def test_sums_of_equal_logits_under_peaks(kernel, gap, base):
+    """Rows of one value with a peak here and there: 151,936 equal terms, whose roundings all point one way."""
+    rows, vocab = 6, 151936
+    logits = torch.full((rows, vocab), base, device=DEV)
+    logits[0:2, 5] = base + gap        # one peak
+    logits[2:4, 5::2048] = base + gap  # one for each 2,048 logits
+    logits[4:6, 5::8192] = base + gap
+    scores = -torch.arange(rows, device=DEV) * 0.125
+    check(kernel, logits, scores, torch.zeros(rows, dtype=torch.bool, device=DEV), 2, -1)
+
+
+@pytest.mark.parametrize("apart", [6e-7, -6e-7])
+@pytest.mark.parametrize("gap", [5.5, 7.3, 9.77])
+def test_nearly_equal_candidates_of_two_rows(kernel, gap, apart):
+    """The best of a row of peaks on a floor of equal logits, and of a scattered row, 6e-7 apart either way: more than
+    the 2^-22 that the sums may be off."""
+    vocab = 151936
+    logits = torch.randn(2, vocab, generator=torch.Generator(device=DEV).manual_seed(9), device=DEV)
+    logits[0] = 0.0
+    logits[0, 5::2048] = gap
+    logits[1, 77] = float(logits[1].max() + 1.0)
+    for _ in range(40):  # the second row's best logit so that the rows are nearly equal, then its score
+        x = logits.cpu().double()
+        best = x[:, [5, 77]].diagonal() - torch.logsumexp(x, 1)
+        logits[1, 77] += (best[0] - best[1]).item()
+    scores = torch.tensor([0.0, (best[0] - best[1]).item() - apart], device=DEV)
+    x = logits.cpu().double()
+    best = x[:, [5, 77]].diagonal() - torch.logsumexp(x, 1) + scores.cpu().double()
+    assert abs(best[0] - best[1] - apart).item() < 1e-7 and x[1].argmax() == 77
+    check(kernel, logits, scores, torch.zeros(2, dtype=torch.bool, device=DEV), 2, -1)
