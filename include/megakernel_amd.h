@@ -261,9 +261,9 @@ hipError_t mk_attention_packed(int q_heads, int kv_heads, const void* q, int64_t
  * whose score is -infinity. A NaN or +infinity among a group's scores or the logits of its rows (a failed
  * decode's are NaN) shows in the whole group: tokens -1, scores NaN, every row its own parent.
  * A row's candidates are ranked by their logits; between rows the scores are compared in 64 bits, each off by at
- * most 2^-22, the accuracy of the logarithm of its row's sum. Asynchronous on `stream`; argument errors (rows not a multiple of beams or over
- * 65,535, eos outside [-1, vocab)) return hipErrorInvalidValue before any launch. No reference counterpart:
- * the reference takes the argmax (/root/reference/model.py:97).
+ * most 2^-22, the accuracy of the logarithm of its row's sum. Asynchronous on `stream`; argument errors (rows not
+ * a multiple of beams or over 65,535, eos outside [-1, vocab)) return hipErrorInvalidValue before any launch. No
+ * reference counterpart: the reference takes the argmax (/root/reference/model.py:97).
  */
 size_t mk_beam_select_workspace_bytes(int rows, int vocab, int beams);
 hipError_t mk_beam_select(int rows, int vocab, int beams, const float* logits, int64_t row_stride,

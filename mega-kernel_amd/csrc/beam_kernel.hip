@@ -303,7 +303,7 @@ __global__ void __launch_bounds__(64 * PICK_WAVES) beam_pick_kernel(const BeamAr
 #pragma unroll
     for (int n = 0; n < NL; ++n) sum += to_reference(st[n].x, st[n].y, m);
     sum = wave_sum64(sum);
-    const double lse = (double)m + log(sum);
+    const double lsum = log(sum);  // beside its reference: together they would lose it in a row of the lowest numbers
     if (lane == 0) state[r] = bad || sum != sum;
     wave_sync();
     // the keys that reach it: W at least (if there are as many), W a chunk of W chunks at most
@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(64 * PICK_WAVES) beam_pick_kernel(const BeamAr
         for (int q = 0; q < 8; ++q) place += near[w][j + q] > key;
       if (place < W) {
         const float x = key_logit(key);
-        score[r * W + place] = x == -INFINITY ? -INFINITY : base + ((double)x - lse);
+        score[r * W + place] = x == -INFINITY ? -INFINITY : base + (((double)x - m) - lsum);
         token[r * W + place] = key_token(key);
       }
     }

@@ -307,3 +307,23 @@ def test_nearly_equal_candidates_of_two_rows(kernel, gap, apart):
     best = x[:, [5, 77]].diagonal() - torch.logsumexp(x, 1) + scores.cpu().double()
     assert abs(best[0] - best[1] - apart).item() < 1e-7 and x[1].argmax() == 77
     check(kernel, logits, scores, torch.zeros(2, dtype=torch.bool, device=DEV), 2, -1)
+
+
+@pytest.mark.parametrize("lowest", [-1e30, torch.finfo(torch.float32).min, -math.inf], ids=str)
+def test_masks_of_the_lowest_value(kernel, lowest):
+    """A constrained vocabulary masked with the type's lowest value. A row that holds nothing else is an even one, of
+    probabilities 1 / vocabulary, and no row's best: the oracle takes the logits less their row's maximum, by which
+    64 bits hold a logarithm of the sum beside such a number."""
+    logits, scores, finished = inputs(6, 20000, seed=8)
+    logits[:, 7000:] = lowest
+    logits[3:] = lowest
+    if lowest == -math.inf:
+        logits[3:, 0] = -50.0
+    logits[1] = lowest if lowest > -math.inf else 0.0
+    want = oracle(logits.double() - logits.double().amax(1, keepdim=True), scores, finished, 3, 1)
+    print(f"[select] masks of {lowest}", flush=True)
+    tokens, parents, out, fin = kernel.beam_select(logits, scores, finished, 3, 1)
+    assert tokens.tolist() == want["tokens"] and parents.tolist() == want["parents"]
+    assert fin.tolist() == want["finished"]
+    for a, b in zip(out.tolist(), want["scores"]):
+        assert abs(a - b) <= 2.0 ** -24 * abs(b) + 2.0 ** -22, (a, b)
