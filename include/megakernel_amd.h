@@ -234,9 +234,11 @@ hipError_t mk_decode_batch(const mk_model_dims* dims, int batch, const int32_t* 
  * to bf16 for the product with v), everything else fp32. fp32 queries: products at fp32 accuracy. A value
  * row that a token may not see does not reach it, whatever it holds; an infinite or NaN value that it sees does,
  * however small the weight; a row whose scores are all -infinity is NaN. Asynchronous on `stream`, no
- * workspace, results independent of what else is in the batch. Argument errors (also more than 2^31 - 256
- * (row, head) pairs) return hipErrorInvalidValue before any launch. No reference counterpart: the
- * reference's attention takes one token's queries (/root/reference/megakernel.cu:228-370).
+ * workspace. No other sequence's values reach a sequence, but the order of its sums, and so the last bits within the
+ * roundings above, goes by the whole batch (which fixes the split of the work). The same call gives the same bits.
+ * `out` may not overlap an input. Argument errors (also more than 2^31 - 256 (row, head) pairs) return
+ * hipErrorInvalidValue before any launch. No reference counterpart: the reference's attention takes one token's
+ * queries (/root/reference/megakernel.cu:228-370).
  */
 hipError_t mk_attention_packed(int q_heads, int kv_heads, const void* q, int64_t q_row_stride, int64_t q_head_stride,
                                const void* k, int64_t k_row_stride, int64_t k_head_stride, const void* v,

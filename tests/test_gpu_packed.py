@@ -391,3 +391,28 @@ def test_a_row_whose_keys_all_have_no_weight(kernel, dtype):
     got = kernel.attention_packed(q, k, v, [300])
     assert torch.isnan(got[:70]).all()
     assert torch.isfinite(got[70:, :, :20]).all() and torch.isfinite(got[70:, :, 21:]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+def test_a_sequence_among_others_differs_by_summation_order_alone(kernel, dtype):
+    """A prompt alone and in batches that other instances of the kernel take: each within the bound of the formula,
+    no other sequence's values in it (theirs are infinite here)."""
+    n = 130
+    q, k, v = inputs(n, 16, 8, dtype, seed=26)
+    want, limit = reference(q, k, v, [n]), bound(q, k, v, dtype)
+    for others in ([], [20], [600, 700], [900] * 6, [2500], [300] * 40):
+        m = sum(others)
+        q2, k2, v2 = inputs(m, 16, 8, dtype, seed=27)
+        v2[:] = math.inf
+        got = kernel.attention_packed(torch.cat([q2, q]), torch.cat([k2, k]), torch.cat([v2, v]), others + [n])
+        err = (got[m:].double() - want).abs().max().item()
+        assert err <= limit, (others, err)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("lengths", SPLITS + [[2500], [900] * 24], ids=lambda v: f"{len(v)}x{v[0]}")
+def test_the_same_call_gives_the_same_bits(kernel, lengths, dtype):
+    q, k, v = inputs(sum(lengths), 16, 8, dtype, seed=29)
+    want = kernel.attention_packed(q, k, v, lengths)
+    for _ in range(5):
+        assert torch.equal(kernel.attention_packed(q, k, v, lengths), want)
