@@ -260,8 +260,11 @@ hipError_t mk_attention_packed(int q_heads, int kv_heads, const void* q, int64_t
  *   workspace    mk_beam_select_workspace_bytes(rows, vocab, beams) bytes of device memory, 256-byte aligned,
  *                owned by the caller, not used after the call's work completes on `stream`
  * A logit of -infinity is a candidate that only fills up (score -infinity), as is every candidate of a row
- * whose score is -infinity. A NaN or +infinity among a group's scores or the logits of its rows (a failed
- * decode's are NaN) shows in the whole group: tokens -1, scores NaN, every row its own parent.
+ * whose score is -infinity. A NaN or +infinity among a group's scores or the logits of its rows that have not
+ * finished (a failed decode's are NaN; a finished row's logits are not looked at) shows in the whole group:
+ * tokens -1, scores NaN, every row its own parent, in this selection and, by its scores, in those that follow.
+ * mk_decode_batch fails for EVERY sequence on a token of -1: replace it (by any token of the vocabulary) before
+ * the next decode if the other groups are to go on.
  * A row's candidates are ranked by their logits; between rows the scores are compared in 64 bits, each off by at
  * most 2^-22, the accuracy of the logarithm of its row's sum. Asynchronous on `stream`; argument errors (rows not
  * a multiple of beams or over 65,535, eos outside [-1, vocab)) return hipErrorInvalidValue before any launch. No

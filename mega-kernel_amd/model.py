@@ -57,7 +57,8 @@ def build_model(shape, max_positions, seed=0):
 def beam_search(kernel, prompts, beams, new, eos, embed, final_norm, layer_weights, cos, sin, max_seq):
     """The best ``beams`` continuations of up to ``new`` tokens of each prompt (lists of token ids), best first, as
     (tokens, score) with the score the sum of their log-probabilities; a continuation ends with ``eos`` (-1: none
-    does). All calls are queued without reading anything back, so ``new`` steps are always made."""
+    does). All calls are queued without reading anything back, so ``new`` steps are always made. A prompt whose
+    logits fail (NaN) has beams of no tokens and the score NaN; the others' searches go on."""
     import torch
     dev, rows = embed.device, len(prompts) * beams
     lengths = [len(p) for p in prompts]
@@ -79,7 +80,8 @@ def beam_search(kernel, prompts, beams, new, eos, embed, final_norm, layer_weigh
         steps.append((tokens, parents, finished))
         if i + 1 < new:
             kernel.beam_reorder(k, v, parents, begin, position, beams)
-            logits, _ = kernel.decode_batch(tokens, position, *weights, k, v, max_seq)
+            # a failed group's tokens are -1, which would fail the decode of every sequence
+            logits, _ = kernel.decode_batch(tokens.clamp(min=0), position, *weights, k, v, max_seq)
             position = position + 1
     steps, scores = [tuple(t.tolist() for t in s) for s in steps], scores.tolist()
     found = []
@@ -87,7 +89,7 @@ def beam_search(kernel, prompts, beams, new, eos, embed, final_norm, layer_weigh
         group = []
         for row in range(s * beams, (s + 1) * beams):
             path, at = [], row
-            for i in reversed(range(new)):
+            for i in reversed(range(new)) if scores[row] == scores[row] else ():  # NaN: failed
                 tokens, parents, _ = steps[i]
                 if i == 0 or not steps[i - 1][2][parents[at]]:  # not the repeated end of a finished one
                     path.append(tokens[at])
@@ -140,11 +142,13 @@ def run(argv=None, keep_prefill_cache=False):
         wall = time.perf_counter() - t0
         for i, group in enumerate(found):
             print(f"prompt {i} ({len(prompts[i])} tokens): " + "; ".join(
-                f"{score:.3f} {tokens[:8]}{' ...' if len(tokens) > 8 else ''}" for tokens, score in group))
+                f"{score:.3f} {tokens[:8]}{' ...' if len(tokens) > 8 else ''}" if score == score else "failed"
+                for tokens, score in group))
         print(f"beam search: {a.prompts} x {a.beams} beams, {new} steps in {wall * 1e3:.1f} ms, device status "
               f"{kernel.status()}")
         return {"prompt": a.prompt, "prompts": prompts, "beams": found, "status": kernel.status(),
-                "generated": [t for group in found for tokens, _ in group for t in tokens],
+                "generated": [t for group in found for tokens, score in group
+                              for t in (tokens if score == score else [-1])],  # -1: a failed beam
                 "inputs": {"embed": embed, "final_norm": final_norm, "layer_weights": layer_weights, "cos": cos,
                            "sin": sin, "max_seq": a.max_seq}}
 

@@ -57,3 +57,28 @@ def test_command_line(driver):
     assert driver.main(ARGS + ["--beams", "4", "--prompts", "3"]) == 0
     with pytest.raises(SystemExit):
         driver.main(ARGS + ["--beams", "17"])
+
+
+def test_a_failed_prompt_leaves_the_others_their_search(driver):
+    """One prompt's logits are NaN (as a failed call reports them): its group is reported as failed, and the other
+    prompt's beams are those of a search in which nothing failed."""
+    import megakernel
+    r = driver.run(ARGS + ["--beams", "3", "--prompts", "2"])
+    inp = r["inputs"]
+
+    class Fails:
+        def __getattr__(self, name):
+            return getattr(megakernel.load(), name)
+
+        def prefill_batch(self, *a):
+            logits, tokens = megakernel.load().prefill_batch(*a)
+            logits[0] = float("nan")
+            return logits, tokens
+
+    found = driver.beam_search(Fails(), r["prompts"], 3, NEW, -1, inp["embed"], inp["final_norm"], inp["layer_weights"],
+                               inp["cos"], inp["sin"], inp["max_seq"])
+    assert len(found[0]) == 3
+    for tokens, score in found[0]:
+        assert tokens == [] and score != score
+    assert [t for t, _ in found[1]] == [t for t, _ in r["beams"][1]]
+    assert [s for _, s in found[1]] == pytest.approx([s for _, s in r["beams"][1]], abs=1e-6)
