@@ -231,3 +231,11 @@ def test_prefill_batch_op(ext):
     refuses("16-byte boundary", k=z(2 * L * 8 * S * 128 + 4)[4:].view(2, L, 8, S, 128))
     refuses("same strides", k=wide[0])
     refuses("cos/sin tables", max_seq=S + 1)
+
+
+def test_version_tells_a_library_with_these_operators(lib, ext):
+    """Libraries up to 0.25 do not have them, or have them with other results."""
+    lib.mk_version.restype = ctypes.c_char_p
+    version = lib.mk_version().decode()
+    assert tuple(int(n) for n in version.split()[1].split(".")) >= (0, 26) and version == ext.version()
+    assert all(name in version for name in ("packed attention", "several prompts", "beam selection"))
