@@ -536,7 +536,8 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 1 ? 1 : 2) packed_attentio
   if constexpr (PARTS > 1) {
     // A query's part may be 0, or of the other sign, where the query is not (or an infinity, for one beyond bf16's
     // range), so on an infinite key component the parts' products are NaN where the query's is an infinity. Such a
-    // score has made its row's sum NaN: these rows are made again from whole queries, key after key in fp32.
+    // score has made its row's sum NaN: these rows are made again from whole queries, key after key in fp32
+    // (8,192 tokens with such a key in every row 16.5 ms, without 0.80).
     const bool again = sum != sum;
     if (__builtin_amdgcn_ballot_w64(again) != 0) {
       int c = col;
@@ -547,23 +548,32 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 1 ? 1 : 2) packed_attentio
       if (again)
 #pragma unroll
         for (int b = 0; b < NB; ++b) out[b] = f32x16{};
+      float qf[64];  // dims 16 s + 8 g + e of the query at 8 s + e
+#pragma unroll
+      for (int s = 0; s < 8; ++s) {
+        const char* qp = (const char*)a.q + qo + (PARTS == 3 ? 64 * s + 32 * g : 32 * s + 16 * g);
+        const uint4 x = *reinterpret_cast<const uint4*>(qp);
+        const uint4 y = *reinterpret_cast<const uint4*>(PARTS == 3 ? qp + 16 : (const char*)a.ql + (qp - (const char*)a.q));
+        const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if constexpr (PARTS == 3) qf[8 * s + e] = __uint_as_float(e < 4 ? xw[e] : yw[e - 4]);
+          else qf[8 * s + e] = (e & 1 ? bf16_hi(xw[e / 2]) : bf16_lo(xw[e / 2])) +
+                               (e & 1 ? bf16_hi(yw[e / 2]) : bf16_lo(yw[e / 2]));
+        }
+      }
 #pragma unroll 1
       for (int key = 0; key <= wlast; ++key) {
+        if (__builtin_amdgcn_ballot_w64(again && l == l) == 0) break;  // a NaN query or key leaves nothing to find
         float dot[8] = {};  // by the lane's 64 dims of query and key, the other half's beside them
-#pragma unroll 1
-        for (int s = 0; s < 8; ++s) {
-          const char* qp = (const char*)a.q + qo + (PARTS == 3 ? 64 : 32) * s + (PARTS == 3 ? 32 : 16) * g;
-          const uint4 x = *reinterpret_cast<const uint4*>(qp);
-          const uint4 y = *reinterpret_cast<const uint4*>(PARTS == 3 ? qp + 16 : (const char*)a.ql + (qp - (const char*)a.q));
-          const uint4 k = *reinterpret_cast<const uint4*>(kbase + key * (2 * a.k_row) + 32 * s + 16 * g);
-          const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w}, kw[4] = {k.x, k.y, k.z, k.w};
+        const char* kr = kbase + key * (2 * a.k_row) + 16 * g;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float qe;
-            if constexpr (PARTS == 3) qe = __uint_as_float(e < 4 ? xw[e] : yw[e - 4]);
-            else qe = (e & 1 ? bf16_hi(xw[e / 2]) : bf16_lo(xw[e / 2])) + (e & 1 ? bf16_hi(yw[e / 2]) : bf16_lo(yw[e / 2]));
-            dot[e] = fmaf(qe, e & 1 ? bf16_hi(kw[e / 2]) : bf16_lo(kw[e / 2]), dot[e]);
-          }
+        for (int s = 0; s < 8; ++s) {
+          const uint4 k = *reinterpret_cast<const uint4*>(kr + 32 * s);
+          const uint32_t kw[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            dot[e] = fmaf(qf[8 * s + e], e & 1 ? bf16_hi(kw[e / 2]) : bf16_lo(kw[e / 2]), dot[e]);
         }
         const float score =
             xsum32(((dot[0] + dot[1]) + (dot[2] + dot[3])) + ((dot[4] + dot[5]) + (dot[6] + dot[7]))) * C;
@@ -602,27 +612,51 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 1 ? 1 : 2) packed_attentio
       for (int j = 0; j < 16; ++j) zero = fmaf(out[b][j], 0.f, zero);
     bad |= zero != zero;
   }
-  if (bad && sum == sum) {
+  if (__builtin_amdgcn_ballot_w64(bad && sum == sum) != 0) {
     f32x16 seen[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) seen[b] = f32x16{};
+    // 32 rows at a time, four to an instruction; the rare one that holds some, dim by dim (8,192 tokens behind an
+    // infinite value 0.60 ms, without 0.30; fp32 1.0 and 0.80)
+    int l16 = lane;
+    asm volatile("" : "+v"(l16));  // so that nothing of it is made before the loop above, and kept there
 #pragma unroll 1
-    for (int key = 0; key <= tok; ++key) {
-      const uint16_t* vr = reinterpret_cast<const uint16_t*>(vbase + key * (2 * a.v_row)) + 32 * b0 + 4 * g;
+    for (int k0 = 0; k0 <= wlast; k0 += 32) {
+      uint32_t hit[8];
 #pragma unroll
-      for (int b = 0; b < NB; ++b)
+      for (int n = 0; n < 8; ++n) {
+        const int key = min(k0 + 4 * n + (l16 >> 4), wlast);
+        const uint4 x = *reinterpret_cast<const uint4*>(vbase + key * (2 * a.v_row) + 16 * (l16 & 15));
+        hit[n] = nonfinite2(x.x) | nonfinite2(x.y) | nonfinite2(x.z) | nonfinite2(x.w);
+      }
+#pragma unroll 1
+      for (int n = 0; n < 8; ++n) {
+        uint32_t h = hit[0];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
+        for (int o = 1; o < 8; ++o) h = n == o ? hit[o] : h;
+        const u64 any = __builtin_amdgcn_ballot_w64(h != 0);
+        if (any == 0) continue;
+#pragma unroll 1
+        for (int e = 0; e < 4; ++e) {
+          const int key = k0 + 4 * n + e;
+          if ((any >> (16 * e) & 0xffff) == 0 || key > wlast) continue;
+          const uint16_t* vr = reinterpret_cast<const uint16_t*>(vbase + key * (2 * a.v_row)) + 32 * b0 + 4 * g;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float f = bf16_to_f32(vr[32 * b + 8 * q + j]);
-            if (!(fabsf(f) < INFINITY)) seen[b][4 * q + j] += f;
-          }
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float f = bf16_to_f32(vr[32 * b + 8 * q + j]);
+                if (key <= tok && !(fabsf(f) < INFINITY)) seen[b][4 * q + j] += f;
+              }
+        }
+      }
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int j = 0; j < 16; ++j) out[b][j] = seen[b][j] != 0.f ? seen[b][j] : out[b][j];
+      for (int j = 0; j < 16; ++j) out[b][j] = bad && seen[b][j] != 0.f ? seen[b][j] : out[b][j];
   }
 
   // the output's columns are queries: 8 dims of one query per lane after a swap between the wave's halves
