@@ -11,8 +11,8 @@
 //                      beams^2 row bests are ranked by their scores in 64 bits, which tell apart any two
 //                      candidates of one row and, between rows, what the sums' 2^-22 resolve.
 // Bound by the read of the logits where there are many rows (8 x 8 beams of a vocabulary of 151,936, 38.9 MB in all:
-// 17.7 us; 16.1 with plain fp32 sums), by launches and round trips where there are few (4 beams
-// 9.4 us). 2,048 logits to a wave: 32 registers hold them, and 64 rows make 4,864 waves, one round on the chip.
+// 17.6 us, 14.0 and 4.5 of them in the two kernels; 16.1 with plain fp32 sums), by launches and round trips where there
+// are few (4 beams 9.4 us). 2,048 logits to a wave: 32 registers hold them, and 64 rows make 4,864 waves, one round on the chip.
 // Equal candidates: the lower row first, within a row the larger logit, then the lower token.
 //
 // Reordering. new[b][p] = old[parents[b]][p] for the rows p of [begin[b], end[b]): a thread takes one 16-byte

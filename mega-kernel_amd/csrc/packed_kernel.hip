@@ -17,17 +17,19 @@
 //                   A operand is V read transposed from LDS (ds_read_b64_tr_b16) in the same order. The
 //                   output's columns are the queries too: rescaling is one factor per lane.
 // K and V tiles are staged through LDS, two deep. 32 rows to a wave rather than 64: the output and the scores of
-// two tiles then stay in the 256 registers of two waves per SIMD (64 rows: 628 us where this takes 372).
+// two tiles then stay in the 256 registers of two waves per SIMD (64 rows: 628 us where 32 took 372 then).
 //
 // Bound by the matrix cores and the exponentials beside them on long sequences: 8,192 + 4,096 + 1,801 tokens of 16
 // heads on 8 take 362 us, 987 TFLOP/s of useful products (a library product of 16,384 cubed: 1,351), MFMA busy 47%
 // and VALU issuing 40% of the time; 3,584 fp32 tokens 141 us, 1,120 TFLOP/s with the three products each. By
-// memory and the blocks' first loads on short ones: 64 prompts of 64 to 960 tokens 153 us (2.6 TB/s, 567 TFLOP/s).
+// memory and the blocks' first loads on short ones: 64 prompts of 64 to 960 tokens 150 us (2.7 TB/s, 580 TFLOP/s).
 // By latency on few: 32 tokens 5.8 us, most of it the fetch of code and operands by one wave per SIMD.
 //
 // Rounding. Queries and weights are multiplied as PARTS bf16 numbers whose sum they are: 1 for bf16
 // queries (a weight is then off by at most 2^-8 of itself, as the output is by its own rounding), 2 for
 // the prefill's hi/lo pairs (2^-16), 3 for fp32 queries (2^-24). Scores, maximum, sum and output are fp32.
+// One bf16 number per weight keeps the second product at one MFMA per fragment; outputs of bf16 queries are then
+// 0.0017 to 0.0020 of their norm from 64 bits, 0.0015 to 0.0016 with weights of 32 bits (the output's own rounding).
 //
 // A masked key weighs nothing, whatever its value row holds: a tile that some query sees in part is looked
 // over for infinities and NaN, and where it has any they are left out of the matrix product (0 times infinity would
@@ -543,7 +545,8 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 1 ? 1 : 2) packed_attentio
       int c = col;
       asm volatile("" : "+v"(c));  // the query's place found again: kept, it would take registers of the loop above
       const int rq = min(r0 + c, rows - 1), tq = div(rq, a.by_g);
-      const int64_t qo = ((int64_t)(row0 + tq) * a.q_row + (kh * a.g + (rq - tq * a.g)) * a.q_head) * (PARTS == 3 ? 4 : 2);
+      const int64_t qo =
+          ((int64_t)(row0 + tq) * a.q_row + (kh * a.g + (rq - tq * a.g)) * a.q_head) * (PARTS == 3 ? 4 : 2);
       float m = -INFINITY, l = 0.f;
       if (again)
 #pragma unroll
@@ -553,7 +556,8 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 1 ? 1 : 2) packed_attentio
       for (int s = 0; s < 8; ++s) {
         const char* qp = (const char*)a.q + qo + (PARTS == 3 ? 64 * s + 32 * g : 32 * s + 16 * g);
         const uint4 x = *reinterpret_cast<const uint4*>(qp);
-        const uint4 y = *reinterpret_cast<const uint4*>(PARTS == 3 ? qp + 16 : (const char*)a.ql + (qp - (const char*)a.q));
+        const uint4 y =
+            *reinterpret_cast<const uint4*>(PARTS == 3 ? qp + 16 : (const char*)a.ql + (qp - (const char*)a.q));
         const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -689,8 +693,9 @@ __global__ void __launch_bounds__(64 * RG * KS, RG == 1 ? 1 : 2) packed_attentio
       }
   } else {
     // Through the wave's own 32 padded rows of LDS, so that a store instruction writes whole lines, BB bytes of
-    // a row at a time, past the L2s: 64 prompts 168 -> 158 us, 3,584 fp32 tokens 151 -> 148 (whole lines into
-    // the L2s 168 and 149, 32 bytes of 32 rows past them 192).
+    // a row at a time, past the L2s. Measured over one set of inputs again and again (some 5 us less than with inputs
+    // that change from call to call, as the header's figures are) and before the later steps: 64 prompts 168 -> 158
+    // us, 3,584 fp32 tokens 151 -> 148 (whole lines into the L2s 168 and 149, 32 bytes of 32 rows past them 192).
     constexpr int ES = PARTS == 1 ? 2 : 4, BB = 32 * NB * ES < 256 ? 32 * NB * ES : 256;
     constexpr int NP = BB / (32 * ES), LR = BB / 16;  // output blocks at a time, lanes to a row
     static_assert(sizeof(sm.tiles) >= KS * RG * 32 * (BB + 16));
@@ -759,8 +764,9 @@ static hipError_t launch_packed(PackedArgs& a, const int32_t* lengths, int num_s
         // Blocks of one sequence after another find its keys in the L2s; blocks in turn, the longest first, end
         // together. So in turn are the last sequences, as many as keep the 512 workgroups that run at once busy
         // for as long as the longest block before them lasts (in units of the keys of one block). Measured on
-        // MI355X, us with all in turn / so / none in turn: 64 prompts of 64 to 960 tokens 158 / 148 / 148, of 512
-        // 136 / 125 / 132, 24 of 1,024 151 / 145 / 153, 8 of 2,048 162 / 163 / 179 (16 query heads on 8, bf16).
+        // MI355X over one set of inputs again and again, us with all in turn / so / none in turn: 64 prompts of 64 to
+        // 960 tokens 158 / 148 / 148, of 512 136 / 125 / 132, 24 of 1,024 151 / 145 / 153, 8 of 2,048 162 / 163 / 179
+        // (16 query heads on 8, bf16).
         int64_t blocks = 0, rest = 0;
         a.alone = 0;
         for (int i = n - 1; i > 0 && a.alone == 0 && pr == 128; --i) {
@@ -787,6 +793,9 @@ static hipError_t launch_packed(PackedArgs& a, const int32_t* lengths, int num_s
       // 18.8. With two / one key groups of 128 rows: bf16 3,584 tokens (448 workgroups) 67.6 / 83.3, 4 of 1,024
       // (512) 30.2 / 29.6, 8 of 512 (512) 21.8 / 18.5, 32 of 128 (512) 17.8 / 11.6; fp32 3,584 155 / 190, 5 of 768
       // (480) 48.9 / 50.7, 6 of 600 (480) 42.5 / 40.8, 32 of 128 27.2 / 20.8.
+      // The first limit of fp32 goes by single prompts. On 257 to 384 workgroups of 32 rows it loses with chains below
+      // about 300: 32 / 64 rows, fp32, 6 of 100 (336) 14.0 / 10.4, 16 of 48 (384) 14.0 / 9.7, 3 of 200 (312) 13.9 /
+      // 12.2, 330 + 300 (320) 14.0 / 14.8, 700 (352) 18.5 / 21.3. The prefill's hi/lo instances go by fp32's limits.
       const int longest = a.len[0];
       dim3 grid = places(32);
       if (grid.x <= (PARTS > 1 ? 384 : 160)) {
