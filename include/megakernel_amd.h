@@ -233,7 +233,8 @@ hipError_t mk_decode_batch(const mk_model_dims* dims, int batch, const int32_t* 
  * All pointers 16-byte aligned. bf16 queries: products of bf16 operands (the softmax's weights rounded
  * to bf16 for the product with v), everything else fp32. fp32 queries: products at fp32 accuracy. A value
  * row that a token may not see does not reach it, whatever it holds; an infinite or NaN value that it sees does,
- * however small the weight; a row whose scores are all -infinity is NaN. Asynchronous on `stream`, no
+ * however small the weight; a row whose scores are all -infinity is NaN. Weights are up to 2^8 before the
+ * division by their sum, so finite values above 2^119 / tokens may overflow. Asynchronous on `stream`, no
  * workspace. No other sequence's values reach a sequence, but the order of its sums, and so the last bits within the
  * roundings above, goes by the whole batch (which fixes the split of the work). The same call gives the same bits.
  * `out` may not overlap an input. Argument errors (also more than 2^31 - 256 (row, head) pairs) return
