@@ -291,6 +291,80 @@ hipError_t mk_beam_reorder(int num_layers, int rows, int beams, int max_seq_len,
                            const int32_t* parents, const int32_t* begin, const int32_t* end, hipStream_t stream);
 
 /*
+ * A K/V cache of many sequences in one pool of pages, for the three entry points below. Position p of
+ * sequence s is row p % page_size of page block_tables[s * table_stride + p / page_size].
+ *   k_pages, v_pages   row r of K/V head h of page i at i * page_stride + h * head_stride + r * row_stride
+ *                      (elements, the same for both, >= 0; multiples of 8, of 16 for 8-bit pages), 128
+ *                      numbers; 16-byte aligned. [num_pages][kv_heads][page_size][128], one layer of
+ *                      mk_decode_paged's pools, is the plain case
+ *   k_scales, v_scales NULL: the pages are bf16. Otherwise they are e4m3 (OCP), and the number of a row is its
+ *                      value times 2^(b - 127), b the byte at i * scale_page_stride + h * scale_head_stride + r
+ *                      (e8m0; 255: the row is NaN, and so are its values)
+ *   block_tables       int32 device array, table_entries (page_size * table_entries at most 2^30) of them
+ *                      for each of num_seqs sequences
+ * page_size is a power of two up to 4096. No reference counterpart: the reference's cache is one
+ * contiguous sequence's (/root/reference/model.py:79-87).
+ */
+typedef struct mk_paged_cache {
+  void *k_pages, *v_pages;
+  void *k_scales, *v_scales;
+  int64_t page_stride, head_stride, row_stride;
+  int64_t scale_page_stride, scale_head_stride;
+  const int32_t* block_tables;
+  int64_t table_stride;
+  int32_t table_entries, num_pages, kv_heads, page_size, num_seqs;
+} mk_paged_cache;
+
+/*
+ * Writes new keys and values into a paged cache. Their rows lie one sequence after the other, lengths[s]
+ * (HOST array of num_seqs, read before the call returns, >= 0) of sequence s, which go to its positions
+ * begin[s], begin[s] + 1, ... (begin: int32 device array).
+ *   k, v   bf16, or fp32 with rows_fp32 != 0; head h of row r at r * k_row_stride + h * k_head_stride (elements,
+ *          >= 0, multiples of 8, of 4 for fp32), 16-byte aligned: slices of one projection's rows will do
+ * bf16 pages: each number rounded to bf16. e4m3 pages: each head's row gets the least power of two, at least
+ * 2^-117, that its largest magnitude is at most 448 times of, and its numbers are rounded to e4m3 in units of it;
+ * a row with an infinity or NaN becomes NaN. A row whose position lies outside [0, table_entries * page_size) or whose
+ * table entry lies outside [0, num_pages) is not written (mk_attention_paged reports the entry). Two rows of one call
+ * may not share a place: what it then holds may be of both. Asynchronous on `stream`, no workspace; argument
+ * errors (also more than 2^31 - 1 rows) return hipErrorInvalidValue before any launch.
+ */
+hipError_t mk_cache_write(const mk_paged_cache* cache, const void* k, int64_t k_row_stride, int64_t k_head_stride,
+                          const void* v, int64_t v_row_stride, int64_t v_head_stride, int rows_fp32,
+                          const int32_t* begin, const int32_t* lengths, hipStream_t stream);
+
+/*
+ * Reads rows of a paged cache back: positions begin[s] .. begin[s] + lengths[s] - 1 of every sequence, one
+ * sequence after the other, into k and v, bf16 [rows][kv_heads][128] (16-byte aligned; they may overlap nothing else).
+ * Exact for what mk_cache_write has written: an e4m3 value times its power of two is a bf16 number (only 2^128, to
+ * which magnitudes from 3.29e38 on are rounded, is an infinity). A position or table entry out of range reads as NaN. Arguments, errors and asynchrony as mk_cache_write.
+ */
+hipError_t mk_cache_read(const mk_paged_cache* cache, const int32_t* begin, const int32_t* lengths, void* k, void* v,
+                         hipStream_t stream);
+
+/*
+ * Attention of one new token per sequence over a paged cache (its own key and value written before):
+ *   out[s][h] = sum over j < lengths[s] of softmax_j(q[s][h] . k[j][h / G] / sqrt(128)) v[j][h / G],
+ * G = q_heads / kv_heads (a whole number, any), heads of 128, up to 4,096 sequences.
+ *   q        bf16, or fp32 with q_fp32 != 0; head h of sequence s at q + s * q_row_stride + h * q_head_stride
+ *            (elements, >= 0; multiples of 8, of 4 for fp32), 16-byte aligned
+ *   lengths  int32 device array: a sequence of 0 keys gets 0, one outside [0, table_entries * page_size] NaN
+ *   out      q's type, [num_seqs][q_heads][128], 16-byte aligned; may not overlap an input
+ *   workspace  mk_attention_paged_workspace_bytes(q_heads, kv_heads) bytes of device memory, 256-byte aligned, owned by
+ *            the caller, not used after the call's work completes on `stream`
+ * A table entry outside [0, num_pages) among a sequence's makes its output NaN (page 0 is read in its place);
+ * entries past its last page are not looked at, nor is a row past its last key. fp32 queries: products at fp32
+ * accuracy. bf16 queries: the weights are products' operands of 16 bits, everything else fp32. An infinite or NaN
+ * value makes the elements of its sequence's output that it is a part of infinite or NaN; a row whose scores are all
+ * -infinity is NaN. The split of the work, and so the order of a sequence's sums, goes by all the lengths; the
+ * same call gives the same bits. Asynchronous on `stream`; argument errors return hipErrorInvalidValue before any
+ * launch. Lengths and tables are read on the device: a captured call can be replayed on other ones.
+ */
+size_t mk_attention_paged_workspace_bytes(int q_heads, int kv_heads);
+hipError_t mk_attention_paged(const mk_paged_cache* cache, int q_heads, const void* q, int64_t q_row_stride,
+                              int64_t q_head_stride, int q_fp32, const int32_t* lengths, void* out, void* workspace,
+                              size_t workspace_bytes, hipStream_t stream);
+
+/*
  * Several decode steps in one call, with no host synchronization between them: the device-side
  * multi-token loop. Step i (0 <= i < n) runs at position + i and reads its input token from device
  * memory, tokens[i] (int32, device array of n + 1 entries, tokens[0] set by the caller).

@@ -1,0 +1,828 @@
+// A K/V cache of many sequences in one pool of pages, on MI355X (gfx950): rows quantised as they are written,
+// read back, and the attention of each sequence's new token over its pages.
+//
+// Rows. A row is the 128 numbers of one position and K/V head. In bf16 pages it is rounded to bf16. In 8-bit
+// pages it is e4m3 values and one power of two: the least 2^e (e >= -117) with max|x| <= 448 * 2^e. A power of
+// two loses nothing against a finer scale (e4m3 keeps its relative precision over 2^15), x / 2^e is exact, so the
+// only rounding is the value's own (2^-4 of it), and value * 2^e is exact in bf16, which the attention multiplies.
+// A row with an infinity or NaN is NaN throughout. Writing and reading take a wave per position, 16 lanes to a row:
+// bound by memory.
+//
+// Attention. out[b][h] = sum over j < len[b] of softmax_j(q[b][h] . k[j][h / G] / sqrt(128)) v[j][h / G].
+// A wave takes 32 keys of one (sequence, K/V head) at a time for up to 16 of its query heads, on the matrix cores
+// and in registers alone (v_mfma_f32_16x16x32_bf16, lane l: n = l % 16, g = l / 16):
+//   S^T = K . Q^T    keys as rows. Row m of half t is key 8 (m / 4) + 4 t + m % 4, so that lane l holds the scores
+//                    of query n against keys 8 g .. 8 g + 7: maximum and sum take registers and two lane swaps;
+//   O^T += V^T . P^T the lane's weights are the B operand as they stand (slots 8 g + j mean keys 8 g + j). For the A
+//                    operand lane l loads dims 8 n .. 8 n + 7 of keys 8 g .. 8 g + 7, whole rows to 16 lanes, and
+//                    swaps them into 8 fragments, the i-th of dims 8 n + i: an 8 x 8 transpose in registers.
+//                    Lane l then holds dims 32 g .. 32 g + 31 of query n.
+// K's loads for the next 32 keys leave when the scores are made, V's when its fragments are. At 2 queries to a K/V head
+// 14 of the 16 columns are zero and the matrix cores are still idle most of the time: the read of the keys bounds it.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <initializer_list>
+#include <type_traits>
+#include <utility>
+
+#include "mk_device.h"
+#include "mk_layers.h"
+#include "../../include/megakernel_amd.h"
+
+namespace mkp {
+
+constexpr int CSEQ = 128;  // sequences per launch of the cache's kernels (their places travel as kernel arguments)
+constexpr int MIN_BYTE = 10;  // e8m0 byte of 2^-117: the least e4m3 value times it is bf16's least normal number
+
+struct PagePool {
+  uint8_t *k, *v;          // bytes
+  uint8_t *ks, *vs;        // scales (8-bit pages)
+  int64_t page, head, row;  // bytes between pages, heads, rows
+  int64_t spage, shead;
+  const int32_t* tables;
+  int64_t tstride;
+  int tn, pages, shift;  // entries of a table, pages of the pool, log2 of the page size
+};
+
+struct CacheArgs {
+  PagePool p;
+  const uint8_t *k, *v;  // written rows
+  uint8_t *ok, *ov;      // read rows, bf16 [rows][heads][128]
+  int64_t k_row, k_head, v_row, v_head;  // bytes
+  const int32_t* begin;
+  int64_t rows, out0;  // rows of this launch, the first of them
+  int hkv, nseq, seq0;
+  int32_t first[CSEQ];  // each sequence's first row, from out0
+};
+
+// The sequence that row r (the same for the whole wave) belongs to: the last one that starts at or before it.
+__device__ __forceinline__ int sequence_of(const CacheArgs& a, int lane, int64_t r) {
+  int n = 0;
+#pragma unroll
+  for (int i = 0; i < CSEQ / 64; ++i) {
+    const int s = 64 * i + lane;
+    n += __popcll(__builtin_amdgcn_ballot_w64(s < a.nseq && a.first[s] <= r));
+  }
+  return n - 1;
+}
+
+__device__ __forceinline__ uint32_t row16_max(uint32_t v) {  // over each 16 lanes
+  auto step = [&](uint32_t o) { v = max(v, o); };
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false));
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, false));
+  step((uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, false));
+  return v;
+}
+
+template <bool FP32, bool E4M3>
+__global__ void __launch_bounds__(256) cache_write_kernel(const CacheArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (r >= a.rows) return;
+  const int s = sequence_of(a, lane, r);
+  const int64_t pos = (int64_t)a.begin[a.seq0 + s] + (r - a.first[s]);
+  if (pos < 0 || (pos >> a.p.shift) >= a.p.tn) return;
+  const int page = a.p.tables[(a.seq0 + s) * a.p.tstride + (pos >> a.p.shift)];
+  if ((uint32_t)page >= (uint32_t)a.p.pages) return;
+  const int in = (int)(pos & ((1 << a.p.shift) - 1)), t = lane & 15;
+  const int64_t at = page * a.p.page + in * a.p.row, sat = page * a.p.spage + in;
+  for (int i = lane >> 4; i < 2 * a.hkv; i += 4) {  // the rows of k's heads, then of v's
+    const bool isv = i >= a.hkv;
+    const int h = isv ? i - a.hkv : i;
+    const uint8_t* src = (isv ? a.v + (a.out0 + r) * a.v_row + h * a.v_head : a.k + (a.out0 + r) * a.k_row + h * a.k_head);
+    float x[8];
+    uint4 w;
+    if constexpr (FP32) {
+      const float4 lo = *reinterpret_cast<const float4*>(src + 32 * t), hi = *reinterpret_cast<const float4*>(src + 32 * t + 16);
+      x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w;
+      x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
+      if constexpr (!E4M3)
+        w = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
+    } else {
+      w = *reinterpret_cast<const uint4*>(src + 16 * t);
+      unpack8(w, x);
+    }
+    uint8_t* dst = (isv ? a.p.v : a.p.k) + at + h * a.p.head;
+    if constexpr (!E4M3) {
+      *reinterpret_cast<uint4*>(dst + 16 * t) = w;
+    } else {
+      uint32_t m = 0;  // the largest magnitude's bits: NaN is above infinity is above the numbers
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7fffffffu);
+      m = row16_max(m);
+      const bool bad = m >= 0x7f800000u;
+      // m = 1.f * 2^(E - 127) <= 1.75 * 2^8 * 2^e
+      const int byte = bad ? 255 : max(MIN_BYTE, (int)(m >> 23) - 8 + ((m & 0x7fffff) > 0x600000));
+      const float inv = __uint_as_float((uint32_t)(254 - (bad ? 127 : byte)) << 23);
+      int lo = 0, hi = 0;
+      lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inv, x[1] * inv, lo, false);
+      lo = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv, x[3] * inv, lo, true);
+      hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[4] * inv, x[5] * inv, hi, false);
+      hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[6] * inv, x[7] * inv, hi, true);
+      *reinterpret_cast<uint2*>(dst + 8 * t) = bad ? make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu) : make_uint2(lo, hi);
+      if (t == 0) ((isv ? a.p.vs : a.p.ks) + sat + h * a.p.shead)[0] = (uint8_t)byte;
+    }
+  }
+}
+
+// Two e4m3 numbers (the low or high half of w) times a power of two, as bf16.
+template <bool HIGH>
+__device__ __forceinline__ uint32_t bf16_of_e4m3(uint32_t w, float scale) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HIGH));
+}
+__device__ __forceinline__ uint4 bf16x8_of_e4m3(uint32_t a, uint32_t b, float scale) {
+  return make_uint4(bf16_of_e4m3<false>(a, scale), bf16_of_e4m3<true>(a, scale), bf16_of_e4m3<false>(b, scale),
+                    bf16_of_e4m3<true>(b, scale));
+}
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+template <bool E4M3>
+__global__ void __launch_bounds__(256) cache_read_kernel(const CacheArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t r = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (r >= a.rows) return;
+  const int s = sequence_of(a, lane, r);
+  const int64_t pos = (int64_t)a.begin[a.seq0 + s] + (r - a.first[s]);
+  int page = -1;
+  if (pos >= 0 && (pos >> a.p.shift) < a.p.tn) page = a.p.tables[(a.seq0 + s) * a.p.tstride + (pos >> a.p.shift)];
+  const bool bad = (uint32_t)page >= (uint32_t)a.p.pages;
+  const int in = (int)(pos & ((1 << a.p.shift) - 1)), t = lane & 15;
+  const int64_t at = page * a.p.page + in * a.p.row, sat = page * a.p.spage + in;
+  for (int i = lane >> 4; i < 2 * a.hkv; i += 4) {
+    const bool isv = i >= a.hkv;
+    const int h = isv ? i - a.hkv : i;
+    const uint8_t* src = (isv ? a.p.v : a.p.k) + at + h * a.p.head;
+    uint4 w = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);  // NaN
+    if (!bad) {
+      if constexpr (E4M3) {
+        const uint2 x = *reinterpret_cast<const uint2*>(src + 8 * t);
+        const uint32_t byte = ((isv ? a.p.vs : a.p.ks) + sat + h * a.p.shead)[0];
+        if (byte != 255) w = bf16x8_of_e4m3(x.x, x.y, scale_of(byte));
+      } else {
+        w = *reinterpret_cast<const uint4*>(src + 16 * t);
+      }
+    }
+    *reinterpret_cast<uint4*>((isv ? a.ov : a.ok) + (((a.out0 + r) * a.hkv + h) * D) * 2 + 16 * t) = w;
+  }
+}
+
+// -----------------------------------------------------------------------------------------------------------
+// attention of one token per sequence
+// -----------------------------------------------------------------------------------------------------------
+constexpr int TK = 32;                 // keys to a tile
+constexpr int AW = 4;                  // waves to a workgroup
+constexpr int NQ = 16;                 // queries to a unit: (sequence, K/V head, 16 of its query heads)
+constexpr int PART = D + 2;            // floats of one query's partial result: sum, maximum, output
+constexpr int SEQ_MAX = 4096;
+constexpr int PAGED_WGS = 512;         // workgroups that share the tiles out
+
+struct PagedArgs {
+  PagePool p;
+  const uint8_t* q;
+  int64_t q_row, q_head;  // bytes
+  uint8_t* out;
+  const int32_t* lengths;
+  float* part;  // [2 * wgs][queries of a unit][PART]
+  int nseq, hkv, g, gt, wgs;  // gt: units to a K/V head
+  int64_t capacity;           // positions of a table
+};
+
+// Keys of sequence b; none if its length is out of range.
+__device__ __forceinline__ int valid_length(const PagedArgs& a, int b) {
+  const int n = a.lengths[b];
+  return n > 0 && n <= a.capacity ? n : 0;
+}
+__device__ __forceinline__ int tiles_of(const PagedArgs& a, int b) { return (valid_length(a, b) + TK - 1) / TK; }
+
+// Sums of v over the workgroup's threads before this one and over all of them.
+template <int THREADS>
+__device__ __forceinline__ int64_t scan_before(int64_t v, int64_t* lds, int64_t& total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int64_t x = v;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int64_t y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 63) lds[w] = x;
+  __syncthreads();
+  int64_t before = x - v;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / 64; ++i) {
+    if (i < w) before += lds[i];
+    total += lds[i];
+  }
+  return before;
+}
+
+// v as the sum of PARTS bf16 numbers, each the rounding of what the ones before it leave
+template <int PARTS>
+__device__ __forceinline__ void parts_of(const float (&v)[8], uint4 (&p)[PARTS]) {
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = v[i];
+#pragma unroll
+  for (int s = 0; s < PARTS; ++s) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      w[i] = pack_bf16x2(r[2 * i], r[2 * i + 1]);
+      if (s + 1 < PARTS) {
+        r[2 * i] -= bf16_lo(w[i]);
+        r[2 * i + 1] -= bf16_hi(w[i]);
+      }
+    }
+    p[s] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+template <bool E4M3>
+struct Tile {
+  uint4 k[2][E4M3 ? 2 : 4];
+  typename std::conditional<E4M3, uint2, uint4>::type v[8];
+  uint32_t ks[2], vs[E4M3 ? 8 : 1];
+};
+
+// One score in fp32 from the whole query: see the NaN of parts below.
+template <bool E4M3>
+__device__ __attribute__((noinline)) float whole_score(const uint8_t* k, float scale, const float* q) {
+  float s = 0.f;
+  for (int d = 0; d < D; ++d) {
+    float x;
+    if constexpr (E4M3) x = __builtin_amdgcn_cvt_f32_fp8((int)k[d], 0) * scale;
+    else x = bf16_to_f32(reinterpret_cast<const uint16_t*>(k)[d]);
+    s = fmaf(q[d], x, s);
+  }
+  return s;
+}
+
+template <int WAVES>
+struct PagedSmem {
+  float m[WAVES][NQ], l[WAVES][NQ];
+  float o[WAVES][NQ][D + 4];
+  int64_t scan[WAVES];
+  int64_t base;
+  int seq;
+};
+
+// E4M3: 8-bit pages. QP, PP: bf16 parts of a query and of a weight (1 and 2 for bf16 queries, 3 for fp32 ones).
+// SMALL: pages of fewer than TK positions, looked up key by key. SPLIT: the tiles of all units in one row are shared
+// out evenly, a unit's parts joined by paged_join_kernel; else a workgroup takes a unit.
+template <bool E4M3, int QP, int PP, bool SMALL, bool SPLIT, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, 2) paged_attention_kernel(const PagedArgs a) {
+  __shared__ PagedSmem<WAVES> sm;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 15, g = lane >> 4;
+  const int units = a.hkv * a.gt;  // of a sequence
+  const int gmax = min(a.g, NQ);
+  int b, u, t0;  // sequence, unit, first tile in it
+  int64_t left;  // tiles still to do
+  if constexpr (SPLIT) {
+    const int each = (a.nseq + 64 * WAVES - 1) / (64 * WAVES);
+    int64_t mine = 0, total;
+    for (int i = 0; i < each; ++i) {
+      const int s = tid * each + i;
+      if (s < a.nseq) mine += tiles_of(a, s);
+    }
+    int64_t before = scan_before<64 * WAVES>(mine, sm.scan, total) * units;
+    total *= units;
+    const int64_t per = max((int64_t)WAVES, (total + a.wgs - 1) / a.wgs);
+    const int64_t lo = blockIdx.x * per;
+    if (lo >= total) return;
+    if (lo >= before && lo < before + mine * units) {
+      for (int i = 0; i < each; ++i) {
+        const int64_t t = (int64_t)tiles_of(a, tid * each + i) * units;
+        if (lo < before + t) {
+          sm.seq = tid * each + i;
+          sm.base = before;
+          break;
+        }
+        before += t;
+      }
+    }
+    __syncthreads();
+    b = __builtin_amdgcn_readfirstlane(sm.seq);
+    const int64_t off = lo - sm.base;
+    const int T = tiles_of(a, b);
+    u = __builtin_amdgcn_readfirstlane((int)(off / T));
+    t0 = __builtin_amdgcn_readfirstlane((int)(off % T));
+    left = min(per, total - lo);
+  } else {
+    b = blockIdx.x / units;
+    u = blockIdx.x % units;
+    t0 = 0;
+    left = INT32_MAX;
+  }
+  const int mask = (1 << a.p.shift) - 1;
+  while (true) {
+    const int len = __builtin_amdgcn_readfirstlane(valid_length(a, b));
+    const int T = (len + TK - 1) / TK, t1 = (int)min((int64_t)T, t0 + left);
+    const int kh = u / a.gt, h0 = kh * a.g + NQ * (u % a.gt), nq = min(NQ, a.g - NQ * (u % a.gt));
+    const int32_t* table = a.p.tables + b * a.p.tstride;
+    const uint8_t* kbase = a.p.k + kh * a.p.head;
+    const uint8_t* vbase = a.p.v + kh * a.p.head;
+    const uint8_t* ksb = E4M3 ? a.p.ks + kh * a.p.shead : nullptr;
+    const uint8_t* vsb = E4M3 ? a.p.vs + kh * a.p.shead : nullptr;
+    bool bad = false;
+
+    // the queries as B operands: dims of step s at 8 lanes' width, as the keys' loads have them
+    auto dim_of = [&](int s) { return E4M3 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g; };
+    uint4 qf[4][QP];
+    const uint8_t* qrow = a.q + b * a.q_row + (int64_t)(h0 + n) * a.q_head;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      if constexpr (QP == 1) {
+        qf[s][0] = n < nq ? *reinterpret_cast<const uint4*>(qrow + 2 * dim_of(s)) : make_uint4(0, 0, 0, 0);
+      } else {
+        float x[8];
+        const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 lo = n < nq ? *reinterpret_cast<const float4*>(qrow + 4 * dim_of(s)) : z;
+        const float4 hi = n < nq ? *reinterpret_cast<const float4*>(qrow + 4 * dim_of(s) + 16) : z;
+        x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w;
+        x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
+        parts_of<QP>(x, qf[s]);
+      }
+    }
+
+    // Places of keys, in bytes from a head's rows; a key past the last is the last one (its weight is 0, and a page
+    // past the sequence's is never looked at).
+    int entry = 0;  // !SMALL: the page of the tile that is loaded next
+    auto page_of = [&](int key) __attribute__((always_inline)) {
+      int page = table[key >> a.p.shift];
+      if ((uint32_t)page >= (uint32_t)a.p.pages) {
+        bad = true;
+        page = 0;
+      }
+      return page;
+    };
+    auto place = [&](int t, int kk, int64_t& at, int64_t& sat) __attribute__((always_inline)) {
+      const int key = min(t * TK + kk, len - 1);
+      const int page = SMALL ? page_of(key) : entry;
+      at = page * a.p.page + (key & mask) * a.p.row;
+      sat = page * a.p.spage + (key & mask);
+    };
+    Tile<E4M3> x;
+    auto load_k = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        int64_t at, sat;
+        place(t, 8 * (n >> 2) + 4 * h + (n & 3), at, sat);
+#pragma unroll
+        for (int s = 0; s < (E4M3 ? 2 : 4); ++s) x.k[h][s] = *reinterpret_cast<const uint4*>(kbase + at + 64 * s + 16 * g);
+        if constexpr (E4M3) x.ks[h] = ksb[sat];
+      }
+    };
+    auto load_v = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        int64_t at, sat;
+        place(t, 8 * g + j, at, sat);
+        if constexpr (E4M3) {
+          x.v[j] = *reinterpret_cast<const uint2*>(vbase + at + 8 * n);
+          x.vs[j] = vsb[sat];
+        } else {
+          x.v[j] = *reinterpret_cast<const uint4*>(vbase + at + 16 * n);
+        }
+      }
+    };
+    auto look_up = [&](int t) __attribute__((always_inline)) {
+      if constexpr (!SMALL) entry = page_of(min(t * TK, len - 1));
+    };
+
+    float m = -INFINITY, l = 0.f;
+    f32x4 o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    int t = t0 + w;
+    if (t < t1) {
+      look_up(t);
+      load_k(t);
+      load_v(t);
+    }
+    for (; t < t1; t += WAVES) {
+      const int next = t + WAVES;
+      // scores
+      f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+          uint4 f;
+          if constexpr (E4M3) {
+            const uint4 r = x.k[h][st >> 1];
+            f = bf16x8_of_e4m3(st & 1 ? r.z : r.x, st & 1 ? r.w : r.y, scale_of(x.ks[h]));
+          } else {
+            f = x.k[h][st];
+          }
+#pragma unroll
+          for (int p = 0; p < QP; ++p) s[h] = mfma(f, qf[st][p], s[h]);
+        }
+      if constexpr (QP > 1) {
+        // Parts of a query may make NaN of an infinite key where the whole query makes an infinity: such scores are
+        // made again, while the query's sum is not NaN already.
+        bool again = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) again |= s[j >> 2][j & 3] != s[j >> 2][j & 3];
+        if (__builtin_amdgcn_ballot_w64(again && n < nq && l == l)) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            int64_t at, sat;
+            place(t, 8 * g + j, at, sat);
+            if (n < nq && l == l && s[j >> 2][j & 3] != s[j >> 2][j & 3])
+              s[j >> 2][j & 3] = whole_score<E4M3>(kbase + at, E4M3 ? scale_of(ksb[sat]) : 1.f,
+                                                   reinterpret_cast<const float*>(qrow));
+          }
+        }
+      }
+      if (next < t1) {
+        look_up(next);
+        load_k(next);
+      }
+      constexpr float C = ATT_SCALE * 1.4426950408889634f;  // weights are powers of two
+      float e[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) e[j] = s[j >> 2][j & 3] * C;
+      if (t * TK + TK > len)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (t * TK + 8 * g + j >= len) e[j] = -INFINITY;
+      float top = e[0];
+#pragma unroll
+      for (int j = 1; j < 8; ++j) top = fmaxf(top, e[j]);
+      top = xmax32(xmax16(top));
+      if (__builtin_amdgcn_ballot_w64(top > m)) {
+        const float up = fmaxf(m, top), f = up == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - up);
+        m = up;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] *= f;
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        e[j] = __builtin_amdgcn_exp2f(e[j] - ref);
+        l += e[j];
+      }
+      uint4 pf[PP];
+      parts_of<PP>(e, pf);
+      // values
+      uint32_t r[8][4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        uint4 f;
+        if constexpr (E4M3) f = bf16x8_of_e4m3(x.v[j].x, x.v[j].y, scale_of(x.vs[j]));
+        else f = x.v[j];
+        r[j][0] = f.x; r[j][1] = f.y; r[j][2] = f.z; r[j][3] = f.w;
+      }
+      if (next < t1) load_v(next);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint32_t f[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          f[q] = __builtin_amdgcn_perm(r[2 * q + 1][i >> 1], r[2 * q][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+        for (int p = 0; p < PP; ++p) o[i] = mfma(make_uint4(f[0], f[1], f[2], f[3]), pf[p], o[i]);
+      }
+    }
+
+    // the waves' results joined: what a query's weights refer to may differ from wave to wave
+    if (__builtin_amdgcn_ballot_w64(bad)) l = __builtin_nanf("");
+    l = xsum32(xsum16(l));
+    if (g == 0) {
+      sm.m[w][n] = m;
+      sm.l[w][n] = l;
+    }
+    if (n < nq)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {  // dims 32 g + 8 r + i
+        float* p = &sm.o[w][n][32 * g + 8 * r];
+        *reinterpret_cast<float4*>(p) = make_float4(o[0][r], o[1][r], o[2][r], o[3][r]);
+        *reinterpret_cast<float4*>(p + 4) = make_float4(o[4][r], o[5][r], o[6][r], o[7][r]);
+      }
+    __syncthreads();
+    const bool whole = t0 == 0 && t1 == T;
+    float* part = SPLIT ? a.part + (int64_t)(2 * blockIdx.x + (t0 == 0)) * gmax * PART : nullptr;
+    for (int i = tid; i < nq * (D / 4); i += 64 * WAVES) {
+      const int qi = i / (D / 4), d = 4 * (i % (D / 4));
+      float M = sm.m[0][qi];
+#pragma unroll
+      for (int v = 1; v < WAVES; ++v) M = fmaxf(M, sm.m[v][qi]);
+      const float ref = M == -INFINITY ? 0.f : M;
+      float sum = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int v = 0; v < WAVES; ++v) {
+        const float f = __builtin_amdgcn_exp2f(sm.m[v][qi] - ref);
+        const float4 y = *reinterpret_cast<const float4*>(&sm.o[v][qi][d]);
+        sum += f * sm.l[v][qi];
+        acc.x += f * y.x; acc.y += f * y.y; acc.z += f * y.z; acc.w += f * y.w;
+      }
+      if (SPLIT && !whole) {
+        float* p = part + qi * PART;
+        if (d == 0) {
+          p[0] = sum;
+          p[1] = M;
+        }
+        // (PART is even: 8-byte aligned)
+        *reinterpret_cast<float2*>(p + 2 + d) = make_float2(acc.x, acc.y);
+        *reinterpret_cast<float2*>(p + 4 + d) = make_float2(acc.z, acc.w);
+        continue;
+      }
+      float inv = sum > 0.f ? 1.f / sum : __builtin_nanf("");  // no key of weight: NaN, as 0 / 0
+      if (!SPLIT && T == 0) {  // an empty sequence, or a length out of range
+        inv = a.lengths[b] == 0 ? 0.f : __builtin_nanf("");
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      const int64_t at = ((int64_t)b * a.hkv * a.g + h0 + qi) * D + d;
+      if constexpr (QP == 1) {
+        *reinterpret_cast<uint2*>(a.out + 2 * at) =
+            make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+      } else {
+        *reinterpret_cast<float4*>(a.out + 4 * at) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+      }
+    }
+    if constexpr (!SPLIT) return;
+    left -= t1 - t0;
+    if (left <= 0) return;
+    __syncthreads();  // the next unit's results take the same places
+    t0 = 0;
+    if (++u == units) {
+      u = 0;
+      do ++b;
+      while (b < a.nseq && tiles_of(a, b) == 0);
+      b = __builtin_amdgcn_readfirstlane(b);
+      if (b >= a.nseq) return;
+    }
+  }
+}
+
+// Joins the parts of the units that more than one workgroup worked on, in their order: a workgroup per (sequence,
+// query head). Sequences without keys get their answer here too.
+template <bool FP32>
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
+  __shared__ int64_t scan[4];
+  __shared__ int64_t sbase;
+  __shared__ float red[4];
+  __shared__ __attribute__((aligned(16))) float acc[8][D];
+  __shared__ float accl[8];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int heads = a.hkv * a.g, b = blockIdx.x / heads, h = blockIdx.x % heads;
+  const int kh = h / a.g, hg = h % a.g, u = kh * a.gt + hg / NQ, qi = hg % NQ, units = a.hkv * a.gt;
+  const int T = tiles_of(a, b);
+  if (T == 0) {
+    const float x = a.lengths[b] == 0 ? 0.f : __builtin_nanf("");
+    const int64_t at = (int64_t)blockIdx.x * D + tid;
+    if (tid < D) {
+      if constexpr (FP32) reinterpret_cast<float*>(a.out)[at] = x;
+      else reinterpret_cast<uint16_t*>(a.out)[at] = f32_to_bf16(x);
+    }
+    return;
+  }
+  const int each = (a.nseq + 255) / 256;
+  int64_t mine = 0, total;
+  for (int i = 0; i < each; ++i) {
+    const int s = tid * each + i;
+    if (s < a.nseq) mine += tiles_of(a, s);
+  }
+  int64_t before = scan_before<256>(mine, scan, total);
+  if (tid == b / each) {
+    for (int s = tid * each; s < b; ++s) before += tiles_of(a, s);
+    sbase = before;
+  }
+  __syncthreads();
+  total *= units;
+  const int64_t per = max((int64_t)AW, (total + a.wgs - 1) / a.wgs);
+  const int64_t u0 = sbase * units + (int64_t)u * T, u1 = u0 + T;
+  const int w0 = (int)(u0 / per), w1 = (int)((u1 - 1) / per);
+  if (w0 == w1) return;
+  const int gmax = min(a.g, NQ);
+  auto slot = [&](int v) { return a.part + ((int64_t)(2 * v + (v == w0)) * gmax + qi) * PART; };
+  float M = -INFINITY;
+  for (int v = w0 + tid; v <= w1; v += 256) M = fmaxf(M, slot(v)[1]);
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+  if (lane == 0) red[w] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float ref = M == -INFINITY ? 0.f : M;
+  const int r = tid >> 5, d = 4 * (tid & 31);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float sum = 0.f;
+  for (int v = w0 + r; v <= w1; v += 8) {
+    const float* p = slot(v);
+    const float f = __builtin_amdgcn_exp2f(p[1] - ref);
+    const float2 x = *reinterpret_cast<const float2*>(p + 2 + d), y = *reinterpret_cast<const float2*>(p + 4 + d);
+    sum += f * p[0];
+    o.x += f * x.x; o.y += f * x.y; o.z += f * y.x; o.w += f * y.y;
+  }
+  *reinterpret_cast<float4*>(&acc[r][d]) = o;
+  if (d == 0) accl[r] = sum;
+  __syncthreads();
+  if (tid >= D) return;
+  float x = 0.f, all = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x += acc[i][tid];
+    all += accl[i];
+  }
+  x *= all > 0.f ? 1.f / all : __builtin_nanf("");
+  const int64_t at = (int64_t)blockIdx.x * D + tid;
+  if constexpr (FP32) reinterpret_cast<float*>(a.out)[at] = x;
+  else reinterpret_cast<uint16_t*>(a.out)[at] = f32_to_bf16(x);
+}
+
+static bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// Whether the rows of `width` elements at these strides are places of their own.
+static bool apart(int64_t width, std::initializer_list<std::pair<int64_t, int64_t>> dims) {  // (stride, count)
+  std::pair<int64_t, int64_t> d[3];
+  int n = 0;
+  for (const auto& x : dims)
+    if (x.second > 1) d[n++] = x;
+  std::sort(d, d + n);
+  for (int i = 0; i < n; ++i) {
+    if (d[i].first < width) return false;
+    width += d[i].first * (d[i].second - 1);
+  }
+  return true;
+}
+
+// The pool as the kernels take it; false where it is not one, or is to be written and has rows that overlap.
+static bool pool_of(const mk_paged_cache* c, PagePool& p, bool written) {
+  if (!c || !c->k_pages || !c->v_pages || c->k_pages == c->v_pages || !c->block_tables) return false;
+  const bool e4m3 = c->k_scales || c->v_scales;
+  if (e4m3 && (!c->k_scales || !c->v_scales || c->k_scales == c->v_scales)) return false;
+  if (c->kv_heads < 1 || c->kv_heads > 65535 || c->num_pages < 1 || c->page_size < 1 || c->page_size > 4096 ||
+      (c->page_size & (c->page_size - 1)) != 0 || c->num_seqs < 1 || c->table_entries < 1 || c->table_stride < 0 ||
+      (int64_t)c->table_entries * c->page_size > 1 << 30)
+    return false;
+  const int64_t size = e4m3 ? 1 : 2, unit = 16 / size;
+  for (int64_t s : {c->page_stride, c->head_stride, c->row_stride})
+    if (s < 0 || s % unit != 0) return false;
+  if (!aligned_to(c->k_pages, 16) || !aligned_to(c->v_pages, 16) || !aligned_to(c->block_tables, 4)) return false;
+  if (e4m3 && (c->scale_page_stride < 0 || c->scale_head_stride < 0)) return false;
+  if (written) {
+    if (!apart(D, {{c->page_stride, c->num_pages}, {c->head_stride, c->kv_heads}, {c->row_stride, c->page_size}})) return false;
+    if (e4m3 && !apart(c->page_size, {{c->scale_page_stride, c->num_pages}, {c->scale_head_stride, c->kv_heads}})) return false;
+  }
+  p.k = static_cast<uint8_t*>(c->k_pages);
+  p.v = static_cast<uint8_t*>(c->v_pages);
+  p.ks = static_cast<uint8_t*>(c->k_scales);
+  p.vs = static_cast<uint8_t*>(c->v_scales);
+  p.page = c->page_stride * size;
+  p.head = c->head_stride * size;
+  p.row = c->row_stride * size;
+  p.spage = c->scale_page_stride;
+  p.shead = c->scale_head_stride;
+  p.tables = c->block_tables;
+  p.tstride = c->table_stride;
+  p.tn = c->table_entries;
+  p.pages = c->num_pages;
+  p.shift = 0;
+  while ((1 << p.shift) < c->page_size) ++p.shift;
+  return true;
+}
+
+// The launches of a cache call: at most CSEQ sequences to each.
+template <typename F>
+static hipError_t cache_launches(CacheArgs& a, const int32_t* lengths, int num_seqs, F launch) {
+  a.out0 = 0;
+  for (int s = 0; s < num_seqs; s += CSEQ) {
+    a.seq0 = s;
+    a.nseq = std::min(CSEQ, num_seqs - s);
+    int64_t at = 0;
+    for (int i = 0; i < a.nseq; ++i) {
+      a.first[i] = (int32_t)at;
+      at += lengths[s + i];
+    }
+    a.rows = at;
+    if (at == 0) continue;
+    launch(dim3((unsigned)((at + 3) / 4)));
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    a.out0 += at;
+  }
+  return hipSuccess;
+}
+
+// Rows in all; -1 where the lengths are not ones.
+static int64_t rows_of(const int32_t* lengths, int num_seqs) {
+  if (!lengths) return -1;
+  int64_t total = 0;
+  for (int i = 0; i < num_seqs; ++i) {
+    if (lengths[i] < 0) return -1;
+    total += lengths[i];
+  }
+  return total <= INT32_MAX ? total : -1;
+}
+
+static bool paged_split(int64_t capacity) { return capacity > 512; }
+
+}  // namespace mkp
+
+using namespace mkp;
+
+extern "C" hipError_t mk_cache_write(const mk_paged_cache* cache, const void* k, int64_t k_row_stride,
+                                     int64_t k_head_stride, const void* v, int64_t v_row_stride, int64_t v_head_stride,
+                                     int rows_fp32, const int32_t* begin, const int32_t* lengths, hipStream_t stream) {
+  CacheArgs a{};
+  if (!pool_of(cache, a.p, true) || !begin) return hipErrorInvalidValue;
+  const int64_t rows = rows_of(lengths, cache->num_seqs);
+  if (rows < 0) return hipErrorInvalidValue;
+  if (rows == 0) return hipSuccess;
+  if (!k || !v || !aligned_to(k, 16) || !aligned_to(v, 16)) return hipErrorInvalidValue;
+  const int size = rows_fp32 ? 4 : 2;
+  for (int64_t s : {k_row_stride, k_head_stride, v_row_stride, v_head_stride})
+    if (s < 0 || s % (16 / size) != 0) return hipErrorInvalidValue;
+  a.k = static_cast<const uint8_t*>(k);
+  a.v = static_cast<const uint8_t*>(v);
+  a.k_row = k_row_stride * size;
+  a.k_head = k_head_stride * size;
+  a.v_row = v_row_stride * size;
+  a.v_head = v_head_stride * size;
+  a.begin = begin;
+  a.hkv = cache->kv_heads;
+  return cache_launches(a, lengths, cache->num_seqs, [&](dim3 grid) {
+    if (a.p.ks) {
+      if (rows_fp32) hipLaunchKernelGGL((cache_write_kernel<true, true>), grid, dim3(256), 0, stream, a);
+      else hipLaunchKernelGGL((cache_write_kernel<false, true>), grid, dim3(256), 0, stream, a);
+    } else {
+      if (rows_fp32) hipLaunchKernelGGL((cache_write_kernel<true, false>), grid, dim3(256), 0, stream, a);
+      else hipLaunchKernelGGL((cache_write_kernel<false, false>), grid, dim3(256), 0, stream, a);
+    }
+  });
+}
+
+extern "C" hipError_t mk_cache_read(const mk_paged_cache* cache, const int32_t* begin, const int32_t* lengths, void* k,
+                                    void* v, hipStream_t stream) {
+  CacheArgs a{};
+  if (!pool_of(cache, a.p, false) || !begin) return hipErrorInvalidValue;
+  const int64_t rows = rows_of(lengths, cache->num_seqs);
+  if (rows < 0) return hipErrorInvalidValue;
+  if (rows == 0) return hipSuccess;
+  if (!k || !v || k == v || !aligned_to(k, 16) || !aligned_to(v, 16)) return hipErrorInvalidValue;
+  a.ok = static_cast<uint8_t*>(k);
+  a.ov = static_cast<uint8_t*>(v);
+  a.begin = begin;
+  a.hkv = cache->kv_heads;
+  return cache_launches(a, lengths, cache->num_seqs, [&](dim3 grid) {
+    if (a.p.ks) hipLaunchKernelGGL(cache_read_kernel<true>, grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL(cache_read_kernel<false>, grid, dim3(256), 0, stream, a);
+  });
+}
+
+extern "C" size_t mk_attention_paged_workspace_bytes(int q_heads, int kv_heads) {
+  if (q_heads < 1 || kv_heads < 1 || q_heads % kv_heads != 0) return 0;
+  return ((size_t)2 * PAGED_WGS * std::min(NQ, q_heads / kv_heads) * PART * sizeof(float) + 255) & ~(size_t)255;
+}
+
+template <bool E4M3, int QP, int PP, bool SMALL>
+static void launch_paged(const PagedArgs& a, hipStream_t stream) {
+  const unsigned units = (unsigned)((int64_t)a.nseq * a.hkv * a.gt);
+  if (!paged_split(a.capacity)) {
+    hipLaunchKernelGGL((paged_attention_kernel<E4M3, QP, PP, SMALL, false, AW>), dim3(units), dim3(64 * AW), 0, stream, a);
+  } else {
+    hipLaunchKernelGGL((paged_attention_kernel<E4M3, QP, PP, SMALL, true, AW>), dim3(a.wgs), dim3(64 * AW), 0, stream, a);
+    hipLaunchKernelGGL(paged_join_kernel<(QP > 1)>, dim3(a.nseq * a.hkv * a.g), dim3(256), 0, stream, a);
+  }
+}
+
+extern "C" hipError_t mk_attention_paged(const mk_paged_cache* cache, int q_heads, const void* q, int64_t q_row_stride,
+                                         int64_t q_head_stride, int q_fp32, const int32_t* lengths, void* out,
+                                         void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  PagedArgs a{};
+  if (!pool_of(cache, a.p, false)) return hipErrorInvalidValue;
+  const size_t need = mk_attention_paged_workspace_bytes(q_heads, cache->kv_heads);
+  if (need == 0 || cache->num_seqs > SEQ_MAX || (int64_t)cache->num_seqs * q_heads > INT32_MAX / D) return hipErrorInvalidValue;
+  if (!q || !out || !lengths || !workspace || workspace_bytes < need || !aligned_to(workspace, 256)) return hipErrorInvalidValue;
+  if (!aligned_to(q, 16) || !aligned_to(out, 16)) return hipErrorInvalidValue;
+  const int size = q_fp32 ? 4 : 2;
+  for (int64_t s : {q_row_stride, q_head_stride})
+    if (s < 0 || s % (16 / size) != 0) return hipErrorInvalidValue;
+  a.q = static_cast<const uint8_t*>(q);
+  a.q_row = q_row_stride * size;
+  a.q_head = q_head_stride * size;
+  a.out = static_cast<uint8_t*>(out);
+  a.lengths = lengths;
+  a.part = static_cast<float*>(workspace);
+  a.nseq = cache->num_seqs;
+  a.hkv = cache->kv_heads;
+  a.g = q_heads / cache->kv_heads;
+  a.gt = (a.g + NQ - 1) / NQ;
+  a.wgs = PAGED_WGS;
+  a.capacity = (int64_t)cache->table_entries * cache->page_size;
+  const bool small = cache->page_size < TK;
+  if (a.p.ks) {
+    if (q_fp32) small ? launch_paged<true, 3, 3, true>(a, stream) : launch_paged<true, 3, 3, false>(a, stream);
+    else small ? launch_paged<true, 1, 2, true>(a, stream) : launch_paged<true, 1, 2, false>(a, stream);
+  } else {
+    if (q_fp32) small ? launch_paged<false, 3, 3, true>(a, stream) : launch_paged<false, 3, 3, false>(a, stream);
+    else small ? launch_paged<false, 1, 2, true>(a, stream) : launch_paged<false, 1, 2, false>(a, stream);
+  }
+  return hipGetLastError();
+}

@@ -18,7 +18,9 @@
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 
+#include <algorithm>
 #include <mutex>
+#include <utility>
 #include <vector>
 
 #include "../../include/megakernel_amd.h"
@@ -585,6 +587,167 @@ void beam_reorder(torch::Tensor kc, torch::Tensor vc, torch::Tensor parents, tor
                                parents.data_ptr<int32_t>(), begin.data_ptr<int32_t>(), end.data_ptr<int32_t>(), stream));
 }
 
+// A paged cache (mk_paged_cache) of tensors: k_pages and v_pages [pages, heads, page_size, 128] bf16, or float8_e4m3fn
+// with k_scales and v_scales float8_e8m0fnu [pages, heads, page_size], of any 16-byte aligned strides that the two
+// share (one layer of decode_paged's pools; the halves of [pages, 2, heads, page_size, 128]); block_tables int32
+// [sequences, entries].
+mk_paged_cache check_paged(const torch::Tensor& kp, const torch::Tensor& vp, const torch::Tensor& tables,
+                           const c10::optional<torch::Tensor>& ks, const c10::optional<torch::Tensor>& vs) {
+  const bool e4m3 = kp.defined() && kp.scalar_type() == torch::kFloat8_e4m3fn;
+  TORCH_CHECK(kp.defined() && kp.dim() == 4 && kp.size(3) == kHeadDim && (e4m3 || kp.scalar_type() == torch::kBFloat16),
+              "megakernel: k_pages must be [pages, heads, page_size, 128], bfloat16 or float8_e4m3fn");
+  const int64_t N = kp.size(0), H = kp.size(1), P = kp.size(2);
+  TORCH_CHECK(P >= 1 && P <= 4096 && (P & (P - 1)) == 0, "megakernel: page_size must be a power of two up to 4096, got ", P);
+  TORCH_CHECK(N >= 1 && N <= INT32_MAX && H >= 1 && H <= 65535, "megakernel: k_pages has no pages or heads, or too many");
+  mk_paged_cache c{};
+  const int64_t unit = 16 / kp.element_size();
+  auto strides = [&](const torch::Tensor& t, const char* name) {
+    TORCH_CHECK(t.defined() && t.device() == kp.device() && t.scalar_type() == kp.scalar_type() && t.sizes() == kp.sizes(),
+                "megakernel: ", name, " must be like k_pages, in type, shape and device");
+    TORCH_CHECK(t.stride(3) == 1, "megakernel: ", name, " must be contiguous in its last dimension");
+    const std::vector<int64_t> s{N > 1 ? t.stride(0) : 0, H > 1 ? t.stride(1) : 0, P > 1 ? t.stride(2) : 0};
+    for (int64_t x : s) TORCH_CHECK(x % unit == 0, "megakernel: ", name, "'s rows must start on 16-byte boundaries");
+    TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "megakernel: ", name,
+                " must start on a 16-byte boundary");
+    return s;
+  };
+  const std::vector<int64_t> st = strides(kp, "k_pages");
+  TORCH_CHECK(strides(vp, "v_pages") == st, "megakernel: k_pages and v_pages must have the same strides");
+  TORCH_CHECK(kp.data_ptr() != vp.data_ptr(), "megakernel: k_pages and v_pages must be distinct");
+  c.k_pages = kp.data_ptr();
+  c.v_pages = vp.data_ptr();
+  c.page_stride = st[0];
+  c.head_stride = st[1];
+  c.row_stride = st[2];
+  TORCH_CHECK(ks.has_value() == e4m3 && vs.has_value() == e4m3, "megakernel: float8_e4m3fn pages need k_scales and "
+              "v_scales, bfloat16 ones have none");
+  if (e4m3) {
+    std::vector<int64_t> ss[2];
+    for (int i = 0; i < 2; ++i) {
+      const torch::Tensor& t = i ? *vs : *ks;
+      const char* name = i ? "v_scales" : "k_scales";
+      TORCH_CHECK(t.defined() && t.device() == kp.device() && t.scalar_type() == torch::kFloat8_e8m0fnu && t.dim() == 3 &&
+                      t.size(0) == N && t.size(1) == H && t.size(2) == P,
+                  "megakernel: ", name, " must be float8_e8m0fnu [pages, heads, page_size] on ", kp.device());
+      TORCH_CHECK(P == 1 || t.stride(2) == 1, "megakernel: ", name, " must be contiguous in its last dimension");
+      ss[i] = {N > 1 ? t.stride(0) : 0, H > 1 ? t.stride(1) : 0};
+    }
+    TORCH_CHECK(ss[0] == ss[1], "megakernel: k_scales and v_scales must have the same strides");
+    TORCH_CHECK(ks->data_ptr() != vs->data_ptr(), "megakernel: k_scales and v_scales must be distinct");
+    c.k_scales = ks->data_ptr();
+    c.v_scales = vs->data_ptr();
+    c.scale_page_stride = ss[0][0];
+    c.scale_head_stride = ss[0][1];
+  }
+  TORCH_CHECK(tables.defined() && tables.device() == kp.device() && tables.scalar_type() == torch::kInt32 &&
+                  tables.dim() == 2 && tables.size(0) >= 1 && tables.size(1) >= 1 &&
+                  (tables.size(1) == 1 || tables.stride(1) == 1) && tables.size(0) <= INT32_MAX,
+              "megakernel: block_tables must be int32 [sequences, entries] on ", kp.device(),
+              ", contiguous in its last dimension");
+  TORCH_CHECK(tables.size(1) * P <= 1 << 30, "megakernel: block_tables covers more than 2^30 positions");
+  c.block_tables = tables.data_ptr<int32_t>();
+  c.table_stride = tables.stride(0);
+  c.table_entries = (int32_t)tables.size(1);
+  c.num_pages = (int32_t)N;
+  c.kv_heads = (int32_t)H;
+  c.page_size = (int32_t)P;
+  c.num_seqs = (int32_t)tables.size(0);
+  return c;
+}
+
+// The lengths of a cache call on the host, and their sum.
+int64_t check_lengths(const std::vector<int64_t>& lengths, const mk_paged_cache& c, std::vector<int32_t>& out) {
+  TORCH_CHECK((int64_t)lengths.size() == c.num_seqs, "megakernel: lengths must name block_tables' ", c.num_seqs,
+              " sequences, got ", lengths.size());
+  int64_t total = 0;
+  for (int64_t n : lengths) {
+    TORCH_CHECK(n >= 0 && n <= INT32_MAX && (total += n) <= INT32_MAX,
+                "megakernel: lengths must be at least 0 and add up to less than 2^31");
+    out.push_back((int32_t)n);
+  }
+  return total;
+}
+
+// Whether every element of t has a place of its own.
+bool apart(const torch::Tensor& t) {
+  std::vector<std::pair<int64_t, int64_t>> d;
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1) d.emplace_back(t.stride(i), t.size(i));
+  std::sort(d.begin(), d.end());
+  int64_t width = 1;
+  for (const auto& x : d) {
+    if (x.first < width) return false;
+    width += x.first * (x.second - 1);
+  }
+  return true;
+}
+
+// Writes packed rows of new keys and values into a paged cache (mk_cache_write): k and v [rows, heads, 128], bf16 or
+// fp32, lengths[s] rows of each sequence in turn to its positions begin[s] on (begin int32 on the device).
+void cache_write(torch::Tensor k, torch::Tensor v, torch::Tensor kp, torch::Tensor vp, torch::Tensor tables,
+                 torch::Tensor begin, std::vector<int64_t> lengths, c10::optional<torch::Tensor> ks,
+                 c10::optional<torch::Tensor> vs) {
+  const mk_paged_cache c = check_paged(kp, vp, tables, ks, vs);
+  std::vector<int32_t> len;
+  const int64_t rows = check_lengths(lengths, c, len);
+  TORCH_CHECK(k.defined() && (k.scalar_type() == torch::kBFloat16 || k.scalar_type() == torch::kFloat32),
+              "megakernel: k must be bfloat16 or float32");
+  const HeadRows sk = check_heads(k, "k", rows, k.scalar_type(), kp.device());
+  const HeadRows sv = check_heads(v, "v", rows, k.scalar_type(), kp.device());
+  TORCH_CHECK(k.size(1) == c.kv_heads && v.size(1) == c.kv_heads, "megakernel: k and v must have the pages' ", c.kv_heads,
+              " heads");
+  check_row_vector(begin, "begin", c.num_seqs, torch::kInt32, kp.device());
+  for (const torch::Tensor& t : {kp, ks.has_value() ? *ks : kp})  // v's are the same
+    TORCH_CHECK(apart(t), "megakernel: k_pages and k_scales must have no elements that overlap");
+  TORCH_CHECK(kp.is_cuda(), "megakernel: k_pages must be a GPU tensor");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(kp.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(kp.device().index()).stream();
+  MK_HIP_CHECK(mk_cache_write(&c, k.data_ptr(), sk.row, sk.head, v.data_ptr(), sv.row, sv.head,
+                              k.scalar_type() == torch::kFloat32, begin.data_ptr<int32_t>(), len.data(), stream));
+}
+
+// Reads rows of a paged cache back (mk_cache_read): positions begin[s] .. begin[s] + lengths[s] - 1 of each sequence
+// in turn. Returns (k, v), bf16 [rows, heads, 128].
+std::tuple<torch::Tensor, torch::Tensor> cache_read(torch::Tensor kp, torch::Tensor vp, torch::Tensor tables,
+                                                    torch::Tensor begin, std::vector<int64_t> lengths,
+                                                    c10::optional<torch::Tensor> ks, c10::optional<torch::Tensor> vs) {
+  const mk_paged_cache c = check_paged(kp, vp, tables, ks, vs);
+  std::vector<int32_t> len;
+  const int64_t rows = check_lengths(lengths, c, len);
+  check_row_vector(begin, "begin", c.num_seqs, torch::kInt32, kp.device());
+  TORCH_CHECK(kp.is_cuda(), "megakernel: k_pages must be a GPU tensor");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(kp.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(kp.device().index()).stream();
+  auto k = torch::empty({rows, c.kv_heads, kHeadDim}, kp.options().dtype(torch::kBFloat16));
+  auto v = torch::empty_like(k);
+  MK_HIP_CHECK(mk_cache_read(&c, begin.data_ptr<int32_t>(), len.data(), k.data_ptr(), v.data_ptr(), stream));
+  return {k, v};
+}
+
+// Attention of one new token per sequence over a paged cache (mk_attention_paged): q [sequences, heads, 128] bf16 or
+// fp32, lengths int32 [sequences] on the device. Returns [sequences, heads, 128] in q's type.
+torch::Tensor attention_paged(torch::Tensor q, torch::Tensor kp, torch::Tensor vp, torch::Tensor tables,
+                              torch::Tensor lengths, c10::optional<torch::Tensor> ks, c10::optional<torch::Tensor> vs) {
+  const mk_paged_cache c = check_paged(kp, vp, tables, ks, vs);
+  TORCH_CHECK(q.defined() && (q.scalar_type() == torch::kBFloat16 || q.scalar_type() == torch::kFloat32),
+              "megakernel: q must be bfloat16 or float32");
+  const HeadRows sq = check_heads(q, "q", c.num_seqs, q.scalar_type(), kp.device());
+  TORCH_CHECK(q.size(1) % c.kv_heads == 0, "megakernel: q's heads (", q.size(1), ") must be a multiple of the pages' (",
+              c.kv_heads, ")");
+  TORCH_CHECK(c.num_seqs <= 4096, "megakernel: at most 4096 sequences, got ", c.num_seqs);
+  TORCH_CHECK(q.size(0) * q.size(1) <= INT32_MAX / kHeadDim, "megakernel: too many heads in one call");
+  check_row_vector(lengths, "lengths", c.num_seqs, torch::kInt32, kp.device());
+  TORCH_CHECK(kp.is_cuda(), "megakernel: k_pages must be a GPU tensor");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(kp.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(kp.device().index()).stream();
+  const size_t bytes = mk_attention_paged_workspace_bytes((int)q.size(1), c.kv_heads);
+  auto ws = torch::empty({(int64_t)bytes}, q.options().dtype(torch::kUInt8));
+  auto out = torch::empty({q.size(0), q.size(1), kHeadDim}, q.options());
+  MK_HIP_CHECK(mk_attention_paged(&c, (int)q.size(1), q.data_ptr(), sq.row, sq.head, q.scalar_type() == torch::kFloat32,
+                                  lengths.data_ptr<int32_t>(), out.data_ptr(), ws.data_ptr(), bytes, stream));
+  return out;
+}
+
 int64_t status() {
   uint32_t s = 0;
   MK_HIP_CHECK(mk_status(&s));
@@ -651,6 +814,22 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("beam_reorder", &beam_reorder,
         "reorder decode_batch's caches in place: row b's positions [begin[b], end[b]) become those of row parents[b] "
         "(int32 [rows] on device, parents inside the row's group of beams)");
+  m.def("cache_write", &cache_write,
+        "write packed rows of new keys and values ([rows, heads, 128] bf16 or fp32; lengths a list, begin int32 on "
+        "device) into a paged cache: pages [pages, heads, page_size, 128] bf16, or float8_e4m3fn with float8_e8m0fnu "
+        "scales [pages, heads, page_size]; block_tables int32 [sequences, entries]",
+        py::arg("k"), py::arg("v"), py::arg("k_pages"), py::arg("v_pages"), py::arg("block_tables"), py::arg("begin"),
+        py::arg("lengths"), py::arg("k_scales") = py::none(), py::arg("v_scales") = py::none());
+  m.def("cache_read", &cache_read,
+        "read lengths[s] rows from begin[s] on of each sequence of a paged cache back (tensors as cache_write); returns "
+        "(k, v), bf16 [rows, heads, 128]",
+        py::arg("k_pages"), py::arg("v_pages"), py::arg("block_tables"), py::arg("begin"), py::arg("lengths"),
+        py::arg("k_scales") = py::none(), py::arg("v_scales") = py::none());
+  m.def("attention_paged", &attention_paged,
+        "attention of one new token per sequence over a paged cache (tensors as cache_write): q [sequences, heads, 128] "
+        "bf16 or fp32, lengths int32 [sequences] on device; returns [sequences, heads, 128] in q's type",
+        py::arg("q"), py::arg("k_pages"), py::arg("v_pages"), py::arg("block_tables"), py::arg("lengths"),
+        py::arg("k_scales") = py::none(), py::arg("v_scales") = py::none());
   m.def("set_batch_engine", &set_batch_engine,
         "engine of decode_batch: 0 automatic (the persistent kernel for <= 16 sequences of the 0.6B shape), "
         "1 layer by layer, 2 persistent where it applies");
