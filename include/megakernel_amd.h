@@ -365,6 +365,31 @@ hipError_t mk_attention_paged(const mk_paged_cache* cache, int q_heads, const vo
                               size_t workspace_bytes, hipStream_t stream);
 
 /*
+ * A token for every row of logits, drawn with a given random number. With x the row's logits, T its temperature and
+ *   w[i] = exp((x[i] - max x) / T),
+ * the candidates are the top_k largest logits (equal ones: the lower token first; top_k <= 0: all); of these, in
+ * that order, the fewest whose w add up to at least top_p of the candidates' sum (top_p >= 1: all); and of these
+ * those with w >= min_p (min_p <= 0: all). The likeliest token always stays. The answer is the first token, in the
+ * order of the vocabulary, at which the running sum of the candidates' w is above u times their whole sum, the last one
+ * if none is. T = 0: the likeliest token. All in 64 bits: sums within 2^-42 of each other count as equal.
+ *   logits     fp32, row r at logits + r * row_stride (elements, >= 0), vocab (1..2^20) of them
+ *   uniforms   [rows] fp32, u in [0, 1)
+ *   temperature, top_k, top_p, min_p     [rows] fp32, int32, fp32, fp32
+ *   tokens     [rows] int32
+ *   logprobs   [rows] fp32 or NULL: log(w / the candidates' sum) of the answer
+ *   workspace  mk_sample_workspace_bytes(rows, vocab) bytes of device memory, 256-byte aligned, owned by the caller,
+ *              not used after the call's work completes on `stream`
+ * A logit of -infinity is never drawn. A row with a NaN or +infinity, without a finite logit, with a negative,
+ * infinite or NaN temperature, or a NaN among u, top_p and min_p gets token -1 and a NaN. Asynchronous on `stream`;
+ * argument errors (also more than 65,535 rows) return hipErrorInvalidValue before any launch. The same call gives
+ * the same answers. Replaces the argmax of the reference's loop (/root/reference/model.py:97).
+ */
+size_t mk_sample_workspace_bytes(int rows, int vocab);
+hipError_t mk_sample(int rows, int vocab, const float* logits, int64_t row_stride, const float* uniforms,
+                     const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p,
+                     int32_t* tokens, float* logprobs, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/*
  * Several decode steps in one call, with no host synchronization between them: the device-side
  * multi-token loop. Step i (0 <= i < n) runs at position + i and reads its input token from device
  * memory, tokens[i] (int32, device array of n + 1 entries, tokens[0] set by the caller).

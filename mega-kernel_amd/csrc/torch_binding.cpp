@@ -748,6 +748,36 @@ torch::Tensor attention_paged(torch::Tensor q, torch::Tensor kp, torch::Tensor v
   return out;
 }
 
+// A token for every row of logits (mk_sample), drawn with the row's uniform number from its logits cut by top_k,
+// top_p and min_p at its temperature: fp32 [rows] each, top_k int32 [rows]. Returns (tokens int32 [rows], fp32
+// log-probabilities [rows]).
+std::tuple<torch::Tensor, torch::Tensor> sample(torch::Tensor logits, torch::Tensor uniforms, torch::Tensor temperature,
+                                                torch::Tensor top_k, torch::Tensor top_p, torch::Tensor min_p) {
+  TORCH_CHECK(logits.defined() && logits.dim() == 2 && logits.scalar_type() == torch::kFloat32 &&
+                  logits.size(1) >= 1 && logits.size(1) <= 1 << 20 && (logits.size(1) == 1 || logits.stride(1) == 1),
+              "megakernel: logits must be float32 [rows, vocab], contiguous in their last dimension, of a vocabulary "
+              "of 1 to 2^20");
+  const int64_t rows = logits.size(0), V = logits.size(1);
+  TORCH_CHECK(rows >= 1 && rows <= 65535, "megakernel: sample takes 1 to 65535 rows, got ", rows);
+  check_row_vector(uniforms, "uniforms", rows, torch::kFloat32, logits.device());
+  check_row_vector(temperature, "temperature", rows, torch::kFloat32, logits.device());
+  check_row_vector(top_k, "top_k", rows, torch::kInt32, logits.device());
+  check_row_vector(top_p, "top_p", rows, torch::kFloat32, logits.device());
+  check_row_vector(min_p, "min_p", rows, torch::kFloat32, logits.device());
+  TORCH_CHECK(logits.is_cuda(), "megakernel: logits must be a GPU tensor");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(logits.device());
+  hipStream_t stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(logits.device().index()).stream();
+  const size_t bytes = mk_sample_workspace_bytes((int)rows, (int)V);
+  auto ws = torch::empty({(int64_t)bytes}, logits.options().dtype(torch::kUInt8));
+  auto toks = torch::empty({rows}, logits.options().dtype(torch::kInt32));
+  auto logprobs = torch::empty({rows}, logits.options());
+  MK_HIP_CHECK(mk_sample((int)rows, (int)V, logits.data_ptr<float>(), rows > 1 ? logits.stride(0) : 0,
+                         uniforms.data_ptr<float>(), temperature.data_ptr<float>(), top_k.data_ptr<int32_t>(),
+                         top_p.data_ptr<float>(), min_p.data_ptr<float>(), toks.data_ptr<int32_t>(),
+                         logprobs.data_ptr<float>(), ws.data_ptr(), bytes, stream));
+  return {toks, logprobs};
+}
+
 int64_t status() {
   uint32_t s = 0;
   MK_HIP_CHECK(mk_status(&s));
@@ -830,6 +860,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "bf16 or fp32, lengths int32 [sequences] on device; returns [sequences, heads, 128] in q's type",
         py::arg("q"), py::arg("k_pages"), py::arg("v_pages"), py::arg("block_tables"), py::arg("lengths"),
         py::arg("k_scales") = py::none(), py::arg("v_scales") = py::none());
+  m.def("sample", &sample,
+        "a token for every row of logits fp32 [rows, vocab], drawn with uniforms fp32 [rows]: temperature, top_p, min_p "
+        "fp32 [rows], top_k int32 [rows] (0, 1 and 0 or less: no limit; temperature 0: the likeliest); returns (int32 "
+        "tokens, fp32 log-probabilities), [rows] each, on device",
+        py::arg("logits"), py::arg("uniforms"), py::arg("temperature"), py::arg("top_k"), py::arg("top_p"),
+        py::arg("min_p"));
   m.def("set_batch_engine", &set_batch_engine,
         "engine of decode_batch: 0 automatic (the persistent kernel for <= 16 sequences of the 0.6B shape), "
         "1 layer by layer, 2 persistent where it applies");
