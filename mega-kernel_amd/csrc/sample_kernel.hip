@@ -5,20 +5,25 @@
 //               order of the logits;
 //   answer      the first token of the vocabulary at which the running sum of the candidates' w exceeds u times
 //               their whole sum.
-// The answer is a whole number that a border may decide, so sums are exact ones of w rounded to 2^-43 of itself, and two
+// The answer is a whole number that a border may decide, so sums are exact ones of w rounded to 2^-37 of itself, and two
 // sums within SAME of each other count as equal: 5 of 10 equal logits reach half of them, and do not exceed it.
 //
 // Bins. p = x * 16 / T falls into bin floor(p), the same for equal logits wherever they are, and within its bin
-// w is exp((p - floor(p)) / 16), a polynomial on [1, 1.065), kept as a whole number of 2^-43: a bin's sum is a sum of
-// whole numbers, the same in any order, and its weight that sum times exp(bin / 16).
+// w is exp((p - floor(p)) / 16), a polynomial on [1, 1.065), kept as a whole number of 2^-36: a bin's sum is a sum of
+// whole numbers, the same in any order, and its weight that sum times exp(bin / 16). Its number of logits shares the
+// 64 bits, so that a logit is one atomic addition in LDS.
 //   sample_chunk_kernel  a workgroup takes 8,192 logits of a row from registers into 512 bins (32 in units of T) below
-//                        their maximum: number and sum of each; what lies lower is a tail of its own;
-//   sample_pick_kernel   a workgroup per row joins the chunks' bins, finds the bin that a border falls into, gathers
-//                        and sorts that bin's logits (narrowing it first where it holds more than 4,096), takes the
-//                        chunks' sums from their bins, and looks for the answer among the 8,192 logits of its chunk.
-// No logit but those of the border's bin and of the answer's chunk is looked at twice in full.
+//                        their maximum (what lies lower is a tail of its own), and lists the logits of the first bins,
+//                        up to 256 of them in all;
+//   sample_pick_kernel   a workgroup per row. Borders lie among the listed logits as a rule: it bins these, finds the
+//                        bin that a border falls into, sorts that bin's logits, and sums the kept ones chunk by chunk.
+//                        Where a border lies deeper it joins the chunks' bins instead and gathers the border's bin from
+//                        the row (narrowing it first where it holds more than 4,096). The answer is looked for among
+//                        the 8,192 logits of its chunk. Without any filter the chunks' sums are all that is needed.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include <algorithm>
 
 #include "mk_device.h"
 #include "mk_layers.h"
@@ -26,25 +31,34 @@
 
 namespace mkp {
 
-constexpr int SL = 2048;            // logits per wave of the first kernel
-constexpr int SC = 4 * SL;          // and per workgroup: a chunk
+constexpr int ST = 1024;            // threads of both kernels
+constexpr int SW = ST / 64;
+constexpr int SC = 8 * ST;          // logits of a chunk
 constexpr int SV_MAX = 1 << 20;
 constexpr int SCH = SV_MAX / SC;    // chunks of a row at most
 constexpr int NB = 512;             // bins; the last one is the tail
 constexpr double RES = 16;          // bins per unit of x / T
-constexpr int FIX = 43;             // bits behind the point of a weight within its bin
+constexpr int FIX = 36;             // bits behind the point of a weight within its bin
+constexpr double ONE = (double)(1ull << FIX);
+constexpr int CNT = 50;             // a bin's number of logits, at most 8,192, from this bit on
+constexpr u64 SUM_MASK = (1ull << CNT) - 1;
 constexpr double SAME = 1.0 / (1ull << 42);
-constexpr int CAP = 4096;           // logits that are sorted
+constexpr int CAP = 4096;           // logits of a bin that are taken together
+constexpr int RANKED = 256;         // logits that are sorted by counting
 constexpr int SUB = 2048;           // narrower bins of a bin that holds more
-constexpr int PT = 1024;            // threads of the second kernel
+constexpr int LISTED = 4;           // listed logits of a row per thread
+constexpr int LIST_MAX = 256;       // and of a chunk, a multiple of 64
 
 typedef float f4a __attribute__((ext_vector_type(4), aligned(4)));  // rows may start at any element
 
 struct SampleStat {
-  double ref;   // the bin of the chunk's maximum; -infinity: no finite logit
-  double tail;  // the weights below the bins, in units of exp(ref / 16)
-  u64 key;      // the largest logit, the lowest token of equal ones
-  int32_t tail_count, bad;
+  double ref;    // the bin of the chunk's maximum; -infinity: no finite logit
+  double total;  // its weights, in units of exp(ref / 16)
+  double tail;   // those below the bins
+  u64 key;       // the largest logit, the lowest token of equal ones; all bits set: the chunk has a NaN or +infinity
+  int32_t tail_count, number;
+  int32_t depth;  // bins 0 .. depth are listed in full; NB: all logits are
+  int32_t pad;
 };
 
 struct SampleArgs {
@@ -54,10 +68,10 @@ struct SampleArgs {
   const int32_t* top_k;
   int32_t* tokens;
   float* logprobs;
-  int vocab, chunks;
+  int vocab, chunks, list;  // list: logits listed of a chunk
   SampleStat* stat;  // [rows][chunks]
-  u64* sum;          // [rows][chunks][NB]
-  uint32_t* count;   // [rows][chunks][NB]
+  u64* bins;         // [rows][chunks][NB]
+  u64* listed;       // [rows][chunks][list], filled up with 0
 };
 
 __device__ __forceinline__ uint32_t logit_order(float x) {  // unsigned order is the numbers'
@@ -68,55 +82,126 @@ __device__ __forceinline__ float logit_of(uint32_t u) {
   return __uint_as_float((u & 0x80000000u) ? u & 0x7fffffffu : ~u);
 }
 __device__ __forceinline__ u64 logit_key(float x, int v) { return (u64)logit_order(x) << 32 | (0xffffffffu - (uint32_t)v); }
-__device__ __forceinline__ int token_of(u64 key) { return (int)(0xffffffffu - (uint32_t)key); }
+__device__ __forceinline__ float key_x(u64 key) { return logit_of((uint32_t)(key >> 32)); }
+__device__ __forceinline__ int key_v(u64 key) { return (int)(0xffffffffu - (uint32_t)key); }
 
-__device__ __forceinline__ double sum_over_wave(double v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
-  return v;
+// v of another lane by DPP, 0 where there is none
+template <int CTRL, int ROWS, typename V>
+__device__ __forceinline__ V from_lane(V v) {
+  if constexpr (sizeof(V) == 4) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+  } else {
+    const u64 u = __builtin_bit_cast(u64, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(V, (u64)hi << 32 | lo);
+  }
+}
+template <typename V>
+__device__ __forceinline__ V at_lane(V v, int lane) {
+  if constexpr (sizeof(V) == 4) {
+    return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+  } else {
+    const u64 u = __builtin_bit_cast(u64, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+    return __builtin_bit_cast(V, (u64)hi << 32 | lo);
+  }
+}
+// op over lanes 0 .. this one of each 16, and of the wave; 0 is op's neutral number
+template <typename V, typename F>
+__device__ __forceinline__ V scan_row16(V v, F op) {
+  v = op(v, from_lane<0x111, 0xf>(v));  // row_shr 1, 2, 4, 8
+  v = op(v, from_lane<0x112, 0xf>(v));
+  v = op(v, from_lane<0x114, 0xf>(v));
+  return op(v, from_lane<0x118, 0xf>(v));
+}
+template <typename V, typename F>
+__device__ __forceinline__ V scan_wave(V v, F op) {
+  v = scan_row16(v, op);
+  v = op(v, from_lane<0x142, 0xa>(v));  // row_bcast 15, 31
+  return op(v, from_lane<0x143, 0xc>(v));
+}
+template <typename V>
+__device__ __forceinline__ V plus(V a, V b) { return a + b; }
+template <typename V>
+__device__ __forceinline__ V sum_over_wave(V v) { return at_lane(scan_wave(v, plus<V>), 63); }
+__device__ __forceinline__ u64 max_over_wave(u64 v) {
+  return at_lane(scan_wave(v, [](u64 a, u64 b) { return a > b ? a : b; }), 63);
 }
 
-// exp(f / 16) for f in [0, 1]: the series about 1/32, whose next term is below 2^-47
-__device__ __forceinline__ double exp_in_bin(double f) {
-  constexpr double A = 1.0 / 16, E = 1.0317434074991028;  // exp(1/32)
-  const double g = f - 0.5;
-  double y = E * A * A * A * A * A * A / 720;
-  y = fma(y, g, E * A * A * A * A * A / 120);
-  y = fma(y, g, E * A * A * A * A / 24);
-  y = fma(y, g, E * A * A * A / 6);
-  y = fma(y, g, E * A * A / 2);
-  y = fma(y, g, E * A);
-  return fma(y, g, E);
+// Sums over the threads before this one and over all (numbers that commute exactly, or in a fixed order).
+template <typename V>
+__device__ __forceinline__ V block_before(V v, V* lds, V& total) {
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const V x = scan_wave(v, plus<V>);
+  __syncthreads();
+  if (lane == 63) lds[w] = x;
+  __syncthreads();
+  const V y = scan_row16(lds[lane & (SW - 1)], plus<V>);  // every wave: the waves' sums, up to each
+  static_assert(SW == 16);
+  total = at_lane(y, SW - 1);
+  const V before = at_lane(y, max(w - 1, 0));
+  return (w ? before : (V)0) + (x - v);
 }
-// the same as a whole number of 2^-FIX
-__device__ __forceinline__ u64 fixed_in_bin(double f) {
-  const u64 b = __builtin_bit_cast(u64, exp_in_bin(f));  // in [1, 2)
-  return (((b & 0xfffffffffffffull) | 1ull << 52) + (1ull << (51 - FIX))) >> (52 - FIX);
+
+// How logits at a temperature fall into bins: c bins per logit. `in` is 1, or 0 where bins are so small (p above 2^45)
+// that different logits lie thousands of bins apart and p has too few digits behind the point: any place in the bin
+// serves.
+struct Scale {
+  double c, in;
+};
+__device__ __forceinline__ Scale scale_of_row(float T, double top) {
+  Scale s;
+  s.c = RES / (double)T;
+  s.in = fabs(top * s.c) < 0x1p45 ? 1.0 : 0.0;
+  return s;
 }
-// The place of a logit in its bin. Above 2^53 p has no digits behind the point, and different logits lie in bins far
-// from each other's: any number serves.
-__device__ __forceinline__ double in_bin(float x, double c, double fl) {
-  return fmin(fmax(fma((double)x, c, -fl), 0.0), 1.0);
+// exp(f / 16) for the place f in [0, 1] of a logit in its bin fl, in whole numbers of 2^-FIX: the series, whose next
+// term is below 2^-40, behind 2^16, where a double's last bit is 2^-36.
+__device__ __forceinline__ u64 fixed_in_bin(float x, const Scale& s, double fl) {
+  constexpr double A = 1.0 / 16, BIG = 1 << (52 - FIX);
+  const double f = fma((double)x, s.c, -fl) * s.in;
+  double y = A * A * A * A * A * A / 720;
+  y = fma(y, f, A * A * A * A * A / 120);
+  y = fma(y, f, A * A * A * A / 24);
+  y = fma(y, f, A * A * A / 6);
+  y = fma(y, f, A * A / 2);
+  y = fma(y, f, A);
+  return __builtin_bit_cast(u64, fma(y, f, 1 + BIG)) - __builtin_bit_cast(u64, BIG);
 }
 // exp(t / 16) for t <= 0 to fp32's accuracy, over the doubles' range: the tail's weights, below exp(-31) of the largest
 __device__ __forceinline__ double exp_tail(double t) {
   const double p = t * (1.4426950408889634 / RES), n = floor(fmax(p, -1100.0));
   return ldexp((double)__builtin_amdgcn_exp2f((float)fmax(p - n, 0.0)), (int)n);
 }
+// the bin of floor(p) below `ref`, the tail's for all from there on
+__device__ __forceinline__ int bin_of(double ref, double fl) {
+  const double k = ref - fl;
+  return k < NB - 1 ? (int)k : NB - 1;
+}
 
-__global__ void __launch_bounds__(256) sample_chunk_kernel(const SampleArgs a) {
-  __shared__ u64 sum[NB];
-  __shared__ uint32_t count[NB];
-  __shared__ u64 skey[4];
-  __shared__ double stail[4];
-  __shared__ int sbad[4], stc[4];
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int row = blockIdx.y, v0 = blockIdx.x * SC + w * SL + 4 * lane;  // this lane's logits: v0 + 256 j + q
-  const float* x = a.logits + row * a.row_stride;
-  const float T = a.temperature[row];
-  float f[SL / 64];
+// Both kernels run each of their instructions a few times at most, and what takes their time beside the loads is the
+// fetch of cold code. So loops are not unrolled: eight numbers in registers turn round instead.
+__device__ __forceinline__ void turn(float (&f)[8]) {
+  const float x = f[0];
 #pragma unroll
-  for (int j = 0; j < SL / 256; ++j) {
+  for (int i = 0; i < 7; ++i) f[i] = f[i + 1];
+  f[7] = x;
+}
+
+__global__ void __launch_bounds__(ST, 8) sample_chunk_kernel(const SampleArgs a) {
+  __shared__ u64 bins[NB];
+  __shared__ u64 skey[SW];
+  __shared__ double stail[SW], stotal[SW];
+  __shared__ int32_t stc[SW], scan[SW];
+  __shared__ int sdepth;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row = blockIdx.y, v0 = blockIdx.x * SC + 512 * w + 4 * lane;  // this lane's logits: v0 + 256 j + q
+  const float* x = a.logits + row * a.row_stride;
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
     const int v = v0 + 256 * j;
     if (v + 3 < a.vocab) {
       const f4a t = *reinterpret_cast<const f4a*>(x + v);
@@ -127,144 +212,125 @@ __global__ void __launch_bounds__(256) sample_chunk_kernel(const SampleArgs a) {
       for (int q = 0; q < 4; ++q) f[4 * j + q] = v + q < a.vocab ? x[v + q] : -INFINITY;
     }
   }
-  for (int i = tid; i < NB; i += 256) {
-    sum[i] = 0;
-    count[i] = 0;
-  }
+  const float T = a.temperature[row];
+  const bool filtered = a.top_k[row] > 0 || !(a.top_p[row] >= 1.f) || a.min_p[row] > 0.f;
+  if (tid < NB) bins[tid] = 0;
+  if (tid == 0) sdepth = -1;
   float m = -INFINITY;
   bool bad = false;
 #pragma unroll
-  for (int i = 0; i < SL / 64; ++i) {
+  for (int i = 0; i < 8; ++i) {
     m = fmaxf(m, f[i]);
     bad |= !(f[i] < INFINITY);  // NaN too
   }
-  int at = INT32_MAX;
+  int at = SV_MAX;
 #pragma unroll
-  for (int i = SL / 64 - 1; i >= 0; --i)
+  for (int i = 7; i >= 0; --i)
     if (f[i] == m) at = v0 + 256 * (i >> 2) + (i & 3);
-  u64 key = logit_key(m, min(at, SV_MAX));
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const u64 y = __shfl_xor(key, o);
-    key = key > y ? key : y;
-  }
+  u64 key = max_over_wave(bad ? ~(u64)0 : logit_key(m, min(at, SV_MAX)));
   if (lane == 0) skey[w] = key;
-  const bool wbad = __builtin_amdgcn_ballot_w64(bad) != 0;
-  if (lane == 0) sbad[w] = wbad;
   __syncthreads();
-  key = max(max(skey[0], skey[1]), max(skey[2], skey[3]));
-  const float top = logit_of((uint32_t)(key >> 32));
-  const bool empty = top == -INFINITY;
-  const double c = RES / (double)T;
-  const double ref = empty ? -INFINITY : floor((double)top * c);
+  key = max_over_wave(skey[lane & (SW - 1)]);
+  const float top = key_x(key);  // NaN, where all bits are set
+  const int64_t slot = (int64_t)row * a.chunks + blockIdx.x;
+  const Scale s = scale_of_row(T, top);
+  SampleStat out{};
+  out.ref = top == -INFINITY ? -INFINITY : floor((double)top * s.c);
+  out.key = key;
+  out.depth = NB;
+  const bool none = !(T > 0.f) || !(top > -INFINITY);  // the likeliest, no number, or an answer that has failed
+  int bin[8];
   double tail = 0;
   int tc = 0;
-  if (T > 0.f && !empty) {
-#pragma unroll
-    for (int i = 0; i < SL / 64; ++i) {
-      const double p = (double)f[i] * c, fl = floor(p);
-      const double k = ref - fl;
-      if (k < NB - 1) {
-        atomicAdd(&sum[(int)k], fixed_in_bin(in_bin(f[i], c, fl)));
-        atomicAdd(&count[(int)k], 1u);
-      } else if (f[i] > -INFINITY) {
-        tail += exp_tail(p - ref);
+  if (!none) {
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      const double p = (double)f[0] * s.c, fl = floor(p);
+      const int j = bin_of(out.ref, fl);
+      if (j < NB - 1) {
+        atomicAdd(&bins[j], fixed_in_bin(f[0], s, fl) + (1ull << CNT));
+      } else if (f[0] > -INFINITY) {
+        tail += exp_tail(p - out.ref);
         ++tc;
       }
-    }
-  }
-  tail = sum_over_wave(tail);
+      turn(f);
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) tc += __shfl_xor(tc, o);
-  if (lane == 0) {
-    stail[w] = tail;
-    stc[w] = tc;
+      for (int k = 0; k < 7; ++k) bin[k] = bin[k + 1];
+      bin[7] = j;
+    }
+    if (__builtin_amdgcn_ballot_w64(tc > 0)) {
+      tail = sum_over_wave(tail);
+      tc = sum_over_wave(tc);
+    }
+    if (lane == 0) {
+      stail[w] = tail;
+      stc[w] = tc;
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  const int64_t slot = (int64_t)row * a.chunks + blockIdx.x;
-  for (int i = tid; i < NB; i += 256) {
-    a.sum[slot * NB + i] = sum[i];
-    a.count[slot * NB + i] = count[i];
+  const u64 b = tid < NB && !none ? bins[tid] : 0;
+  if (!none) {
+    const double weight = w < NB / 64 ? sum_over_wave((double)(b & SUM_MASK) / ONE * exp(-tid / RES)) : 0;
+    if (lane == 0) stotal[w] = weight;
+    int all;
+    const int upto = block_before<int32_t>((int)(b >> CNT), scan, all) + (int)(b >> CNT);  // (stotal is written behind it)
+    const u64 in = __builtin_amdgcn_ballot_w64(tid < NB - 1 && upto <= a.list);
+    if (filtered && lane == 0 && in) atomicAdd(&sdepth, __popcll(in));
+#pragma unroll 1
+    for (int i = 0; i < SW; ++i) {
+      out.tail += stail[i];
+      out.tail_count += stc[i];
+      out.total += stotal[i];
+    }
+    out.total += out.tail;
+    out.number = all + out.tail_count;
   }
-  if (tid == 0) {
-    SampleStat s;
-    s.ref = ref;
-    s.tail = (stail[0] + stail[1]) + (stail[2] + stail[3]);
-    s.key = key;
-    s.tail_count = stc[0] + stc[1] + stc[2] + stc[3];
-    s.bad = sbad[0] | sbad[1] | sbad[2] | sbad[3];
-    a.stat[slot] = s;
+  if (filtered) {
+    if (tid < NB) a.bins[slot * NB + tid] = b;
+    // the bins that the list holds in full, and their logits in the threads' order
+    int n = 0;
+    if (!none) {
+      __syncthreads();
+      out.depth = out.number <= a.list ? NB : sdepth;
+      int mine = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mine += f[i] > -INFINITY && bin[i] <= out.depth;
+      int to = block_before<int32_t>(mine, scan, n);
+      if (mine > 0)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (f[i] > -INFINITY && bin[i] <= out.depth)
+            a.listed[slot * a.list + to++] = logit_key(f[i], v0 + 256 * (i >> 2) + (i & 3));
+    }
+    for (int i = n + tid; i < a.list; i += ST) a.listed[slot * a.list + i] = 0;
   }
+  if (tid == 0) a.stat[slot] = out;
 }
 
 // The least u32 in [lo, hi] for which `test`, false up to some number and true from there on, is true (hi, if none
-// below it is): by all lanes of a wave, 64 places at a time.
+// below it is), by all lanes of a wave: 64 numbers around a guess as a rule decide, else 64 places at a time.
 template <typename F>
-__device__ __forceinline__ uint32_t least_true(uint32_t lo, uint32_t hi, F test) {
+__device__ __forceinline__ uint32_t least_true(uint32_t lo, uint32_t hi, uint32_t guess, F test) {
   const int lane = threadIdx.x & 63;
-  uint64_t a = lo, n = (uint64_t)hi - lo;  // the answer lies in [a, a + n]
-  while (n > 0) {
-    const uint64_t step = (n + 63) / 64;  // places a + step - 1, a + 2 step - 1, ...: is it at or before there?
-    const uint64_t at = a + (lane + 1) * step - 1;
-    const u64 hit = __builtin_amdgcn_ballot_w64(at >= a + n || test((uint32_t)at));
+  uint64_t a = max(lo, min(hi, max(guess, 32u) - 32)), n = 63;
+  bool near = true;
+#pragma unroll 1
+  while (n > 0) {  // the answer lies in [a, a + n], once it is not near
+    const uint64_t step = (n + 63) / 64, end = min((uint64_t)hi, a + n);
+    const uint64_t at = near ? a + lane : a + (lane + 1) * step - 1;  // is it at or before there?
+    const u64 hit = __builtin_amdgcn_ballot_w64(at >= (near ? (uint64_t)hi : end) || test((uint32_t)min((uint64_t)hi, at)));
     const int first = hit ? __ffsll(hit) - 1 : 64;
-    const uint64_t end = a + n;
-    a += first * step;
-    n = min((uint64_t)(step - 1), end - a);
-    if (a > end) { a = end; n = 0; }
+    if (near) {
+      near = false;
+      if (hit && (first > 0 || a == lo)) return (uint32_t)min((uint64_t)hi, a + first);
+      a = lo;
+      n = hi - lo;
+    } else {
+      a = min(end, a + first * step);
+      n = min(step - 1, end - a);
+    }
   }
   return (uint32_t)a;
-}
-
-struct PickSmem {
-  double et[NB];        // exp(-j / 16)
-  double upto[NB];      // weights of bins 0 .. j
-  int32_t cupto[NB];    // their logits
-  int32_t delta[SCH];   // bins of the row above the chunk's first (at most 2^20)
-  double scale[SCH], ref[SCH], tail[SCH], csum[SCH];
-  int32_t tcount[SCH];
-  u64 part[SCH];        // kept weights of the border's bin, by chunk
-  union {
-    u64 list[CAP];
-    struct {
-      u64 sum[SUB];
-      uint32_t count[SUB];
-    } sub;
-    struct {
-      u64 sum[NB];
-      int32_t count[NB];
-      double tail[PT / 64];
-      int32_t tcount[PT / 64];
-    } half;
-  };
-  double wsum[PT / 64];
-  int32_t wcount[PT / 64];
-  u64 wfix[PT / 64];
-  int found, n, last;
-  uint32_t klo, khi;
-  double w0;
-};
-
-// Sums over the threads before this one and over all (numbers that commute exactly, or in the threads' order).
-template <typename V>
-__device__ __forceinline__ V block_before(V v, V* lds, V& total) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  V x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const V y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();
-  if (lane == 63) lds[w] = x;
-  __syncthreads();
-  V before = 0, all = 0;
-  for (int i = 0; i < PT / 64; ++i) {
-    if (i == w) before = all;
-    all += lds[i];
-  }
-  total = all;
-  return before + (x - v);
 }
 
 // A row's border: kept are bins 0 .. bin - 1 and, of bin `bin`, all (part false) or the logits above x and those
@@ -274,24 +340,202 @@ struct Cut {
   bool part;
   float x;
   int token;
+  __device__ __forceinline__ bool keeps(int j, float y, int v) const {
+    return j < bin || (j == bin && (!part || y > x || (y == x && v <= token)));
+  }
 };
+
+// What the threads of a row share.
+struct PickSmem {
+  double et[NB];        // exp(-j / 16)
+  double upto[NB];      // weights of bins 0 .. j
+  int32_t cupto[NB];    // their logits
+  int32_t delta[SCH];   // bins of the row above the chunk's first (at most 2^20)
+  double scale[SCH], csum[SCH];
+  u64 part[SCH];        // kept weights of the border's bin, by chunk
+  u64 lkey[LISTED * ST];  // the listed logits; where a border lies deeper, no longer needed
+  u64 lbin[LISTED * ST];  // their bins, above LBIN, and weights in their bins
+  u64 list[CAP];  // logits of a bin
+  union {
+    u64 bins[NB];
+    u64 sub[SUB];  // numbers and sums of narrower bins
+    struct {
+      u64 sum[SUB];
+      uint32_t count[SUB];
+    } many;
+    struct {
+      u64 raw[RANKED], key[RANKED];
+    } sort;
+    struct {
+      u64 sum[NB];
+      int32_t count[NB];
+      double tail[SW];
+      int32_t tcount[SW];
+    } half;
+    double lsum[LISTED * SW];  // kept weights of 64 listed logits each
+  };
+  double wsum[SW];
+  int32_t wcount[SW];
+  u64 wfix[SW], wfix2[SW];
+  int first[SW], last[SW];
+  int found, n, above, depth, number;
+  u64 sum, key;
+  uint32_t klo, khi;
+  double z, goal;
+  Cut cut;
+};
+__device__ __forceinline__ PickSmem& smem() {
+  __shared__ PickSmem s;
+  return s;
+}
+constexpr int LBIN = 40;
 
 struct Row {
   const float* x;
-  int vocab, chunks;
-  double c, ref;  // bins per logit; the bin of the largest
+  int vocab;
+  Scale s;
+  double ref;  // the bin of the largest
   uint32_t ktop, kmin;
 };
 
-// fn(logit, token) for every logit of the row whose order's number lies in [lo, hi], by the whole workgroup.
+__device__ __forceinline__ double weight_below(int j) { return j > 0 ? smem().upto[j - 1] : 0.0; }
+__device__ __forceinline__ int number_below(int j) { return j > 0 ? smem().cupto[j - 1] : 0; }
+// the first bin that passes a test that stays passed, the last one if none does
+template <typename F>
+__device__ __forceinline__ int first_bin(F test) {
+  PickSmem& sm = smem();
+  const int tid = threadIdx.x;
+  __syncthreads();
+  if (tid < NB && (tid == 0 || !test(tid - 1)) && (tid == NB - 1 || test(tid))) sm.found = tid;
+  __syncthreads();
+  return sm.found;
+}
+
+// The weight of a logit of the row's bin j, in 2^-FIX of exp(-j / 16).
+__device__ __forceinline__ u64 fixed_weight(const Scale& s, double ref, float x, int j) {
+  const double p = (double)x * s.c, fl = floor(p);
+  if (j == NB - 1) return (u64)(exp_tail(p - ref + (NB - 1)) * ONE);
+  return fixed_in_bin(x, s, fl);
+}
+
+// The border among sm.list, n <= CAP logits of bin j: the first of them, in order, at which their number reaches `rank`
+// (by_rank), or their sum reaches `goal` (in 2^-FIX of the bin's unit; the last of `most` logits, if none of them does),
+// `above` and `sabove` being those of the bin before the list. Into sm.key, and the sum up to it into sm.sum.
+// The range of the keys is narrowed, SUB bins at a time, to the few that are sorted.
+__device__ __attribute__((noinline)) void border_in_list(int n, int j, double c, double in, double ref, bool by_rank,
+                                                         int rank, double goal, int most, int above, u64 sabove) {
+  PickSmem& sm = smem();
+  const int tid = threadIdx.x;
+  const Scale s = {c, in};
+  const int size = n;
+  auto reached = [&](int number, u64 sum) { return by_rank ? number >= rank : (double)sum >= goal || number >= most; };
+  u64 lo = 0, hi = ~(u64)0;
+  if (n > RANKED) {  // the list's own range
+    u64 l = ~(u64)0, h = 0;
+#pragma unroll 1
+    for (int i = tid; i < size; i += ST) {
+      l = min(l, sm.list[i]);
+      h = max(h, sm.list[i]);
+    }
+    h = max_over_wave(h);
+    l = ~max_over_wave(~l);
+    __syncthreads();
+    if ((tid & 63) == 0) {
+      sm.wfix[tid >> 6] = h;
+      sm.wfix2[tid >> 6] = l;
+    }
+    __syncthreads();
+    hi = max_over_wave(sm.wfix[tid & (SW - 1)]);
+    lo = ~max_over_wave(~sm.wfix2[tid & (SW - 1)]);
+  }
+#pragma unroll 1
+  while (n > RANKED) {
+    const int bits = 64 - __clzll((hi - lo) | 1), shift = max(0, bits - 11);
+    __syncthreads();
+    for (int i = tid; i < SUB; i += ST) sm.sub[i] = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int i = tid; i < size; i += ST) {
+      const u64 k = sm.list[i];
+      if (k >= lo && k <= hi) atomicAdd(&sm.sub[(hi - k) >> shift], fixed_weight(s, ref, key_x(k), j) + (1ull << CNT));
+    }
+    __syncthreads();
+    const u64 b0 = sm.sub[2 * tid], b1 = sm.sub[2 * tid + 1];
+    u64 all;
+    const u64 before = block_before<u64>(b0 + b1, sm.wfix, all);
+    const int c0 = above + (int)(before >> CNT);
+    const u64 s0 = sabove + (before & SUM_MASK);
+    const int c1 = c0 + (int)(b0 >> CNT), c2 = c1 + (int)(b1 >> CNT);
+    const u64 s1 = s0 + (b0 & SUM_MASK), s2 = s1 + (b1 & SUM_MASK);
+    // the one bin where it is reached, the last one with any logits if nowhere
+    const int end = above + n;
+    const bool r0 = c0 > above && (reached(c0, s0) || c0 == end), r1 = c1 > above && (reached(c1, s1) || c1 == end);
+    const bool r2 = c2 > above && (reached(c2, s2) || c2 == end);
+    if (!r0 && r2) {
+      sm.found = r1 ? 2 * tid : 2 * tid + 1;
+      sm.n = (int)((r1 ? b0 : b1) >> CNT);
+      sm.above = r1 ? c0 : c1;
+      sm.sum = r1 ? s0 : s1;
+    }
+    __syncthreads();
+    n = sm.n;
+    above = sm.above;
+    sabove = sm.sum;
+    hi -= (u64)sm.found << shift;
+    const u64 width = (1ull << shift) - 1;
+    lo = hi - lo > width ? hi - width : lo;
+  }
+  // the rest sorted: a key's place is how many are larger, four lanes to a key
+  __syncthreads();
+  if (tid == 0) sm.n = 0;
+  __syncthreads();
+#pragma unroll 1
+  for (int i = tid; i < size; i += ST) {
+    const u64 k = sm.list[i];
+    if (k >= lo && k <= hi) {
+      const int at = atomicAdd(&sm.n, 1);
+      if (at < RANKED) sm.sort.raw[at] = k;
+    }
+  }
+  __syncthreads();
+  {
+    const int i = tid >> 2;
+    const u64 k = i < n ? sm.sort.raw[i] : 0;
+    int place = 0;
+    if (i < n)
+#pragma unroll 1
+      for (int e = tid & 3; e < n; e += 4) place += sm.sort.raw[e] > k;
+    place += __shfl_xor(place, 1);
+    place += __shfl_xor(place, 2);
+    if (i < n && (tid & 3) == 0) sm.sort.key[place] = k;
+  }
+  __syncthreads();
+  const u64 k = tid < n ? sm.sort.key[tid] : 0, mine = tid < n ? fixed_weight(s, ref, key_x(k), j) : 0;
+  u64 all;
+  const u64 before = sabove + block_before<u64>(mine, sm.wfix, all);
+  if (tid < n && (tid == 0 || !reached(above + tid, before)) && (tid == n - 1 || reached(above + tid + 1, before + mine))) {
+    sm.key = k;
+    sm.sum = before + mine;
+  }
+  __syncthreads();
+}
+
+// -----------------------------------------------------------------------------------------------------------
+// Borders that lie deeper than the listed logits: from the chunks' bins and the row's logits.
+// -----------------------------------------------------------------------------------------------------------
+
+// fn(logit, token) for every logit of the row whose order's number lies in [lo, hi], by the whole workgroup. 32 logits
+// to a thread are compared as numbers (both zeros are one, with one place in the order); the few that pass are read again.
 template <typename F>
 __device__ __forceinline__ void sweep(const Row& r, uint32_t lo, uint32_t hi, F fn) {
   const int tid = threadIdx.x;
-  for (int base = 0; base < r.vocab; base += 8 * 4 * PT) {
+  const float flo = logit_of(lo), fhi = logit_of(hi);
+#pragma unroll 1
+  for (int base = 0; base < r.vocab; base += 8 * 4 * ST) {
     float f[8][4];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int v = base + 4 * PT * j + 4 * tid;
+      const int v = base + 4 * ST * j + 4 * tid;
       if (v + 3 < r.vocab) {
         const f4a t = *reinterpret_cast<const f4a*>(r.x + v);
 #pragma unroll
@@ -301,133 +545,107 @@ __device__ __forceinline__ void sweep(const Row& r, uint32_t lo, uint32_t hi, F 
         for (int q = 0; q < 4; ++q) f[j][q] = v + q < r.vocab ? r.x[v + q] : -INFINITY;
       }
     }
+    uint32_t mask = 0;  // the first logit in the highest bit
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const uint32_t o = logit_order(f[j][q]);  // not the numbers: -0 and 0 are one number, and one place alone
-        if (o >= lo && o <= hi) fn(f[j][q], base + 4 * PT * j + 4 * tid + q);
-      }
+      for (int q = 0; q < 4; ++q) mask = mask + mask + (__builtin_amdgcn_fmed3f(f[j][q], flo, fhi) == f[j][q]);
+#pragma unroll 1
+    while (mask) {
+      const int e = __clz(mask), v = base + 4 * ST * (e >> 2) + 4 * tid + (e & 3);
+      mask &= ~(0x80000000u >> e);
+      const float x = r.x[v];
+      const uint32_t o = logit_order(x);
+      if (o >= lo && o <= hi) fn(x, v);
+    }
   }
 }
 
-// The weight of a logit of bin j (the row's), in 2^-FIX of exp(-j / 16).
-__device__ __forceinline__ u64 fixed_weight(const Row& r, float x, int j) {
-  const double p = (double)x * r.c, fl = floor(p);
-  if (j == NB - 1) return (u64)(exp_tail(p - r.ref + (NB - 1)) * (double)(1ull << FIX));
-  return fixed_in_bin(in_bin(x, r.c, fl));
-}
+__device__ __forceinline__ u64 fixed_weight(const Row& r, float x, int j) { return fixed_weight(r.s, r.ref, x, j); }
 
-// The order's numbers of bin j's logits, by wave 0.
-__device__ __forceinline__ void bin_range(const Row& r, int j, PickSmem& sm) {
-  if (threadIdx.x < 64) {
-    auto from = [&](double b) {  // the least logit of bin b or above
-      return least_true(r.kmin, r.ktop, [&](uint32_t k) { return floor((double)logit_of(k) * r.c) >= b; });
-    };
-    const uint32_t lo = j == NB - 1 ? r.kmin : from(r.ref - j);
-    const uint32_t hi = j == 0 ? r.ktop : from(r.ref - (j - 1)) - 1;
-    if (threadIdx.x == 0) {
-      sm.klo = lo;
-      sm.khi = hi;
+// The order's numbers of bin j's logits, by two waves.
+__device__ __forceinline__ void bin_range(const Row& r, int j) {
+  PickSmem& sm = smem();
+  __syncthreads();
+  if (threadIdx.x < 128) {
+    const bool high = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const double b = r.ref - j + high;  // the least logit of bin j, or of the one above
+    uint32_t k = high ? r.ktop + 1 : r.kmin;
+    if (high ? j > 0 : j < NB - 1) {
+      const float guess = (float)fmin(fmax(b / r.s.c, -3.4028234663852886e38), (double)logit_of(r.ktop));
+      k = least_true(r.kmin, r.ktop, logit_order(guess), [&](uint32_t o) { return floor((double)logit_of(o) * r.s.c) >= b; });
+    }
+    if ((threadIdx.x & 63) == 0) {
+      if (high) sm.khi = k - 1;
+      else sm.klo = k;
     }
   }
   __syncthreads();
 }
 
-// Gathers the logits of the order's numbers [klo, khi] (n <= CAP of them) and sorts them, the first of the order first.
-__device__ __forceinline__ void gather(const Row& r, uint32_t klo, uint32_t khi, int n, PickSmem& sm) {
-  const int tid = threadIdx.x;
+// Gathers the logits of the order's numbers [klo, khi], at most CAP.
+__device__ __forceinline__ void gather(const Row& r, uint32_t klo, uint32_t khi) {
+  PickSmem& sm = smem();
   __syncthreads();
-  if (tid == 0) sm.n = 0;
+  if (threadIdx.x == 0) sm.n = 0;
   __syncthreads();
   sweep(r, klo, khi, [&](float x, int v) {
     const int at = atomicAdd(&sm.n, 1);
     if (at < CAP) sm.list[at] = logit_key(x, v);
   });
   __syncthreads();
-  const int got = min(sm.n, CAP);  // n
-  int size = 64;
-  while (size < max(n, got)) size *= 2;
-  for (int i = got + tid; i < size; i += PT) sm.list[i] = 0;
-  __syncthreads();
-  if (size <= 256) {  // a key's place is how many are larger: four lanes to a key
-    const int i = tid >> 2;
-    u64 key = 0;
-    int place = 0;
-    if (i < n) {
-      key = sm.list[i];
-      for (int e = tid & 3; e < n; e += 4) place += sm.list[e] > key;
-    }
-    place += __shfl_xor(place, 1);
-    place += __shfl_xor(place, 2);
-    __syncthreads();
-    if (i < n && (tid & 3) == 0) sm.list[place] = key;
-    __syncthreads();
-    return;
-  }
-  for (int k = 2; k <= size; k *= 2)
-    for (int j = k / 2; j > 0; j /= 2) {
-      for (int p = tid; p < size / 2; p += PT) {
-        const int lo = 2 * p - (p & (j - 1)), hi = lo + j;
-        const u64 a = sm.list[lo], b = sm.list[hi];
-        if ((a < b) == ((lo & k) == 0)) {
-          sm.list[lo] = b;
-          sm.list[hi] = a;
-        }
-      }
-      __syncthreads();
-    }
 }
 
-// Finds the border within bin j: the first of its logits, in order, at which their number reaches `rank` (by_rank), or
-// their sum reaches `goal` (in 2^-FIX of the bin's unit; the last of `most` logits, if none of them does). Returns
-// the sum up to it. Leaves the list of the whole bin where it holds no more than CAP (listed).
-__device__ u64 border_in_bin(const Row& r, int j, int count, bool by_rank, int rank, double goal, int most, bool& listed,
-                             Cut& cut, PickSmem& sm) {
+// Finds the border within bin j, which has `count` logits: the first of them, in order, at which their number reaches
+// `rank` (by_rank), or their sum reaches `goal` (in 2^-FIX of the bin's unit; the last of `most` logits, if none of
+// them does). Returns the sum up to it. Leaves the list of the whole bin where it holds no more than CAP.
+__device__ __forceinline__ u64 border_in_bin(const Row& r, int j, int count, bool by_rank, int rank, double goal,
+                                             int most, Cut& cut) {
+  PickSmem& sm = smem();
   const int tid = threadIdx.x;
-  bin_range(r, j, sm);
+  bin_range(r, j);
   uint32_t klo = sm.klo, khi = sm.khi;
   int n = count, above = 0;  // logits in [klo, khi], and of the bin above khi
   u64 sabove = 0;
-  listed = n <= CAP;
+  auto reached = [&](int number, u64 sum) { return by_rank ? number >= rank : (double)sum >= goal || number >= most; };
   while (n > CAP && klo < khi) {  // narrow: SUB bins of the order's numbers, the first of the order first
     int shift = 0;
     while (((khi - klo) >> shift) >= SUB) ++shift;
     __syncthreads();
-    for (int i = tid; i < SUB; i += PT) {
-      sm.sub.sum[i] = 0;
-      sm.sub.count[i] = 0;
+    for (int i = tid; i < SUB; i += ST) {
+      sm.many.sum[i] = 0;
+      sm.many.count[i] = 0;
     }
-    if (tid == 0) sm.found = SUB - 1;
     __syncthreads();
     sweep(r, klo, khi, [&](float x, int) {
       const uint32_t b = (khi - logit_order(x)) >> shift;
-      atomicAdd(&sm.sub.count[b], 1u);
-      atomicAdd(&sm.sub.sum[b], fixed_weight(r, x, j));
+      atomicAdd(&sm.many.count[b], 1u);
+      atomicAdd(&sm.many.sum[b], fixed_weight(r, x, j));
     });
     __syncthreads();
-    int c0 = (int)sm.sub.count[2 * tid], c1 = (int)sm.sub.count[2 * tid + 1], call;
-    u64 s0 = sm.sub.sum[2 * tid], s1 = sm.sub.sum[2 * tid + 1], sall;
-    const int cb = above + block_before<int32_t>(c0 + c1, sm.wcount, call);
-    const u64 sb = sabove + block_before<u64>(s0 + s1, sm.wfix, sall);
-    auto reached = [&](int number, u64 sum) { return by_rank ? number >= rank : (double)sum >= goal || number >= most; };
-    if (reached(cb + c0, sb + s0)) atomicMin(&sm.found, 2 * tid);
-    else if (reached(cb + c0 + c1, sb + s0 + s1)) atomicMin(&sm.found, 2 * tid + 1);
-    __syncthreads();
-    const int b = min(sm.found, (int)((khi - klo) >> shift));
-    if (tid == b / 2) {
-      sm.n = b & 1 ? c1 : c0;
-      sm.last = b & 1 ? cb + c0 : cb;
-      sm.wfix[0] = b & 1 ? sb + s0 : sb;
+    const int c0 = (int)sm.many.count[2 * tid], c1 = (int)sm.many.count[2 * tid + 1];
+    const u64 s0 = sm.many.sum[2 * tid], s1 = sm.many.sum[2 * tid + 1];
+    int call;
+    u64 sall;
+    int cb = above + block_before<int32_t>(c0 + c1, sm.wcount, call);
+    u64 sb = sabove + block_before<u64>(s0 + s1, sm.wfix, sall);
+    // the one place where it is reached, at the end of the range if nowhere before
+    const int lastb = (int)((khi - klo) >> shift);
+    const bool r0 = reached(cb + c0, sb + s0) || 2 * tid >= lastb, r1 = reached(cb + c0 + c1, sb + s0 + s1) || 2 * tid + 1 >= lastb;
+    const bool rb = tid > 0 && (reached(cb, sb) || 2 * tid - 1 >= lastb);
+    if (!rb && r1) {
+      sm.found = r0 ? 2 * tid : 2 * tid + 1;
+      sm.n = r0 ? c0 : c1;
+      sm.above = r0 ? cb : cb + c0;
+      sm.sum = r0 ? sb : sb + s0;
     }
     __syncthreads();
     n = sm.n;
-    above = sm.last;
-    sabove = sm.wfix[0];
-    const uint32_t top = khi - ((uint32_t)b << shift);
-    const uint32_t width = (1u << shift) - 1;
-    klo = top - klo > width ? top - width : klo;
-    khi = top;
+    above = sm.above;
+    sabove = sm.sum;
+    const uint32_t hi = khi - ((uint32_t)sm.found << shift), width = (1u << shift) - 1;
+    klo = hi - klo > width ? hi - width : klo;
+    khi = hi;
     __syncthreads();
   }
   if (n > CAP) {  // equal logits: so many of them, the lowest tokens
@@ -444,7 +662,7 @@ __device__ u64 border_in_bin(const Row& r, int j, int count, bool by_rank, int r
     // the token of the take-th: tokens in their order, a piece of 4 to a thread
     int seen = 0;
     if (tid == 0) sm.found = 0;
-    for (int base = 0; base < r.vocab && seen < take; base += 4 * PT) {
+    for (int base = 0; base < r.vocab && seen < take; base += 4 * ST) {
       int mine = 0, all;
       for (int q = 0; q < 4; ++q) {
         const int v = base + 4 * tid + q;
@@ -462,118 +680,44 @@ __device__ u64 border_in_bin(const Row& r, int j, int count, bool by_rank, int r
     cut = {j, true, x, sm.found};
     return sabove + (u64)take * w;
   }
-  gather(r, klo, khi, n, sm);
-  // running sums of the sorted logits, four to a thread
-  u64 s[4], mine = 0, all;
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int i = 4 * tid + q;
-    s[q] = i < n ? fixed_weight(r, logit_of((uint32_t)(sm.list[i] >> 32)), j) : 0;
-    mine += s[q];
-  }
-  if (tid == 0) sm.found = max(0, min(n, most - above) - 1);
-  u64 run = sabove + block_before<u64>(mine, sm.wfix, all);
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int i = 4 * tid + q;
-    run += s[q];
-    s[q] = run;
-    if (i < n && (by_rank ? above + i + 1 >= rank : (double)run >= goal)) atomicMin(&sm.found, i);
-  }
-  __syncthreads();
-  const int at = sm.found;
-  if (tid == at / 4) sm.wfix[0] = at % 4 == 0 ? s[0] : at % 4 == 1 ? s[1] : at % 4 == 2 ? s[2] : s[3];
-  const u64 key = sm.list[at];
-  __syncthreads();
-  cut = {j, true, logit_of((uint32_t)(key >> 32)), token_of(key)};
-  return sm.wfix[0];
+  gather(r, klo, khi);
+  border_in_list(n, j, r.s.c, r.s.in, r.ref, by_rank, rank, goal, most, above, sabove);
+  cut = {j, true, key_x(sm.key), key_v(sm.key)};
+  return sm.sum;
 }
 
-__global__ void __launch_bounds__(PT) sample_pick_kernel(const SampleArgs a) {
-  __shared__ PickSmem sm;
+// The border by all filters, into sm.cut, and the chunks' sums of what is kept, into sm.csum.
+__device__ __attribute__((noinline)) void deep_cut(const u64* bins, const SampleStat* stat, int chunks, const float* x,
+                                                   int vocab, double c, double in, double ref, uint32_t ktop, int number,
+                                                   double whole, int top_k, float top_p, float xm, int jm) {
+  PickSmem& sm = smem();
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int row = blockIdx.x, chunks = a.chunks;
-  const int64_t s0 = (int64_t)row * chunks;
-  const float T = a.temperature[row], u = a.uniforms[row], top_p = a.top_p[row], min_p = a.min_p[row];
-  const int top_k = a.top_k[row];
-  auto answer = [&](int token, float logprob) {
-    a.tokens[row] = token;
-    if (a.logprobs) a.logprobs[row] = logprob;
-  };
-  // the row's maximum, and what is wrong with it
-  u64 key = 0;
-  int bad = 0;
-  double ref = -INFINITY;
-  for (int i = lane; i < chunks; i += 64) {  // every wave for itself
-    const SampleStat s = a.stat[s0 + i];
-    key = key > s.key ? key : s.key;
-    bad |= s.bad;
-    ref = fmax(ref, s.ref);
-    if (w == 0) {
-      sm.ref[i] = s.ref;
-      sm.tail[i] = s.tail;
-      sm.tcount[i] = s.tail_count;
-      sm.part[i] = 0;
-    }
-  }
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const u64 y = __shfl_xor(key, o);
-    key = key > y ? key : y;
-    bad |= __shfl_xor(bad, o);
-    ref = fmax(ref, __shfl_xor(ref, o));
-  }
-  const float top = logit_of((uint32_t)(key >> 32));
-  if (bad || top == -INFINITY || !(T >= 0.f && T < INFINITY) || u != u || top_p != top_p || min_p != min_p) {
-    if (tid == 0) answer(-1, __builtin_nanf(""));
-    return;
-  }
-  if (T == 0.f) {
-    if (tid == 0) answer(token_of(key), 0.f);
-    return;
-  }
-  Row r;
-  r.x = a.logits + row * a.row_stride;
-  r.vocab = a.vocab;
-  r.chunks = chunks;
-  r.c = RES / (double)T;
-  r.ref = ref;
-  r.ktop = (uint32_t)(key >> 32);
-  r.kmin = logit_order(-3.4028234663852886e38f);
-  if (tid < NB) sm.et[tid] = exp(-tid / RES);
+  const Row r = {x, vocab, {c, in}, ref, ktop, logit_order(-3.4028234663852886e38f)};
   __syncthreads();
-  if (tid < chunks) {
-    const double d = ref - sm.ref[tid];
-    sm.delta[tid] = d < (1 << 20) ? (int)d : 1 << 20;
-    sm.scale[tid] = exp(-d / RES);
-  }
-  __syncthreads();
-
-  // the chunks' bins joined: two threads to a bin
-  {
-    constexpr double UNIT = 1.0 / (double)(1ull << FIX);
+  {  // the chunks' bins joined, two threads to a bin
     const int j = tid % NB, half = tid / NB;
     u64 s = 0;
     int n = 0, tn = 0;
     double t = 0;
-    for (int c = half; c < chunks; c += PT / NB) {
-      const int d = sm.delta[c];
-      if (j >= d && j - d < NB - 1) {
-        s += a.sum[(s0 + c) * NB + j - d];
-        n += (int)a.count[(s0 + c) * NB + j - d];
-      }
-      if (j < NB - 1 && j + d >= NB - 1) {  // the chunk's bin lies in the row's tail
-        t += (double)a.sum[(s0 + c) * NB + j] * UNIT * (sm.et[j] * sm.scale[c]);
-        tn += (int)a.count[(s0 + c) * NB + j];
+#pragma unroll 8
+    for (int k = half; k < chunks; k += ST / NB) {
+      const int d = sm.delta[k];
+      const u64 b = bins[k * NB + max(j - d, 0)];
+      const bool have = j >= d && j - d < NB - 1;
+      s += have ? b & SUM_MASK : 0;
+      n += have ? (int)(b >> CNT) : 0;
+      if (d > 0 && j < NB - 1 && j + d >= NB - 1) {  // the chunk's bin lies in the row's tail
+        const u64 o = bins[k * NB + j];
+        t += (double)(o & SUM_MASK) / ONE * (sm.et[j] * sm.scale[k]);
+        tn += (int)(o >> CNT);
       }
       if (j == NB - 1) {
-        t += sm.tail[c] * sm.scale[c];
-        tn += sm.tcount[c];
+        t += stat[k].tail * sm.scale[k];
+        tn += stat[k].tail_count;
       }
     }
     t = sum_over_wave(t);
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) tn += __shfl_xor(tn, o);
+    tn = sum_over_wave(tn);
     if (lane == 0) {
       sm.half.tail[w] = t;
       sm.half.tcount[w] = tn;
@@ -587,11 +731,11 @@ __global__ void __launch_bounds__(PT) sample_pick_kernel(const SampleArgs a) {
     if (!half) {
       s += sm.half.sum[j];
       n += sm.half.count[j];
-      weight = (double)s * UNIT * sm.et[j];
+      weight = (double)s / ONE * sm.et[j];
       if (j == NB - 1) {
         weight = 0;
         n = 0;
-        for (int i = 0; i < PT / 64; ++i) {
+        for (int i = 0; i < SW; ++i) {
           weight += sm.half.tail[i];
           n += sm.half.tcount[i];
         }
@@ -599,159 +743,342 @@ __global__ void __launch_bounds__(PT) sample_pick_kernel(const SampleArgs a) {
     } else {
       n = 0;
     }
-    double all;
+    double wall;
     int call;
-    const double wb = block_before<double>(weight, sm.wsum, all);
+    const double wb = block_before<double>(weight, sm.wsum, wall);
     const int cb = block_before<int32_t>(n, sm.wcount, call);
     if (!half) {
       sm.upto[j] = wb + weight;
       sm.cupto[j] = cb + n;
     }
-    __syncthreads();
   }
-  const int number = sm.cupto[NB - 1];
-  constexpr double ONE = (double)(1ull << FIX);
-  auto below = [&](int j) { return j > 0 ? sm.upto[j - 1] : 0.0; };
-  auto cbelow = [&](int j) { return j > 0 ? sm.cupto[j - 1] : 0; };
-  auto first_bin = [&](auto test) {  // the first bin that passes, the last one if none does
-    __syncthreads();
-    if (tid == 0) sm.found = NB - 1;
-    __syncthreads();
-    if (tid < NB && test(tid)) atomicMin(&sm.found, tid);
-    __syncthreads();
-    return sm.found;
-  };
+  Cut cut = {NB - 1, false, 0.f, 0};
+  int kept = number, holds = -1;  // candidates; the bin whose logits the list holds
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    const bool by_rank = pass == 0;
+    if (by_rank ? top_k <= 0 || top_k >= number : !(top_p < 1.f)) continue;
+    const double goal = (double)top_p * whole * (1 - SAME);
+    const int j = min(cut.bin, first_bin([&](int i) {
+      return by_rank ? sm.cupto[i] >= top_k : sm.cupto[i] > 0 && sm.upto[i] >= goal;
+    }));
+    const int n = sm.cupto[j] - number_below(j);
+    const u64 s = border_in_bin(r, j, n, by_rank, top_k - number_below(j), (goal - weight_below(j)) / sm.et[j] * ONE,
+                                min(n, kept - number_below(j)), cut);
+    holds = n <= CAP ? j : -1;
+    if (by_rank) {
+      kept = top_k;
+      whole = weight_below(j) + (double)s / ONE * sm.et[j];
+    }
+  }
+  if (jm < cut.bin || (jm == cut.bin && (!cut.part || xm > cut.x))) cut = {jm, true, xm, INT32_MAX};
+  if (tid == 0) sm.cut = cut;
+  if (!cut.part) return;  // everything
+  {  // the kept weights of the border's bin
+    const int j = cut.bin, n = sm.cupto[j] - number_below(j);
+    if (n <= CAP) {
+      if (holds != j) {
+        bin_range(r, j);
+        gather(r, sm.klo, sm.khi);
+      }
+      for (int i = tid; i < n; i += ST) {
+        const float y = key_x(sm.list[i]);
+        const int v = key_v(sm.list[i]);
+        if (cut.keeps(j, y, v)) atomicAdd(&sm.part[v / SC], fixed_weight(r, y, j));
+      }
+    } else {
+      bin_range(r, j);
+      sweep(r, logit_order(cut.x), sm.khi, [&](float y, int v) {
+        if (cut.keeps(j, y, v)) atomicAdd(&sm.part[v / SC], fixed_weight(r, y, j));
+      });
+    }
+  }
+  __syncthreads();
+  for (int k = w; k < chunks; k += SW) {
+    const int d = sm.delta[k];
+    double s = 0;
+#pragma unroll
+    for (int i = 0; i < NB / 64; ++i) {
+      const int j = 64 * i + lane;
+      const u64 b = bins[k * NB + j];
+      if (j < NB - 1 && j + d < cut.bin) s += (double)(b & SUM_MASK) / ONE * (sm.et[j] * sm.scale[k]);
+    }
+    s = sum_over_wave(s);
+    if (lane == 0) sm.csum[k] = s + (double)sm.part[k] / ONE * sm.et[cut.bin];
+  }
+}
+
+__global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
+  PickSmem& sm = smem();
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row = blockIdx.x, chunks = a.chunks;
+  const int64_t s0 = (int64_t)row * chunks;
+  const float T = a.temperature[row], u = a.uniforms[row], top_p = a.top_p[row], min_p = a.min_p[row];
+  const int top_k = a.top_k[row];
+  const bool filtered = top_k > 0 || !(top_p >= 1.f) || min_p > 0.f;
+  u64 key = 0;
+  SampleStat st{};
+  const int ci = tid - NB;  // the threads behind the bins' take a chunk each
+  if (ci >= 0 && ci < chunks) st = a.stat[s0 + ci];
+  if (lane < chunks) key = a.stat[s0 + lane].key;
+  if (64 + lane < chunks) key = max(key, a.stat[s0 + 64 + lane].key);
+  if (filtered)
+#pragma unroll
+    for (int i = 0; i < LISTED; ++i)
+      sm.lkey[i * ST + tid] = i * ST + tid < chunks * a.list ? a.listed[s0 * a.list + i * ST + tid] : 0;
+  key = max_over_wave(key);
+  const float top = key_x(key);  // NaN for a row that has failed
+  if (!(top > -INFINITY) || !(T >= 0.f && T < INFINITY) || u != u || top_p != top_p || min_p != min_p || T == 0.f) {
+    if (tid == 0) {
+      const bool likeliest = T == 0.f && top > -INFINITY && u == u && top_p == top_p && min_p == min_p;
+      a.tokens[row] = likeliest ? key_v(key) : -1;
+      if (a.logprobs) a.logprobs[row] = likeliest ? 0.f : __builtin_nanf("");
+    }
+    return;
+  }
+  const float* x = a.logits + row * a.row_stride;
+  const Scale sc = scale_of_row(T, top);
+  const double ref = floor((double)top * sc.c);
+  if (tid == 0) {
+    sm.depth = NB - 2;
+    sm.number = 0;
+  }
+  const double d = ref - st.ref;
+  const double y = exp((tid < NB ? -tid : -d) / RES);
+  if (tid < NB) {
+    sm.et[tid] = y;
+    sm.bins[tid] = 0;
+  }
+  __syncthreads();
+  if (ci >= 0 && ci < chunks) {
+    const int delta = d < (1 << 20) ? (int)d : 1 << 20;
+    sm.delta[ci] = delta;
+    sm.scale[ci] = y;
+    sm.csum[ci] = st.total * y;
+    sm.part[ci] = 0;
+    if (st.depth < NB) atomicMin(&sm.depth, st.depth + delta);
+    atomicAdd(&sm.number, st.number);
+  }
+  __syncthreads();
 
   Cut cut = {NB - 1, false, 0.f, 0};
-  double whole = sm.upto[NB - 1];  // the candidates' sum
-  int listed = -1, kept = number;  // the bin whose logits the list holds; candidates
-  if (top_k > 0 && top_k < number) {
-    const int j = first_bin([&](int i) { return sm.cupto[i] >= top_k; });
-    const int rank = top_k - cbelow(j), n = sm.cupto[j] - cbelow(j);
-    kept = top_k;
-    if (rank == n) {
-      cut.bin = j;
-      whole = sm.upto[j];
-    } else {
-      bool l;
-      const u64 s = border_in_bin(r, j, n, true, rank, 0, INT32_MAX, l, cut, sm);
-      listed = l ? j : -1;
-      whole = below(j) + (double)s / ONE * sm.et[j];
-    }
-  }
-  if (top_p < 1.f) {
-    const double goal = (double)top_p * whole * (1 - SAME);
-    const int j = min(cut.bin, first_bin([&](int i) { return sm.cupto[i] > 0 && sm.upto[i] >= goal; }));
-    const int n = sm.cupto[j] - cbelow(j);
-    bool l;
-    border_in_bin(r, j, n, false, 0, (goal - below(j)) / sm.et[j] * ONE, min(n, kept - cbelow(j)), l, cut, sm);
-    listed = l ? j : -1;
-  }
-  if (min_p > 0.f) {
-    // the least logit with w >= min_p, and its bin
-    if (tid < 64) {
-      const double lim = fmin((double)min_p, 1.0);
-      const uint32_t k = least_true(r.kmin, r.ktop, [&](uint32_t o) {
-        return exp(((double)logit_of(o) - (double)top) / (double)T) >= lim;
-      });
-      if (tid == 0) sm.klo = k;
+  bool from_list = false;  // what is kept is listed, its weights in sm.lbin
+  if (filtered) {
+    const int number = sm.number, depth = sm.depth;
+    double whole = (lane < chunks ? sm.csum[lane] : 0) + (64 + lane < chunks ? sm.csum[64 + lane] : 0);
+    whole = sum_over_wave(whole);
+    // the listed logits' bins: the row's, as far down as `depth`
+#pragma unroll 1
+    for (int i = tid; i < LISTED * ST; i += ST) {
+      const u64 k = sm.lkey[i];
+      u64 packed = (u64)NB << LBIN;  // none
+      if (k) {
+        const float y = key_x(k);
+        const double fl = floor((double)y * sc.c);
+        const int j = bin_of(ref, fl);
+        const u64 f = fixed_in_bin(y, sc, fl);
+        if (j <= depth) {
+          packed = (u64)j << LBIN | f;
+          atomicAdd(&sm.bins[j], f + (1ull << CNT));
+        }
+      }
+      sm.lbin[i] = packed;
     }
     __syncthreads();
-    const float x = logit_of(sm.klo);
-    const double d = ref - floor((double)x * r.c);
-    const int j = d < NB - 1 ? (int)d : NB - 1;
-    if (j < cut.bin || (j == cut.bin && (!cut.part || x > cut.x))) cut = {j, true, x, INT32_MAX};
+    {
+      const u64 b = tid < NB - 1 ? sm.bins[tid] : 0;
+      const double weight = tid < NB ? (double)(b & SUM_MASK) / ONE * sm.et[tid] : 0;
+      double all;
+      int call;
+      const double wb = block_before<double>(weight, sm.wsum, all);
+      const int cb = block_before<int32_t>((int)(b >> CNT), sm.wcount, call);
+      if (tid < NB) {
+        sm.upto[tid] = wb + weight;
+        sm.cupto[tid] = cb + (int)(b >> CNT);
+      }
+    }
+    // the least logit with w >= min_p, and its bin
+    float xm = 0;
+    int jm = NB;
+    const uint32_t ktop = (uint32_t)(key >> 32), kmin = logit_order(-3.4028234663852886e38f);
+    if (min_p > 0.f) {
+      if (tid < 64) {
+        const double lim = fmin((double)min_p, 1.0);
+        const float guess = (float)fmax((double)top + (double)T * log(lim), -3.4028234663852886e38);
+        const uint32_t k = least_true(kmin, ktop, logit_order(guess), [&](uint32_t o) {
+          return exp(((double)logit_of(o) - (double)top) / (double)T) >= lim;
+        });
+        if (tid == 0) sm.klo = k;
+      }
+      __syncthreads();
+      xm = logit_of(sm.klo);
+      jm = bin_of(ref, floor((double)xm * sc.c));
+    }
+    // the borders among the listed logits: by number, then by weight
+    int kept = number;
+    bool deep = false;
+    double sum = whole;  // the candidates'
+#pragma unroll 1
+    for (int pass = 0; pass < 2 && !deep; ++pass) {
+      const bool by_rank = pass == 0;
+      if (by_rank ? top_k <= 0 || top_k >= number : !(top_p < 1.f)) continue;
+      const double goal = (double)top_p * sum * (1 - SAME);
+      const int j = min(cut.bin, first_bin([&](int i) {
+        return by_rank ? sm.cupto[i] >= top_k : sm.cupto[i] > 0 && sm.upto[i] >= goal;
+      }));
+      const int n = sm.cupto[j] - number_below(j);
+      if (j > depth) {
+        deep = true;
+        break;
+      }
+      if (tid == 0) sm.n = 0;
+      __syncthreads();
+#pragma unroll 1
+      for (int i = tid; i < LISTED * ST; i += ST)
+        if ((int)(sm.lbin[i] >> LBIN) == j) sm.list[atomicAdd(&sm.n, 1)] = sm.lkey[i];
+      __syncthreads();
+      border_in_list(n, j, sc.c, sc.in, ref, by_rank, top_k - number_below(j), (goal - weight_below(j)) / sm.et[j] * ONE,
+                     min(n, kept - number_below(j)), 0, 0);
+      cut = {j, true, key_x(sm.key), key_v(sm.key)};
+      if (by_rank) {
+        kept = top_k;
+        sum = weight_below(j) + (double)sm.sum / ONE * sm.et[j];
+      }
+      __syncthreads();
+    }
+    if (!deep) {
+      if (jm < cut.bin || (jm == cut.bin && (!cut.part || xm > cut.x))) cut = {jm, true, xm, INT32_MAX};
+      deep = cut.part && cut.bin > depth;
+    }
+    if (deep) {
+      deep_cut(a.bins + s0 * NB, a.stat + s0, chunks, x, a.vocab, sc.c, sc.in, ref, ktop, number, whole, top_k, top_p, xm, jm);
+      __syncthreads();
+      cut = sm.cut;
+    } else if (cut.part) {  // the chunks' sums of what is kept: all of it is listed, a wave's 64 are of one chunk
+      from_list = true;
+      __syncthreads();
+#pragma unroll 1
+      for (int i = tid; i < LISTED * ST; i += ST) {
+        const u64 k = sm.lkey[i], b = sm.lbin[i];
+        const int j = (int)(b >> LBIN);
+        double s = 0;
+        if (j < NB && cut.keeps(j, key_x(k), key_v(k))) s = (double)(b & ((1ull << LBIN) - 1)) / ONE * sm.et[j];
+        sm.lbin[i] = __builtin_bit_cast(u64, s);
+        if (__builtin_amdgcn_ballot_w64(s > 0)) s = sum_over_wave(s);
+        if (lane == 0) sm.lsum[i / 64] = s;
+      }
+      __syncthreads();
+      if (tid < chunks) {
+        const int n = a.list / 64;
+        double s = 0;
+#pragma unroll 1
+        for (int i = 0; i < n; ++i) s += sm.lsum[tid * n + i];
+        sm.csum[tid] = s;
+      }
+    }
+    __syncthreads();
   }
 
-  // the kept weights of the border's bin, by chunk
-  if (cut.part) {
-    const int j = cut.bin, n = sm.cupto[j] - cbelow(j);
-    if (n <= CAP) {
-      if (listed != j) {
-        bin_range(r, j, sm);
-        gather(r, sm.klo, sm.khi, n, sm);
-      }
-      for (int i = tid; i < n; i += PT) {
-        const float x = logit_of((uint32_t)(sm.list[i] >> 32));
-        const int v = token_of(sm.list[i]);
-        if (x > cut.x || (x == cut.x && v <= cut.token)) atomicAdd(&sm.part[v / SC], fixed_weight(r, x, j));
-      }
-    } else {
-      bin_range(r, j, sm);
-      sweep(r, logit_order(cut.x), sm.khi, [&](float x, int v) {
-        if (x > cut.x || v <= cut.token) atomicAdd(&sm.part[v / SC], fixed_weight(r, x, j));
-      });
+  // the chunk of the answer: the first one whose running sum exceeds u times the whole
+  if (w == 0) {
+    const double c0 = 2 * lane < chunks ? sm.csum[2 * lane] : 0, c1 = 2 * lane + 1 < chunks ? sm.csum[2 * lane + 1] : 0;
+    const double run = scan_wave(c0 + c1, plus<double>);
+    const double z = at_lane(run, 63), goal = fmax((double)u, 0.0) * z * (1 + SAME);
+    double before = __shfl_up(run, 1);
+    if (lane == 0) before = 0;
+    const bool h0 = c0 > 0 && before + c0 > goal, h1 = c1 > 0 && run > goal;
+    const u64 hit = __builtin_amdgcn_ballot_w64(h0 || h1), some = __builtin_amdgcn_ballot_w64(c0 > 0 || c1 > 0);
+    const int at = hit ? __ffsll(hit) - 1 : 63 - __clzll(some);  // none: the last one with any weight
+    if (lane == at) {
+      const bool second = hit ? !h0 : c1 > 0;
+      sm.found = 2 * lane + second;
+      sm.goal = goal - (second ? before + c0 : before);
+      sm.z = z;
+      sm.first[0] = INT32_MAX;
+      sm.last[0] = -1;
     }
   }
   __syncthreads();
-
-  // the chunks' sums: a wave to a chunk
-  const int full = cut.part ? cut.bin : cut.bin + 1;  // bins kept in full
-  for (int c = w; c < chunks; c += PT / 64) {
-    const int d = sm.delta[c];
-    double s = 0;
-    for (int j = lane; j < NB - 1; j += 64)
-      if (full == NB || j + d < full) s += (double)a.sum[(s0 + c) * NB + j] / ONE * (sm.et[j] * sm.scale[c]);
-    s = sum_over_wave(s);
-    if (full == NB) s += sm.tail[c] * sm.scale[c];
-    if (cut.part) s += (double)sm.part[c] / ONE * sm.et[cut.bin];
-    if (lane == 0) sm.csum[c] = s;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    double z = 0;
-    for (int c = 0; c < chunks; ++c) z += sm.csum[c];
-    const double goal = (double)u * z * (1 + SAME);
-    double before = 0;
-    int at = 0;
-    double at_before = 0;
-    for (int c = 0; c < chunks; ++c) {
-      if (sm.csum[c] > 0) {
-        at = c;
-        at_before = before;
-        if (before + sm.csum[c] > goal) break;
-      }
-      before += sm.csum[c];
+  const double goal = sm.goal, z = sm.z;
+  if (from_list) {  // four lanes to a logit add up what is before it
+    const u64* keys = sm.lkey + sm.found * a.list;
+    const u64* weights = sm.lbin + sm.found * a.list;
+    const int i = tid >> 2;
+    const bool mine = i < a.list;
+    const uint32_t low = mine ? (uint32_t)keys[i] : 0;  // falls as the token rises
+    const double weight = mine ? __builtin_bit_cast(double, weights[i]) : 0;
+    double run = 0;
+    if (weight > 0)
+#pragma unroll 1
+      for (int e = tid & 3; e < a.list; e += 4)
+        if ((uint32_t)keys[e] > low) run += __builtin_bit_cast(double, weights[e]);
+    run += __shfl_xor(run, 1);
+    run += __shfl_xor(run, 2);
+    const int v = (int)(0xffffffffu - low);
+    if (weight > 0) {
+      if (run + weight > goal) atomicMin(&sm.first[0], v);
+      atomicMax(&sm.last[0], v);
     }
-    sm.found = at;
-    sm.w0 = goal - at_before;
-    sm.upto[0] = z;
-    sm.n = INT32_MAX;
-    sm.last = -1;
+    __syncthreads();
+    if (weight > 0 && (tid & 3) == 0 && v == (sm.first[0] < INT32_MAX ? sm.first[0] : sm.last[0])) {
+      a.tokens[row] = v;
+      if (a.logprobs) a.logprobs[row] = (float)fmin(log(weight / z), 0.0);
+    }
+    return;
   }
-  __syncthreads();
   // the answer among the chunk's logits, eight to a thread
   const int v0 = sm.found * SC + 8 * tid;
-  const double goal = sm.w0, z = sm.upto[0];
-  double s[8], mine = 0;
+  float f[8];
+  if (v0 + 7 < a.vocab) {
+    const f4a y0 = *reinterpret_cast<const f4a*>(x + v0), y1 = *reinterpret_cast<const f4a*>(x + v0 + 4);
 #pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    const float x = v0 + q < a.vocab ? r.x[v0 + q] : -INFINITY;
-    const double fl = floor((double)x * r.c), d = ref - fl;
-    double weight = 0;
-    if (x > -INFINITY) {
-      const int j = d < NB - 1 ? (int)d : NB - 1;
-      if (j < full || (cut.part && j == cut.bin && (x > cut.x || (x == cut.x && v0 + q <= cut.token))))
-        weight = j < NB - 1 ? exp_in_bin(in_bin(x, r.c, fl)) * sm.et[j] : exp_tail((double)x * r.c - ref);
+    for (int q = 0; q < 4; ++q) {
+      f[q] = y0[q];
+      f[4 + q] = y1[q];
     }
-    s[q] = weight;
-    mine += weight;
-  }
-  double all;
-  double run = block_before<double>(mine, sm.wsum, all);
+  } else {
 #pragma unroll
-  for (int q = 0; q < 8; ++q) {
-    run += s[q];
-    if (s[q] > 0) {
-      if (run > goal) atomicMin(&sm.n, v0 + q);
-      atomicMax(&sm.last, v0 + q);
+    for (int q = 0; q < 8; ++q) f[q] = v0 + q < a.vocab ? x[v0 + q] : -INFINITY;
+  }
+  // a thread's sum, then, by the waves that the answer may be in, the place in it: the first logit with which the running
+  // sum exceeds the goal, or the last one of any weight
+  double before = 0, weight = 0;
+  int hit = -1, last = -1;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    double run = before;
+#pragma unroll 1
+    for (int q = 0; q < 8; ++q) {
+      const double p = (double)f[0] * sc.c, fl = floor(p);
+      const int j = bin_of(ref, fl);
+      if (f[0] > -INFINITY && cut.keeps(j, f[0], v0 + q)) {
+        const double s = j < NB - 1 ? (double)fixed_in_bin(f[0], sc, fl) / ONE * sm.et[j] : exp_tail(p - ref);
+        run += s;
+        if (s > 0 && hit < 0 && pass == 1) {
+          if (run > goal) hit = v0 + q;
+          last = v0 + q;
+          weight = s;
+        }
+      }
+      turn(f);
+    }
+    if (pass == 0) {
+      const double mine = run;
+      double all;
+      before = block_before<double>(mine, sm.wsum, all);
+      // sums in another order may differ in their last digits: a little more than the thread that has it
+      const bool here = mine > 0 && (before + mine) * (1 + SAME) > goal && before * (1 - SAME) <= goal;
+      if (!__builtin_amdgcn_ballot_w64(here) && all * (1 - SAME) > goal) break;
     }
   }
+  if (hit >= 0) atomicMin(&sm.first[0], hit);
+  if (last >= 0) atomicMax(&sm.last[0], last);
   __syncthreads();
-  const int v = sm.n < INT32_MAX ? sm.n : sm.last;
-#pragma unroll
-  for (int q = 0; q < 8; ++q)
-    if (v0 + q == v) answer(v, (float)fmin(log(s[q]) - log(z), 0.0));
+  const int v = sm.first[0] < INT32_MAX ? sm.first[0] : sm.last[0];
+  if (v >= 0 && (v == hit || v == last)) {
+    a.tokens[row] = v;
+    if (a.logprobs) a.logprobs[row] = (float)fmin(log(weight / z), 0.0);
+  }
 }
 
 static size_t sample_align(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -763,7 +1090,7 @@ using namespace mkp;
 extern "C" size_t mk_sample_workspace_bytes(int rows, int vocab) {
   if (rows < 1 || rows > 65535 || vocab < 1 || vocab > SV_MAX) return 0;
   const size_t slots = (size_t)rows * ((vocab + SC - 1) / SC);
-  return sample_align(slots * sizeof(SampleStat)) + slots * NB * (sizeof(u64) + sizeof(uint32_t));
+  return sample_align(slots * sizeof(SampleStat)) + slots * (NB + LIST_MAX) * sizeof(u64);
 }
 
 extern "C" hipError_t mk_sample(int rows, int vocab, const float* logits, int64_t row_stride, const float* uniforms,
@@ -789,11 +1116,12 @@ extern "C" hipError_t mk_sample(int rows, int vocab, const float* logits, int64_
   const size_t slots = (size_t)rows * a.chunks;
   char* ws = static_cast<char*>(workspace);
   a.stat = reinterpret_cast<SampleStat*>(ws);
-  a.sum = reinterpret_cast<u64*>(ws + sample_align(slots * sizeof(SampleStat)));
-  a.count = reinterpret_cast<uint32_t*>(a.sum + slots * NB);
-  hipLaunchKernelGGL(sample_chunk_kernel, dim3(a.chunks, rows), dim3(256), 0, stream, a);
+  a.list = std::min(LIST_MAX, LISTED * ST / a.chunks & ~63);
+  a.bins = reinterpret_cast<u64*>(ws + sample_align(slots * sizeof(SampleStat)));
+  a.listed = a.bins + slots * NB;
+  hipLaunchKernelGGL(sample_chunk_kernel, dim3(a.chunks, rows), dim3(ST), 0, stream, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(sample_pick_kernel, dim3(rows), dim3(PT), 0, stream, a);
+  hipLaunchKernelGGL(sample_pick_kernel, dim3(rows), dim3(ST), 0, stream, a);
   return hipGetLastError();
 }
