@@ -8,17 +8,17 @@
 // The answer is a whole number that a border may decide, so sums are exact ones of w rounded to 2^-37 of itself, and two
 // sums within SAME of each other count as equal: 5 of 10 equal logits reach half of them, and do not exceed it.
 //
-// Bins. p = x * 16 / T falls into bin floor(p), the same for equal logits wherever they are, and within its bin
-// w is exp((p - floor(p)) / 16), a polynomial on [1, 1.065), kept as a whole number of 2^-36: a bin's sum is a sum of
-// whole numbers, the same in any order, and its weight that sum times exp(bin / 16). Its number of logits shares the
-// 64 bits, so that a logit is one atomic addition in LDS.
-//   sample_chunk_kernel  a workgroup takes 8,192 logits of a row from registers into 512 bins (32 in units of T) below
+// Bins, 11 to a factor of 2. p = x * 11 log2(e) / T falls into bin floor(p), the same for equal logits wherever they
+// are, and within its bin w is 2^((p - floor(p)) / 11), a polynomial on [1, 1.066), kept as a whole number of 2^-36: a
+// bin's sum is a sum of whole numbers, the same in any order, and its weight that sum times 2^(bin / 11). Its number of
+// logits shares the 64 bits, so that a logit is one atomic addition in LDS.
+//   sample_chunk_kernel  a workgroup takes 8,192 logits of a row from registers into 512 bins (a factor of 2^46) below
 //                        their maximum (what lies lower is a tail of its own), and lists the logits of the first bins,
 //                        up to 256 of them in all;
 //   sample_pick_kernel   a workgroup per row. Borders lie among the listed logits as a rule: it bins these, finds the
 //                        bin that a border falls into, sorts that bin's logits, and sums the kept ones chunk by chunk.
 //                        Where a border lies deeper it joins the chunks' bins instead and gathers the border's bin from
-//                        the row (narrowing it first where it holds more than 4,096). The answer is looked for among
+//                        the row, by its logits' bins in a byte each (narrowing it first where it holds more than 4,096). The answer is looked for among
 //                        the 8,192 logits of its chunk. Without any filter the chunks' sums are all that is needed.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -37,7 +37,7 @@ constexpr int SC = 8 * ST;          // logits of a chunk
 constexpr int SV_MAX = 1 << 20;
 constexpr int SCH = SV_MAX / SC;    // chunks of a row at most
 constexpr int NB = 512;             // bins; the last one is the tail
-constexpr double RES = 16;          // bins per unit of x / T
+constexpr int RES = 11;             // bins to a factor of 2
 constexpr int FIX = 36;             // bits behind the point of a weight within its bin
 constexpr double ONE = (double)(1ull << FIX);
 constexpr int CNT = 50;             // a bin's number of logits, at most 8,192, from this bit on
@@ -53,7 +53,7 @@ typedef float f4a __attribute__((ext_vector_type(4), aligned(4)));  // rows may 
 
 struct SampleStat {
   double ref;    // the bin of the chunk's maximum; -infinity: no finite logit
-  double total;  // its weights, in units of exp(ref / 16)
+  double total;  // its weights, in units of 2^(ref / 11)
   double tail;   // those below the bins
   u64 key;       // the largest logit, the lowest token of equal ones; all bits set: the chunk has a NaN or +infinity
   int32_t tail_count, number;
@@ -72,6 +72,7 @@ struct SampleArgs {
   SampleStat* stat;  // [rows][chunks]
   u64* bins;         // [rows][chunks][NB]
   u64* listed;       // [rows][chunks][list], filled up with 0
+  uint8_t* codes;    // [rows][chunks][SC]: half of each logit's bin, of rows whose border may lie deeper
 };
 
 __device__ __forceinline__ uint32_t logit_order(float x) {  // unsigned order is the numbers'
@@ -153,14 +154,39 @@ struct Scale {
 };
 __device__ __forceinline__ Scale scale_of_row(float T, double top) {
   Scale s;
-  s.c = RES / (double)T;
+  s.c = RES * 1.4426950408889634 / (double)T;
   s.in = fabs(top * s.c) < 0x1p45 ? 1.0 : 0.0;
   return s;
 }
-// exp(f / 16) for the place f in [0, 1] of a logit in its bin fl, in whole numbers of 2^-FIX: the series, whose next
+// 2^(-k / RES) for a whole number k >= 0, to 2^-51 of itself
+__device__ __forceinline__ double bin_weight(double k) {
+  k = fmin(k, 2.0e4);  // 0 from about 11,800 on
+  const double q = floor(k * (1.0 / RES) + 1.0 / (2 * RES));
+  const int i = (int)(k - q * RES);  // its powers of 2: 2^(-2^b / 11)
+  double y = i & 1 ? 0x1.e0bb8d64fdb5ap-1 : 1.0;
+  y *= i & 2 ? 0x1.c35fedd14b862p-1 : 1.0;
+  y *= i & 4 ? 0x1.8ded91f0e72eep-1 : 1.0;
+  y *= i & 8 ? 0x1.3545598e5c232p-1 : 1.0;
+  return ldexp(y, -(int)q);
+}
+// log x to 2^-48 of itself: 2 artanh((m - 1) / (m + 1)) of the mantissa m in [0.7, 1.42)
+__device__ __forceinline__ double log64(double x) {
+  int e;
+  double m = frexp(x, &e);
+  if (m < 0.70710678) {
+    m *= 2;
+    --e;
+  }
+  const double t = (m - 1) / (m + 1), q = t * t;
+  double y = 1.0 / 21;
+#pragma unroll
+  for (int k = 19; k >= 3; k -= 2) y = fma(y, q, 1.0 / k);
+  return fma((double)e, 0.6931471805599453, 2 * fma(t * q, y, t));
+}
+// 2^(f / 11) for the place f in [0, 1] of a logit in its bin fl, in whole numbers of 2^-FIX: the series, whose next
 // term is below 2^-40, behind 2^16, where a double's last bit is 2^-36.
 __device__ __forceinline__ u64 fixed_in_bin(float x, const Scale& s, double fl) {
-  constexpr double A = 1.0 / 16, BIG = 1 << (52 - FIX);
+  constexpr double A = 0.6931471805599453 / RES, BIG = 1 << (52 - FIX);
   const double f = fma((double)x, s.c, -fl) * s.in;
   double y = A * A * A * A * A * A / 720;
   y = fma(y, f, A * A * A * A * A / 120);
@@ -170,9 +196,9 @@ __device__ __forceinline__ u64 fixed_in_bin(float x, const Scale& s, double fl) 
   y = fma(y, f, A);
   return __builtin_bit_cast(u64, fma(y, f, 1 + BIG)) - __builtin_bit_cast(u64, BIG);
 }
-// exp(t / 16) for t <= 0 to fp32's accuracy, over the doubles' range: the tail's weights, below exp(-31) of the largest
+// 2^(t / 11) for t <= 0 to fp32's accuracy, over the doubles' range: the tail's weights, below 2^-46 of the largest
 __device__ __forceinline__ double exp_tail(double t) {
-  const double p = t * (1.4426950408889634 / RES), n = floor(fmax(p, -1100.0));
+  const double p = t * (1.0 / RES), n = floor(fmax(p, -1100.0));
   return ldexp((double)__builtin_amdgcn_exp2f((float)fmax(p - n, 0.0)), (int)n);
 }
 // the bin of floor(p) below `ref`, the tail's for all from there on
@@ -213,7 +239,8 @@ __global__ void __launch_bounds__(ST, 8) sample_chunk_kernel(const SampleArgs a)
     }
   }
   const float T = a.temperature[row];
-  const bool filtered = a.top_k[row] > 0 || !(a.top_p[row] >= 1.f) || a.min_p[row] > 0.f;
+  const int top_k = a.top_k[row];
+  const bool filtered = top_k > 0 || !(a.top_p[row] >= 1.f) || a.min_p[row] > 0.f;
   if (tid < NB) bins[tid] = 0;
   if (tid == 0) sdepth = -1;
   float m = -INFINITY;
@@ -270,7 +297,7 @@ __global__ void __launch_bounds__(ST, 8) sample_chunk_kernel(const SampleArgs a)
   }
   const u64 b = tid < NB && !none ? bins[tid] : 0;
   if (!none) {
-    const double weight = w < NB / 64 ? sum_over_wave((double)(b & SUM_MASK) / ONE * exp(-tid / RES)) : 0;
+    const double weight = w < NB / 64 ? sum_over_wave((double)(b & SUM_MASK) / ONE * bin_weight(tid)) : 0;
     if (lane == 0) stotal[w] = weight;
     int all;
     const int upto = block_before<int32_t>((int)(b >> CNT), scan, all) + (int)(b >> CNT);  // (stotal is written behind it)
@@ -287,6 +314,14 @@ __global__ void __launch_bounds__(ST, 8) sample_chunk_kernel(const SampleArgs a)
   }
   if (filtered) {
     if (tid < NB) a.bins[slot * NB + tid] = b;
+    if (!none && (top_k <= 0 || top_k > a.list)) {
+      uint8_t* codes = a.codes + slot * SC + (v0 - (int)blockIdx.x * SC);
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        *reinterpret_cast<uint32_t*>(codes + 256 * j) = (uint32_t)(bin[4 * j] >> 1) | (uint32_t)(bin[4 * j + 1] >> 1) << 8 |
+                                                        (uint32_t)(bin[4 * j + 2] >> 1) << 16 |
+                                                        (uint32_t)(bin[4 * j + 3] >> 1) << 24;
+    }
     // the bins that the list holds in full, and their logits in the threads' order
     int n = 0;
     if (!none) {
@@ -347,7 +382,7 @@ struct Cut {
 
 // What the threads of a row share.
 struct PickSmem {
-  double et[NB];        // exp(-j / 16)
+  double et[NB];        // 2^(-j / 11)
   double upto[NB];      // weights of bins 0 .. j
   int32_t cupto[NB];    // their logits
   int32_t delta[SCH];   // bins of the row above the chunk's first (at most 2^20)
@@ -366,12 +401,6 @@ struct PickSmem {
     struct {
       u64 raw[RANKED], key[RANKED];
     } sort;
-    struct {
-      u64 sum[NB];
-      int32_t count[NB];
-      double tail[SW];
-      int32_t tcount[SW];
-    } half;
     double lsum[LISTED * SW];  // kept weights of 64 listed logits each
   };
   double wsum[SW];
@@ -411,7 +440,7 @@ __device__ __forceinline__ int first_bin(F test) {
   return sm.found;
 }
 
-// The weight of a logit of the row's bin j, in 2^-FIX of exp(-j / 16).
+// The weight of a logit of the row's bin j, in 2^-FIX of 2^(-j / 11).
 __device__ __forceinline__ u64 fixed_weight(const Scale& s, double ref, float x, int j) {
   const double p = (double)x * s.c, fl = floor(p);
   if (j == NB - 1) return (u64)(exp_tail(p - ref + (NB - 1)) * ONE);
@@ -503,7 +532,7 @@ __device__ __attribute__((noinline)) void border_in_list(int n, int j, double c,
     const u64 k = i < n ? sm.sort.raw[i] : 0;
     int place = 0;
     if (i < n)
-#pragma unroll 1
+#pragma unroll 4
       for (int e = tid & 3; e < n; e += 4) place += sm.sort.raw[e] > k;
     place += __shfl_xor(place, 1);
     place += __shfl_xor(place, 2);
@@ -596,13 +625,64 @@ __device__ __forceinline__ void gather(const Row& r, uint32_t klo, uint32_t khi)
   __syncthreads();
 }
 
+// Gathers the logits of bin j, not the tail's, at most CAP, by the codes: 16 of them to a load.
+__device__ __forceinline__ void gather_bin(const Row& r, const uint8_t* codes, int chunks, int j) {
+  PickSmem& sm = smem();
+  const int tid = threadIdx.x;
+  __syncthreads();
+  if (tid == 0) sm.n = 0;
+  __syncthreads();
+  const double fl = r.ref - j;
+  const int units = chunks * (SC / 16);
+#pragma unroll 1
+  for (int base = 0; base < units; base += 4 * ST) {
+    uint4 q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = base + i * ST + tid;
+      q[i] = at < units ? *reinterpret_cast<const uint4*>(codes + (int64_t)16 * at) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int at = base + i * ST + tid, k = j - sm.delta[min(at / (SC / 16), chunks - 1)];  // the chunk's bin
+      if (at >= units || k < 0) continue;
+      const uint32_t code = (uint32_t)(k >> 1) * 0x01010101u, w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+      uint32_t mask = 0;  // bit 4 byte + word: a byte that is the code
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t y = w[e] ^ code, z = ~(((y & 0x7f7f7f7fu) + 0x7f7f7f7fu) | y) & 0x80808080u;
+        mask |= z >> (7 - e);
+      }
+#pragma unroll 1
+      while (mask) {
+        const int bit = __ffs(mask) - 1, v = 16 * at + 4 * (bit & 7) + (bit >> 3);
+        mask &= mask - 1;
+        if (v < r.vocab) {
+          const float x = r.x[v];
+          if (floor((double)x * r.s.c) == fl) {
+            const int to = atomicAdd(&sm.n, 1);
+            if (to < CAP) sm.list[to] = logit_key(x, v);
+          }
+        }
+      }
+    }
+  }
+  __syncthreads();
+}
+
 // Finds the border within bin j, which has `count` logits: the first of them, in order, at which their number reaches
 // `rank` (by_rank), or their sum reaches `goal` (in 2^-FIX of the bin's unit; the last of `most` logits, if none of
 // them does). Returns the sum up to it. Leaves the list of the whole bin where it holds no more than CAP.
-__device__ __forceinline__ u64 border_in_bin(const Row& r, int j, int count, bool by_rank, int rank, double goal,
-                                             int most, Cut& cut) {
+__device__ __forceinline__ u64 border_in_bin(const Row& r, const uint8_t* codes, int chunks, int j, int count, bool by_rank,
+                                             int rank, double goal, int most, Cut& cut) {
   PickSmem& sm = smem();
   const int tid = threadIdx.x;
+  if (count <= CAP && j < NB - 1 && codes) {
+    gather_bin(r, codes, chunks, j);
+    border_in_list(count, j, r.s.c, r.s.in, r.ref, by_rank, rank, goal, most, 0, 0);
+    cut = {j, true, key_x(sm.key), key_v(sm.key)};
+    return sm.sum;
+  }
   bin_range(r, j);
   uint32_t klo = sm.klo, khi = sm.khi;
   int n = count, above = 0;  // logits in [klo, khi], and of the bin above khi
@@ -687,69 +767,67 @@ __device__ __forceinline__ u64 border_in_bin(const Row& r, int j, int count, boo
 }
 
 // The border by all filters, into sm.cut, and the chunks' sums of what is kept, into sm.csum.
-__device__ __attribute__((noinline)) void deep_cut(const u64* bins, const SampleStat* stat, int chunks, const float* x,
+__device__ __attribute__((noinline)) void deep_cut(const u64* bins, const SampleStat* stat,
+                                                   const uint8_t* codes, int chunks, const float* x,
                                                    int vocab, double c, double in, double ref, uint32_t ktop, int number,
                                                    double whole, int top_k, float top_p, float xm, int jm) {
   PickSmem& sm = smem();
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Row r = {x, vocab, {c, in}, ref, ktop, logit_order(-3.4028234663852886e38f)};
   __syncthreads();
-  {  // the chunks' bins joined, two threads to a bin
-    const int j = tid % NB, half = tid / NB;
-    u64 s = 0;
-    int n = 0, tn = 0;
+  // the chunks' bins joined, a wave to a chunk
+  for (int i = tid; i < NB; i += ST) {
+    sm.many.sum[i] = 0;
+    sm.many.count[i] = 0;
+  }
+  __syncthreads();
+  int tn = 0;
+#pragma unroll 1
+  for (int k = w; k < chunks; k += SW) {
+    const int d = sm.delta[k];
+    const double f = sm.scale[k];
+    u64 b[NB / 64];
+#pragma unroll
+    for (int i = 0; i < NB / 64; ++i) b[i] = bins[k * NB + 64 * i + lane];
     double t = 0;
-#pragma unroll 8
-    for (int k = half; k < chunks; k += ST / NB) {
-      const int d = sm.delta[k];
-      const u64 b = bins[k * NB + max(j - d, 0)];
-      const bool have = j >= d && j - d < NB - 1;
-      s += have ? b & SUM_MASK : 0;
-      n += have ? (int)(b >> CNT) : 0;
-      if (d > 0 && j < NB - 1 && j + d >= NB - 1) {  // the chunk's bin lies in the row's tail
-        const u64 o = bins[k * NB + j];
-        t += (double)(o & SUM_MASK) / ONE * (sm.et[j] * sm.scale[k]);
-        tn += (int)(o >> CNT);
-      }
-      if (j == NB - 1) {
-        t += stat[k].tail * sm.scale[k];
-        tn += stat[k].tail_count;
+#pragma unroll
+    for (int i = 0; i < NB / 64; ++i) {
+      const int j = 64 * i + lane;
+      if (j + d < NB - 1) {
+        if (b[i]) {
+          atomicAdd(&sm.many.sum[j + d], b[i] & SUM_MASK);
+          atomicAdd(&sm.many.count[j + d], (uint32_t)(b[i] >> CNT));
+        }
+      } else if (j < NB - 1) {  // in the row's tail
+        t += (double)(b[i] & SUM_MASK) / ONE * (sm.et[j] * f);
+        tn += (int)(b[i] >> CNT);
       }
     }
     t = sum_over_wave(t);
-    tn = sum_over_wave(tn);
     if (lane == 0) {
-      sm.half.tail[w] = t;
-      sm.half.tcount[w] = tn;
+      sm.csum[k] = t + stat[k].tail * f;
+      tn += stat[k].tail_count;
     }
-    if (half) {
-      sm.half.sum[j] = s;
-      sm.half.count[j] = n;
+  }
+  if (tid == 0) sm.n = 0;
+  __syncthreads();
+  tn = sum_over_wave(tn);
+  if (lane == 0) atomicAdd(&sm.n, tn);
+  double t = (lane < chunks ? sm.csum[lane] : 0) + (64 + lane < chunks ? sm.csum[64 + lane] : 0);
+  t = sum_over_wave(t);
+  __syncthreads();
+  {
+    double weight = 0, wall;
+    int n = 0, call;
+    if (tid < NB) {
+      n = tid < NB - 1 ? (int)sm.many.count[tid] : sm.n;
+      weight = tid < NB - 1 ? (double)sm.many.sum[tid] / ONE * sm.et[tid] : t;
     }
-    __syncthreads();
-    double weight = 0;
-    if (!half) {
-      s += sm.half.sum[j];
-      n += sm.half.count[j];
-      weight = (double)s / ONE * sm.et[j];
-      if (j == NB - 1) {
-        weight = 0;
-        n = 0;
-        for (int i = 0; i < SW; ++i) {
-          weight += sm.half.tail[i];
-          n += sm.half.tcount[i];
-        }
-      }
-    } else {
-      n = 0;
-    }
-    double wall;
-    int call;
     const double wb = block_before<double>(weight, sm.wsum, wall);
     const int cb = block_before<int32_t>(n, sm.wcount, call);
-    if (!half) {
-      sm.upto[j] = wb + weight;
-      sm.cupto[j] = cb + n;
+    if (tid < NB) {
+      sm.upto[tid] = wb + weight;
+      sm.cupto[tid] = cb + n;
     }
   }
   Cut cut = {NB - 1, false, 0.f, 0};
@@ -763,7 +841,7 @@ __device__ __attribute__((noinline)) void deep_cut(const u64* bins, const Sample
       return by_rank ? sm.cupto[i] >= top_k : sm.cupto[i] > 0 && sm.upto[i] >= goal;
     }));
     const int n = sm.cupto[j] - number_below(j);
-    const u64 s = border_in_bin(r, j, n, by_rank, top_k - number_below(j), (goal - weight_below(j)) / sm.et[j] * ONE,
+    const u64 s = border_in_bin(r, codes, chunks, j, n, by_rank, top_k - number_below(j), (goal - weight_below(j)) / sm.et[j] * ONE,
                                 min(n, kept - number_below(j)), cut);
     holds = n <= CAP ? j : -1;
     if (by_rank) {
@@ -778,8 +856,12 @@ __device__ __attribute__((noinline)) void deep_cut(const u64* bins, const Sample
     const int j = cut.bin, n = sm.cupto[j] - number_below(j);
     if (n <= CAP) {
       if (holds != j) {
-        bin_range(r, j);
-        gather(r, sm.klo, sm.khi);
+        if (j < NB - 1 && codes) {
+          gather_bin(r, codes, chunks, j);
+        } else {
+          bin_range(r, j);
+          gather(r, sm.klo, sm.khi);
+        }
       }
       for (int i = tid; i < n; i += ST) {
         const float y = key_x(sm.list[i]);
@@ -844,14 +926,14 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
     sm.number = 0;
   }
   const double d = ref - st.ref;
-  const double y = exp((tid < NB ? -tid : -d) / RES);
+  const double y = bin_weight(tid < NB ? tid : d);
   if (tid < NB) {
     sm.et[tid] = y;
     sm.bins[tid] = 0;
   }
   __syncthreads();
   if (ci >= 0 && ci < chunks) {
-    const int delta = d < (1 << 20) ? (int)d : 1 << 20;
+    const int delta = d < (1 << 20) ? (int)d : 1 << 20;  // (-infinity: no finite logit, no weight)
     sm.delta[ci] = delta;
     sm.scale[ci] = y;
     sm.csum[ci] = st.total * y;
@@ -900,18 +982,11 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
     // the least logit with w >= min_p, and its bin
     float xm = 0;
     int jm = NB;
-    const uint32_t ktop = (uint32_t)(key >> 32), kmin = logit_order(-3.4028234663852886e38f);
+    const uint32_t ktop = (uint32_t)(key >> 32);
     if (min_p > 0.f) {
-      if (tid < 64) {
-        const double lim = fmin((double)min_p, 1.0);
-        const float guess = (float)fmax((double)top + (double)T * log(lim), -3.4028234663852886e38);
-        const uint32_t k = least_true(kmin, ktop, logit_order(guess), [&](uint32_t o) {
-          return exp(((double)logit_of(o) - (double)top) / (double)T) >= lim;
-        });
-        if (tid == 0) sm.klo = k;
-      }
-      __syncthreads();
-      xm = logit_of(sm.klo);
+      const double y = (double)top + (double)T * log64(fmin((double)min_p, 1.0));
+      xm = fmaxf((float)y, -3.4028234663852886e38f);
+      if ((double)xm < y) xm = logit_of(logit_order(xm) + 1);  // rounded up
       jm = bin_of(ref, floor((double)xm * sc.c));
     }
     // the borders among the listed logits: by number, then by weight
@@ -951,7 +1026,7 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
       deep = cut.part && cut.bin > depth;
     }
     if (deep) {
-      deep_cut(a.bins + s0 * NB, a.stat + s0, chunks, x, a.vocab, sc.c, sc.in, ref, ktop, number, whole, top_k, top_p, xm, jm);
+      deep_cut(a.bins + s0 * NB, a.stat + s0, top_k <= 0 || top_k > a.list ? a.codes + s0 * SC : nullptr, chunks, x, a.vocab, sc.c, sc.in, ref, ktop, number, whole, top_k, top_p, xm, jm);
       __syncthreads();
       cut = sm.cut;
     } else if (cut.part) {  // the chunks' sums of what is kept: all of it is listed, a wave's 64 are of one chunk
@@ -1009,8 +1084,8 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
     const double weight = mine ? __builtin_bit_cast(double, weights[i]) : 0;
     double run = 0;
     if (weight > 0)
-#pragma unroll 1
-      for (int e = tid & 3; e < a.list; e += 4)
+#pragma unroll 8
+      for (int e = tid & 3; e < a.list; e += 4)  // (list: a multiple of 64)
         if ((uint32_t)keys[e] > low) run += __builtin_bit_cast(double, weights[e]);
     run += __shfl_xor(run, 1);
     run += __shfl_xor(run, 2);
@@ -1022,7 +1097,7 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
     __syncthreads();
     if (weight > 0 && (tid & 3) == 0 && v == (sm.first[0] < INT32_MAX ? sm.first[0] : sm.last[0])) {
       a.tokens[row] = v;
-      if (a.logprobs) a.logprobs[row] = (float)fmin(log(weight / z), 0.0);
+      if (a.logprobs) a.logprobs[row] = (float)fmin(log64(weight / z), 0.0);
     }
     return;
   }
@@ -1042,33 +1117,34 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
   }
   // a thread's sum, then, by the waves that the answer may be in, the place in it: the first logit with which the running
   // sum exceeds the goal, or the last one of any weight
-  double before = 0, weight = 0;
+  double* weights = reinterpret_cast<double*>(sm.lkey) + tid;  // (and on into lbin)
+  static_assert(sizeof(sm.lkey) + sizeof(sm.lbin) >= SC * sizeof(double));
+  double mine = 0, weight = 0, all;
+#pragma unroll 1
+  for (int q = 0; q < 8; ++q) {
+    const double p = (double)f[0] * sc.c, fl = floor(p);
+    const int j = bin_of(ref, fl);
+    double s = 0;
+    if (f[0] > -INFINITY && cut.keeps(j, f[0], v0 + q))
+      s = j < NB - 1 ? (double)fixed_in_bin(f[0], sc, fl) / ONE * sm.et[j] : exp_tail(p - ref);
+    weights[q * ST] = s;
+    mine += s;
+    turn(f);
+  }
+  double run = block_before<double>(mine, sm.wsum, all);
   int hit = -1, last = -1;
-#pragma unroll 1
-  for (int pass = 0; pass < 2; ++pass) {
-    double run = before;
-#pragma unroll 1
+  // sums in another order may differ in their last digits: a little more than the thread that has it
+  const bool here = mine > 0 && (run + mine) * (1 + SAME) > goal && run * (1 - SAME) <= goal;
+  if (__builtin_amdgcn_ballot_w64(here) || all * (1 - SAME) <= goal) {
+#pragma unroll
     for (int q = 0; q < 8; ++q) {
-      const double p = (double)f[0] * sc.c, fl = floor(p);
-      const int j = bin_of(ref, fl);
-      if (f[0] > -INFINITY && cut.keeps(j, f[0], v0 + q)) {
-        const double s = j < NB - 1 ? (double)fixed_in_bin(f[0], sc, fl) / ONE * sm.et[j] : exp_tail(p - ref);
-        run += s;
-        if (s > 0 && hit < 0 && pass == 1) {
-          if (run > goal) hit = v0 + q;
-          last = v0 + q;
-          weight = s;
-        }
+      const double s = weights[q * ST];
+      run += s;
+      if (s > 0 && hit < 0) {
+        if (run > goal) hit = v0 + q;
+        last = v0 + q;
+        weight = s;
       }
-      turn(f);
-    }
-    if (pass == 0) {
-      const double mine = run;
-      double all;
-      before = block_before<double>(mine, sm.wsum, all);
-      // sums in another order may differ in their last digits: a little more than the thread that has it
-      const bool here = mine > 0 && (before + mine) * (1 + SAME) > goal && before * (1 - SAME) <= goal;
-      if (!__builtin_amdgcn_ballot_w64(here) && all * (1 - SAME) > goal) break;
     }
   }
   if (hit >= 0) atomicMin(&sm.first[0], hit);
@@ -1077,7 +1153,7 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
   const int v = sm.first[0] < INT32_MAX ? sm.first[0] : sm.last[0];
   if (v >= 0 && (v == hit || v == last)) {
     a.tokens[row] = v;
-    if (a.logprobs) a.logprobs[row] = (float)fmin(log(weight / z), 0.0);
+    if (a.logprobs) a.logprobs[row] = (float)fmin(log64(weight / z), 0.0);
   }
 }
 
@@ -1090,7 +1166,7 @@ using namespace mkp;
 extern "C" size_t mk_sample_workspace_bytes(int rows, int vocab) {
   if (rows < 1 || rows > 65535 || vocab < 1 || vocab > SV_MAX) return 0;
   const size_t slots = (size_t)rows * ((vocab + SC - 1) / SC);
-  return sample_align(slots * sizeof(SampleStat)) + slots * (NB + LIST_MAX) * sizeof(u64);
+  return sample_align(slots * sizeof(SampleStat)) + slots * ((NB + LIST_MAX) * sizeof(u64) + SC);
 }
 
 extern "C" hipError_t mk_sample(int rows, int vocab, const float* logits, int64_t row_stride, const float* uniforms,
@@ -1119,6 +1195,7 @@ extern "C" hipError_t mk_sample(int rows, int vocab, const float* logits, int64_
   a.list = std::min(LIST_MAX, LISTED * ST / a.chunks & ~63);
   a.bins = reinterpret_cast<u64*>(ws + sample_align(slots * sizeof(SampleStat)));
   a.listed = a.bins + slots * NB;
+  a.codes = reinterpret_cast<uint8_t*>(a.listed + slots * LIST_MAX);
   hipLaunchKernelGGL(sample_chunk_kernel, dim3(a.chunks, rows), dim3(ST), 0, stream, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
