@@ -31,9 +31,9 @@
 
 namespace mkp {
 
-constexpr int ST = 1024;            // threads of both kernels
+constexpr int ST = 1024;            // threads of the second kernel
 constexpr int SW = ST / 64;
-constexpr int SC = 8 * ST;          // logits of a chunk
+constexpr int SC = 8192;            // logits of a chunk
 constexpr int SV_MAX = 1 << 20;
 constexpr int SCH = SV_MAX / SC;    // chunks of a row at most
 constexpr int NB = 512;             // bins; the last one is the tail
@@ -132,16 +132,16 @@ __device__ __forceinline__ u64 max_over_wave(u64 v) {
 }
 
 // Sums over the threads before this one and over all (numbers that commute exactly, or in a fixed order).
-template <typename V>
+template <int WAVES = SW, typename V>
 __device__ __forceinline__ V block_before(V v, V* lds, V& total) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const V x = scan_wave(v, plus<V>);
   __syncthreads();
   if (lane == 63) lds[w] = x;
   __syncthreads();
-  const V y = scan_row16(lds[lane & (SW - 1)], plus<V>);  // every wave: the waves' sums, up to each
-  static_assert(SW == 16);
-  total = at_lane(y, SW - 1);
+  const V y = scan_row16(lds[lane & (WAVES - 1)], plus<V>);  // every wave: the waves' sums, up to each
+  static_assert(WAVES <= 16 && (WAVES & (WAVES - 1)) == 0);
+  total = at_lane(y, WAVES - 1);
   const V before = at_lane(y, max(w - 1, 0));
   return (w ? before : (V)0) + (x - v);
 }
@@ -207,8 +207,8 @@ __device__ __forceinline__ int bin_of(double ref, double fl) {
   return k < NB - 1 ? (int)k : NB - 1;
 }
 
-// Both kernels run each of their instructions a few times at most, and what takes their time beside the loads is the
-// fetch of cold code. So loops are not unrolled: eight numbers in registers turn round instead.
+// The second kernel runs each of its instructions a few times at most, and what takes its time beside the loads is the
+// fetch of cold code. So its loops are not unrolled: eight numbers in registers turn round instead.
 __device__ __forceinline__ void turn(float (&f)[8]) {
   const float x = f[0];
 #pragma unroll
@@ -216,18 +216,21 @@ __device__ __forceinline__ void turn(float (&f)[8]) {
   f[7] = x;
 }
 
-__global__ void __launch_bounds__(ST, 8) sample_chunk_kernel(const SampleArgs a) {
+// W waves to a chunk's 8,192 logits.
+template <int W>
+__global__ void __launch_bounds__(64 * W) sample_chunk_kernel(const SampleArgs a) {
+  constexpr int N = SC / (64 * W), PB = (NB + 64 * W - 1) / (64 * W);  // logits and bins to a thread
   __shared__ u64 bins[NB];
-  __shared__ u64 skey[SW];
-  __shared__ double stail[SW], stotal[SW];
-  __shared__ int32_t stc[SW], scan[SW];
+  __shared__ u64 skey[W];
+  __shared__ double stail[W], stotal[W];
+  __shared__ int32_t stc[W], scan[W];
   __shared__ int sdepth;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int row = blockIdx.y, v0 = blockIdx.x * SC + 512 * w + 4 * lane;  // this lane's logits: v0 + 256 j + q
+  const int row = blockIdx.y, v0 = blockIdx.x * SC + 64 * N * w + 4 * lane;  // this lane's logits: v0 + 256 j + q
   const float* x = a.logits + row * a.row_stride;
-  float f[8];
+  float f[N];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
+  for (int j = 0; j < N / 4; ++j) {
     const int v = v0 + 256 * j;
     if (v + 3 < a.vocab) {
       const f4a t = *reinterpret_cast<const f4a*>(x + v);
@@ -240,24 +243,26 @@ __global__ void __launch_bounds__(ST, 8) sample_chunk_kernel(const SampleArgs a)
   }
   const float T = a.temperature[row];
   const int top_k = a.top_k[row];
-  const bool filtered = top_k > 0 || !(a.top_p[row] >= 1.f) || a.min_p[row] > 0.f;
-  if (tid < NB) bins[tid] = 0;
+  const float top_p = a.top_p[row], min_p = a.min_p[row];
+  const bool filtered = top_k > 0 || !(top_p >= 1.f) || min_p > 0.f;
+  for (int i = tid; i < NB; i += 64 * W) bins[i] = 0;
   if (tid == 0) sdepth = -1;
   float m = -INFINITY;
   bool bad = false;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < N; ++i) {
     m = fmaxf(m, f[i]);
     bad |= !(f[i] < INFINITY);  // NaN too
   }
-  int at = SV_MAX;
+  int at = 0;
+  if (T == 0.f)  // nobody else asks for the token
 #pragma unroll
-  for (int i = 7; i >= 0; --i)
-    if (f[i] == m) at = v0 + 256 * (i >> 2) + (i & 3);
-  u64 key = max_over_wave(bad ? ~(u64)0 : logit_key(m, min(at, SV_MAX)));
+    for (int i = N - 1; i >= 0; --i)
+      if (f[i] == m) at = v0 + 256 * (i >> 2) + (i & 3);
+  u64 key = max_over_wave(bad ? ~(u64)0 : logit_key(m, at));
   if (lane == 0) skey[w] = key;
   __syncthreads();
-  key = max_over_wave(skey[lane & (SW - 1)]);
+  key = max_over_wave(skey[lane & (W - 1)]);
   const float top = key_x(key);  // NaN, where all bits are set
   const int64_t slot = (int64_t)row * a.chunks + blockIdx.x;
   const Scale s = scale_of_row(T, top);
@@ -265,79 +270,109 @@ __global__ void __launch_bounds__(ST, 8) sample_chunk_kernel(const SampleArgs a)
   out.ref = top == -INFINITY ? -INFINITY : floor((double)top * s.c);
   out.key = key;
   out.depth = NB;
-  const bool none = !(T > 0.f) || !(top > -INFINITY);  // the likeliest, no number, or an answer that has failed
-  int bin[8];
+  if (!(T > 0.f) || !(top > -INFINITY)) {  // the likeliest, no number, or an answer that has failed
+    if (filtered) {
+      for (int i = tid; i < NB; i += 64 * W) a.bins[slot * NB + i] = 0;
+      for (int i = tid; i < a.list; i += 64 * W) a.listed[slot * a.list + i] = 0;
+    }
+    if (tid == 0) a.stat[slot] = out;
+    return;
+  }
+  if (min_p > 0.f && top_p >= 1.f) {  // what min_p leaves out against the chunk's maximum nobody asks for
+    const float low = (float)((double)top + (double)T * log64(fmin((double)min_p, 1.0)));
+    const float lim = low - fmaxf(fabsf(low) * 0x1p-22f, 1e-37f);
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = f[i] >= lim ? f[i] : -INFINITY;
+  }
+  const bool coded = filtered && (top_k <= 0 || top_k > a.list);
+  uint32_t* codes = reinterpret_cast<uint32_t*>(a.codes + slot * SC + 64 * N * w + 4 * lane);
   double tail = 0;
   int tc = 0;
-  if (!none) {
-#pragma unroll 1
-    for (int i = 0; i < 8; ++i) {
-      const double p = (double)f[0] * s.c, fl = floor(p);
-      const int j = bin_of(out.ref, fl);
-      if (j < NB - 1) {
-        atomicAdd(&bins[j], fixed_in_bin(f[0], s, fl) + (1ull << CNT));
-      } else if (f[0] > -INFINITY) {
+#pragma unroll
+  for (int j = 0; j < N / 4; ++j) {
+    uint32_t code = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int i = 4 * j + q;
+      const double p = (double)f[i] * s.c, fl = floor(p);
+      const int bin = bin_of(out.ref, fl);
+      if (bin < NB - 1) {
+        atomicAdd(&bins[bin], fixed_in_bin(f[i], s, fl) + (1ull << CNT));
+      } else if (f[i] > -INFINITY) {
         tail += exp_tail(p - out.ref);
         ++tc;
       }
-      turn(f);
-#pragma unroll
-      for (int k = 0; k < 7; ++k) bin[k] = bin[k + 1];
-      bin[7] = j;
+      code |= (uint32_t)(bin >> 1) << (8 * q);
     }
-    if (__builtin_amdgcn_ballot_w64(tc > 0)) {
-      tail = sum_over_wave(tail);
-      tc = sum_over_wave(tc);
-    }
-    if (lane == 0) {
-      stail[w] = tail;
-      stc[w] = tc;
-    }
-    __syncthreads();
+    if (coded) codes[64 * j] = code;
   }
-  const u64 b = tid < NB && !none ? bins[tid] : 0;
-  if (!none) {
-    const double weight = w < NB / 64 ? sum_over_wave((double)(b & SUM_MASK) / ONE * bin_weight(tid)) : 0;
-    if (lane == 0) stotal[w] = weight;
-    int all;
-    const int upto = block_before<int32_t>((int)(b >> CNT), scan, all) + (int)(b >> CNT);  // (stotal is written behind it)
-    const u64 in = __builtin_amdgcn_ballot_w64(tid < NB - 1 && upto <= a.list);
-    if (filtered && lane == 0 && in) atomicAdd(&sdepth, __popcll(in));
+  if (__builtin_amdgcn_ballot_w64(tc > 0)) {
+    tail = sum_over_wave(tail);
+    tc = sum_over_wave(tc);
+  }
+  if (lane == 0) {
+    stail[w] = tail;
+    stc[w] = tc;
+  }
+  __syncthreads();
+  // the bins' weights and numbers, PB to a thread
+  u64 b[PB];
+  double weight = 0;
+  int number = 0, all;
+#pragma unroll
+  for (int i = 0; i < PB; ++i) {
+    const int j = PB * tid + i;
+    b[i] = j < NB ? bins[j] : 0;
+    weight += (double)(b[i] & SUM_MASK) / ONE * bin_weight(j);
+    number += (int)(b[i] >> CNT);
+  }
+  weight = sum_over_wave(weight);
+  if (lane == 0) stotal[w] = weight;
+  int upto = block_before<W>(number, scan, all);  // (stotal is written behind it)
 #pragma unroll 1
-    for (int i = 0; i < SW; ++i) {
-      out.tail += stail[i];
-      out.tail_count += stc[i];
-      out.total += stotal[i];
-    }
-    out.total += out.tail;
-    out.number = all + out.tail_count;
+  for (int i = 0; i < W; ++i) {
+    out.tail += stail[i];
+    out.tail_count += stc[i];
+    out.total += stotal[i];
   }
+  out.total += out.tail;
+  out.number = all + out.tail_count;
   if (filtered) {
-    if (tid < NB) a.bins[slot * NB + tid] = b;
-    if (!none && (top_k <= 0 || top_k > a.list)) {
-      uint8_t* codes = a.codes + slot * SC + (v0 - (int)blockIdx.x * SC);
+    // the bins that the list holds in full
+    int in = 0;
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        *reinterpret_cast<uint32_t*>(codes + 256 * j) = (uint32_t)(bin[4 * j] >> 1) | (uint32_t)(bin[4 * j + 1] >> 1) << 8 |
-                                                        (uint32_t)(bin[4 * j + 2] >> 1) << 16 |
-                                                        (uint32_t)(bin[4 * j + 3] >> 1) << 24;
+    for (int i = 0; i < PB; ++i) {
+      const int j = PB * tid + i;
+      upto += (int)(b[i] >> CNT);
+      if (j < NB) a.bins[slot * NB + j] = b[i];
+      in += __popcll(__builtin_amdgcn_ballot_w64(j < NB - 1 && upto <= a.list));
     }
-    // the bins that the list holds in full, and their logits in the threads' order
-    int n = 0;
-    if (!none) {
-      __syncthreads();
-      out.depth = out.number <= a.list ? NB : sdepth;
-      int mine = 0;
+    if (lane == 0 && in) atomicAdd(&sdepth, in);
+    __syncthreads();
+    out.depth = out.number <= a.list ? NB : sdepth;
+    // their logits, in the threads' order: first those that cannot be lower, to a part of a bin
+    const double low = out.ref - out.depth;
+    const float lim = out.depth == NB ? -INFINITY : (float)fmax((low - 0.5) / s.c, -3.4028234663852886e38);
+    uint32_t mine = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mine += f[i] > -INFINITY && bin[i] <= out.depth;
-      int to = block_before<int32_t>(mine, scan, n);
-      if (mine > 0)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (f[i] > -INFINITY && bin[i] <= out.depth)
-            a.listed[slot * a.list + to++] = logit_key(f[i], v0 + 256 * (i >> 2) + (i & 3));
+    for (int i = 0; i < N; ++i) mine = mine + mine + (f[i] >= lim && f[i] > -INFINITY);
+    uint32_t keep = 0;
+    for (uint32_t todo = mine; todo;) {
+      const int e = 31 - __clz(todo);
+      todo &= ~(1u << e);
+      const int i = N - 1 - e;
+      const float y = x[v0 + 256 * (i >> 2) + (i & 3)];  // again: cheaper than finding it among the registers
+      if (out.depth == NB || floor((double)y * s.c) >= low) keep |= 1u << e;
     }
-    for (int i = n + tid; i < a.list; i += ST) a.listed[slot * a.list + i] = 0;
+    int n;
+    int to = block_before<W>((int)__popc(keep), scan, n);
+    while (keep) {
+      const int e = 31 - __clz(keep);
+      keep &= ~(1u << e);
+      const int i = N - 1 - e, v = v0 + 256 * (i >> 2) + (i & 3);
+      a.listed[slot * a.list + to++] = logit_key(x[v], v);
+    }
+    for (int i = n + tid; i < a.list; i += 64 * W) a.listed[slot * a.list + i] = 0;
   }
   if (tid == 0) a.stat[slot] = out;
 }
@@ -402,6 +437,11 @@ struct PickSmem {
       u64 raw[RANKED], key[RANKED];
     } sort;
     double lsum[LISTED * SW];  // kept weights of 64 listed logits each
+    struct {
+      uint32_t map[SC / 32];
+      int mapped[SC / 32], token[LIST_MAX];
+      double inorder[LIST_MAX];
+    };
   };
   double wsum[SW];
   int32_t wcount[SW];
@@ -491,7 +531,7 @@ __device__ __attribute__((noinline)) void border_in_list(int n, int j, double c,
     __syncthreads();
     const u64 b0 = sm.sub[2 * tid], b1 = sm.sub[2 * tid + 1];
     u64 all;
-    const u64 before = block_before<u64>(b0 + b1, sm.wfix, all);
+    const u64 before = block_before(b0 + b1, sm.wfix, all);
     const int c0 = above + (int)(before >> CNT);
     const u64 s0 = sabove + (before & SUM_MASK);
     const int c1 = c0 + (int)(b0 >> CNT), c2 = c1 + (int)(b1 >> CNT);
@@ -541,7 +581,7 @@ __device__ __attribute__((noinline)) void border_in_list(int n, int j, double c,
   __syncthreads();
   const u64 k = tid < n ? sm.sort.key[tid] : 0, mine = tid < n ? fixed_weight(s, ref, key_x(k), j) : 0;
   u64 all;
-  const u64 before = sabove + block_before<u64>(mine, sm.wfix, all);
+  const u64 before = sabove + block_before(mine, sm.wfix, all);
   if (tid < n && (tid == 0 || !reached(above + tid, before)) && (tid == n - 1 || reached(above + tid + 1, before + mine))) {
     sm.key = k;
     sm.sum = before + mine;
@@ -625,25 +665,28 @@ __device__ __forceinline__ void gather(const Row& r, uint32_t klo, uint32_t khi)
   __syncthreads();
 }
 
-// Gathers the logits of bin j, not the tail's, at most CAP, by the codes: 16 of them to a load.
-__device__ __forceinline__ void gather_bin(const Row& r, const uint8_t* codes, int chunks, int j) {
+// Gathers the logits of bin j, not the tail's, at most CAP, by the codes: 16 of them to a load. False if too many others
+// have their code.
+__device__ __forceinline__ bool gather_bin(const Row& r, const uint8_t* codes, int chunks, int j) {
   PickSmem& sm = smem();
+  int* maybe = reinterpret_cast<int*>(sm.lkey);
+  static_assert(sizeof(sm.lkey) >= 2 * CAP * sizeof(int));
   const int tid = threadIdx.x;
   __syncthreads();
-  if (tid == 0) sm.n = 0;
+  if (tid == 0) sm.n = sm.found = 0;
   __syncthreads();
   const double fl = r.ref - j;
   const int units = chunks * (SC / 16);
 #pragma unroll 1
-  for (int base = 0; base < units; base += 4 * ST) {
-    uint4 q[4];
+  for (int base = 0; base < units; base += 5 * ST) {
+    uint4 q[5];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 5; ++i) {
       const int at = base + i * ST + tid;
       q[i] = at < units ? *reinterpret_cast<const uint4*>(codes + (int64_t)16 * at) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 5; ++i) {
       const int at = base + i * ST + tid, k = j - sm.delta[min(at / (SC / 16), chunks - 1)];  // the chunk's bin
       if (at >= units || k < 0) continue;
       const uint32_t code = (uint32_t)(k >> 1) * 0x01010101u, w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
@@ -657,17 +700,25 @@ __device__ __forceinline__ void gather_bin(const Row& r, const uint8_t* codes, i
       while (mask) {
         const int bit = __ffs(mask) - 1, v = 16 * at + 4 * (bit & 7) + (bit >> 3);
         mask &= mask - 1;
-        if (v < r.vocab) {
-          const float x = r.x[v];
-          if (floor((double)x * r.s.c) == fl) {
-            const int to = atomicAdd(&sm.n, 1);
-            if (to < CAP) sm.list[to] = logit_key(x, v);
-          }
-        }
+        const int to = atomicAdd(&sm.found, 1);
+        if (to < 2 * CAP) maybe[to] = v;
       }
     }
   }
   __syncthreads();
+  const int all = sm.found;
+  if (all > 2 * CAP) return false;
+#pragma unroll 4
+  for (int i = tid; i < all; i += ST) {
+    const int v = maybe[i];
+    const float x = v < r.vocab ? r.x[v] : -INFINITY;
+    if (floor((double)x * r.s.c) == fl) {
+      const int to = atomicAdd(&sm.n, 1);
+      if (to < CAP) sm.list[to] = logit_key(x, v);
+    }
+  }
+  __syncthreads();
+  return true;
 }
 
 // Finds the border within bin j, which has `count` logits: the first of them, in order, at which their number reaches
@@ -677,8 +728,7 @@ __device__ __forceinline__ u64 border_in_bin(const Row& r, const uint8_t* codes,
                                              int rank, double goal, int most, Cut& cut) {
   PickSmem& sm = smem();
   const int tid = threadIdx.x;
-  if (count <= CAP && j < NB - 1 && codes) {
-    gather_bin(r, codes, chunks, j);
+  if (count <= CAP && j < NB - 1 && codes && gather_bin(r, codes, chunks, j)) {
     border_in_list(count, j, r.s.c, r.s.in, r.ref, by_rank, rank, goal, most, 0, 0);
     cut = {j, true, key_x(sm.key), key_v(sm.key)};
     return sm.sum;
@@ -707,8 +757,8 @@ __device__ __forceinline__ u64 border_in_bin(const Row& r, const uint8_t* codes,
     const u64 s0 = sm.many.sum[2 * tid], s1 = sm.many.sum[2 * tid + 1];
     int call;
     u64 sall;
-    int cb = above + block_before<int32_t>(c0 + c1, sm.wcount, call);
-    u64 sb = sabove + block_before<u64>(s0 + s1, sm.wfix, sall);
+    int cb = above + block_before(c0 + c1, sm.wcount, call);
+    u64 sb = sabove + block_before(s0 + s1, sm.wfix, sall);
     // the one place where it is reached, at the end of the range if nowhere before
     const int lastb = (int)((khi - klo) >> shift);
     const bool r0 = reached(cb + c0, sb + s0) || 2 * tid >= lastb, r1 = reached(cb + c0 + c1, sb + s0 + s1) || 2 * tid + 1 >= lastb;
@@ -748,7 +798,7 @@ __device__ __forceinline__ u64 border_in_bin(const Row& r, const uint8_t* codes,
         const int v = base + 4 * tid + q;
         mine += v < r.vocab && r.x[v] == x;
       }
-      int before = seen + block_before<int32_t>(mine, sm.wcount, all);
+      int before = seen + block_before(mine, sm.wcount, all);
       if (before < take && before + mine >= take)
         for (int q = 0; q < 4; ++q) {
           const int v = base + 4 * tid + q;
@@ -823,8 +873,8 @@ __device__ __attribute__((noinline)) void deep_cut(const u64* bins, const Sample
       n = tid < NB - 1 ? (int)sm.many.count[tid] : sm.n;
       weight = tid < NB - 1 ? (double)sm.many.sum[tid] / ONE * sm.et[tid] : t;
     }
-    const double wb = block_before<double>(weight, sm.wsum, wall);
-    const int cb = block_before<int32_t>(n, sm.wcount, call);
+    const double wb = block_before(weight, sm.wsum, wall);
+    const int cb = block_before(n, sm.wcount, call);
     if (tid < NB) {
       sm.upto[tid] = wb + weight;
       sm.cupto[tid] = cb + n;
@@ -856,9 +906,7 @@ __device__ __attribute__((noinline)) void deep_cut(const u64* bins, const Sample
     const int j = cut.bin, n = sm.cupto[j] - number_below(j);
     if (n <= CAP) {
       if (holds != j) {
-        if (j < NB - 1 && codes) {
-          gather_bin(r, codes, chunks, j);
-        } else {
+        if (j == NB - 1 || !codes || !gather_bin(r, codes, chunks, j)) {
           bin_range(r, j);
           gather(r, sm.klo, sm.khi);
         }
@@ -972,8 +1020,8 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
       const double weight = tid < NB ? (double)(b & SUM_MASK) / ONE * sm.et[tid] : 0;
       double all;
       int call;
-      const double wb = block_before<double>(weight, sm.wsum, all);
-      const int cb = block_before<int32_t>((int)(b >> CNT), sm.wcount, call);
+      const double wb = block_before(weight, sm.wsum, all);
+      const int cb = block_before((int)(b >> CNT), sm.wcount, call);
       if (tid < NB) {
         sm.upto[tid] = wb + weight;
         sm.cupto[tid] = cb + (int)(b >> CNT);
@@ -1075,28 +1123,33 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
   }
   __syncthreads();
   const double goal = sm.goal, z = sm.z;
-  if (from_list) {  // four lanes to a logit add up what is before it
-    const u64* keys = sm.lkey + sm.found * a.list;
-    const u64* weights = sm.lbin + sm.found * a.list;
-    const int i = tid >> 2;
-    const bool mine = i < a.list;
-    const uint32_t low = mine ? (uint32_t)keys[i] : 0;  // falls as the token rises
-    const double weight = mine ? __builtin_bit_cast(double, weights[i]) : 0;
-    double run = 0;
-    if (weight > 0)
-#pragma unroll 8
-      for (int e = tid & 3; e < a.list; e += 4)  // (list: a multiple of 64)
-        if ((uint32_t)keys[e] > low) run += __builtin_bit_cast(double, weights[e]);
-    run += __shfl_xor(run, 1);
-    run += __shfl_xor(run, 2);
-    const int v = (int)(0xffffffffu - low);
+  if (from_list) {  // the kept logits of the chunk in the order of their tokens: a bit map tells each its place
+    const int i = sm.found * a.list + tid, first = sm.found * SC;
+    double weight = tid < a.list ? __builtin_bit_cast(double, sm.lbin[i]) : 0;
+    const int v = tid < a.list ? key_v(sm.lkey[i]) : 0, off = weight > 0 ? v - first : 0;
+    if (tid < SC / 32) sm.map[tid] = 0;
+    __syncthreads();
+    if (weight > 0) atomicOr(&sm.map[off >> 5], 1u << (off & 31));
+    __syncthreads();
+    const uint32_t bits = tid < SC / 32 ? sm.map[tid] : 0;
+    int n;
+    const int place = block_before((int)__popc(bits), sm.wcount, n);
+    if (tid < SC / 32) sm.mapped[tid] = place;
+    __syncthreads();
     if (weight > 0) {
-      if (run + weight > goal) atomicMin(&sm.first[0], v);
-      atomicMax(&sm.last[0], v);
+      const int at = sm.mapped[off >> 5] + __popc(sm.map[off >> 5] & ((1u << (off & 31)) - 1));
+      sm.inorder[at] = weight;
+      sm.token[at] = v;
     }
     __syncthreads();
-    if (weight > 0 && (tid & 3) == 0 && v == (sm.first[0] < INT32_MAX ? sm.first[0] : sm.last[0])) {
-      a.tokens[row] = v;
+    weight = tid < n ? sm.inorder[tid] : 0;
+    double all;
+    const double run = block_before(weight, sm.wsum, all);
+    // the first one whose running sum exceeds the goal, the last one if none does
+    if (tid < n && (run + weight > goal || tid == n - 1) && (tid == 0 || !(run > goal))) atomicMin(&sm.first[0], tid);
+    __syncthreads();
+    if (tid == sm.first[0]) {
+      a.tokens[row] = sm.token[tid];
       if (a.logprobs) a.logprobs[row] = (float)fmin(log64(weight / z), 0.0);
     }
     return;
@@ -1131,7 +1184,7 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
     mine += s;
     turn(f);
   }
-  double run = block_before<double>(mine, sm.wsum, all);
+  double run = block_before(mine, sm.wsum, all);
   int hit = -1, last = -1;
   // sums in another order may differ in their last digits: a little more than the thread that has it
   const bool here = mine > 0 && (run + mine) * (1 + SAME) > goal && run * (1 - SAME) <= goal;
@@ -1196,7 +1249,9 @@ extern "C" hipError_t mk_sample(int rows, int vocab, const float* logits, int64_
   a.bins = reinterpret_cast<u64*>(ws + sample_align(slots * sizeof(SampleStat)));
   a.listed = a.bins + slots * NB;
   a.codes = reinterpret_cast<uint8_t*>(a.listed + slots * LIST_MAX);
-  hipLaunchKernelGGL(sample_chunk_kernel, dim3(a.chunks, rows), dim3(ST), 0, stream, a);
+  const dim3 grid(a.chunks, rows);
+  if ((int64_t)a.chunks * rows <= 512) hipLaunchKernelGGL(sample_chunk_kernel<16>, grid, dim3(1024), 0, stream, a);
+  else hipLaunchKernelGGL(sample_chunk_kernel<4>, grid, dim3(256), 0, stream, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(sample_pick_kernel, dim3(rows), dim3(ST), 0, stream, a);
