@@ -491,7 +491,7 @@ __device__ __forceinline__ u64 fixed_weight(const Scale& s, double ref, float x,
 // (by_rank), or their sum reaches `goal` (in 2^-FIX of the bin's unit; the last of `most` logits, if none of them does),
 // `above` and `sabove` being those of the bin before the list. Into sm.key, and the sum up to it into sm.sum.
 // The range of the keys is narrowed, SUB bins at a time, to the few that are sorted.
-__device__ __attribute__((noinline)) void border_in_list(int n, int j, double c, double in, double ref, bool by_rank,
+__device__ __forceinline__ void border_in_list(int n, int j, double c, double in, double ref, bool by_rank,
                                                          int rank, double goal, int most, int above, u64 sabove) {
   PickSmem& sm = smem();
   const int tid = threadIdx.x;
@@ -817,7 +817,7 @@ __device__ __forceinline__ u64 border_in_bin(const Row& r, const uint8_t* codes,
 }
 
 // The border by all filters, into sm.cut, and the chunks' sums of what is kept, into sm.csum.
-__device__ __attribute__((noinline)) void deep_cut(const u64* bins, const SampleStat* stat,
+__device__ __forceinline__ void deep_cut(const u64* bins, const SampleStat* stat,
                                                    const uint8_t* codes, int chunks, const float* x,
                                                    int vocab, double c, double in, double ref, uint32_t ktop, int number,
                                                    double whole, int top_k, float top_p, float xm, int jm) {
