@@ -172,12 +172,14 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const CacheArgs a) {
 // -----------------------------------------------------------------------------------------------------------
 // attention of one token per sequence
 // -----------------------------------------------------------------------------------------------------------
-constexpr int TK = 32;                 // keys to a tile
-constexpr int AW = 4;                  // waves to a workgroup
-constexpr int NQ = 16;                 // queries to a unit: (sequence, K/V head, 16 of its query heads)
-constexpr int PART = D + 2;            // floats of one query's partial result: sum, maximum, output
+constexpr int TK = 32;           // keys to a tile
+constexpr int AW = 4;            // waves to a workgroup
+constexpr int NQ = 16;           // queries to a unit: (sequence, K/V head, 16 of its query heads)
+constexpr int OROW = D + 4;      // floats of a query's output in LDS
+constexpr int PART = D + 2;      // floats of one query's partial result: sum, maximum, output
 constexpr int SEQ_MAX = 4096;
-constexpr int PAGED_WGS = 512;         // workgroups that share the tiles out
+constexpr int PAGED_WGS = 512;   // workgroups that share the tiles out
+constexpr int START = 3;         // tiles that the start of a unit costs as much as: see Plan
 
 struct PagedArgs {
   PagePool p;
@@ -195,21 +197,28 @@ __device__ __forceinline__ int valid_length(const PagedArgs& a, int b) {
   const int n = a.lengths[b];
   return n > 0 && n <= a.capacity ? n : 0;
 }
-__device__ __forceinline__ int tiles_of(const PagedArgs& a, int b) { return (valid_length(a, b) + TK - 1) / TK; }
+
+// How the work is shared out. Each unit with keys takes START + its tiles places in one row of all units, sequence by
+// sequence, and every workgroup `per` places of the row, its waves a part each; the places before a unit's first tile
+// stand for what a unit costs by itself (its queries, its first loads). Places are counted in doubles, exactly.
+__device__ __forceinline__ double places_of(int length) { return length > 0 ? START + (length + TK - 1) / TK : 0; }
+__device__ __forceinline__ double places_per(const PagedArgs& a, double total, int waves) {
+  return fmax(floor((total + a.wgs - 1) / a.wgs), (double)((START + 1) * waves));
+}
 
 // Sums of v over the workgroup's threads before this one and over all of them.
 template <int THREADS>
-__device__ __forceinline__ int64_t scan_before(int64_t v, int64_t* lds, int64_t& total) {
+__device__ __forceinline__ double scan_before(double v, double* lds, double& total) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int64_t x = v;
+  double x = v;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int64_t y = __shfl_up(x, o);
+    const double y = __shfl_up(x, o);
     if (lane >= o) x += y;
   }
   if (lane == 63) lds[w] = x;
   __syncthreads();
-  int64_t before = x - v;
+  double before = x - v;
   total = 0;
 #pragma unroll
   for (int i = 0; i < THREADS / 64; ++i) {
@@ -260,323 +269,379 @@ __device__ __attribute__((noinline)) float whole_score(const uint8_t* k, float s
   return s;
 }
 
+// What a wave has of a unit that it did not do alone, in LDS: up to two to a wave, its first and its last unit.
+struct Piece {
+  int seq, unit, t0, t1;  // t0 == t1: none
+};
 template <int WAVES>
 struct PagedSmem {
-  float m[WAVES][NQ], l[WAVES][NQ];
-  float o[WAVES][NQ][D + 4];
-  int64_t scan[WAVES];
-  int64_t base;
-  int seq;
+  Piece piece[2 * WAVES];
+  float m[2 * WAVES][NQ], l[2 * WAVES][NQ];
+  double scan[WAVES], base[WAVES];
+  int seq[WAVES], len[WAVES];
 };
 
+template <int QP>
+__device__ __forceinline__ void store_out(uint8_t* out, int64_t at, float4 y) {  // 4 numbers of the output from at on
+  if constexpr (QP == 1) *reinterpret_cast<uint2*>(out + 2 * at) = make_uint2(pack_bf16x2(y.x, y.y), pack_bf16x2(y.z, y.w));
+  else *reinterpret_cast<float4*>(out + 4 * at) = y;
+}
+
 // E4M3: 8-bit pages. QP, PP: bf16 parts of a query and of a weight (1 and 2 for bf16 queries, 3 for fp32 ones).
-// SMALL: pages of fewer than TK positions, looked up key by key. SPLIT: the tiles of all units in one row are shared
-// out evenly, a unit's parts joined by paged_join_kernel; else a workgroup takes a unit.
+// SMALL: pages of fewer than TK positions, looked up key by key. SPLIT: the tiles of all units are shared out evenly, a
+// unit's parts joined by paged_join_kernel; else a workgroup takes a unit, a wave a run of its tiles.
 template <bool E4M3, int QP, int PP, bool SMALL, bool SPLIT, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, 2) paged_attention_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(64 * WAVES, WAVES <= 8 ? 2 : 4) paged_attention_kernel(const PagedArgs a) {
   __shared__ PagedSmem<WAVES> sm;
+  extern __shared__ __attribute__((aligned(16))) float outs[];  // [pieces][queries of a unit][OROW]
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int units = a.hkv * a.gt;  // of a sequence
   const int gmax = min(a.g, NQ);
-  int b, u, t0;  // sequence, unit, first tile in it
-  int64_t left;  // tiles still to do
+  int b, u, len;       // sequence, unit of it, its keys
+  double p = 0, left;  // places of the unit that are behind the wave, places that it has still to do
+  if (tid < 2 * WAVES) sm.piece[tid] = Piece{0, 0, 0, 0};
   if constexpr (SPLIT) {
     const int each = (a.nseq + 64 * WAVES - 1) / (64 * WAVES);
-    int64_t mine = 0, total;
+    double mine = 0, total;
+    int len0 = 0;
     for (int i = 0; i < each; ++i) {
       const int s = tid * each + i;
-      if (s < a.nseq) mine += tiles_of(a, s);
+      if (s < a.nseq) mine += places_of(len0 = valid_length(a, s));
     }
-    int64_t before = scan_before<64 * WAVES>(mine, sm.scan, total) * units;
+    double before = scan_before<64 * WAVES>(mine, sm.scan, total) * units;
     total *= units;
-    const int64_t per = max((int64_t)WAVES, (total + a.wgs - 1) / a.wgs);
-    const int64_t lo = blockIdx.x * per;
-    if (lo >= total) return;
-    if (lo >= before && lo < before + mine * units) {
-      for (int i = 0; i < each; ++i) {
-        const int64_t t = (int64_t)tiles_of(a, tid * each + i) * units;
-        if (lo < before + t) {
-          sm.seq = tid * each + i;
-          sm.base = before;
-          break;
-        }
-        before += t;
+    mine *= units;
+    const double per = places_per(a, total, WAVES), wper = floor((per + WAVES - 1) / WAVES);
+    if (blockIdx.x * per >= total) return;
+#pragma unroll 1
+    for (int v = 0; v < WAVES; ++v) {
+      const double lo = blockIdx.x * per + v * wper;
+      if (lo >= before && lo < before + mine) {
+        double base = before;
+        int s = tid * each;
+        if (each > 1)
+          while (true) {
+            len0 = valid_length(a, s);
+            const double end = base + places_of(len0) * units;
+            if (lo < end) break;
+            base = end;
+            ++s;
+          }
+        sm.seq[v] = s;
+        sm.len[v] = len0;
+        sm.base[v] = base;
       }
     }
     __syncthreads();
-    b = __builtin_amdgcn_readfirstlane(sm.seq);
-    const int64_t off = lo - sm.base;
-    const int T = tiles_of(a, b);
-    u = __builtin_amdgcn_readfirstlane((int)(off / T));
-    t0 = __builtin_amdgcn_readfirstlane((int)(off % T));
-    left = min(per, total - lo);
+    const double lo = blockIdx.x * per + w * wper;
+    left = fmin(fmin(wper, per - w * wper), total - lo);
+    b = __builtin_amdgcn_readfirstlane(sm.seq[w]);
+    len = __builtin_amdgcn_readfirstlane(sm.len[w]);
+    if (left > 0) {
+      const double cost = places_of(len), off = lo - sm.base[w];
+      double q = floor(off / cost);
+      if (q * cost > off) --q;
+      u = __builtin_amdgcn_readfirstlane((int)q);
+      p = off - q * cost;
+    }
   } else {
     b = blockIdx.x / units;
     u = blockIdx.x % units;
-    t0 = 0;
-    left = INT32_MAX;
+    len = __builtin_amdgcn_readfirstlane(valid_length(a, b));
+    const int T = (len + TK - 1) / TK, each = (T + WAVES - 1) / WAVES;
+    p = START + min(T, w * each);
+    left = min(each, T - min(T, w * each));
   }
   const int mask = (1 << a.p.shift) - 1;
-  while (true) {
-    const int len = __builtin_amdgcn_readfirstlane(valid_length(a, b));
-    const int T = (len + TK - 1) / TK, t1 = (int)min((int64_t)T, t0 + left);
-    const int kh = u / a.gt, h0 = kh * a.g + NQ * (u % a.gt), nq = min(NQ, a.g - NQ * (u % a.gt));
-    const int32_t* table = a.p.tables + b * a.p.tstride;
-    const uint8_t* kbase = a.p.k + kh * a.p.head;
-    const uint8_t* vbase = a.p.v + kh * a.p.head;
-    const uint8_t* ksb = E4M3 ? a.p.ks + kh * a.p.shead : nullptr;
-    const uint8_t* vsb = E4M3 ? a.p.vs + kh * a.p.shead : nullptr;
-    bool bad = false;
+  int piece = 2 * w;
+#pragma unroll 1
+  while (left > 0) {
+    const int T = (len + TK - 1) / TK;
+    const int t0 = __builtin_amdgcn_readfirstlane(max(0, (int)(p - START)));
+    const int t1 = __builtin_amdgcn_readfirstlane((int)fmin((double)T, fmax(0.0, p + left - START)));
+    if (t1 > t0) {
+      const int kh = u / a.gt, h0 = kh * a.g + NQ * (u % a.gt), nq = min(NQ, a.g - NQ * (u % a.gt));
+      const int32_t* table = a.p.tables + b * a.p.tstride;
+      const uint8_t* kbase = a.p.k + kh * a.p.head;
+      const uint8_t* vbase = a.p.v + kh * a.p.head;
+      const uint8_t* ksb = E4M3 ? a.p.ks + kh * a.p.shead : nullptr;
+      const uint8_t* vsb = E4M3 ? a.p.vs + kh * a.p.shead : nullptr;
+      bool bad = false;
 
-    // the queries as B operands: dims of step s at 8 lanes' width, as the keys' loads have them
-    auto dim_of = [&](int s) { return E4M3 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g; };
-    uint4 qf[4][QP];
-    const uint8_t* qrow = a.q + b * a.q_row + (int64_t)(h0 + n) * a.q_head;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      if constexpr (QP == 1) {
-        qf[s][0] = n < nq ? *reinterpret_cast<const uint4*>(qrow + 2 * dim_of(s)) : make_uint4(0, 0, 0, 0);
-      } else {
-        float x[8];
-        const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-        const float4 lo = n < nq ? *reinterpret_cast<const float4*>(qrow + 4 * dim_of(s)) : z;
-        const float4 hi = n < nq ? *reinterpret_cast<const float4*>(qrow + 4 * dim_of(s) + 16) : z;
-        x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w;
-        x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
-        parts_of<QP>(x, qf[s]);
-      }
-    }
-
-    // Places of keys, in bytes from a head's rows; a key past the last is the last one (its weight is 0, and a page
-    // past the sequence's is never looked at).
-    int entry = 0;  // !SMALL: the page of the tile that is loaded next
-    auto page_of = [&](int key) __attribute__((always_inline)) {
-      int page = table[key >> a.p.shift];
-      if ((uint32_t)page >= (uint32_t)a.p.pages) {
-        bad = true;
-        page = 0;
-      }
-      return page;
-    };
-    auto place = [&](int t, int kk, int64_t& at, int64_t& sat) __attribute__((always_inline)) {
-      const int key = min(t * TK + kk, len - 1);
-      const int page = SMALL ? page_of(key) : entry;
-      at = page * a.p.page + (key & mask) * a.p.row;
-      sat = page * a.p.spage + (key & mask);
-    };
-    Tile<E4M3> x;
-    auto load_k = [&](int t) __attribute__((always_inline)) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        int64_t at, sat;
-        place(t, 8 * (n >> 2) + 4 * h + (n & 3), at, sat);
-#pragma unroll
-        for (int s = 0; s < (E4M3 ? 2 : 4); ++s) x.k[h][s] = *reinterpret_cast<const uint4*>(kbase + at + 64 * s + 16 * g);
-        if constexpr (E4M3) x.ks[h] = ksb[sat];
-      }
-    };
-    auto load_v = [&](int t) __attribute__((always_inline)) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        int64_t at, sat;
-        place(t, 8 * g + j, at, sat);
-        if constexpr (E4M3) {
-          x.v[j] = *reinterpret_cast<const uint2*>(vbase + at + 8 * n);
-          x.vs[j] = vsb[sat];
-        } else {
-          x.v[j] = *reinterpret_cast<const uint4*>(vbase + at + 16 * n);
+      // Places of keys, in bytes from a head's rows; a key past the last is the last one (its weight is 0, and a page
+      // past the sequence's is never looked at).
+      int entry = 0;  // !SMALL: the page of the tile that is loaded next
+      auto page_of = [&](int key) __attribute__((always_inline)) {
+        int page = table[key >> a.p.shift];
+        if ((uint32_t)page >= (uint32_t)a.p.pages) {
+          bad = true;
+          page = 0;
         }
-      }
-    };
-    auto look_up = [&](int t) __attribute__((always_inline)) {
-      if constexpr (!SMALL) entry = page_of(min(t * TK, len - 1));
-    };
-
-    float m = -INFINITY, l = 0.f;
-    f32x4 o[8];
+        return page;
+      };
+      auto place = [&](int t, int kk, int64_t& at, int64_t& sat) __attribute__((always_inline)) {
+        const int key = min(t * TK + kk, len - 1);
+        const int page = SMALL ? page_of(key) : entry;
+        at = page * a.p.page + (key & mask) * a.p.row;
+        sat = page * a.p.spage + (key & mask);
+      };
+      Tile<E4M3> x;
+      auto load_k = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    int t = t0 + w;
-    if (t < t1) {
-      look_up(t);
-      load_k(t);
-      load_v(t);
-    }
-    for (; t < t1; t += WAVES) {
-      const int next = t + WAVES;
-      // scores
-      f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+        for (int h = 0; h < 2; ++h) {
+          int64_t at, sat;
+          place(t, 8 * (n >> 2) + 4 * h + (n & 3), at, sat);
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+          for (int s = 0; s < (E4M3 ? 2 : 4); ++s) x.k[h][s] = *reinterpret_cast<const uint4*>(kbase + at + 64 * s + 16 * g);
+          if constexpr (E4M3) x.ks[h] = ksb[sat];
+        }
+      };
+      auto load_v = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
-        for (int st = 0; st < 4; ++st) {
-          uint4 f;
+        for (int j = 0; j < 8; ++j) {
+          int64_t at, sat;
+          place(t, 8 * g + j, at, sat);
           if constexpr (E4M3) {
-            const uint4 r = x.k[h][st >> 1];
-            f = bf16x8_of_e4m3(st & 1 ? r.z : r.x, st & 1 ? r.w : r.y, scale_of(x.ks[h]));
+            x.v[j] = *reinterpret_cast<const uint2*>(vbase + at + 8 * n);
+            x.vs[j] = vsb[sat];
           } else {
-            f = x.k[h][st];
-          }
-#pragma unroll
-          for (int p = 0; p < QP; ++p) s[h] = mfma(f, qf[st][p], s[h]);
-        }
-      if constexpr (QP > 1) {
-        // Parts of a query may make NaN of an infinite key where the whole query makes an infinity: such scores are
-        // made again, while the query's sum is not NaN already.
-        bool again = false;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) again |= s[j >> 2][j & 3] != s[j >> 2][j & 3];
-        if (__builtin_amdgcn_ballot_w64(again && n < nq && l == l)) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            int64_t at, sat;
-            place(t, 8 * g + j, at, sat);
-            if (n < nq && l == l && s[j >> 2][j & 3] != s[j >> 2][j & 3])
-              s[j >> 2][j & 3] = whole_score<E4M3>(kbase + at, E4M3 ? scale_of(ksb[sat]) : 1.f,
-                                                   reinterpret_cast<const float*>(qrow));
+            x.v[j] = *reinterpret_cast<const uint4*>(vbase + at + 16 * n);
           }
         }
-      }
-      if (next < t1) {
-        look_up(next);
-        load_k(next);
-      }
-      constexpr float C = ATT_SCALE * 1.4426950408889634f;  // weights are powers of two
-      float e[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) e[j] = s[j >> 2][j & 3] * C;
-      if (t * TK + TK > len)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (t * TK + 8 * g + j >= len) e[j] = -INFINITY;
-      float top = e[0];
-#pragma unroll
-      for (int j = 1; j < 8; ++j) top = fmaxf(top, e[j]);
-      top = xmax32(xmax16(top));
-      if (__builtin_amdgcn_ballot_w64(top > m)) {
-        const float up = fmaxf(m, top), f = up == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - up);
-        m = up;
-        l *= f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] *= f;
-      }
-      const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        e[j] = __builtin_amdgcn_exp2f(e[j] - ref);
-        l += e[j];
-      }
-      uint4 pf[PP];
-      parts_of<PP>(e, pf);
-      // values
-      uint32_t r[8][4];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        uint4 f;
-        if constexpr (E4M3) f = bf16x8_of_e4m3(x.v[j].x, x.v[j].y, scale_of(x.vs[j]));
-        else f = x.v[j];
-        r[j][0] = f.x; r[j][1] = f.y; r[j][2] = f.z; r[j][3] = f.w;
-      }
-      if (next < t1) load_v(next);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        uint32_t f[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          f[q] = __builtin_amdgcn_perm(r[2 * q + 1][i >> 1], r[2 * q][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-        for (int p = 0; p < PP; ++p) o[i] = mfma(make_uint4(f[0], f[1], f[2], f[3]), pf[p], o[i]);
-      }
-    }
+      };
+      auto look_up = [&](int t) __attribute__((always_inline)) {
+        if constexpr (!SMALL) entry = page_of(min(t * TK, len - 1));
+      };
 
-    // the waves' results joined: what a query's weights refer to may differ from wave to wave
-    if (__builtin_amdgcn_ballot_w64(bad)) l = __builtin_nanf("");
-    l = xsum32(xsum16(l));
-    if (g == 0) {
-      sm.m[w][n] = m;
-      sm.l[w][n] = l;
-    }
-    if (n < nq)
+      look_up(t0);
+      load_k(t0);
+      load_v(t0);
+      // the queries as B operands: dims of step s at 8 lanes' width, as the keys' loads have them
+      auto dim_of = [&](int s) { return E4M3 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g; };
+      uint4 qf[4][QP];
+      const uint8_t* qrow = a.q + b * a.q_row + (int64_t)(h0 + n) * a.q_head;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {  // dims 32 g + 8 r + i
-        float* p = &sm.o[w][n][32 * g + 8 * r];
-        *reinterpret_cast<float4*>(p) = make_float4(o[0][r], o[1][r], o[2][r], o[3][r]);
-        *reinterpret_cast<float4*>(p + 4) = make_float4(o[4][r], o[5][r], o[6][r], o[7][r]);
+      for (int s = 0; s < 4; ++s) {
+        if constexpr (QP == 1) {
+          qf[s][0] = n < nq ? *reinterpret_cast<const uint4*>(qrow + 2 * dim_of(s)) : make_uint4(0, 0, 0, 0);
+        } else {
+          float y[8];
+          const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+          const float4 lo = n < nq ? *reinterpret_cast<const float4*>(qrow + 4 * dim_of(s)) : z;
+          const float4 hi = n < nq ? *reinterpret_cast<const float4*>(qrow + 4 * dim_of(s) + 16) : z;
+          y[0] = lo.x; y[1] = lo.y; y[2] = lo.z; y[3] = lo.w;
+          y[4] = hi.x; y[5] = hi.y; y[6] = hi.z; y[7] = hi.w;
+          parts_of<QP>(y, qf[s]);
+        }
       }
-    __syncthreads();
-    const bool whole = t0 == 0 && t1 == T;
-    float* part = SPLIT ? a.part + (int64_t)(2 * blockIdx.x + (t0 == 0)) * gmax * PART : nullptr;
+
+      float m = -INFINITY, l = 0.f;
+      f32x4 o[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int t = t0; t < t1; ++t) {
+        // scores
+        f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int st = 0; st < 4; ++st) {
+            uint4 f;
+            if constexpr (E4M3) {
+              const uint4 r = x.k[h][st >> 1];
+              f = bf16x8_of_e4m3(st & 1 ? r.z : r.x, st & 1 ? r.w : r.y, scale_of(x.ks[h]));
+            } else {
+              f = x.k[h][st];
+            }
+#pragma unroll
+            for (int i = 0; i < QP; ++i) s[h] = mfma(f, qf[st][i], s[h]);
+          }
+        if constexpr (QP > 1) {
+          // Parts of a query may make NaN of an infinite key where the whole query makes an infinity: such scores are
+          // made again, while the query's sum is not NaN already.
+          bool again = false;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) again |= s[j >> 2][j & 3] != s[j >> 2][j & 3];
+          if (__builtin_amdgcn_ballot_w64(again && n < nq && l == l)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              int64_t at, sat;
+              place(t, 8 * g + j, at, sat);
+              if (n < nq && l == l && s[j >> 2][j & 3] != s[j >> 2][j & 3])
+                s[j >> 2][j & 3] = whole_score<E4M3>(kbase + at, E4M3 ? scale_of(ksb[sat]) : 1.f,
+                                                     reinterpret_cast<const float*>(qrow));
+            }
+          }
+        }
+        if (t + 1 < t1) {
+          look_up(t + 1);
+          load_k(t + 1);
+        }
+        constexpr float C = ATT_SCALE * 1.4426950408889634f;  // weights are powers of two
+        float e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = s[j >> 2][j & 3] * C;
+        if (t * TK + TK > len)
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (t * TK + 8 * g + j >= len) e[j] = -INFINITY;
+        float top = e[0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) top = fmaxf(top, e[j]);
+        top = xmax32(xmax16(top));
+        if (__builtin_amdgcn_ballot_w64(top > m)) {
+          const float up = fmaxf(m, top), f = up == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - up);
+          m = up;
+          l *= f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] *= f;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          e[j] = __builtin_amdgcn_exp2f(e[j] - ref);
+          l += e[j];
+        }
+        uint4 pf[PP];
+        parts_of<PP>(e, pf);
+        // values
+        uint32_t r[8][4];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          uint4 f;
+          if constexpr (E4M3) f = bf16x8_of_e4m3(x.v[j].x, x.v[j].y, scale_of(x.vs[j]));
+          else f = x.v[j];
+          r[j][0] = f.x; r[j][1] = f.y; r[j][2] = f.z; r[j][3] = f.w;
+        }
+        if (t + 1 < t1) load_v(t + 1);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t f[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            f[q] = __builtin_amdgcn_perm(r[2 * q + 1][i >> 1], r[2 * q][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
+#pragma unroll
+          for (int k = 0; k < PP; ++k) o[i] = mfma(make_uint4(f[0], f[1], f[2], f[3]), pf[k], o[i]);
+        }
+      }
+      if (__builtin_amdgcn_ballot_w64(bad)) l = __builtin_nanf("");
+      l = xsum32(xsum16(l));
+
+      // the lane's dims 32 g + 8 r + i of query n: the output if the wave had the whole unit, else a piece of it
+      const bool whole = t0 == 0 && t1 == T;
+      const float inv = whole ? (l > 0.f ? 1.f / l : __builtin_nanf("")) : 1.f;  // no key of weight: NaN, as 0 / 0
+      if (n < nq) {
+        float* to = outs + (piece * gmax + n) * OROW + 32 * g;
+        const int64_t at = ((int64_t)b * a.hkv * a.g + h0 + n) * D + 32 * g;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int i = 0; i < 8; i += 4) {
+            const float4 y = make_float4(o[i][r] * inv, o[i + 1][r] * inv, o[i + 2][r] * inv, o[i + 3][r] * inv);
+            if (whole) store_out<QP>(a.out, at + 8 * r + i, y);
+            else *reinterpret_cast<float4*>(to + 8 * r + i) = y;
+          }
+      }
+      if (!whole) {
+        if (g == 0) {
+          sm.m[piece][n] = m;
+          sm.l[piece][n] = l;
+        }
+        if (lane == 0) sm.piece[piece] = Piece{b, u, t0, t1};
+        piece = 2 * w + 1;
+      }
+    }
+    const double cost = places_of(len);
+    left -= cost - p;
+    p = 0;
+    if (left > 0 && ++u == units) {
+      u = 0;
+      do ++b;
+      while (b < a.nseq && valid_length(a, b) == 0);
+      b = __builtin_amdgcn_readfirstlane(b);
+      if (b >= a.nseq) break;
+      len = __builtin_amdgcn_readfirstlane(valid_length(a, b));
+    }
+  }
+  __syncthreads();
+
+  // The pieces joined, unit by unit: what a query's weights refer to differs from piece to piece. A unit that the
+  // workgroup had whole is done, others go to the join.
+#pragma unroll 1
+  for (int e0 = 0; e0 < 2 * WAVES;) {
+    const Piece first = sm.piece[e0];
+    if (first.t0 == first.t1) {
+      ++e0;
+      continue;
+    }
+    int e1 = e0 + 1, t1 = first.t1;
+    for (int e = e1; e < 2 * WAVES; ++e) {
+      const Piece y = sm.piece[e];
+      if (y.t0 == y.t1) continue;
+      if (y.seq != first.seq || y.unit != first.unit) break;
+      e1 = e + 1;
+      t1 = y.t1;
+    }
+    const int T = ((SPLIT ? valid_length(a, first.seq) : len) + TK - 1) / TK;
+    const bool whole = first.t0 == 0 && t1 == T;
+    const int kh = first.unit / a.gt, h0 = kh * a.g + NQ * (first.unit % a.gt), nq = min(NQ, a.g - NQ * (first.unit % a.gt));
     for (int i = tid; i < nq * (D / 4); i += 64 * WAVES) {
       const int qi = i / (D / 4), d = 4 * (i % (D / 4));
-      float M = sm.m[0][qi];
-#pragma unroll
-      for (int v = 1; v < WAVES; ++v) M = fmaxf(M, sm.m[v][qi]);
+      float M = -INFINITY;
+      for (int e = e0; e < e1; ++e)
+        if (sm.piece[e].t0 != sm.piece[e].t1) M = fmaxf(M, sm.m[e][qi]);
       const float ref = M == -INFINITY ? 0.f : M;
       float sum = 0.f;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int v = 0; v < WAVES; ++v) {
-        const float f = __builtin_amdgcn_exp2f(sm.m[v][qi] - ref);
-        const float4 y = *reinterpret_cast<const float4*>(&sm.o[v][qi][d]);
-        sum += f * sm.l[v][qi];
+      for (int e = e0; e < e1; ++e) {
+        if (sm.piece[e].t0 == sm.piece[e].t1) continue;
+        const float f = __builtin_amdgcn_exp2f(sm.m[e][qi] - ref);
+        const float4 y = *reinterpret_cast<const float4*>(outs + (e * gmax + qi) * OROW + d);
+        sum += f * sm.l[e][qi];
         acc.x += f * y.x; acc.y += f * y.y; acc.z += f * y.z; acc.w += f * y.w;
       }
-      if (SPLIT && !whole) {
-        float* p = part + qi * PART;
-        if (d == 0) {
-          p[0] = sum;
-          p[1] = M;
-        }
-        // (PART is even: 8-byte aligned)
-        *reinterpret_cast<float2*>(p + 2 + d) = make_float2(acc.x, acc.y);
-        *reinterpret_cast<float2*>(p + 4 + d) = make_float2(acc.z, acc.w);
-        continue;
-      }
-      float inv = sum > 0.f ? 1.f / sum : __builtin_nanf("");  // no key of weight: NaN, as 0 / 0
-      if (!SPLIT && T == 0) {  // an empty sequence, or a length out of range
-        inv = a.lengths[b] == 0 ? 0.f : __builtin_nanf("");
-        acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      const int64_t at = ((int64_t)b * a.hkv * a.g + h0 + qi) * D + d;
-      if constexpr (QP == 1) {
-        *reinterpret_cast<uint2*>(a.out + 2 * at) =
-            make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+      if (whole) {
+        const float inv = sum > 0.f ? 1.f / sum : __builtin_nanf("");
+        store_out<QP>(a.out, ((int64_t)first.seq * a.hkv * a.g + h0 + qi) * D + d,
+                      make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
       } else {
-        *reinterpret_cast<float4*>(a.out + 4 * at) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+        float* to = a.part + ((int64_t)(2 * blockIdx.x + (first.t0 == 0)) * gmax + qi) * PART;
+        if (d == 0) {
+          to[0] = sum;
+          to[1] = M;
+        }
+        *reinterpret_cast<float2*>(to + 2 + d) = make_float2(acc.x, acc.y);  // (PART is even: 8-byte aligned)
+        *reinterpret_cast<float2*>(to + 4 + d) = make_float2(acc.z, acc.w);
       }
     }
-    if constexpr (!SPLIT) return;
-    left -= t1 - t0;
-    if (left <= 0) return;
-    __syncthreads();  // the next unit's results take the same places
-    t0 = 0;
-    if (++u == units) {
-      u = 0;
-      do ++b;
-      while (b < a.nseq && tiles_of(a, b) == 0);
-      b = __builtin_amdgcn_readfirstlane(b);
-      if (b >= a.nseq) return;
-    }
+    e0 = e1;
   }
+  if constexpr (!SPLIT)
+    if (len == 0) {  // an empty sequence, or a length out of range
+      const float y = a.lengths[b] == 0 ? 0.f : __builtin_nanf("");
+      const int kh = u / a.gt, h0 = kh * a.g + NQ * (u % a.gt), nq = min(NQ, a.g - NQ * (u % a.gt));
+      for (int i = tid; i < nq * (D / 4); i += 64 * WAVES)
+        store_out<QP>(a.out, ((int64_t)b * a.hkv * a.g + h0) * D + 4 * i, make_float4(y, y, y, y));
+    }
 }
 
 // Joins the parts of the units that more than one workgroup worked on, in their order: a workgroup per (sequence,
 // query head). Sequences without keys get their answer here too.
 template <bool FP32>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
-  __shared__ int64_t scan[4];
-  __shared__ int64_t sbase;
+  __shared__ double scan[4], sbase;
   __shared__ float red[4];
   __shared__ __attribute__((aligned(16))) float acc[8][D];
   __shared__ float accl[8];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int heads = a.hkv * a.g, b = blockIdx.x / heads, h = blockIdx.x % heads;
   const int kh = h / a.g, hg = h % a.g, u = kh * a.gt + hg / NQ, qi = hg % NQ, units = a.hkv * a.gt;
-  const int T = tiles_of(a, b);
-  if (T == 0) {
+  const int len = valid_length(a, b);
+  const int64_t at = (int64_t)blockIdx.x * D + tid;
+  if (len == 0) {
     const float x = a.lengths[b] == 0 ? 0.f : __builtin_nanf("");
-    const int64_t at = (int64_t)blockIdx.x * D + tid;
     if (tid < D) {
       if constexpr (FP32) reinterpret_cast<float*>(a.out)[at] = x;
       else reinterpret_cast<uint16_t*>(a.out)[at] = f32_to_bf16(x);
@@ -584,21 +649,20 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
     return;
   }
   const int each = (a.nseq + 255) / 256;
-  int64_t mine = 0, total;
+  double mine = 0, total;
   for (int i = 0; i < each; ++i) {
     const int s = tid * each + i;
-    if (s < a.nseq) mine += tiles_of(a, s);
+    if (s < a.nseq) mine += places_of(valid_length(a, s));
   }
-  int64_t before = scan_before<256>(mine, scan, total);
+  double before = scan_before<256>(mine, scan, total);
   if (tid == b / each) {
-    for (int s = tid * each; s < b; ++s) before += tiles_of(a, s);
+    for (int s = tid * each; s < b; ++s) before += places_of(valid_length(a, s));
     sbase = before;
   }
   __syncthreads();
-  total *= units;
-  const int64_t per = max((int64_t)AW, (total + a.wgs - 1) / a.wgs);
-  const int64_t u0 = sbase * units + (int64_t)u * T, u1 = u0 + T;
-  const int w0 = (int)(u0 / per), w1 = (int)((u1 - 1) / per);
+  const double per = places_per(a, total * units, AW);
+  const double u0 = sbase * units + u * places_of(len);
+  const int w0 = (int)floor((u0 + START) / per), w1 = (int)floor((u0 + places_of(len) - 1) / per);
   if (w0 == w1) return;
   const int gmax = min(a.g, NQ);
   auto slot = [&](int v) { return a.part + ((int64_t)(2 * v + (v == w0)) * gmax + qi) * PART; };
@@ -631,7 +695,6 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
     all += accl[i];
   }
   x *= all > 0.f ? 1.f / all : __builtin_nanf("");
-  const int64_t at = (int64_t)blockIdx.x * D + tid;
   if constexpr (FP32) reinterpret_cast<float*>(a.out)[at] = x;
   else reinterpret_cast<uint16_t*>(a.out)[at] = f32_to_bf16(x);
 }
@@ -784,10 +847,11 @@ extern "C" size_t mk_attention_paged_workspace_bytes(int q_heads, int kv_heads) 
 template <bool E4M3, int QP, int PP, bool SMALL>
 static void launch_paged(const PagedArgs& a, hipStream_t stream) {
   const unsigned units = (unsigned)((int64_t)a.nseq * a.hkv * a.gt);
+  const unsigned lds = 2 * AW * std::min(a.g, NQ) * OROW * sizeof(float);
   if (!paged_split(a.capacity)) {
-    hipLaunchKernelGGL((paged_attention_kernel<E4M3, QP, PP, SMALL, false, AW>), dim3(units), dim3(64 * AW), 0, stream, a);
+    hipLaunchKernelGGL((paged_attention_kernel<E4M3, QP, PP, SMALL, false, AW>), dim3(units), dim3(64 * AW), lds, stream, a);
   } else {
-    hipLaunchKernelGGL((paged_attention_kernel<E4M3, QP, PP, SMALL, true, AW>), dim3(a.wgs), dim3(64 * AW), 0, stream, a);
+    hipLaunchKernelGGL((paged_attention_kernel<E4M3, QP, PP, SMALL, true, AW>), dim3(a.wgs), dim3(64 * AW), lds, stream, a);
     hipLaunchKernelGGL(paged_join_kernel<(QP > 1)>, dim3(a.nseq * a.hkv * a.g), dim3(256), 0, stream, a);
   }
 }
