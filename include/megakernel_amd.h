@@ -294,7 +294,8 @@ hipError_t mk_beam_reorder(int num_layers, int rows, int beams, int max_seq_len,
  * A K/V cache of many sequences in one pool of pages, for the three entry points below. Position p of
  * sequence s is row p % page_size of page block_tables[s * table_stride + p / page_size].
  *   k_pages, v_pages   row r of K/V head h of page i at i * page_stride + h * head_stride + r * row_stride
- *                      (elements, the same for both, >= 0; multiples of 8, of 16 for 8-bit pages), 128
+ *                      (elements, the same for both, >= 0; multiples of 8, of 16 for 8-bit pages; row_stride at
+ *                      most 2^24), 128
  *                      numbers; 16-byte aligned. [num_pages][kv_heads][page_size][128], one layer of
  *                      mk_decode_paged's pools, is the plain case
  *   k_scales, v_scales NULL: the pages are bf16. Otherwise they are e4m3 (OCP), and the number of a row is its

@@ -179,6 +179,7 @@ constexpr int OROW = D + 4;      // floats of a query's output in LDS
 constexpr int PART = D + 2;      // floats of one query's partial result: sum, maximum, output
 constexpr int SEQ_MAX = 4096;
 constexpr int PAGED_WGS = 512;   // workgroups that share the tiles out
+constexpr size_t BASE_BYTES = ((SEQ_MAX + 1) * sizeof(double) + 255) & ~(size_t)255;
 constexpr int START = 3;         // tiles that the start of a unit costs as much as: see Plan
 
 struct PagedArgs {
@@ -187,7 +188,8 @@ struct PagedArgs {
   int64_t q_row, q_head;  // bytes
   uint8_t* out;
   const int32_t* lengths;
-  float* part;  // [2 * wgs][queries of a unit][PART]
+  float* part;   // [2 * wgs][queries of a unit][PART]
+  double* base;  // [nseq + 1]: the first place of each sequence's first unit, and `per`
   int nseq, hkv, g, gt, wgs;  // gt: units to a K/V head
   int64_t capacity;           // positions of a table
 };
@@ -253,8 +255,9 @@ template <bool E4M3>
 struct Tile {
   uint4 k[2][E4M3 ? 2 : 4];
   typename std::conditional<E4M3, uint2, uint4>::type v[8];
-  uint32_t ks[2], vs[E4M3 ? 8 : 1];
+  uint32_t ks[2], vs[2];  // bytes
 };
+__device__ __forceinline__ uint32_t byte_of(uint32_t w, int i) { return w >> (8 * i) & 255; }
 
 // One score in fp32 from the whole query: see the NaN of parts below.
 template <bool E4M3>
@@ -288,9 +291,9 @@ __device__ __forceinline__ void store_out(uint8_t* out, int64_t at, float4 y) { 
 }
 
 // E4M3: 8-bit pages. QP, PP: bf16 parts of a query and of a weight (1 and 2 for bf16 queries, 3 for fp32 ones).
-// SMALL: pages of fewer than TK positions, looked up key by key. SPLIT: the tiles of all units are shared out evenly, a
+// PG: 2, a tile lies in one page; 1, each 8 keys of it do; 0, pages are looked up key by key. SPLIT: the tiles of all units are shared out evenly, a
 // unit's parts joined by paged_join_kernel; else a workgroup takes a unit, a wave a run of its tiles.
-template <bool E4M3, int QP, int PP, bool SMALL, bool SPLIT, int WAVES>
+template <bool E4M3, int QP, int PP, int PG, bool SPLIT, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES, WAVES <= 8 ? 2 : 4) paged_attention_kernel(const PagedArgs a) {
   __shared__ PagedSmem<WAVES> sm;
   extern __shared__ __attribute__((aligned(16))) float outs[];  // [pieces][queries of a unit][OROW]
@@ -313,6 +316,15 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES <= 8 ? 2 : 4) paged_attentio
     total *= units;
     mine *= units;
     const double per = places_per(a, total, WAVES), wper = floor((per + WAVES - 1) / WAVES);
+    if (blockIdx.x == 0) {  // for the join
+      double at = before;
+      for (int i = 0; i < each; ++i) {
+        const int s = tid * each + i;
+        if (s < a.nseq) a.base[s] = at;
+        if (each > 1 && s < a.nseq) at += places_of(valid_length(a, s)) * units;
+      }
+      if (tid == 0) a.base[a.nseq] = per;
+    }
     if (blockIdx.x * per >= total) return;
 #pragma unroll 1
     for (int v = 0; v < WAVES; ++v) {
@@ -369,9 +381,9 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES <= 8 ? 2 : 4) paged_attentio
       const uint8_t* vsb = E4M3 ? a.p.vs + kh * a.p.shead : nullptr;
       bool bad = false;
 
-      // Places of keys, in bytes from a head's rows; a key past the last is the last one (its weight is 0, and a page
-      // past the sequence's is never looked at).
-      int entry = 0;  // !SMALL: the page of the tile that is loaded next
+      // Places of keys, in bytes from a head's rows: a page's, or that of the first of 8 keys of the lane's (8 (n / 4) of
+      // k, 8 g of v), and the rows' from there. In a unit's last tile a key past the last is the last one: its weight is
+      // 0, and neither a row past the sequence's nor a page past its last is looked at.
       auto page_of = [&](int key) __attribute__((always_inline)) {
         int page = table[key >> a.p.shift];
         if ((uint32_t)page >= (uint32_t)a.p.pages) {
@@ -380,9 +392,33 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES <= 8 ? 2 : 4) paged_attentio
         }
         return page;
       };
-      auto place = [&](int t, int kk, int64_t& at, int64_t& sat) __attribute__((always_inline)) {
-        const int key = min(t * TK + kk, len - 1);
-        const int page = SMALL ? page_of(key) : entry;
+      const int row = (int)a.p.row, gk = 8 * (n >> 2), gv = 8 * g;
+      uint32_t rk[2], rv[8];  // PG 0: not used
+      int64_t pk = 0, pv = 0, sk = 0, sv = 0;
+      auto rows_from = [&](int last) __attribute__((always_inline)) {  // keys of the tile up to `last`
+        const int k0 = PG == 2 ? 0 : min(gk, last & ~7), v0 = PG == 2 ? 0 : min(gv, last & ~7);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) rk[h] = (uint32_t)((min(gk + 4 * h + (n & 3), last) - k0) * row + 16 * g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) rv[j] = (uint32_t)((min(gv + j, last) - v0) * row + (E4M3 ? 8 : 16) * n);
+      };
+      auto look_up = [&](int t) __attribute__((always_inline)) {
+        if constexpr (PG == 2) {
+          const int page = page_of(t * TK), in = t * TK & mask;
+          pk = pv = page * a.p.page + in * a.p.row;
+          sk = sv = page * a.p.spage + in;
+        } else if constexpr (PG == 1) {
+          const int last = min(TK, len - t * TK) - 1, k0 = t * TK + min(gk, last & ~7), v0 = t * TK + min(gv, last & ~7);
+          const int page = page_of(k0), page2 = page_of(v0);
+          pk = page * a.p.page + (k0 & mask) * a.p.row;
+          pv = page2 * a.p.page + (v0 & mask) * a.p.row;
+          sk = page * a.p.spage + (k0 & mask);
+          sv = page2 * a.p.spage + (v0 & mask);
+        }
+        if (t * TK + TK > len) rows_from(len - t * TK - 1);
+      };
+      auto place = [&](int t, int kk, int64_t& at, int64_t& sat) __attribute__((always_inline)) {  // of any key
+        const int key = min(t * TK + kk, len - 1), page = page_of(key);
         at = page * a.p.page + (key & mask) * a.p.row;
         sat = page * a.p.spage + (key & mask);
       };
@@ -390,30 +426,48 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES <= 8 ? 2 : 4) paged_attentio
       auto load_k = [&](int t) __attribute__((always_inline)) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          int64_t at, sat;
-          place(t, 8 * (n >> 2) + 4 * h + (n & 3), at, sat);
+          const uint8_t* from;
+          if constexpr (PG == 0) {
+            int64_t at, sat;
+            place(t, gk + 4 * h + (n & 3), at, sat);
+            from = kbase + at + 16 * g;
+            if constexpr (E4M3) x.ks[h] = ksb[sat];
+          } else {
+            from = kbase + pk + rk[h];
+          }
 #pragma unroll
-          for (int s = 0; s < (E4M3 ? 2 : 4); ++s) x.k[h][s] = *reinterpret_cast<const uint4*>(kbase + at + 64 * s + 16 * g);
-          if constexpr (E4M3) x.ks[h] = ksb[sat];
+          for (int s = 0; s < (E4M3 ? 2 : 4); ++s) x.k[h][s] = *reinterpret_cast<const uint4*>(from + 64 * s);
+        }
+        if constexpr (E4M3 && PG > 0) {  // the 8 scales of the lane's 8 keys, of which it takes two
+          const uint2 y = *reinterpret_cast<const uint2*>(ksb + sk + (PG == 2 ? gk : 0));
+          x.ks[0] = byte_of(y.x, n & 3);
+          x.ks[1] = byte_of(y.y, n & 3);
         }
       };
       auto load_v = [&](int t) __attribute__((always_inline)) {
+        if constexpr (E4M3 && PG == 0) x.vs[0] = x.vs[1] = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          int64_t at, sat;
-          place(t, 8 * g + j, at, sat);
-          if constexpr (E4M3) {
-            x.v[j] = *reinterpret_cast<const uint2*>(vbase + at + 8 * n);
-            x.vs[j] = vsb[sat];
+          const uint8_t* from;
+          if constexpr (PG == 0) {
+            int64_t at, sat;
+            place(t, gv + j, at, sat);
+            from = vbase + at + (E4M3 ? 8 : 16) * n;
+            if constexpr (E4M3) x.vs[j >> 2] |= (uint32_t)vsb[sat] << (8 * (j & 3));
           } else {
-            x.v[j] = *reinterpret_cast<const uint4*>(vbase + at + 16 * n);
+            from = vbase + pv + rv[j];
           }
+          if constexpr (E4M3) x.v[j] = *reinterpret_cast<const uint2*>(from);
+          else x.v[j] = *reinterpret_cast<const uint4*>(from);
+        }
+        if constexpr (E4M3 && PG > 0) {
+          const uint2 y = *reinterpret_cast<const uint2*>(vsb + sv + (PG == 2 ? gv : 0));
+          x.vs[0] = y.x;
+          x.vs[1] = y.y;
         }
       };
-      auto look_up = [&](int t) __attribute__((always_inline)) {
-        if constexpr (!SMALL) entry = page_of(min(t * TK, len - 1));
-      };
 
+      if constexpr (PG > 0) rows_from(TK - 1);
       look_up(t0);
       load_k(t0);
       load_v(t0);
@@ -507,11 +561,16 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES <= 8 ? 2 : 4) paged_attentio
         uint4 pf[PP];
         parts_of<PP>(e, pf);
         // values
+        if constexpr (E4M3 && PG > 0)
+          if (t * TK + TK > len)  // scales behind the last row may be anything
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (t * TK + gv + j >= len) x.vs[j >> 2] = (x.vs[j >> 2] & ~(255u << (8 * (j & 3)))) | 127u << (8 * (j & 3));
         uint32_t r[8][4];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           uint4 f;
-          if constexpr (E4M3) f = bf16x8_of_e4m3(x.v[j].x, x.v[j].y, scale_of(x.vs[j]));
+          if constexpr (E4M3) f = bf16x8_of_e4m3(x.v[j].x, x.v[j].y, scale_of(byte_of(x.vs[j >> 2], j & 3)));
           else f = x.v[j];
           r[j][0] = f.x; r[j][1] = f.y; r[j][2] = f.z; r[j][3] = f.w;
         }
@@ -631,7 +690,6 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES <= 8 ? 2 : 4) paged_attentio
 // query head). Sequences without keys get their answer here too.
 template <bool FP32>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
-  __shared__ double scan[4], sbase;
   __shared__ float red[4];
   __shared__ __attribute__((aligned(16))) float acc[8][D];
   __shared__ float accl[8];
@@ -648,20 +706,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
     }
     return;
   }
-  const int each = (a.nseq + 255) / 256;
-  double mine = 0, total;
-  for (int i = 0; i < each; ++i) {
-    const int s = tid * each + i;
-    if (s < a.nseq) mine += places_of(valid_length(a, s));
-  }
-  double before = scan_before<256>(mine, scan, total);
-  if (tid == b / each) {
-    for (int s = tid * each; s < b; ++s) before += places_of(valid_length(a, s));
-    sbase = before;
-  }
-  __syncthreads();
-  const double per = places_per(a, total * units, AW);
-  const double u0 = sbase * units + u * places_of(len);
+  const double per = a.base[a.nseq], u0 = a.base[b] + u * places_of(len);
   const int w0 = (int)floor((u0 + START) / per), w1 = (int)floor((u0 + places_of(len) - 1) / per);
   if (w0 == w1) return;
   const int gmax = min(a.g, NQ);
@@ -727,6 +772,7 @@ static bool pool_of(const mk_paged_cache* c, PagePool& p, bool written) {
   const int64_t size = e4m3 ? 1 : 2, unit = 16 / size;
   for (int64_t s : {c->page_stride, c->head_stride, c->row_stride})
     if (s < 0 || s % unit != 0) return false;
+  if (c->row_stride > (1 << 24)) return false;  // a page's rows are told apart by 32 bits
   if (!aligned_to(c->k_pages, 16) || !aligned_to(c->v_pages, 16) || !aligned_to(c->block_tables, 4)) return false;
   if (e4m3 && (c->scale_page_stride < 0 || c->scale_head_stride < 0)) return false;
   if (written) {
@@ -841,17 +887,17 @@ extern "C" hipError_t mk_cache_read(const mk_paged_cache* cache, const int32_t* 
 
 extern "C" size_t mk_attention_paged_workspace_bytes(int q_heads, int kv_heads) {
   if (q_heads < 1 || kv_heads < 1 || q_heads % kv_heads != 0) return 0;
-  return ((size_t)2 * PAGED_WGS * std::min(NQ, q_heads / kv_heads) * PART * sizeof(float) + 255) & ~(size_t)255;
+  return BASE_BYTES + (((size_t)2 * PAGED_WGS * std::min(NQ, q_heads / kv_heads) * PART * sizeof(float) + 255) & ~(size_t)255);
 }
 
-template <bool E4M3, int QP, int PP, bool SMALL>
+template <bool E4M3, int QP, int PP, int PG>
 static void launch_paged(const PagedArgs& a, hipStream_t stream) {
   const unsigned units = (unsigned)((int64_t)a.nseq * a.hkv * a.gt);
   const unsigned lds = 2 * AW * std::min(a.g, NQ) * OROW * sizeof(float);
   if (!paged_split(a.capacity)) {
-    hipLaunchKernelGGL((paged_attention_kernel<E4M3, QP, PP, SMALL, false, AW>), dim3(units), dim3(64 * AW), lds, stream, a);
+    hipLaunchKernelGGL((paged_attention_kernel<E4M3, QP, PP, PG, false, AW>), dim3(units), dim3(64 * AW), lds, stream, a);
   } else {
-    hipLaunchKernelGGL((paged_attention_kernel<E4M3, QP, PP, SMALL, true, AW>), dim3(a.wgs), dim3(64 * AW), lds, stream, a);
+    hipLaunchKernelGGL((paged_attention_kernel<E4M3, QP, PP, PG, true, AW>), dim3(a.wgs), dim3(64 * AW), lds, stream, a);
     hipLaunchKernelGGL(paged_join_kernel<(QP > 1)>, dim3(a.nseq * a.hkv * a.g), dim3(256), 0, stream, a);
   }
 }
@@ -873,20 +919,29 @@ extern "C" hipError_t mk_attention_paged(const mk_paged_cache* cache, int q_head
   a.q_head = q_head_stride * size;
   a.out = static_cast<uint8_t*>(out);
   a.lengths = lengths;
-  a.part = static_cast<float*>(workspace);
+  a.base = static_cast<double*>(workspace);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + BASE_BYTES);
   a.nseq = cache->num_seqs;
   a.hkv = cache->kv_heads;
   a.g = q_heads / cache->kv_heads;
   a.gt = (a.g + NQ - 1) / NQ;
   a.wgs = PAGED_WGS;
   a.capacity = (int64_t)cache->table_entries * cache->page_size;
-  const bool small = cache->page_size < TK;
+  // the keys of a tile that surely share a page, and scales that can be loaded 8 at a time
+  int pg = cache->page_size >= TK ? 2 : cache->page_size >= 8 ? 1 : 0;
+  if (a.p.ks && (!aligned_to(a.p.ks, 8) || !aligned_to(a.p.vs, 8) || a.p.spage % 8 != 0 || a.p.shead % 8 != 0)) pg = 0;
+  auto launch = [&](auto e4m3, auto qp, auto pp) {
+    if (pg == 2) launch_paged<e4m3.value, qp.value, pp.value, 2>(a, stream);
+    else if (pg == 1) launch_paged<e4m3.value, qp.value, pp.value, 1>(a, stream);
+    else launch_paged<e4m3.value, qp.value, pp.value, 0>(a, stream);
+  };
+  using std::integral_constant;
   if (a.p.ks) {
-    if (q_fp32) small ? launch_paged<true, 3, 3, true>(a, stream) : launch_paged<true, 3, 3, false>(a, stream);
-    else small ? launch_paged<true, 1, 2, true>(a, stream) : launch_paged<true, 1, 2, false>(a, stream);
+    if (q_fp32) launch(std::true_type(), integral_constant<int, 3>(), integral_constant<int, 3>());
+    else launch(std::true_type(), integral_constant<int, 1>(), integral_constant<int, 2>());
   } else {
-    if (q_fp32) small ? launch_paged<false, 3, 3, true>(a, stream) : launch_paged<false, 3, 3, false>(a, stream);
-    else small ? launch_paged<false, 1, 2, true>(a, stream) : launch_paged<false, 1, 2, false>(a, stream);
+    if (q_fp32) launch(std::false_type(), integral_constant<int, 3>(), integral_constant<int, 3>());
+    else launch(std::false_type(), integral_constant<int, 1>(), integral_constant<int, 2>());
   }
   return hipGetLastError();
 }

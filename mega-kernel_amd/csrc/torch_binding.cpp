@@ -606,6 +606,7 @@ mk_paged_cache check_paged(const torch::Tensor& kp, const torch::Tensor& vp, con
                 "megakernel: ", name, " must be like k_pages, in type, shape and device");
     TORCH_CHECK(t.stride(3) == 1, "megakernel: ", name, " must be contiguous in its last dimension");
     const std::vector<int64_t> s{N > 1 ? t.stride(0) : 0, H > 1 ? t.stride(1) : 0, P > 1 ? t.stride(2) : 0};
+    TORCH_CHECK(s[2] <= 1 << 24, "megakernel: ", name, "'s rows must be at most 2^24 elements apart");
     for (int64_t x : s) TORCH_CHECK(x % unit == 0, "megakernel: ", name, "'s rows must start on 16-byte boundaries");
     TORCH_CHECK(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "megakernel: ", name,
                 " must start on a 16-byte boundary");

@@ -44,7 +44,7 @@ def lib():
 
 BAD_POOLS = [dict(k_pages=None), dict(v_pages=None), dict(v_pages=P), dict(block_tables=None), dict(k_pages=P + 8),
              dict(v_pages=Q + 8), dict(block_tables=P + 2), dict(page_stride=-8), dict(head_stride=-8), dict(row_stride=-8),
-             dict(page_stride=8 * 16 * 128 + 4), dict(head_stride=16 * 128 + 4), dict(row_stride=132), dict(num_pages=0),
+             dict(page_stride=8 * 16 * 128 + 4), dict(head_stride=16 * 128 + 4), dict(row_stride=132), dict(row_stride=(1 << 24) + 8), dict(num_pages=0),
              dict(kv_heads=0), dict(kv_heads=65536), dict(page_size=0), dict(page_size=24), dict(page_size=8192),
              dict(num_seqs=0), dict(table_entries=0), dict(table_stride=-1), dict(table_entries=(1 << 26) + 1),
              dict(k_scales=R), dict(v_scales=S), dict(k_scales=R, v_scales=R)]
@@ -176,6 +176,8 @@ def test_pools_of_the_ops(ext):
         _refuses("same strides", f, bk, both[:, 1], t, None, None)
         _refuses("must be distinct", f, bk, bk, t, None, None)
         _refuses("contiguous in its last", f, torch.zeros(10, 8, 16, 256, dtype=BF)[..., ::2], bv, t, None, None)
+        far = torch.empty((1 << 24) + 256, dtype=BF).as_strided((1, 1, 2, 128), (0, 0, (1 << 24) + 8, 1))
+        _refuses("at most 2\\^24", f, far, far, t, None, None)
         _refuses("16-byte boundaries", f, torch.zeros(10, 8, 16, 132, dtype=BF)[..., :128], bv, t, None, None)
         _refuses("16-byte boundary", f, torch.zeros(10 * 16384 + 4, dtype=BF)[4:].view(10, 8, 16, 128), bv, t, None, None)
         _refuses("need k_scales", f, ek, ev, t, None, None)
