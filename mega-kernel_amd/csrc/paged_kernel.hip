@@ -29,6 +29,7 @@
 
 #include "mk_device.h"
 #include "mk_layers.h"
+#include "mk_scan.h"
 #include "../../include/megakernel_amd.h"
 
 namespace mkp {
@@ -178,9 +179,12 @@ constexpr int NQ = 16;           // queries to a unit: (sequence, K/V head, 16 o
 constexpr int OROW = D + 4;      // floats of a query's output in LDS
 constexpr int PART = D + 2;      // floats of one query's partial result: sum, maximum, output
 constexpr int SEQ_MAX = 4096;
-constexpr int PAGED_WGS = 512;   // workgroups that share the tiles out
+// Workgroups that share the tiles out: two to a CU, as the registers of two waves to a SIMD allow. (With three waves of
+// bf16 queries, on 168 registers: 64 sequences of 900 to 4,095 keys in bf16 pages 132 us instead of 121, as six registers
+// spill; of 64 to 960 in 8-bit pages 23.1 instead of 23.9.)
+constexpr int PAGED_WGS = 512;
 constexpr size_t BASE_BYTES = ((SEQ_MAX + 1) * sizeof(double) + 255) & ~(size_t)255;
-constexpr int START = 3;         // tiles that the start of a unit costs as much as: see Plan
+constexpr int START = 2;         // tiles that the start of a unit costs as much as: see Plan
 
 struct PagedArgs {
   PagePool p;
@@ -205,29 +209,7 @@ __device__ __forceinline__ int valid_length(const PagedArgs& a, int b) {
 // stand for what a unit costs by itself (its queries, its first loads). Places are counted in doubles, exactly.
 __device__ __forceinline__ double places_of(int length) { return length > 0 ? START + (length + TK - 1) / TK : 0; }
 __device__ __forceinline__ double places_per(const PagedArgs& a, double total, int waves) {
-  return fmax(floor((total + a.wgs - 1) / a.wgs), (double)((START + 1) * waves));
-}
-
-// Sums of v over the workgroup's threads before this one and over all of them.
-template <int THREADS>
-__device__ __forceinline__ double scan_before(double v, double* lds, double& total) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  double x = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double y = __shfl_up(x, o);
-    if (lane >= o) x += y;
-  }
-  if (lane == 63) lds[w] = x;
-  __syncthreads();
-  double before = x - v;
-  total = 0;
-#pragma unroll
-  for (int i = 0; i < THREADS / 64; ++i) {
-    if (i < w) before += lds[i];
-    total += lds[i];
-  }
-  return before;
+  return fmax(floor((total + a.wgs - 1) / a.wgs), (double)waves);
 }
 
 // v as the sum of PARTS bf16 numbers, each the rounding of what the ones before it leave
@@ -274,7 +256,8 @@ __device__ __attribute__((noinline)) float whole_score(const uint8_t* k, float s
 
 // What a wave has of a unit that it did not do alone, in LDS: up to two to a wave, its first and its last unit.
 struct Piece {
-  int seq, unit, t0, t1;  // t0 == t1: none
+  int id, t0, t1, tiles;  // seq * units + unit; t0 == t1: none; the unit's tiles
+  int row, nq;            // of the output's (sequence, head) rows, the unit's first; their number
 };
 template <int WAVES>
 struct PagedSmem {
@@ -294,7 +277,7 @@ __device__ __forceinline__ void store_out(uint8_t* out, int64_t at, float4 y) { 
 // PG: 2, a tile lies in one page; 1, each 8 keys of it do; 0, pages are looked up key by key. SPLIT: the tiles of all units are shared out evenly, a
 // unit's parts joined by paged_join_kernel; else a workgroup takes a unit, a wave a run of its tiles.
 template <bool E4M3, int QP, int PP, int PG, bool SPLIT, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, WAVES <= 8 ? 2 : 4) paged_attention_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(64 * WAVES, 2) paged_attention_kernel(const PagedArgs a) {
   __shared__ PagedSmem<WAVES> sm;
   extern __shared__ __attribute__((aligned(16))) float outs[];  // [pieces][queries of a unit][OROW]
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -303,7 +286,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES <= 8 ? 2 : 4) paged_attentio
   const int gmax = min(a.g, NQ);
   int b, u, len;       // sequence, unit of it, its keys
   double p = 0, left;  // places of the unit that are behind the wave, places that it has still to do
-  if (tid < 2 * WAVES) sm.piece[tid] = Piece{0, 0, 0, 0};
+  if (tid < 2 * WAVES) sm.piece[tid].t0 = sm.piece[tid].t1 = 0;
   if constexpr (SPLIT) {
     const int each = (a.nseq + 64 * WAVES - 1) / (64 * WAVES);
     double mine = 0, total;
@@ -312,7 +295,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES <= 8 ? 2 : 4) paged_attentio
       const int s = tid * each + i;
       if (s < a.nseq) mine += places_of(len0 = valid_length(a, s));
     }
-    double before = scan_before<64 * WAVES>(mine, sm.scan, total) * units;
+    double before = block_before<WAVES>(mine, sm.scan, total) * units;
     total *= units;
     mine *= units;
     const double per = places_per(a, total, WAVES), wper = floor((per + WAVES - 1) / WAVES);
@@ -566,24 +549,30 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES <= 8 ? 2 : 4) paged_attentio
 #pragma unroll
             for (int j = 0; j < 8; ++j)
               if (t * TK + gv + j >= len) x.vs[j >> 2] = (x.vs[j >> 2] & ~(255u << (8 * (j & 3)))) | 127u << (8 * (j & 3));
-        uint32_t r[8][4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          uint4 f;
-          if constexpr (E4M3) f = bf16x8_of_e4m3(x.v[j].x, x.v[j].y, scale_of(byte_of(x.vs[j >> 2], j & 3)));
-          else f = x.v[j];
-          r[j][0] = f.x; r[j][1] = f.y; r[j][2] = f.z; r[j][3] = f.w;
+        for (int c = 0; c < 4; ++c) {  // dims 8 n + 2 c and the next
+          uint32_t r[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if constexpr (E4M3) {
+              const float sc = scale_of(byte_of(x.vs[j >> 2], j & 3));
+              const uint32_t y = c < 2 ? x.v[j].x : x.v[j].y;
+              r[j] = c & 1 ? bf16_of_e4m3<true>(y, sc) : bf16_of_e4m3<false>(y, sc);
+            } else {
+              r[j] = c == 0 ? x.v[j].x : c == 1 ? x.v[j].y : c == 2 ? x.v[j].z : x.v[j].w;
+            }
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            uint32_t f[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              f[q] = __builtin_amdgcn_perm(r[2 * q + 1], r[2 * q], h ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int k = 0; k < PP; ++k) o[2 * c + h] = mfma(make_uint4(f[0], f[1], f[2], f[3]), pf[k], o[2 * c + h]);
+          }
         }
         if (t + 1 < t1) load_v(t + 1);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint32_t f[4];
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            f[q] = __builtin_amdgcn_perm(r[2 * q + 1][i >> 1], r[2 * q][i >> 1], i & 1 ? 0x07060302u : 0x05040100u);
-#pragma unroll
-          for (int k = 0; k < PP; ++k) o[i] = mfma(make_uint4(f[0], f[1], f[2], f[3]), pf[k], o[i]);
-        }
       }
       if (__builtin_amdgcn_ballot_w64(bad)) l = __builtin_nanf("");
       l = xsum32(xsum16(l));
@@ -608,7 +597,7 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES <= 8 ? 2 : 4) paged_attentio
           sm.m[piece][n] = m;
           sm.l[piece][n] = l;
         }
-        if (lane == 0) sm.piece[piece] = Piece{b, u, t0, t1};
+        if (lane == 0) sm.piece[piece] = Piece{b * units + u, t0, t1, T, b * a.hkv * a.g + h0, nq};
         piece = 2 * w + 1;
       }
     }
@@ -626,47 +615,41 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES <= 8 ? 2 : 4) paged_attentio
   }
   __syncthreads();
 
-  // The pieces joined, unit by unit: what a query's weights refer to differs from piece to piece. A unit that the
-  // workgroup had whole is done, others go to the join.
+  // The pieces joined, unit by unit, by the wave that has the unit's first: what a query's weights refer to differs from
+  // piece to piece. A unit that the workgroup had whole is done, others go to the join.
+  const Piece y = sm.piece[min(lane, 2 * WAVES - 1)];  // lane e: piece e
+  const uint32_t some = (uint32_t)__builtin_amdgcn_ballot_w64(lane < 2 * WAVES && y.t0 != y.t1);
 #pragma unroll 1
-  for (int e0 = 0; e0 < 2 * WAVES;) {
-    const Piece first = sm.piece[e0];
-    if (first.t0 == first.t1) {
-      ++e0;
-      continue;
-    }
-    int e1 = e0 + 1, t1 = first.t1;
-    for (int e = e1; e < 2 * WAVES; ++e) {
-      const Piece y = sm.piece[e];
-      if (y.t0 == y.t1) continue;
-      if (y.seq != first.seq || y.unit != first.unit) break;
-      e1 = e + 1;
-      t1 = y.t1;
-    }
-    const int T = ((SPLIT ? valid_length(a, first.seq) : len) + TK - 1) / TK;
-    const bool whole = first.t0 == 0 && t1 == T;
-    const int kh = first.unit / a.gt, h0 = kh * a.g + NQ * (first.unit % a.gt), nq = min(NQ, a.g - NQ * (first.unit % a.gt));
-    for (int i = tid; i < nq * (D / 4); i += 64 * WAVES) {
+  for (int e0 = 2 * w; e0 < 2 * w + 2; ++e0) {
+    if (!(some >> e0 & 1)) continue;
+    const int id = __builtin_amdgcn_readlane(y.id, e0);
+    const uint32_t run = some & (uint32_t)__builtin_amdgcn_ballot_w64(y.id == id);
+    if (__ffs(run) - 1 != e0) continue;  // an earlier wave's
+    const int t0 = __builtin_amdgcn_readlane(y.t0, e0), t1 = __builtin_amdgcn_readlane(y.t1, 31 - __clz(run));
+    const bool whole = t0 == 0 && t1 == __builtin_amdgcn_readlane(y.tiles, e0);
+    const int nq = __builtin_amdgcn_readlane(y.nq, e0), row = __builtin_amdgcn_readlane(y.row, e0);
+#pragma unroll 1
+    for (int i = lane; i < nq * (D / 4); i += 64) {
       const int qi = i / (D / 4), d = 4 * (i % (D / 4));
       float M = -INFINITY;
-      for (int e = e0; e < e1; ++e)
-        if (sm.piece[e].t0 != sm.piece[e].t1) M = fmaxf(M, sm.m[e][qi]);
+#pragma unroll 2
+      for (int e = 0; e < 2 * WAVES; ++e) M = run >> e & 1 ? fmaxf(M, sm.m[e][qi]) : M;
       const float ref = M == -INFINITY ? 0.f : M;
       float sum = 0.f;
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int e = e0; e < e1; ++e) {
-        if (sm.piece[e].t0 == sm.piece[e].t1) continue;
+#pragma unroll 1
+      for (uint32_t todo = run; todo; todo &= todo - 1) {
+        const int e = __ffs(todo) - 1;
         const float f = __builtin_amdgcn_exp2f(sm.m[e][qi] - ref);
-        const float4 y = *reinterpret_cast<const float4*>(outs + (e * gmax + qi) * OROW + d);
+        const float4 z = *reinterpret_cast<const float4*>(outs + (e * gmax + qi) * OROW + d);
         sum += f * sm.l[e][qi];
-        acc.x += f * y.x; acc.y += f * y.y; acc.z += f * y.z; acc.w += f * y.w;
+        acc.x += f * z.x; acc.y += f * z.y; acc.z += f * z.z; acc.w += f * z.w;
       }
       if (whole) {
         const float inv = sum > 0.f ? 1.f / sum : __builtin_nanf("");
-        store_out<QP>(a.out, ((int64_t)first.seq * a.hkv * a.g + h0 + qi) * D + d,
-                      make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
+        store_out<QP>(a.out, (int64_t)(row + qi) * D + d, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
       } else {
-        float* to = a.part + ((int64_t)(2 * blockIdx.x + (first.t0 == 0)) * gmax + qi) * PART;
+        float* to = a.part + ((int64_t)(2 * blockIdx.x + (t0 == 0)) * gmax + qi) * PART;
         if (d == 0) {
           to[0] = sum;
           to[1] = M;
@@ -675,7 +658,6 @@ __global__ void __launch_bounds__(64 * WAVES, WAVES <= 8 ? 2 : 4) paged_attentio
         *reinterpret_cast<float2*>(to + 4 + d) = make_float2(acc.z, acc.w);
       }
     }
-    e0 = e1;
   }
   if constexpr (!SPLIT)
     if (len == 0) {  // an empty sequence, or a length out of range

@@ -27,6 +27,7 @@
 
 #include "mk_device.h"
 #include "mk_layers.h"
+#include "mk_scan.h"
 #include "../../include/megakernel_amd.h"
 
 namespace mkp {
@@ -85,66 +86,6 @@ __device__ __forceinline__ float logit_of(uint32_t u) {
 __device__ __forceinline__ u64 logit_key(float x, int v) { return (u64)logit_order(x) << 32 | (0xffffffffu - (uint32_t)v); }
 __device__ __forceinline__ float key_x(u64 key) { return logit_of((uint32_t)(key >> 32)); }
 __device__ __forceinline__ int key_v(u64 key) { return (int)(0xffffffffu - (uint32_t)key); }
-
-// v of another lane by DPP, 0 where there is none
-template <int CTRL, int ROWS, typename V>
-__device__ __forceinline__ V from_lane(V v) {
-  if constexpr (sizeof(V) == 4) {
-    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
-  } else {
-    const u64 u = __builtin_bit_cast(u64, v);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
-    return __builtin_bit_cast(V, (u64)hi << 32 | lo);
-  }
-}
-template <typename V>
-__device__ __forceinline__ V at_lane(V v, int lane) {
-  if constexpr (sizeof(V) == 4) {
-    return __builtin_bit_cast(V, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
-  } else {
-    const u64 u = __builtin_bit_cast(u64, v);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
-    return __builtin_bit_cast(V, (u64)hi << 32 | lo);
-  }
-}
-// op over lanes 0 .. this one of each 16, and of the wave; 0 is op's neutral number
-template <typename V, typename F>
-__device__ __forceinline__ V scan_row16(V v, F op) {
-  v = op(v, from_lane<0x111, 0xf>(v));  // row_shr 1, 2, 4, 8
-  v = op(v, from_lane<0x112, 0xf>(v));
-  v = op(v, from_lane<0x114, 0xf>(v));
-  return op(v, from_lane<0x118, 0xf>(v));
-}
-template <typename V, typename F>
-__device__ __forceinline__ V scan_wave(V v, F op) {
-  v = scan_row16(v, op);
-  v = op(v, from_lane<0x142, 0xa>(v));  // row_bcast 15, 31
-  return op(v, from_lane<0x143, 0xc>(v));
-}
-template <typename V>
-__device__ __forceinline__ V plus(V a, V b) { return a + b; }
-template <typename V>
-__device__ __forceinline__ V sum_over_wave(V v) { return at_lane(scan_wave(v, plus<V>), 63); }
-__device__ __forceinline__ u64 max_over_wave(u64 v) {
-  return at_lane(scan_wave(v, [](u64 a, u64 b) { return a > b ? a : b; }), 63);
-}
-
-// Sums over the threads before this one and over all (numbers that commute exactly, or in a fixed order).
-template <int WAVES = SW, typename V>
-__device__ __forceinline__ V block_before(V v, V* lds, V& total) {
-  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const V x = scan_wave(v, plus<V>);
-  __syncthreads();
-  if (lane == 63) lds[w] = x;
-  __syncthreads();
-  const V y = scan_row16(lds[lane & (WAVES - 1)], plus<V>);  // every wave: the waves' sums, up to each
-  static_assert(WAVES <= 16 && (WAVES & (WAVES - 1)) == 0);
-  total = at_lane(y, WAVES - 1);
-  const V before = at_lane(y, max(w - 1, 0));
-  return (w ? before : (V)0) + (x - v);
-}
 
 // How logits at a temperature fall into bins: c bins per logit. `in` is 1, or 0 where bins are so small (p above 2^45)
 // that different logits lie thousands of bins apart and p has too few digits behind the point: any place in the bin
@@ -531,7 +472,7 @@ __device__ __forceinline__ void border_in_list(int n, int j, double c, double in
     __syncthreads();
     const u64 b0 = sm.sub[2 * tid], b1 = sm.sub[2 * tid + 1];
     u64 all;
-    const u64 before = block_before(b0 + b1, sm.wfix, all);
+    const u64 before = block_before<SW>(b0 + b1, sm.wfix, all);
     const int c0 = above + (int)(before >> CNT);
     const u64 s0 = sabove + (before & SUM_MASK);
     const int c1 = c0 + (int)(b0 >> CNT), c2 = c1 + (int)(b1 >> CNT);
@@ -581,7 +522,7 @@ __device__ __forceinline__ void border_in_list(int n, int j, double c, double in
   __syncthreads();
   const u64 k = tid < n ? sm.sort.key[tid] : 0, mine = tid < n ? fixed_weight(s, ref, key_x(k), j) : 0;
   u64 all;
-  const u64 before = sabove + block_before(mine, sm.wfix, all);
+  const u64 before = sabove + block_before<SW>(mine, sm.wfix, all);
   if (tid < n && (tid == 0 || !reached(above + tid, before)) && (tid == n - 1 || reached(above + tid + 1, before + mine))) {
     sm.key = k;
     sm.sum = before + mine;
@@ -757,8 +698,8 @@ __device__ __forceinline__ u64 border_in_bin(const Row& r, const uint8_t* codes,
     const u64 s0 = sm.many.sum[2 * tid], s1 = sm.many.sum[2 * tid + 1];
     int call;
     u64 sall;
-    int cb = above + block_before(c0 + c1, sm.wcount, call);
-    u64 sb = sabove + block_before(s0 + s1, sm.wfix, sall);
+    int cb = above + block_before<SW>(c0 + c1, sm.wcount, call);
+    u64 sb = sabove + block_before<SW>(s0 + s1, sm.wfix, sall);
     // the one place where it is reached, at the end of the range if nowhere before
     const int lastb = (int)((khi - klo) >> shift);
     const bool r0 = reached(cb + c0, sb + s0) || 2 * tid >= lastb, r1 = reached(cb + c0 + c1, sb + s0 + s1) || 2 * tid + 1 >= lastb;
@@ -798,7 +739,7 @@ __device__ __forceinline__ u64 border_in_bin(const Row& r, const uint8_t* codes,
         const int v = base + 4 * tid + q;
         mine += v < r.vocab && r.x[v] == x;
       }
-      int before = seen + block_before(mine, sm.wcount, all);
+      int before = seen + block_before<SW>(mine, sm.wcount, all);
       if (before < take && before + mine >= take)
         for (int q = 0; q < 4; ++q) {
           const int v = base + 4 * tid + q;
@@ -873,8 +814,8 @@ __device__ __forceinline__ void deep_cut(const u64* bins, const SampleStat* stat
       n = tid < NB - 1 ? (int)sm.many.count[tid] : sm.n;
       weight = tid < NB - 1 ? (double)sm.many.sum[tid] / ONE * sm.et[tid] : t;
     }
-    const double wb = block_before(weight, sm.wsum, wall);
-    const int cb = block_before(n, sm.wcount, call);
+    const double wb = block_before<SW>(weight, sm.wsum, wall);
+    const int cb = block_before<SW>(n, sm.wcount, call);
     if (tid < NB) {
       sm.upto[tid] = wb + weight;
       sm.cupto[tid] = cb + n;
@@ -1020,8 +961,8 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
       const double weight = tid < NB ? (double)(b & SUM_MASK) / ONE * sm.et[tid] : 0;
       double all;
       int call;
-      const double wb = block_before(weight, sm.wsum, all);
-      const int cb = block_before((int)(b >> CNT), sm.wcount, call);
+      const double wb = block_before<SW>(weight, sm.wsum, all);
+      const int cb = block_before<SW>((int)(b >> CNT), sm.wcount, call);
       if (tid < NB) {
         sm.upto[tid] = wb + weight;
         sm.cupto[tid] = cb + (int)(b >> CNT);
@@ -1133,7 +1074,7 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
     __syncthreads();
     const uint32_t bits = tid < SC / 32 ? sm.map[tid] : 0;
     int n;
-    const int place = block_before((int)__popc(bits), sm.wcount, n);
+    const int place = block_before<SW>((int)__popc(bits), sm.wcount, n);
     if (tid < SC / 32) sm.mapped[tid] = place;
     __syncthreads();
     if (weight > 0) {
@@ -1144,7 +1085,7 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
     __syncthreads();
     weight = tid < n ? sm.inorder[tid] : 0;
     double all;
-    const double run = block_before(weight, sm.wsum, all);
+    const double run = block_before<SW>(weight, sm.wsum, all);
     // the first one whose running sum exceeds the goal, the last one if none does
     if (tid < n && (run + weight > goal || tid == n - 1) && (tid == 0 || !(run > goal))) atomicMin(&sm.first[0], tid);
     __syncthreads();
@@ -1184,7 +1125,7 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
     mine += s;
     turn(f);
   }
-  double run = block_before(mine, sm.wsum, all);
+  double run = block_before<SW>(mine, sm.wsum, all);
   int hit = -1, last = -1;
   // sums in another order may differ in their last digits: a little more than the thread that has it
   const bool here = mine > 0 && (run + mine) * (1 + SAME) > goal && run * (1 - SAME) <= goal;
