@@ -263,8 +263,6 @@ template <int WAVES>
 struct PagedSmem {
   Piece piece[2 * WAVES];
   float m[2 * WAVES][NQ], l[2 * WAVES][NQ];
-  double scan[WAVES], base[WAVES];
-  int seq[WAVES], len[WAVES];
 };
 
 template <int QP>
@@ -288,53 +286,52 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attention_kernel(const Pa
   double p = 0, left;  // places of the unit that are behind the wave, places that it has still to do
   if (tid < 2 * WAVES) sm.piece[tid].t0 = sm.piece[tid].t1 = 0;
   if constexpr (SPLIT) {
-    const int each = (a.nseq + 64 * WAVES - 1) / (64 * WAVES);
-    double mine = 0, total;
+    // Every wave for itself: a lane adds up `each` sequences, and the lane that the wave's first place falls to tells
+    // the sequence, or (more than 64 of them) the 64 lanes look among its sequences.
+    const int each = (a.nseq + 63) / 64;
+    double mine = 0;
     int len0 = 0;
+#pragma unroll 1
     for (int i = 0; i < each; ++i) {
-      const int s = tid * each + i;
-      if (s < a.nseq) mine += places_of(len0 = valid_length(a, s));
+      const int s = lane * each + i;
+      len0 = s < a.nseq ? valid_length(a, s) : 0;
+      mine += places_of(len0);
     }
-    double before = block_before<WAVES>(mine, sm.scan, total) * units;
-    total *= units;
     mine *= units;
+    double upto = scan_wave(mine, plus<double>);
+    const double total = at_lane(upto, 63);
     const double per = places_per(a, total, WAVES), wper = floor((per + WAVES - 1) / WAVES);
-    if (blockIdx.x == 0) {  // for the join
-      double at = before;
+    if (blockIdx.x == 0 && w == 0) {  // for the join
+      double at = upto - mine;
+#pragma unroll 1
       for (int i = 0; i < each; ++i) {
-        const int s = tid * each + i;
-        if (s < a.nseq) a.base[s] = at;
-        if (each > 1 && s < a.nseq) at += places_of(valid_length(a, s)) * units;
+        const int s = lane * each + i;
+        if (s < a.nseq) {
+          a.base[s] = at;
+          if (each > 1) at += places_of(valid_length(a, s)) * units;
+        }
       }
-      if (tid == 0) a.base[a.nseq] = per;
+      if (lane == 0) a.base[a.nseq] = per;
     }
     if (blockIdx.x * per >= total) return;
-#pragma unroll 1
-    for (int v = 0; v < WAVES; ++v) {
-      const double lo = blockIdx.x * per + v * wper;
-      if (lo >= before && lo < before + mine) {
-        double base = before;
-        int s = tid * each;
-        if (each > 1)
-          while (true) {
-            len0 = valid_length(a, s);
-            const double end = base + places_of(len0) * units;
-            if (lo < end) break;
-            base = end;
-            ++s;
-          }
-        sm.seq[v] = s;
-        sm.len[v] = len0;
-        sm.base[v] = base;
-      }
-    }
-    __syncthreads();
     const double lo = blockIdx.x * per + w * wper;
     left = fmin(fmin(wper, per - w * wper), total - lo);
-    b = __builtin_amdgcn_readfirstlane(sm.seq[w]);
-    len = __builtin_amdgcn_readfirstlane(sm.len[w]);
+    b = u = len = 0;
     if (left > 0) {
-      const double cost = places_of(len), off = lo - sm.base[w];
+      int at = __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(lo < upto)) - 1;
+      b = at;
+      if (each > 1) {
+        const double before = at_lane(upto - mine, at);
+        const int s = at * each + lane;
+        len0 = lane < each && s < a.nseq ? valid_length(a, s) : 0;
+        mine = places_of(len0) * units;
+        upto = before + scan_wave(mine, plus<double>);
+        b = at * each;
+        at = __ffsll((unsigned long long)__builtin_amdgcn_ballot_w64(lo < upto)) - 1;
+        b += at;
+      }
+      len = at_lane(len0, at);
+      const double cost = places_of(len), off = lo - at_lane(upto - mine, at);
       double q = floor(off / cost);
       if (q * cost > off) --q;
       u = __builtin_amdgcn_readfirstlane((int)q);
@@ -451,24 +448,29 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attention_kernel(const Pa
       };
 
       if constexpr (PG > 0) rows_from(TK - 1);
+      // the queries as B operands: dims of step s at 8 lanes' width, as the keys' loads have them
+      auto dim_of = [&](int s) { return E4M3 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g; };
+      uint4 qf[4][QP], raw[4][2];
+      const uint8_t* qrow = a.q + b * a.q_row + (int64_t)(h0 + n) * a.q_head;
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int h = 0; h < (QP > 1 ? 2 : 1); ++h)
+          raw[s][h] = n < nq ? *reinterpret_cast<const uint4*>(qrow + (QP > 1 ? 4 : 2) * dim_of(s) + 16 * h) : make_uint4(0, 0, 0, 0);
       look_up(t0);
       load_k(t0);
       load_v(t0);
-      // the queries as B operands: dims of step s at 8 lanes' width, as the keys' loads have them
-      auto dim_of = [&](int s) { return E4M3 ? 64 * (s >> 1) + 16 * g + 8 * (s & 1) : 32 * s + 8 * g; };
-      uint4 qf[4][QP];
-      const uint8_t* qrow = a.q + b * a.q_row + (int64_t)(h0 + n) * a.q_head;
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
         if constexpr (QP == 1) {
-          qf[s][0] = n < nq ? *reinterpret_cast<const uint4*>(qrow + 2 * dim_of(s)) : make_uint4(0, 0, 0, 0);
+          qf[s][0] = raw[s][0];
         } else {
           float y[8];
-          const float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-          const float4 lo = n < nq ? *reinterpret_cast<const float4*>(qrow + 4 * dim_of(s)) : z;
-          const float4 hi = n < nq ? *reinterpret_cast<const float4*>(qrow + 4 * dim_of(s) + 16) : z;
-          y[0] = lo.x; y[1] = lo.y; y[2] = lo.z; y[3] = lo.w;
-          y[4] = hi.x; y[5] = hi.y; y[6] = hi.z; y[7] = hi.w;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float4 z = __builtin_bit_cast(float4, raw[s][h]);
+            y[4 * h] = z.x; y[4 * h + 1] = z.y; y[4 * h + 2] = z.z; y[4 * h + 3] = z.w;
+          }
           parts_of<QP>(y, qf[s]);
         }
       }
@@ -672,10 +674,9 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attention_kernel(const Pa
 // query head). Sequences without keys get their answer here too.
 template <bool FP32>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
-  __shared__ float red[4];
   __shared__ __attribute__((aligned(16))) float acc[8][D];
-  __shared__ float accl[8];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  __shared__ float accl[8], accm[8];
+  const int tid = threadIdx.x;
   const int heads = a.hkv * a.g, b = blockIdx.x / heads, h = blockIdx.x % heads;
   const int kh = h / a.g, hg = h % a.g, u = kh * a.gt + hg / NQ, qi = hg % NQ, units = a.hkv * a.gt;
   const int len = valid_length(a, b);
@@ -693,33 +694,52 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a) {
   if (w0 == w1) return;
   const int gmax = min(a.g, NQ);
   auto slot = [&](int v) { return a.part + ((int64_t)(2 * v + (v == w0)) * gmax + qi) * PART; };
-  float M = -INFINITY;
-  for (int v = w0 + tid; v <= w1; v += 256) M = fmaxf(M, slot(v)[1]);
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
-  if (lane == 0) red[w] = M;
-  __syncthreads();
-  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  const float ref = M == -INFINITY ? 0.f : M;
+  // 32 lanes to a part, eight parts of a lane at a time, so that their loads are made together
   const int r = tid >> 5, d = 4 * (tid & 31);
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  float sum = 0.f;
-  for (int v = w0 + r; v <= w1; v += 8) {
-    const float* p = slot(v);
-    const float f = __builtin_amdgcn_exp2f(p[1] - ref);
-    const float2 x = *reinterpret_cast<const float2*>(p + 2 + d), y = *reinterpret_cast<const float2*>(p + 4 + d);
-    sum += f * p[0];
-    o.x += f * x.x; o.y += f * x.y; o.z += f * y.x; o.w += f * y.y;
+  float sum = 0.f, M = -INFINITY;
+#pragma unroll 1
+  for (int v0 = w0 + r; v0 <= w1; v0 += 64) {
+    float2 ml[8], x[8], y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float* p = slot(min(v0 + 8 * i, w1));
+      ml[i] = *reinterpret_cast<const float2*>(p);
+      x[i] = *reinterpret_cast<const float2*>(p + 2 + d);
+      y[i] = *reinterpret_cast<const float2*>(p + 4 + d);
+    }
+    float top = M;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, v0 + 8 * i <= w1 ? ml[i].y : -INFINITY);
+    const float ref = top == -INFINITY ? 0.f : top, f0 = __builtin_amdgcn_exp2f(M - ref);
+    M = top;
+    sum *= f0;
+    o.x *= f0; o.y *= f0; o.z *= f0; o.w *= f0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (v0 + 8 * i > w1) continue;
+      const float f = __builtin_amdgcn_exp2f(ml[i].y - ref);
+      sum += f * ml[i].x;
+      o.x += f * x[i].x; o.y += f * x[i].y; o.z += f * y[i].x; o.w += f * y[i].y;
+    }
   }
   *reinterpret_cast<float4*>(&acc[r][d]) = o;
-  if (d == 0) accl[r] = sum;
+  if (d == 0) {
+    accl[r] = sum;
+    accm[r] = M;
+  }
   __syncthreads();
   if (tid >= D) return;
+  M = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) M = fmaxf(M, accm[i]);
+  const float ref = M == -INFINITY ? 0.f : M;
   float x = 0.f, all = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    x += acc[i][tid];
-    all += accl[i];
+    const float f = __builtin_amdgcn_exp2f(accm[i] - ref);
+    x += f * acc[i][tid];
+    all += f * accl[i];
   }
   x *= all > 0.f ? 1.f / all : __builtin_nanf("");
   if constexpr (FP32) reinterpret_cast<float*>(a.out)[at] = x;
