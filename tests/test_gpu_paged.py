@@ -186,6 +186,18 @@ def test_cache_of_many_sequences(kernel, e4m3):
     write_and_check(kernel, pool, k[:0], k[:0], ints(begin), [0] * seqs, [])
 
 
+@KINDS
+@PAGES
+def test_cache_of_more_rows_than_the_caches_hold(kernel, dtype, e4m3):
+    """More than 32 MiB of rows (read past the L2s)."""
+    pool = Pool(2, 150, 64, 8, e4m3, DEV, "rows")
+    n = (33 << 20) // (8 * 2 * D * (2 if dtype == BF else 4)) + 1
+    lengths = [n - 700, 700]
+    rows = torch.randn(n, 16, D, generator=torch.Generator(device=DEV).manual_seed(2), device=DEV).to(dtype)
+    at = [(s, 9 + i) for s, c in enumerate(lengths) for i in range(c)]
+    write_and_check(kernel, pool, rows[:, :8], rows[:, 8:], ints([9, 9]), lengths, at)
+
+
 # ---------------------------------------------------------------------------------------------
 # the attention
 # ---------------------------------------------------------------------------------------------
