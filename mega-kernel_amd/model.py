@@ -23,9 +23,13 @@ Mirrors ``/root/reference/model.py`` step for step:
     prompt in one call and ``beam_reorder`` spreads it over the others; each step is ``beam_select``,
     ``beam_reorder`` of the rows generated so far, and ``decode_batch`` of all beams. Nothing is read
     back until the last step.
+  * ``--temperature T`` (with ``--top-k``, ``--top-p``, ``--min-p``, ``--seed`` and ``--prompts S``): S prompts of
+    different lengths are continued together with tokens drawn from their logits (S <= 64). ``prefill_batch`` fills
+    their caches, and each step is ``sample`` and ``decode_batch``. Nothing is read back until the last step.
 
     python mega-kernel_amd/model.py [--shape qwen3-0.6b] [--prompt 32] [--max-seq 512] [--new 64]
                                     [--device-loop] [--native-prefill] [--beams 4 [--prompts 2] [--eos ID]]
+                                    [--temperature 0.8 [--top-k 50] [--top-p 0.9] [--min-p 0.05] [--seed 0]]
 """
 import argparse
 import os
@@ -99,6 +103,47 @@ def beam_search(kernel, prompts, beams, new, eos, embed, final_norm, layer_weigh
     return found
 
 
+def sample_texts(kernel, prompts, new, eos, temperature, top_k, top_p, min_p, seed, embed, final_norm, layer_weights, cos,
+                 sin, max_seq):
+    """Up to ``new`` tokens after each prompt (lists of token ids), drawn with ``sample``, as (tokens, the sum of their
+    log-probabilities); a continuation ends with ``eos`` (-1: none does). All calls are queued without reading
+    anything back, so ``new`` steps are always made. A prompt whose logits fail (NaN) ends there, with the sum NaN; the
+    others go on."""
+    import torch
+    dev, rows = embed.device, len(prompts)
+    lengths = [len(p) for p in prompts]
+    shape = (rows, len(layer_weights) // 11, 8, max_seq, 128)
+    k, v = (torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    packed = torch.tensor([t for p in prompts for t in p], dtype=torch.int32, device=dev)
+    weights = (embed, embed, final_norm, layer_weights, cos, sin)
+    settings = [torch.full((rows,), x, dtype=t, device=dev) for x, t in (
+        (temperature, torch.float32), (top_k, torch.int32), (top_p, torch.float32), (min_p, torch.float32))]
+    numbers = torch.rand(new, rows, generator=torch.Generator().manual_seed(seed)).to(dev)
+    logits, _ = kernel.prefill_batch(packed, lengths, *weights, k, v, max_seq)
+    position, steps = torch.tensor(lengths, dtype=torch.int32, device=dev), []
+    for i in range(new):
+        tokens, logprobs = kernel.sample(logits, numbers[i], *settings)
+        steps.append((tokens, logprobs))
+        if i + 1 < new:
+            # a failed row's token is -1, which would fail the decode of every sequence
+            logits, _ = kernel.decode_batch(tokens.clamp(min=0), position, *weights, k, v, max_seq)
+            position = position + 1
+    steps = [(t.tolist(), p.tolist()) for t, p in steps]
+    found = []
+    for row in range(rows):
+        text, total = [], 0.0
+        for tokens, logprobs in steps:
+            if tokens[row] < 0:
+                total = float("nan")
+                break
+            text.append(tokens[row])
+            total += logprobs[row]
+            if tokens[row] == eos:
+                break
+        found.append((text, total))
+    return found
+
+
 def run(argv=None, keep_prefill_cache=False):
     """Runs the driver and returns what it did: the generated tokens (the prefill's greedy token
     first), the prompt length, the device status after the loop, ms per token, and, with
@@ -114,9 +159,23 @@ def run(argv=None, keep_prefill_cache=False):
                     help="fill the cache with the batched prefill kernel (prefill) instead of the Transformers "
                          "prefill and cache copy")
     ap.add_argument("--beams", type=int, default=0, help="beam search with this many beams per prompt (1 to 16)")
-    ap.add_argument("--prompts", type=int, default=1, help="with --beams: prompts searched together")
-    ap.add_argument("--eos", type=int, default=-1, help="with --beams: the token that ends a continuation")
+    ap.add_argument("--prompts", type=int, default=1, help="with --beams or --temperature: prompts taken together")
+    ap.add_argument("--eos", type=int, default=-1, help="with --beams or --temperature: the token that ends a continuation")
+    ap.add_argument("--temperature", type=float, default=None, help="draw the tokens at this temperature (0: the likeliest)")
+    ap.add_argument("--top-k", type=int, default=0, help="with --temperature: from the k largest logits (0: all)")
+    ap.add_argument("--top-p", type=float, default=1.0, help="with --temperature: from the fewest that reach this share")
+    ap.add_argument("--min-p", type=float, default=0.0, help="with --temperature: from those this likely against the likeliest")
+    ap.add_argument("--seed", type=int, default=0, help="with --temperature: of the random numbers")
     a = ap.parse_args(argv)
+    if a.temperature is not None:
+        if a.beams or a.device_loop or a.native_prefill:
+            ap.error("--temperature goes without --beams, --device-loop and --native-prefill")
+        if not (0 <= a.temperature < float("inf") and 0 <= a.top_p <= 1 and 0 <= a.min_p <= 1 and a.top_k >= 0):
+            ap.error("--temperature and --top-k must be at least 0, --top-p and --min-p between 0 and 1")
+        if not 1 <= a.prompts <= 64:
+            ap.error("--temperature takes 1 to 64 prompts")
+        if not 1 <= a.prompt < a.max_seq:
+            ap.error("--temperature needs a prompt that leaves room in --max-seq")
     if a.beams and (a.beams > 16 or a.beams < 0 or a.prompts < 1 or a.beams * a.prompts > 64):
         ap.error("--beams takes 1 to 16 beams per prompt, and at most 64 in all")
     if a.beams and not 1 <= a.prompt < a.max_seq:
@@ -133,9 +192,24 @@ def run(argv=None, keep_prefill_cache=False):
     final_norm = model.model.norm.weight.detach().to(dev)
     cos, sin = megakernel.rope_tables(model, a.max_seq, dev)
 
+    # prompts of different lengths, the longest of --prompt tokens: pieces of the same random ids
+    prompts = [ids[0, :max(1, a.prompt - 5 * i)].tolist() for i in range(a.prompts)]
+    if a.temperature is not None:
+        new = min(a.new, a.max_seq - a.prompt)
+        t0 = time.perf_counter()
+        found = sample_texts(kernel, prompts, new, a.eos, a.temperature, a.top_k, a.top_p, a.min_p, a.seed, embed,
+                             final_norm, layer_weights, cos, sin, a.max_seq)
+        wall = time.perf_counter() - t0
+        for i, (tokens, score) in enumerate(found):
+            print(f"prompt {i} ({len(prompts[i])} tokens): " + (
+                f"{score:.3f} {tokens[:8]}{' ...' if len(tokens) > 8 else ''}" if score == score else "failed"))
+        print(f"sampling: {a.prompts} prompts, {new} steps in {wall * 1e3:.1f} ms, device status {kernel.status()}")
+        return {"prompt": a.prompt, "prompts": prompts, "texts": found, "status": kernel.status(),
+                "generated": [t for tokens, score in found for t in (tokens if score == score else [-1])],
+                "inputs": {"embed": embed, "final_norm": final_norm, "layer_weights": layer_weights, "cos": cos,
+                           "sin": sin, "max_seq": a.max_seq}}
+
     if a.beams:
-        # prompts of different lengths, the longest of --prompt tokens: pieces of the same random ids
-        prompts = [ids[0, :max(1, a.prompt - 5 * i)].tolist() for i in range(a.prompts)]
         new = min(a.new, a.max_seq - a.prompt)
         t0 = time.perf_counter()
         found = beam_search(kernel, prompts, a.beams, new, a.eos, embed, final_norm, layer_weights, cos, sin, a.max_seq)
