@@ -327,7 +327,7 @@ typedef struct mk_paged_cache {
  * a row with an infinity or NaN becomes NaN. A row whose position lies outside [0, table_entries * page_size) or whose
  * table entry lies outside [0, num_pages) is not written (mk_attention_paged reports the entry). Two rows of one call
  * may not share a place: what it then holds may be of both. Asynchronous on `stream`, no workspace; argument
- * errors (also more than 2^31 - 1 rows) return hipErrorInvalidValue before any launch.
+ * errors (also more than 2^25 rows) return hipErrorInvalidValue before any launch.
  */
 hipError_t mk_cache_write(const mk_paged_cache* cache, const void* k, int64_t k_row_stride, int64_t k_head_stride,
                           const void* v, int64_t v_row_stride, int64_t v_head_stride, int rows_fp32,

@@ -34,6 +34,7 @@
 
 namespace mkp {
 
+constexpr int64_t ROWS_MAX = 1 << 25;  // of a call: 64 threads each, and a launch has less than 2^32
 constexpr int CSEQ = 128;  // sequences per launch of the cache's kernels (their places travel as kernel arguments)
 constexpr int MIN_BYTE = 10;  // e8m0 byte of 2^-117: the least e4m3 value times it is bf16's least normal number
 
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const CacheArgs a) {
 // attention of one token per sequence
 // -----------------------------------------------------------------------------------------------------------
 constexpr int TK = 32;           // keys to a tile
-constexpr int AW = 4;            // waves to a workgroup
+constexpr int WAVES = 4;         // to a workgroup
 constexpr int NQ = 16;           // queries to a unit: (sequence, K/V head, 16 of its query heads)
 constexpr int OROW = D + 4;      // floats of a query's output in LDS
 constexpr int PART = D + 2;      // floats of one query's partial result: sum, maximum, output
@@ -232,7 +233,7 @@ constexpr int SEQ_MAX = 4096;
 // spill; of 64 to 960 in 8-bit pages 23.1 instead of 23.9.)
 constexpr int PAGED_WGS = 512;
 constexpr size_t BASE_BYTES = ((SEQ_MAX + 1) * sizeof(double) + 255) & ~(size_t)255;
-constexpr int START = 2;         // tiles that the start of a unit costs as much as: see Plan
+constexpr int START = 2;         // tiles that the start of a unit costs as much as
 
 struct PagedArgs {
   PagePool p;
@@ -240,9 +241,9 @@ struct PagedArgs {
   int64_t q_row, q_head;  // bytes
   uint8_t* out;
   const int32_t* lengths;
-  float* part;   // [2 * wgs][queries of a unit][PART]
+  float* part;   // [2 * PAGED_WGS][queries of a unit][PART]
   double* base;  // [nseq + 1]: the first place of each sequence's first unit, and `per`
-  int nseq, hkv, g, gt, wgs;  // gt: units to a K/V head
+  int nseq, hkv, g, gt;  // gt: units to a K/V head
   int64_t capacity;           // positions of a table
 };
 
@@ -256,8 +257,8 @@ __device__ __forceinline__ int valid_length(const PagedArgs& a, int b) {
 // sequence, and every workgroup `per` places of the row, its waves a part each; the places before a unit's first tile
 // stand for what a unit costs by itself (its queries, its first loads). Places are counted in doubles, exactly.
 __device__ __forceinline__ double places_of(int length) { return length > 0 ? START + (length + TK - 1) / TK : 0; }
-__device__ __forceinline__ double places_per(const PagedArgs& a, double total, int waves) {
-  return fmax(floor((total + a.wgs - 1) / a.wgs), (double)waves);
+__device__ __forceinline__ double places_per(double total) {
+  return fmax(floor((total + PAGED_WGS - 1) / PAGED_WGS), (double)WAVES);
 }
 
 // v as the sum of PARTS bf16 numbers, each the rounding of what the ones before it leave
@@ -307,7 +308,6 @@ struct Piece {
   int id, t0, t1, tiles;  // seq * units + unit; t0 == t1: none; the unit's tiles
   int row, nq;            // of the output's (sequence, head) rows, the unit's first; their number
 };
-template <int WAVES>
 struct PagedSmem {
   Piece piece[2 * WAVES];
   float m[2 * WAVES][NQ], l[2 * WAVES][NQ];
@@ -322,9 +322,9 @@ __device__ __forceinline__ void store_out(uint8_t* out, int64_t at, float4 y) { 
 // E4M3: 8-bit pages. QP, PP: bf16 parts of a query and of a weight (1 and 2 for bf16 queries, 3 for fp32 ones).
 // PG: 2, a tile lies in one page; 1, each 8 keys of it do; 0, pages are looked up key by key. SPLIT: the tiles of all units are shared out evenly, a
 // unit's parts joined by paged_join_kernel; else a workgroup takes a unit, a wave a run of its tiles.
-template <bool E4M3, int QP, int PP, int PG, bool SPLIT, int WAVES>
+template <bool E4M3, int QP, int PP, int PG, bool SPLIT>
 __global__ void __launch_bounds__(64 * WAVES, 2) paged_attention_kernel(const PagedArgs a) {
-  __shared__ PagedSmem<WAVES> sm;
+  __shared__ PagedSmem sm;
   extern __shared__ __attribute__((aligned(16))) float outs[];  // [pieces][queries of a unit][OROW]
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, g = lane >> 4;
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attention_kernel(const Pa
     mine *= units;
     double upto = scan_wave(mine, plus<double>);
     const double total = at_lane(upto, 63);
-    const double per = places_per(a, total, WAVES), wper = floor((per + WAVES - 1) / WAVES);
+    const double per = places_per(total), wper = floor((per + WAVES - 1) / WAVES);
     if (blockIdx.x == 0 && w == 0) {  // for the join
       double at = upto - mine;
 #pragma unroll 1
@@ -879,7 +879,7 @@ static int64_t rows_of(const int32_t* lengths, int num_seqs) {
     if (lengths[i] < 0) return -1;
     total += lengths[i];
   }
-  return total <= INT32_MAX ? total : -1;
+  return total <= ROWS_MAX ? total : -1;
 }
 
 static bool paged_split(int64_t capacity) { return capacity > 512; }
@@ -945,11 +945,11 @@ extern "C" size_t mk_attention_paged_workspace_bytes(int q_heads, int kv_heads) 
 template <bool E4M3, int QP, int PP, int PG>
 static void launch_paged(const PagedArgs& a, hipStream_t stream) {
   const unsigned units = (unsigned)((int64_t)a.nseq * a.hkv * a.gt);
-  const unsigned lds = 2 * AW * std::min(a.g, NQ) * OROW * sizeof(float);
+  const unsigned lds = 2 * WAVES * std::min(a.g, NQ) * OROW * sizeof(float);
   if (!paged_split(a.capacity)) {
-    hipLaunchKernelGGL((paged_attention_kernel<E4M3, QP, PP, PG, false, AW>), dim3(units), dim3(64 * AW), lds, stream, a);
+    hipLaunchKernelGGL((paged_attention_kernel<E4M3, QP, PP, PG, false>), dim3(units), dim3(64 * WAVES), lds, stream, a);
   } else {
-    hipLaunchKernelGGL((paged_attention_kernel<E4M3, QP, PP, PG, true, AW>), dim3(a.wgs), dim3(64 * AW), lds, stream, a);
+    hipLaunchKernelGGL((paged_attention_kernel<E4M3, QP, PP, PG, true>), dim3(PAGED_WGS), dim3(64 * WAVES), lds, stream, a);
     hipLaunchKernelGGL(paged_join_kernel<(QP > 1)>, dim3(a.nseq * a.hkv * a.g), dim3(256), 0, stream, a);
   }
 }
@@ -977,7 +977,6 @@ extern "C" hipError_t mk_attention_paged(const mk_paged_cache* cache, int q_head
   a.hkv = cache->kv_heads;
   a.g = q_heads / cache->kv_heads;
   a.gt = (a.g + NQ - 1) / NQ;
-  a.wgs = PAGED_WGS;
   a.capacity = (int64_t)cache->table_entries * cache->page_size;
   // the keys of a tile that surely share a page, and scales that can be loaded 8 at a time
   int pg = cache->page_size >= TK ? 2 : cache->page_size >= 8 ? 1 : 0;

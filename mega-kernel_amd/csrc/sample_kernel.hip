@@ -59,7 +59,6 @@ struct SampleStat {
   u64 key;       // the largest logit, the lowest token of equal ones; all bits set: the chunk has a NaN or +infinity
   int32_t tail_count, number;
   int32_t depth;  // bins 0 .. depth are listed in full; NB: all logits are
-  int32_t pad;
 };
 
 struct SampleArgs {

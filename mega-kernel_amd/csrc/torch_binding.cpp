@@ -662,8 +662,8 @@ int64_t check_lengths(const std::vector<int64_t>& lengths, const mk_paged_cache&
               " sequences, got ", lengths.size());
   int64_t total = 0;
   for (int64_t n : lengths) {
-    TORCH_CHECK(n >= 0 && n <= INT32_MAX && (total += n) <= INT32_MAX,
-                "megakernel: lengths must be at least 0 and add up to less than 2^31");
+    TORCH_CHECK(n >= 0 && n <= INT32_MAX && (total += n) <= 1 << 25,
+                "megakernel: lengths must be at least 0 and add up to at most 2^25");
     out.push_back((int32_t)n);
   }
   return total;

@@ -66,7 +66,7 @@ def test_cache_write_c(lib, fp32):
 
     assert call() == call(k=None) == call(pool(True)) == 0  # no rows: nothing to do
     assert call(False) == call(begin=None) == call(lengths=None) == call(lengths=(3, -1)) == INVALID
-    assert call(lengths=(2 ** 31 - 1, 1)) == INVALID
+    assert call(lengths=(2 ** 31 - 1, 1)) == call(lengths=(2 ** 25, 1)) == INVALID
     one = (1, 1)
     assert call(k=None, lengths=one) == call(v=None, lengths=one) == call(k=P + 8, lengths=one) == INVALID
     assert call(v=P + 8, lengths=one) == call(ks=(1022, 128), lengths=one) == call(vs=(1024, 126), lengths=one) == INVALID
@@ -215,6 +215,7 @@ def test_cache_write_op(ext):
     refuses("lengths must name", lengths=(5,))
     refuses("lengths must be at least 0", lengths=(6, -1))
     refuses("lengths must be at least 0", lengths=(2 ** 31 - 1, 1))
+    refuses("add up to at most 2", lengths=(2 ** 25, 1))
     refuses("k must be bfloat16 or float32", k=k.half())
     refuses("v must be Float", v=v.to(BF))
     refuses("k must have 5 rows", k=k[:4])
