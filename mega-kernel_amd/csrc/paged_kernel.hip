@@ -6,7 +6,9 @@
 // two loses nothing against a finer scale (e4m3 keeps its relative precision over 2^15), x / 2^e is exact, so the
 // only rounding is the value's own (2^-4 of it), and value * 2^e is exact in bf16, which the attention multiplies.
 // A row with an infinity or NaN is NaN throughout. Writing and reading take a wave per position, 16 lanes to a row:
-// bound by memory.
+// bound by memory. Measured on MI355X, a write and a read of the same rows: 11,994 fp32 rows of 8 heads through bf16
+// pages (319 MB moved) 58 us, 5.5 TB/s, where a copy of 4 GiB runs at 4.8; one row to each of 8 sequences 3.6 and 3.3 us
+// by the kernels' own times, a launch and three loads that wait for each other (begin, table, row).
 //
 // Attention. out[b][h] = sum over j < len[b] of softmax_j(q[b][h] . k[j][h / G] / sqrt(128)) v[j][h / G].
 // A wave takes 32 keys of one (sequence, K/V head) at a time for up to 16 of its query heads, on the matrix cores
@@ -19,6 +21,10 @@
 //                    Lane l then holds dims 32 g .. 32 g + 31 of query n.
 // K's loads for the next 32 keys leave when the scores are made, V's when its fragments are. At 2 queries to a K/V head
 // 14 of the 16 columns are zero and the matrix cores are still idle most of the time: the read of the keys bounds it.
+// Measured, bf16 queries of 16 heads on 8, both launches: 64 sequences of 900 to 4,095 keys in bf16 pages (655 MB) 119 us,
+// 5.5 TB/s; 30,001 keys of one (123 MB) 30 us, 4.1 TB/s, of which 5 are the join; 64 of 64 to 960 in 8-bit pages (69 MB) 23 us;
+// one of 300 keys 7.7 us: launch, cold code, and lengths, table and keys one after the other. Tiles through LDS would only
+// add a trip: a wave's keys are its own, and no second wave reads them.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -233,7 +239,9 @@ constexpr int SEQ_MAX = 4096;
 // spill; of 64 to 960 in 8-bit pages 23.1 instead of 23.9.)
 constexpr int PAGED_WGS = 512;
 constexpr size_t BASE_BYTES = ((SEQ_MAX + 1) * sizeof(double) + 255) & ~(size_t)255;
-constexpr int START = 2;         // tiles that the start of a unit costs as much as
+// Tiles that the start of a unit costs as much as: 1, 2 and 4 measure within 2% of each other from 1 to 256 sequences,
+// except 8-bit pages of 8 keys, where 4 takes 25.8 us and 1 and 2 take 24.4.
+constexpr int START = 2;
 
 struct PagedArgs {
   PagePool p;
@@ -320,8 +328,11 @@ __device__ __forceinline__ void store_out(uint8_t* out, int64_t at, float4 y) { 
 }
 
 // E4M3: 8-bit pages. QP, PP: bf16 parts of a query and of a weight (1 and 2 for bf16 queries, 3 for fp32 ones).
-// PG: 2, a tile lies in one page; 1, each 8 keys of it do; 0, pages are looked up key by key. SPLIT: the tiles of all units are shared out evenly, a
-// unit's parts joined by paged_join_kernel; else a workgroup takes a unit, a wave a run of its tiles.
+// PG: 2, a tile lies in one page (8-bit pages: one look-up and one address for all scales, 22.7 us instead of 23.6 for 64
+// sequences of 256 to 1,024 keys; bf16 pages gain nothing and take 1); 1, each 8 keys of it do; 0, pages are looked up key
+// by key (13 sequences of 128 to 512 keys 10.5 us instead of 9.6, 8-bit pages of 8 keys 25.9 instead of 24.4).
+// SPLIT: the tiles of all units are shared out evenly, a unit's parts joined by paged_join_kernel; else a workgroup takes a
+// unit, a wave a run of its tiles.
 template <bool E4M3, int QP, int PP, int PG, bool SPLIT>
 __global__ void __launch_bounds__(64 * WAVES, 2) paged_attention_kernel(const PagedArgs a) {
   __shared__ PagedSmem sm;
@@ -882,6 +893,10 @@ static int64_t rows_of(const int32_t* lengths, int num_seqs) {
   return total <= ROWS_MAX ? total : -1;
 }
 
+// Tables of at most 512 positions, 16 tiles to a unit, take one launch: four tiles to a wave at most. Measured, heads 16 / 8,
+// bf16 pages, lengths even over capacity / 4 .. capacity, without and with the split: capacity 512 one sequence 6.4 and
+// 8.5 us, 13 of them 9.6 and 10.7, 64 17.9 and 20.7, 256 63.0 and 65.4; capacity 1,024 one 13.2 and 8.9, 13 16.5 and 12.9,
+// 64 30.6 and 33.2, 256 128 and 135, but 64 of which one is full and the others have up to 64 keys 14.7 and 10.7.
 static bool paged_split(int64_t capacity) { return capacity > 512; }
 
 }  // namespace mkp
@@ -979,11 +994,12 @@ extern "C" hipError_t mk_attention_paged(const mk_paged_cache* cache, int q_head
   a.gt = (a.g + NQ - 1) / NQ;
   a.capacity = (int64_t)cache->table_entries * cache->page_size;
   // the keys of a tile that surely share a page, and scales that can be loaded 8 at a time
-  int pg = cache->page_size >= TK ? 2 : cache->page_size >= 8 ? 1 : 0;
+  int pg = a.p.ks && cache->page_size >= TK ? 2 : cache->page_size >= 8 ? 1 : 0;
   if (a.p.ks && (!aligned_to(a.p.ks, 8) || !aligned_to(a.p.vs, 8) || a.p.spage % 8 != 0 || a.p.shead % 8 != 0)) pg = 0;
   auto launch = [&](auto e4m3, auto qp, auto pp) {
-    if (pg == 2) launch_paged<e4m3.value, qp.value, pp.value, 2>(a, stream);
-    else if (pg == 1) launch_paged<e4m3.value, qp.value, pp.value, 1>(a, stream);
+    if constexpr (e4m3.value)
+      if (pg == 2) return launch_paged<true, qp.value, pp.value, 2>(a, stream);
+    if (pg == 1) launch_paged<e4m3.value, qp.value, pp.value, 1>(a, stream);
     else launch_paged<e4m3.value, qp.value, pp.value, 0>(a, stream);
   };
   using std::integral_constant;

@@ -20,6 +20,11 @@
 //                        Where a border lies deeper it joins the chunks' bins instead and gathers the border's bin from
 //                        the row, by its logits' bins in a byte each (narrowing it first where it holds more than 4,096). The answer is looked for among
 //                        the 8,192 logits of its chunk. Without any filter the chunks' sums are all that is needed.
+// The logits are read once and the chunk of the answer, or its listed logits, again. Measured on MI355X: one row of 151,936 22
+// to 27 us, 9 of them the first kernel, a chain of seven barriers through cold code, and 14 the second; with a border
+// deeper than the lists 31 to 34 us of the second kernel in one workgroup (the gather by codes, the sort, the chunks' sums).
+// 64 rows (39 MB) 56 us with such borders among them: 23 us of the first kernel, which the 64-bit
+// products and whole-number atomics of the weights bound (its read alone takes 8 us), and the deepest row's second.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -44,11 +49,12 @@ constexpr double ONE = (double)(1ull << FIX);
 constexpr int CNT = 50;             // a bin's number of logits, at most 8,192, from this bit on
 constexpr u64 SUM_MASK = (1ull << CNT) - 1;
 constexpr double SAME = 1.0 / (1ull << 42);
-constexpr int CAP = 4096;           // logits of a bin that are taken together
-constexpr int RANKED = 256;         // logits that are sorted by counting
+constexpr int CAP = 4096;           // logits of a bin that are taken together: what LDS holds
+constexpr int RANKED = 256;         // logits that are sorted by counting, four threads of the 1,024 to each
 constexpr int SUB = 2048;           // narrower bins of a bin that holds more
 constexpr int LISTED = 4;           // listed logits of a row per thread
-constexpr int LIST_MAX = 256;       // and of a chunk, a multiple of 64
+constexpr int LIST_MAX = 256;       // and of a chunk, a multiple of 64 (above 64 chunks, 524,288 logits, none: all borders
+                                    // are deep ones)
 
 typedef float f4a __attribute__((ext_vector_type(4), aligned(4)));  // rows may start at any element
 
@@ -1190,7 +1196,10 @@ extern "C" hipError_t mk_sample(int rows, int vocab, const float* logits, int64_
   a.listed = a.bins + slots * NB;
   a.codes = reinterpret_cast<uint8_t*>(a.listed + slots * LIST_MAX);
   const dim3 grid(a.chunks, rows);
-  if ((int64_t)a.chunks * rows <= 512) hipLaunchKernelGGL(sample_chunk_kernel<16>, grid, dim3(1024), 0, stream, a);
+  // A workgroup of 16 waves to a CU at most; beyond that, smaller ones overlap better. Measured on MI355X, top 50 of 0.95, 16
+  // waves and 4: 151,936 logits (19 chunks) 1 row 25.0 and 26.6 us, 13 rows 26.0 and 27.7, 20 rows 29.8 and 28.8, 64 rows
+  // 45.6 and 37.9; 32,000 (4 chunks) 64 rows 23.2 and 24.6, 128 rows 27.9 and 26.6. (8 waves: within 1% of 4 at 64 rows.)
+  if ((int64_t)a.chunks * rows <= 256) hipLaunchKernelGGL(sample_chunk_kernel<16>, grid, dim3(1024), 0, stream, a);
   else hipLaunchKernelGGL(sample_chunk_kernel<4>, grid, dim3(256), 0, stream, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
