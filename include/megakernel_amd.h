@@ -321,7 +321,8 @@ typedef struct mk_paged_cache {
  * (HOST array of num_seqs, read before the call returns, >= 0) of sequence s, which go to its positions
  * begin[s], begin[s] + 1, ... (begin: int32 device array).
  *   k, v   bf16, or fp32 with rows_fp32 != 0; head h of row r at r * k_row_stride + h * k_head_stride (elements,
- *          >= 0, multiples of 8, of 4 for fp32), 16-byte aligned: slices of one projection's rows will do
+ *          >= 0, multiples of 8, of 4 for fp32), 16-byte aligned: slices of one projection's rows will do;
+ *          they may not overlap the pages
  * bf16 pages: each number rounded to bf16. e4m3 pages: each head's row gets the least power of two, at least
  * 2^-117, that its largest magnitude is at most 448 times of, and its numbers are rounded to e4m3 in units of it;
  * a row with an infinity or NaN becomes NaN. A row whose position lies outside [0, table_entries * page_size) or whose

@@ -6,8 +6,8 @@
 // two loses nothing against a finer scale (e4m3 keeps its relative precision over 2^15), x / 2^e is exact, so the
 // only rounding is the value's own (2^-4 of it), and value * 2^e is exact in bf16, which the attention multiplies.
 // A row with an infinity or NaN is NaN throughout. Writing and reading take a wave per position, 16 lanes to a row:
-// bound by memory. Measured on MI355X, a write and a read of the same rows: 11,994 fp32 rows of 8 heads through bf16
-// pages (319 MB moved) 58 us, 5.5 TB/s, where a copy of 4 GiB runs at 4.8; one row to each of 8 sequences 3.6 and 3.3 us
+// bound by memory. Measured on MI355X, a write and a read: 14,992 fp32 rows of 8 heads into bf16 pages, and
+// 16,492 read back (319 MB moved) 58 us, 5.5 TB/s, where a copy of 4 GiB runs at 4.8; one row to each of 8 sequences 3.6 and 3.3 us
 // by the kernels' own times, a launch and three loads that wait for each other (begin, table, row).
 //
 // Attention. out[b][h] = sum over j < len[b] of softmax_j(q[b][h] . k[j][h / G] / sqrt(128)) v[j][h / G].
@@ -108,7 +108,7 @@ __device__ __forceinline__ Spot spot_of(const CacheArgs& a, int s, int64_t r) {
 
 // A wave to a position, 16 lanes to a row; the rows of k's heads, then of v's, 16 of them at a time. What a wave writes is
 // loaded before its place is looked up. ONCE: past the L2s, where the rows are more than these hold. Measured on MI355X:
-// 11,994 fp32 rows of 8 heads (98 MB) into bf16 pages and read back 58 us with and 65 us without; 873 rows (7 MB,
+// 14,992 fp32 rows of 8 heads (123 MB) into bf16 pages and 16,492 read back 58 us with and 65 us without; 1,092 rows (9 MB,
 // still in the L2s from call to call) 14.9 and 13.8.
 template <bool FP32, bool E4M3, bool ONCE>
 __global__ void __launch_bounds__(256) cache_write_kernel(const CacheArgs a) {
