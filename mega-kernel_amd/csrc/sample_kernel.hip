@@ -611,9 +611,9 @@ __device__ __forceinline__ void gather(const Row& r, uint32_t klo, uint32_t khi)
   __syncthreads();
 }
 
-// Gathers the logits of bin j, not the tail's, at most CAP, by the codes: 16 of them to a load. False if too many others
-// have their code.
-__device__ __forceinline__ bool gather_bin(const Row& r, const uint8_t* codes, int chunks, int j) {
+// Gathers the logits of bin j, not the tail's, from `low` on, at most CAP, by the codes: 16 of them to a load. False if too
+// many others have their code.
+__device__ __forceinline__ bool gather_bin(const Row& r, const uint8_t* codes, int chunks, int j, float low) {
   PickSmem& sm = smem();
   int* maybe = reinterpret_cast<int*>(sm.lkey);
   static_assert(sizeof(sm.lkey) >= 2 * CAP * sizeof(int));
@@ -658,7 +658,7 @@ __device__ __forceinline__ bool gather_bin(const Row& r, const uint8_t* codes, i
   for (int i = tid; i < all; i += ST) {
     const int v = maybe[i];
     const float x = v < r.vocab ? r.x[v] : -INFINITY;
-    if (floor((double)x * r.s.c) == fl) {
+    if (floor((double)x * r.s.c) == fl && x >= low) {
       const int to = atomicAdd(&sm.n, 1);
       if (to < CAP) sm.list[to] = logit_key(x, v);
     }
@@ -669,94 +669,102 @@ __device__ __forceinline__ bool gather_bin(const Row& r, const uint8_t* codes, i
 
 // Finds the border within bin j, which has `count` logits: the first of them, in order, at which their number reaches
 // `rank` (by_rank), or their sum reaches `goal` (in 2^-FIX of the bin's unit; the last of `most` logits, if none of
-// them does). Returns the sum up to it. Leaves the list of the whole bin where it holds no more than CAP.
+// them does). Returns the sum up to it. `low`: the count may leave out logits below it, which the first kernel has dropped
+// for min_p; a border among these is put at `low`. held: how many of the bin's logits from `low` on sm.list then
+// holds, all of them, or -1.
 __device__ __forceinline__ u64 border_in_bin(const Row& r, const uint8_t* codes, int chunks, int j, int count, bool by_rank,
-                                             int rank, double goal, int most, Cut& cut) {
+                                             int rank, double goal, int most, float low, Cut& cut, int& held) {
   PickSmem& sm = smem();
   const int tid = threadIdx.x;
-  if (count <= CAP && j < NB - 1 && codes && gather_bin(r, codes, chunks, j)) {
-    border_in_list(count, j, r.s.c, r.s.in, r.ref, by_rank, rank, goal, most, 0, 0);
-    cut = {j, true, key_x(sm.key), key_v(sm.key)};
-    return sm.sum;
-  }
-  bin_range(r, j);
-  uint32_t klo = sm.klo, khi = sm.khi;
   int n = count, above = 0;  // logits in [klo, khi], and of the bin above khi
   u64 sabove = 0;
-  auto reached = [&](int number, u64 sum) { return by_rank ? number >= rank : (double)sum >= goal || number >= most; };
-  while (n > CAP && klo < khi) {  // narrow: SUB bins of the order's numbers, the first of the order first
-    int shift = 0;
-    while (((khi - klo) >> shift) >= SUB) ++shift;
-    __syncthreads();
-    for (int i = tid; i < SUB; i += ST) {
-      sm.many.sum[i] = 0;
-      sm.many.count[i] = 0;
-    }
-    __syncthreads();
-    sweep(r, klo, khi, [&](float x, int) {
-      const uint32_t b = (khi - logit_order(x)) >> shift;
-      atomicAdd(&sm.many.count[b], 1u);
-      atomicAdd(&sm.many.sum[b], fixed_weight(r, x, j));
-    });
-    __syncthreads();
-    const int c0 = (int)sm.many.count[2 * tid], c1 = (int)sm.many.count[2 * tid + 1];
-    const u64 s0 = sm.many.sum[2 * tid], s1 = sm.many.sum[2 * tid + 1];
-    int call;
-    u64 sall;
-    int cb = above + block_before<SW>(c0 + c1, sm.wcount, call);
-    u64 sb = sabove + block_before<SW>(s0 + s1, sm.wfix, sall);
-    // the one place where it is reached, at the end of the range if nowhere before
-    const int lastb = (int)((khi - klo) >> shift);
-    const bool r0 = reached(cb + c0, sb + s0) || 2 * tid >= lastb, r1 = reached(cb + c0 + c1, sb + s0 + s1) || 2 * tid + 1 >= lastb;
-    const bool rb = tid > 0 && (reached(cb, sb) || 2 * tid - 1 >= lastb);
-    if (!rb && r1) {
-      sm.found = r0 ? 2 * tid : 2 * tid + 1;
-      sm.n = r0 ? c0 : c1;
-      sm.above = r0 ? cb : cb + c0;
-      sm.sum = r0 ? sb : sb + s0;
-    }
-    __syncthreads();
-    n = sm.n;
-    above = sm.above;
-    sabove = sm.sum;
-    const uint32_t hi = khi - ((uint32_t)sm.found << shift), width = (1u << shift) - 1;
-    klo = hi - klo > width ? hi - width : klo;
-    khi = hi;
-    __syncthreads();
-  }
-  if (n > CAP) {  // equal logits: so many of them, the lowest tokens
-    const float x = logit_of(khi);
-    const u64 w = fixed_weight(r, x, j);
-    int take;
-    if (by_rank) {
-      take = rank - above;
-    } else {
-      take = w ? (int)fmin(ceil((goal - (double)sabove) / (double)w), (double)n) : n;
-      take = min(take, most - above);
-    }
-    take = max(1, min(take, n));
-    // the token of the take-th: tokens in their order, a piece of 4 to a thread
-    int seen = 0;
-    if (tid == 0) sm.found = 0;
-    for (int base = 0; base < r.vocab && seen < take; base += 4 * ST) {
-      int mine = 0, all;
-      for (int q = 0; q < 4; ++q) {
-        const int v = base + 4 * tid + q;
-        mine += v < r.vocab && r.x[v] == x;
+  held = -1;
+  if (!(count <= CAP && j < NB - 1 && codes && gather_bin(r, codes, chunks, j, low))) {
+    bin_range(r, j);
+    uint32_t klo = sm.klo, khi = sm.khi;
+    if (count <= CAP) klo = max(klo, logit_order(low));
+    auto reached = [&](int number, u64 sum) { return by_rank ? number >= rank : (double)sum >= goal || number >= most; };
+    while (n > CAP && klo < khi) {  // narrow: SUB bins of the order's numbers, the first of the order first
+      int shift = 0;
+      while (((khi - klo) >> shift) >= SUB) ++shift;
+      __syncthreads();
+      for (int i = tid; i < SUB; i += ST) {
+        sm.many.sum[i] = 0;
+        sm.many.count[i] = 0;
       }
-      int before = seen + block_before<SW>(mine, sm.wcount, all);
-      if (before < take && before + mine >= take)
+      __syncthreads();
+      sweep(r, klo, khi, [&](float x, int) {
+        const uint32_t b = (khi - logit_order(x)) >> shift;
+        atomicAdd(&sm.many.count[b], 1u);
+        atomicAdd(&sm.many.sum[b], fixed_weight(r, x, j));
+      });
+      __syncthreads();
+      const int c0 = (int)sm.many.count[2 * tid], c1 = (int)sm.many.count[2 * tid + 1];
+      const u64 s0 = sm.many.sum[2 * tid], s1 = sm.many.sum[2 * tid + 1];
+      int call;
+      u64 sall;
+      int cb = above + block_before<SW>(c0 + c1, sm.wcount, call);
+      u64 sb = sabove + block_before<SW>(s0 + s1, sm.wfix, sall);
+      // the one place where it is reached, at the end of the range if nowhere before
+      const int lastb = (int)((khi - klo) >> shift);
+      const bool r0 = reached(cb + c0, sb + s0) || 2 * tid >= lastb, r1 = reached(cb + c0 + c1, sb + s0 + s1) || 2 * tid + 1 >= lastb;
+      const bool rb = tid > 0 && (reached(cb, sb) || 2 * tid - 1 >= lastb);
+      if (!rb && r1) {
+        sm.found = r0 ? 2 * tid : 2 * tid + 1;
+        sm.n = r0 ? c0 : c1;
+        sm.above = r0 ? cb : cb + c0;
+        sm.sum = r0 ? sb : sb + s0;
+      }
+      __syncthreads();
+      n = sm.n;
+      above = sm.above;
+      sabove = sm.sum;
+      const uint32_t hi = khi - ((uint32_t)sm.found << shift), width = (1u << shift) - 1;
+      klo = hi - klo > width ? hi - width : klo;
+      khi = hi;
+      __syncthreads();
+    }
+    if (n > CAP) {  // equal logits: so many of them, the lowest tokens
+      const float x = logit_of(khi);
+      const u64 w = fixed_weight(r, x, j);
+      int take;
+      if (by_rank) {
+        take = rank - above;
+      } else {
+        take = w ? (int)fmin(ceil((goal - (double)sabove) / (double)w), (double)n) : n;
+        take = min(take, most - above);
+      }
+      take = max(1, min(take, n));
+      // the token of the take-th: tokens in their order, a piece of 4 to a thread
+      int seen = 0;
+      if (tid == 0) sm.found = 0;
+      for (int base = 0; base < r.vocab && seen < take; base += 4 * ST) {
+        int mine = 0, all;
         for (int q = 0; q < 4; ++q) {
           const int v = base + 4 * tid + q;
-          if (v < r.vocab && r.x[v] == x && ++before == take) sm.found = v;
+          mine += v < r.vocab && r.x[v] == x;
         }
-      seen += all;
+        int before = seen + block_before<SW>(mine, sm.wcount, all);
+        if (before < take && before + mine >= take)
+          for (int q = 0; q < 4; ++q) {
+            const int v = base + 4 * tid + q;
+            if (v < r.vocab && r.x[v] == x && ++before == take) sm.found = v;
+          }
+        seen += all;
+      }
+      __syncthreads();
+      cut = {j, true, x, sm.found};
+      return sabove + (u64)take * w;
     }
-    __syncthreads();
-    cut = {j, true, x, sm.found};
-    return sabove + (u64)take * w;
+    gather(r, klo, khi);
   }
-  gather(r, klo, khi);
+  if (count <= CAP) {
+    n = held = sm.n;
+    if (by_rank ? rank > n : n == 0) {
+      cut = {j, true, low, INT32_MAX};
+      return 0;
+    }
+  }
   border_in_list(n, j, r.s.c, r.s.in, r.ref, by_rank, rank, goal, most, above, sabove);
   cut = {j, true, key_x(sm.key), key_v(sm.key)};
   return sm.sum;
@@ -827,7 +835,8 @@ __device__ __forceinline__ void deep_cut(const u64* bins, const SampleStat* stat
     }
   }
   Cut cut = {NB - 1, false, 0.f, 0};
-  int kept = number, holds = -1;  // candidates; the bin whose logits the list holds
+  const float low = top_p >= 1.f && jm < NB ? xm : -3.4028234663852886e38f;  // the first kernel may have dropped those below
+  int kept = number, holds = -1, held = -1;  // candidates; the bin whose logits the list holds, and their number
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
     const bool by_rank = pass == 0;
@@ -838,8 +847,8 @@ __device__ __forceinline__ void deep_cut(const u64* bins, const SampleStat* stat
     }));
     const int n = sm.cupto[j] - number_below(j);
     const u64 s = border_in_bin(r, codes, chunks, j, n, by_rank, top_k - number_below(j), (goal - weight_below(j)) / sm.et[j] * ONE,
-                                min(n, kept - number_below(j)), cut);
-    holds = n <= CAP ? j : -1;
+                                min(n, kept - number_below(j)), low, cut, held);
+    holds = held >= 0 ? j : -1;
     if (by_rank) {
       kept = top_k;
       whole = weight_below(j) + (double)s / ONE * sm.et[j];
@@ -852,12 +861,13 @@ __device__ __forceinline__ void deep_cut(const u64* bins, const SampleStat* stat
     const int j = cut.bin, n = sm.cupto[j] - number_below(j);
     if (n <= CAP) {
       if (holds != j) {
-        if (j == NB - 1 || !codes || !gather_bin(r, codes, chunks, j)) {
+        if (j == NB - 1 || !codes || !gather_bin(r, codes, chunks, j, cut.x)) {
           bin_range(r, j);
-          gather(r, sm.klo, sm.khi);
+          gather(r, max(sm.klo, logit_order(cut.x)), sm.khi);
         }
+        held = sm.n;
       }
-      for (int i = tid; i < n; i += ST) {
+      for (int i = tid; i < held; i += ST) {
         const float y = key_x(sm.list[i]);
         const int v = key_v(sm.list[i]);
         if (cut.keeps(j, y, v)) atomicAdd(&sm.part[v / SC], fixed_weight(r, y, j));

@@ -161,6 +161,26 @@ def test_a_crowded_bin_is_narrowed(kernel):
             check(kernel, x, u, T, k, p, m)
 
 
+@pytest.mark.parametrize("above", [0, 6000])
+def test_min_p_in_a_crowded_bin(kernel, above):
+    """A border in a bin of which min_p leaves some logits, too many to be listed, and not many more; with 6,000 spread over the
+    bin above, that bin's and its own logits are more than are told apart by their bins alone."""
+    gen = torch.Generator(device=DEV).manual_seed(above + 1)
+    top = 2.14 if above else 2.07  # bins of x log2(e) 11: 32 up to 2.0797, 33 up to 2.1427
+    x = 2.02 + 0.03 * torch.rand(6, V, generator=gen, device=DEV)
+    for c in range(3):
+        x[:, 40000 * c:40000 * c + 1200] = 2.06 + 0.009 * torch.rand(6, 1200, generator=gen, device=DEV)
+    if above:
+        x[:, 100000:100000 + above] = 2.09 + 0.049 * torch.rand(6, above, generator=gen, device=DEV)
+    x[:, 8191::8192] = top
+    x[:, V - 1] = top
+    u = torch.tensor([0.0, 0.2, 0.5, 0.7, 0.9, 0.9999], device=DEV)
+    for k in (0, 50, 150, 1000, 3000, 3617, 7000, 9000, 9621, 100000):
+        for threshold in (2.055, 2.065, 2.0695, 2.08, 2.03):
+            if threshold < top:
+                check(kernel, x, u, 1.0, k, 1.0, math.exp(threshold - top))
+
+
 def test_temperatures(kernel):
     x, u = logits(12, 40000, 5)
     check(kernel, x, u, [0.0, 1e-45, 1e-30, 1e-3, 0.05, 0.5, 3.0, 100.0, 1e6, 1e30, 3.4e38, 0.01], [0, 300])
