@@ -343,7 +343,8 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attention_kernel(const Pa
   const int gmax = min(a.g, NQ);
   int b, u, len;       // sequence, unit of it, its keys
   double p = 0, left;  // places of the unit that are behind the wave, places that it has still to do
-  if (tid < 2 * WAVES) sm.piece[tid].t0 = sm.piece[tid].t1 = 0;
+  // each wave its own two, which nobody else touches before the barrier behind the loop
+  if (lane < 2) sm.piece[2 * w + lane].t0 = sm.piece[2 * w + lane].t1 = 0;
   if constexpr (SPLIT) {
     // Every wave for itself: a lane adds up `each` sequences, and the lane that the wave's first place falls to tells
     // the sequence, or (more than 64 of them) the 64 lanes look among its sequences.
