@@ -53,10 +53,11 @@ __device__ __forceinline__ V max_over_wave(V v) {  // of numbers that are not ne
   return at_lane(scan_wave(v, [](V a, V b) { return a > b ? a : b; }), 63);
 }
 
-// Sums over the threads before this one and over all WAVES waves of the workgroup (numbers that commute exactly, or in a
-// fixed order). `lds` holds WAVES numbers.
+// Sums over the threads up to this one, over all WAVES waves of the workgroup and over the waves before this one, each in
+// an order of its own. `lds` holds WAVES numbers. For numbers that round: the sum before a thread is the one up to the
+// thread before it. (Taken as a difference, a small sum before a large number would be rounded to the large one's digits.)
 template <int WAVES, typename V>
-__device__ __forceinline__ V block_before(V v, V* lds, V& total) {
+__device__ __forceinline__ V block_upto(V v, V* lds, V& total, V& waves) {
   static_assert(WAVES <= 16 && (WAVES & (WAVES - 1)) == 0);
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const V x = scan_wave(v, plus<V>);
@@ -66,7 +67,19 @@ __device__ __forceinline__ V block_before(V v, V* lds, V& total) {
   const V y = scan_row16(lds[lane & (WAVES - 1)], plus<V>);  // every wave: the waves' sums, up to each
   total = at_lane(y, WAVES - 1);
   const V before = at_lane(y, w > 0 ? w - 1 : 0);
-  return (w ? before : (V)0) + (x - v);
+  waves = w ? before : (V)0;
+  return waves + x;
+}
+template <int WAVES, typename V>
+__device__ __forceinline__ V block_upto(V v, V* lds, V& total) {
+  V waves;
+  return block_upto<WAVES>(v, lds, total, waves);
+}
+// Sums over the threads before this one and over all, of whole numbers.
+template <int WAVES, typename V>
+__device__ __forceinline__ V block_before(V v, V* lds, V& total) {
+  static_assert(V(0.5) == V(0), "a sum that rounds has no exact difference");
+  return block_upto<WAVES>(v, lds, total) - v;
 }
 
 }  // namespace mk

@@ -827,11 +827,11 @@ __device__ __forceinline__ void deep_cut(const u64* bins, const SampleStat* stat
       n = tid < NB - 1 ? (int)sm.many.count[tid] : sm.n;
       weight = tid < NB - 1 ? (double)sm.many.sum[tid] / ONE * sm.et[tid] : t;
     }
-    const double wb = block_before<SW>(weight, sm.wsum, wall);
-    const int cb = block_before<SW>(n, sm.wcount, call);
+    const double upto = block_upto<SW>(weight, sm.wsum, wall);
+    const int cupto = block_upto<SW>(n, sm.wcount, call);
     if (tid < NB) {
-      sm.upto[tid] = wb + weight;
-      sm.cupto[tid] = cb + n;
+      sm.upto[tid] = upto;
+      sm.cupto[tid] = cupto;
     }
   }
   Cut cut = {NB - 1, false, 0.f, 0};
@@ -976,11 +976,11 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
       const double weight = tid < NB ? (double)(b & SUM_MASK) / ONE * sm.et[tid] : 0;
       double all;
       int call;
-      const double wb = block_before<SW>(weight, sm.wsum, all);
-      const int cb = block_before<SW>((int)(b >> CNT), sm.wcount, call);
+      const double upto = block_upto<SW>(weight, sm.wsum, all);
+      const int cupto = block_upto<SW>((int)(b >> CNT), sm.wcount, call);
       if (tid < NB) {
-        sm.upto[tid] = wb + weight;
-        sm.cupto[tid] = cb + (int)(b >> CNT);
+        sm.upto[tid] = upto;
+        sm.cupto[tid] = cupto;
       }
     }
     // the least logit with w >= min_p, and its bin
@@ -1071,7 +1071,7 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
     if (lane == at) {
       const bool second = hit ? !h0 : c1 > 0;
       sm.found = 2 * lane + second;
-      sm.goal = goal - (second ? before + c0 : before);
+      sm.goal = fmax(goal - (second ? before + c0 : before), 0.0);  // (the sums before it may have been rounded up)
       sm.z = z;
       sm.first[0] = INT32_MAX;
       sm.last[0] = -1;
@@ -1100,11 +1100,11 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
     __syncthreads();
     weight = tid < n ? sm.inorder[tid] : 0;
     double all;
-    const double run = block_before<SW>(weight, sm.wsum, all);
     // the first one whose running sum exceeds the goal, the last one if none does
-    if (tid < n && (run + weight > goal || tid == n - 1) && (tid == 0 || !(run > goal))) atomicMin(&sm.first[0], tid);
+    const u64 hit = __builtin_amdgcn_ballot_w64(block_upto<SW>(weight, sm.wsum, all) > goal && tid < n);
+    if (hit && lane == __ffsll(hit) - 1) atomicMin(&sm.first[0], tid);
     __syncthreads();
-    if (tid == sm.first[0]) {
+    if (tid == min(sm.first[0], n - 1)) {
       a.tokens[row] = sm.token[tid];
       if (a.logprobs) a.logprobs[row] = (float)fmin(log64(weight / z), 0.0);
     }
@@ -1124,11 +1124,12 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
 #pragma unroll
     for (int q = 0; q < 8; ++q) f[q] = v0 + q < a.vocab ? x[v0 + q] : -INFINITY;
   }
-  // a thread's sum, then, by the waves that the answer may be in, the place in it: the first logit with which the running
-  // sum exceeds the goal, or the last one of any weight
+  // a thread's sum and its last logit of any weight, then, by the waves that the answer may be in, the first logit with which
+  // the running sum exceeds the goal; the row's last one of any weight if none does
   double* weights = reinterpret_cast<double*>(sm.lkey) + tid;  // (and on into lbin)
   static_assert(sizeof(sm.lkey) + sizeof(sm.lbin) >= SC * sizeof(double));
-  double mine = 0, weight = 0, all;
+  double mine = 0, all, waves;
+  int last = -1;
 #pragma unroll 1
   for (int q = 0; q < 8; ++q) {
     const double p = (double)f[0] * sc.c, fl = floor(p);
@@ -1138,31 +1139,32 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
       s = j < NB - 1 ? (double)fixed_in_bin(f[0], sc, fl) / ONE * sm.et[j] : exp_tail(p - ref);
     weights[q * ST] = s;
     mine += s;
+    last = s > 0 ? v0 + q : last;
     turn(f);
   }
-  double run = block_before<SW>(mine, sm.wsum, all);
-  int hit = -1, last = -1;
-  // sums in another order may differ in their last digits: a little more than the thread that has it
+  const double upto = block_upto<SW>(mine, sm.wsum, all, waves);
+  double run = __shfl_up(upto, 1);
+  if (lane == 0) run = waves;
+  const u64 some = __builtin_amdgcn_ballot_w64(last >= 0);
+  if (some && lane == 63 - __clzll(some)) atomicMax(&sm.last[0], last);
+  // Sums in another order may differ in their last digits: a little more than the thread that has it, so that one of these has
+  // it wherever the goal is below all of them.
   const bool here = mine > 0 && (run + mine) * (1 + SAME) > goal && run * (1 - SAME) <= goal;
-  if (__builtin_amdgcn_ballot_w64(here) || all * (1 - SAME) <= goal) {
+  int hit = INT32_MAX;
+  if (__builtin_amdgcn_ballot_w64(here)) {
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
       const double s = weights[q * ST];
       run += s;
-      if (s > 0 && hit < 0) {
-        if (run > goal) hit = v0 + q;
-        last = v0 + q;
-        weight = s;
-      }
+      if (here && s > 0 && run > goal) hit = min(hit, v0 + q);
     }
   }
-  if (hit >= 0) atomicMin(&sm.first[0], hit);
-  if (last >= 0) atomicMax(&sm.last[0], last);
+  if (hit < INT32_MAX) atomicMin(&sm.first[0], hit);
   __syncthreads();
   const int v = sm.first[0] < INT32_MAX ? sm.first[0] : sm.last[0];
-  if (v >= 0 && (v == hit || v == last)) {
+  if (v >= v0 && v < v0 + 8) {
     a.tokens[row] = v;
-    if (a.logprobs) a.logprobs[row] = (float)fmin(log64(weight / z), 0.0);
+    if (a.logprobs) a.logprobs[row] = (float)fmin(log64(weights[(v - v0) * ST] / z), 0.0);
   }
 }
 
