@@ -393,7 +393,7 @@ struct PickSmem {
   int32_t wcount[SW];
   u64 wfix[SW], wfix2[SW];
   int first[SW], last[SW];
-  int found, n, above, depth, number;
+  int found, border, n, above, depth, number;
   u64 sum, key;
   uint32_t klo, khi;
   double z, goal;
@@ -415,15 +415,21 @@ struct Row {
 
 __device__ __forceinline__ double weight_below(int j) { return j > 0 ? smem().upto[j - 1] : 0.0; }
 __device__ __forceinline__ int number_below(int j) { return j > 0 ? smem().cupto[j - 1] : 0; }
-// the first bin that passes a test that stays passed, the last one if none does
-template <typename F>
-__device__ __forceinline__ int first_bin(F test) {
+// The bin that a border falls into: the first one up to which there are `rank` logits (by_rank), or, of those that have any,
+// weights of `goal`; the last one if none is. (Running sums are added up in orders of their own: a bin without logits may have
+// a larger one than the bins around it, by the last digit.)
+__device__ __forceinline__ int border_bin(bool by_rank, int rank, double goal) {
   PickSmem& sm = smem();
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63;
+  if (tid == 0) sm.border = NB - 1;
   __syncthreads();
-  if (tid < NB && (tid == 0 || !test(tid - 1)) && (tid == NB - 1 || test(tid))) sm.found = tid;
+  if (tid < NB) {
+    const int n = sm.cupto[tid];
+    const u64 hit = __builtin_amdgcn_ballot_w64(by_rank ? n >= rank : n > number_below(tid) && sm.upto[tid] >= goal);
+    if (hit && lane == __ffsll(hit) - 1) atomicMin(&sm.border, tid);
+  }
   __syncthreads();
-  return sm.found;
+  return sm.border;
 }
 
 // The weight of a logit of the row's bin j, in 2^-FIX of 2^(-j / 11).
@@ -842,9 +848,7 @@ __device__ __forceinline__ void deep_cut(const u64* bins, const SampleStat* stat
     const bool by_rank = pass == 0;
     if (by_rank ? top_k <= 0 || top_k >= number : !(top_p < 1.f)) continue;
     const double goal = (double)top_p * whole * (1 - SAME);
-    const int j = min(cut.bin, first_bin([&](int i) {
-      return by_rank ? sm.cupto[i] >= top_k : sm.cupto[i] > 0 && sm.upto[i] >= goal;
-    }));
+    const int j = min(cut.bin, border_bin(by_rank, top_k, goal));
     const int n = sm.cupto[j] - number_below(j);
     const u64 s = border_in_bin(r, codes, chunks, j, n, by_rank, top_k - number_below(j), (goal - weight_below(j)) / sm.et[j] * ONE,
                                 min(n, kept - number_below(j)), low, cut, held);
@@ -1002,9 +1006,7 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
       const bool by_rank = pass == 0;
       if (by_rank ? top_k <= 0 || top_k >= number : !(top_p < 1.f)) continue;
       const double goal = (double)top_p * sum * (1 - SAME);
-      const int j = min(cut.bin, first_bin([&](int i) {
-        return by_rank ? sm.cupto[i] >= top_k : sm.cupto[i] > 0 && sm.upto[i] >= goal;
-      }));
+      const int j = min(cut.bin, border_bin(by_rank, top_k, goal));
       const int n = sm.cupto[j] - number_below(j);
       if (j > depth) {
         deep = true;
