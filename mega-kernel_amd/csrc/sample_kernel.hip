@@ -297,8 +297,8 @@ __global__ void __launch_bounds__(64 * W) sample_chunk_kernel(const SampleArgs a
     __syncthreads();
     out.depth = out.number <= a.list ? NB : sdepth;
     // their logits, in the threads' order: first those that cannot be lower, to a part of a bin
-    const double low = out.ref - out.depth;
-    const float lim = out.depth == NB ? -INFINITY : (float)fmax((low - 0.5) / s.c, -3.4028234663852886e38);
+    // (their bins decide as they did above: beyond 2^53 the number of the bin that is next to `ref` is `ref` again)
+    const float lim = out.depth == NB ? -INFINITY : (float)fmax((out.ref - out.depth - 0.5) / s.c, -3.4028234663852886e38);
     uint32_t mine = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) mine = mine + mine + (f[i] >= lim && f[i] > -INFINITY);
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(64 * W) sample_chunk_kernel(const SampleArgs a
       todo &= ~(1u << e);
       const int i = N - 1 - e;
       const float y = x[v0 + 256 * (i >> 2) + (i & 3)];  // again: cheaper than finding it among the registers
-      if (out.depth == NB || floor((double)y * s.c) >= low) keep |= 1u << e;
+      if (bin_of(out.ref, floor((double)y * s.c)) <= out.depth) keep |= 1u << e;
     }
     int n;
     int to = block_before<W>((int)__popc(keep), scan, n);

@@ -1,12 +1,14 @@
 """``sample`` on the GPU where sums of very different sizes meet and at the ends of its filters, against its definition in
 64 bits (``test_gpu_sample``). Numbers u are single precision, 2^-24 of themselves apart, and running sums are good to
 2^-36 of themselves, so that nearly no u is too near a border to tell; ``apart`` leaves these few out."""
+import ctypes
 import math
 
 import pytest
 import torch
 
-from test_gpu_sample import DEV, INF, check
+from megakernel import build as mkbuild
+from test_gpu_sample import DEV, INF, check, rows
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +63,38 @@ def test_weights_that_grow_along_the_vocabulary(kernel, vocab, k, p, m):
     assert len(u) > 700
     tokens, _ = poisoned(kernel, x.expand(len(u), -1), u, 1.0, k, p, m)
     assert len(set(tokens.tolist())) > 2
+
+
+def guarded(x, u, T, k, p, m):
+    """The C entry on a workspace of just the bytes that it asks for, with a megabyte behind it that has to stay as it is."""
+    lib = ctypes.CDLL(mkbuild.LIB)
+    lib.mk_sample_workspace_bytes.restype = ctypes.c_size_t
+    n, vocab = x.shape
+    need = lib.mk_sample_workspace_bytes(n, vocab)
+    memory = torch.full((need + (1 << 20),), 0xa5, dtype=torch.uint8, device=DEV)
+    tokens, logprobs = torch.full((n,), -7, dtype=torch.int32, device=DEV), torch.full((n,), math.nan, device=DEV)
+    ins = [ctypes.c_void_p(t.data_ptr()) for t in (u, rows(T, n), rows(k, n, torch.int32), rows(p, n), rows(m, n))]
+    torch.cuda.synchronize()
+    assert lib.mk_sample(n, vocab, ctypes.c_void_p(x.data_ptr()), ctypes.c_int64(x.stride(0)), *ins,
+                         ctypes.c_void_p(tokens.data_ptr()), ctypes.c_void_p(logprobs.data_ptr()),
+                         ctypes.c_void_p(memory.data_ptr()), ctypes.c_size_t(need), None) == 0
+    torch.cuda.synchronize()
+    assert (memory[need:] == 0xa5).all()
+    return tokens, logprobs
+
+
+@pytest.mark.parametrize("value", [-3.4e38, 3.3e38, -1e16, torch.finfo(torch.float32).min])
+@pytest.mark.parametrize("vocab,equal", [(300, 300), (8192, 5000), (20000, 257), (20000, 20000), (151936, 151936)])
+def test_equal_logits_so_large_that_bins_have_no_numbers_of_their_own(kernel, vocab, equal, value):
+    """Rows masked whole with the type's lowest value, and others whose largest logits, more than are listed, are 2^53 bins and
+    more from 0."""
+    gen = torch.Generator().manual_seed(vocab + equal)
+    x = torch.full((5, vocab), -INF if value < 0 else 0.0)
+    x[:, torch.randperm(vocab, generator=gen)[:equal]] = value
+    x, u = x.to(DEV), torch.tensor([0.0, 0.3, 0.5, 0.9, 1 - 2.0 ** -24], device=DEV)
+    for T, k, p, m in ((1.0, 50, 1.0, 0.0), (1.0, 0, 0.9, 0.0), (0.7, 0, 1.0, 0.5), (1.3, 3, 0.5, 0.1), (1.0, 6000, 0.8, 1.0),
+                       (1.0, 0, 1.0, 0.0), (1e-3, 257, 1.0, 0.0)):
+        tokens, logprobs = check(kernel, x, u, T, k, p, m)
+        for _ in range(3):
+            again, lp = guarded(x, u, T, k, p, m)
+            assert torch.equal(again, tokens) and torch.equal(lp.double().cpu(), logprobs)
