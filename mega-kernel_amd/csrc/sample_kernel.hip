@@ -839,6 +839,7 @@ __device__ __forceinline__ void deep_cut(const u64* bins, const SampleStat* stat
       sm.upto[tid] = upto;
       sm.cupto[tid] = cupto;
     }
+    __syncthreads();  // min_p's border alone is looked for without another one
   }
   Cut cut = {NB - 1, false, 0.f, 0};
   const float low = top_p >= 1.f && jm < NB ? xm : -3.4028234663852886e38f;  // the first kernel may have dropped those below

@@ -98,3 +98,21 @@ def test_equal_logits_so_large_that_bins_have_no_numbers_of_their_own(kernel, vo
         for _ in range(3):
             again, lp = guarded(x, u, T, k, p, m)
             assert torch.equal(again, tokens) and torch.equal(lp.double().cpu(), logprobs)
+
+
+@pytest.mark.parametrize("crowd", [300, 4000, 5000, 140000])
+def test_min_p_alone_in_a_bin_of_many(kernel, crowd):
+    """The bin that min_p's border falls into holds more logits than are listed, than are taken together and fewer: no other
+    filter looks for a bin before it. The same answers every time."""
+    gen = torch.Generator(device=DEV).manual_seed(crowd)
+    x = torch.full((8, 151936), -5.0, device=DEV)
+    for row in x:
+        row[torch.randperm(151936, generator=gen, device=DEV)[:crowd]] = 2.02 + 0.05 * torch.rand(crowd, generator=gen, device=DEV)
+    x[:, 77] = 2.07
+    u = torch.rand(8, generator=gen, device=DEV)
+    for m in (math.exp(2.05 - 2.07), math.exp(2.0201 - 2.07), math.exp(-7.0)):
+        tokens, logprobs = check(kernel, x, u, 1.0, 0, 1.0, m)
+        args = (x, u, rows(1.0, 8), rows(0, 8, torch.int32), rows(1.0, 8), rows(m, 8))
+        for _ in range(20):
+            again, lp = kernel.sample(*args)
+            assert torch.equal(again, tokens) and torch.equal(lp.double().cpu(), logprobs)
