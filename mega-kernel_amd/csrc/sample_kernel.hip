@@ -81,6 +81,9 @@ struct SampleArgs {
   uint8_t* codes;    // [rows][chunks][SC]: half of each logit's bin, of rows whose border may lie deeper
 };
 
+// No weight is above 1: a larger min_p leaves the likeliest token alone, the lowest of equal ones, as a top_k of 1 does.
+__device__ __forceinline__ int top_k_under(float min_p, int top_k) { return min_p > 1.f ? 1 : top_k; }
+
 __device__ __forceinline__ uint32_t logit_order(float x) {  // unsigned order is the numbers'
   const uint32_t u = __float_as_uint(x + 0.f);  // -0 as 0
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
@@ -188,8 +191,8 @@ __global__ void __launch_bounds__(64 * W) sample_chunk_kernel(const SampleArgs a
     }
   }
   const float T = a.temperature[row];
-  const int top_k = a.top_k[row];
   const float top_p = a.top_p[row], min_p = a.min_p[row];
+  const int top_k = top_k_under(min_p, a.top_k[row]);
   const bool filtered = top_k > 0 || !(top_p >= 1.f) || min_p > 0.f;
   for (int i = tid; i < NB; i += 64 * W) bins[i] = 0;
   if (tid == 0) sdepth = -1;
@@ -905,7 +908,7 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
   const int row = blockIdx.x, chunks = a.chunks;
   const int64_t s0 = (int64_t)row * chunks;
   const float T = a.temperature[row], u = a.uniforms[row], top_p = a.top_p[row], min_p = a.min_p[row];
-  const int top_k = a.top_k[row];
+  const int top_k = top_k_under(min_p, a.top_k[row]);
   const bool filtered = top_k > 0 || !(top_p >= 1.f) || min_p > 0.f;
   u64 key = 0;
   SampleStat st{};

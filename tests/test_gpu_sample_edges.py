@@ -116,3 +116,26 @@ def test_min_p_alone_in_a_bin_of_many(kernel, crowd):
         for _ in range(20):
             again, lp = kernel.sample(*args)
             assert torch.equal(again, tokens) and torch.equal(lp.double().cpu(), logprobs)
+
+
+@pytest.mark.parametrize("vocab", [2, 300, 20000, 151936, 1 << 20])
+@pytest.mark.parametrize("equal", [2, 8, 5000])
+def test_min_p_above_1_leaves_the_likeliest_token(kernel, vocab, equal):
+    """No weight is above 1, so that of equal logits the lowest token stays alone; min_p of 1 keeps all of them."""
+    gen = torch.Generator().manual_seed(vocab + equal)
+    equal = min(equal, vocab)
+    at = torch.randperm(vocab, generator=gen)[:equal].sort().values
+    for value in (5.0, -3.4e38, 0.0):
+        x = torch.full((4, vocab), -INF)
+        if value == 5.0 and vocab > 2 * equal:
+            x = torch.randn(4, vocab, generator=gen).clamp(max=4.0)
+        x[:, at] = value
+        x = x.to(DEV)
+        u = torch.tensor([0.0, 0.6, 0.9, 1 - 2.0 ** -24], device=DEV)
+        for T, k, p in ((1.0, 0, 1.0), (0.5, 3, 1.0), (2.0, 0, 0.9), (1.0, 100000, 0.5)):
+            for m in (1.5, 1 + 2.0 ** -23, INF):
+                m = torch.full((4,), m, device=DEV)
+                tokens, logprobs = kernel.sample(x, u, torch.full_like(u, T), torch.full_like(u, k).int(),
+                                                 torch.full_like(u, p), m)
+                assert tokens.tolist() == [at[0].item()] * 4 and logprobs.tolist() == [0.0] * 4
+        check(kernel, x, u, 1.0, 0, 1.0, 1.0)
