@@ -557,6 +557,10 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attention_kernel(const Pa
 #pragma unroll
             for (int i = 0; i < QP; ++i) s[h] = mfma(f, qf[st][i], s[h]);
           }
+        if (t * TK + TK > len)  // keys past the last weigh nothing, whatever their scales have made of them
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (t * TK + 8 * g + j >= len) s[j >> 2][j & 3] = -INFINITY;
         if constexpr (QP > 1) {
           // Parts of a query may make NaN of an infinite key where the whole query makes an infinity: such scores are
           // made again, while the query's sum is not NaN already.
@@ -582,10 +586,6 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attention_kernel(const Pa
         float e[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) e[j] = s[j >> 2][j & 3] * C;
-        if (t * TK + TK > len)
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (t * TK + 8 * g + j >= len) e[j] = -INFINITY;
         float top = e[0];
 #pragma unroll
         for (int j = 1; j < 8; ++j) top = fmaxf(top, e[j]);

@@ -22,3 +22,35 @@ def test_attention_where_a_wave_has_one_tile(kernel, dtype, e4m3, lengths):
         for size in (33024 + 2 * 512 * 2 * 130 * 4, q.numel() * q.element_size()):  # the workspace's bytes and the output's
             torch.full((size // 4,), float("nan"), device=DEV)
         assert torch.equal(kernel.attention_paged(q, *pool.args(), n, *pool.scales()), first)
+
+
+def milliseconds(call):
+    """The least of eight measured runs of ten calls."""
+    best = float("inf")
+    for _ in range(8):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        for _ in range(10):
+            call()
+        b.record()
+        torch.cuda.synchronize()
+        best = min(best, a.elapsed_time(b) / 10)
+    return best
+
+
+@pytest.mark.parametrize("capacity", [512, 1024])
+def test_attention_takes_no_longer_for_what_is_behind_the_last_key(kernel, capacity):
+    """fp32 queries, 8-bit pages: a scale of NaN behind the last key makes NaN of scores that nobody asks for. None of them is
+    made again (when they were, calls like these took about twice as long)."""
+    gen = torch.Generator().manual_seed(capacity)
+    lengths = [8 * int(n) + 1 for n in torch.randint(8, capacity // 8 - 1, (256,), generator=gen)]
+    pool = Pool(256, capacity // 64, 64, 8, True, DEV)
+    q, n = queries(256, 16, torch.float32), ints(lengths)
+    call = lambda: kernel.attention_paged(q, *pool.args(), n, *pool.scales())  # noqa: E731
+    expected, before = call(), milliseconds(call)
+    for s, length in enumerate(lengths):
+        for scales in (pool.ks, pool.vs):
+            scales.view(torch.uint8)[pool.tables[s, length // 64].item(), :, length % 64:] = 255
+    assert torch.equal(call(), expected)
+    after = milliseconds(call)
+    assert after < 1.3 * before, (before, after)
