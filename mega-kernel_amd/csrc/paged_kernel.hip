@@ -731,37 +731,44 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attention_kernel(const Pa
 }
 
 // Joins the parts of the units that more than one workgroup worked on, in their order: a workgroup to `take` pairs of
-// (sequence, query head), a lane to look at each, and the whole of it to join the few that need it. Sequences without
-// keys get their answer here too.
+// (sequence, query head), a lane to look at each, and the whole of it to join the few that need it. The pairs of a workgroup lie
+// far apart, as all heads of a long sequence need it (one of 8,000 keys among 256 short ones 19 us, 41 with neighbours). Sequences
+// without keys get their answer here too.
 template <bool FP32>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedArgs a, int take) {
   __shared__ __attribute__((aligned(16))) float acc[8][D];
   __shared__ float accl[8], accm[8];
   const int tid = threadIdx.x, lane = tid & 63;
-  const int heads = a.hkv * a.g, gmax = min(a.g, NQ), first = blockIdx.x * take;
+  const int heads = a.hkv * a.g, gmax = min(a.g, NQ), step = gridDim.x, pairs = a.nseq * heads;
   int len = 0, w0 = 0, w1 = 0;
   bool some = false;
-  if (lane < take && first + lane < a.nseq * heads) {
-    const int b = (first + lane) / heads, h = (first + lane) % heads;
+  auto pair_of = [&](int e) { return (int)blockIdx.x + e * step; };
+  if (lane < take && pair_of(lane) < pairs) {
+    const int b = pair_of(lane) / heads, h = pair_of(lane) % heads;
     len = valid_length(a, b);
     const double per = a.base[a.nseq], cost = places_of(len);
     const double u0 = a.base[b] + (h / a.g * a.gt + h % a.g / NQ) * cost;
     w0 = (int)floor((u0 + START) / per);
     w1 = (int)floor((u0 + cost - 1) / per);
-    some = len == 0 || w0 != w1;
+    some = len > 0 && w0 != w1;
+  }
+  {  // sequences without keys, 16 lanes to a pair
+    const int e = tid >> 4, item = pair_of(e), keys = __shfl(len, e);
+    if (e < take && item < pairs && keys == 0) {
+      const float y = a.lengths[item / heads] == 0 ? 0.f : __builtin_nanf("");
+#pragma unroll
+      for (int i = 0; i < 8; i += 4)
+        store_out<FP32 ? 2 : 1>(a.out, (int64_t)item * D + 8 * (tid & 15) + i, make_float4(y, y, y, y));
+    }
   }
 #pragma unroll 1
   for (u64 todo = __builtin_amdgcn_ballot_w64(some); todo; todo &= todo - 1) {
-    const int e = __ffsll(todo) - 1, item = first + e;
+    const int e = __ffsll(todo) - 1, item = pair_of(e);
     const int64_t at = (int64_t)item * D + tid;
     auto store = [&](float x) {
       if constexpr (FP32) reinterpret_cast<float*>(a.out)[at] = x;
       else reinterpret_cast<uint16_t*>(a.out)[at] = f32_to_bf16(x);
     };
-    if (at_lane(len, e) == 0) {
-      if (tid < D) store(a.lengths[item / heads] == 0 ? 0.f : __builtin_nanf(""));
-      continue;
-    }
     const int v1 = at_lane(w1, e), vs = at_lane(w0, e), qi = item % heads % a.g % NQ;
     auto slot = [&](int v) { return a.part + ((int64_t)(2 * v + (v == vs)) * gmax + qi) * PART; };
     // 32 lanes to a part, eight parts of a lane at a time, so that their loads are made together
@@ -970,7 +977,7 @@ extern "C" size_t mk_attention_paged_workspace_bytes(int q_heads, int kv_heads) 
 }
 
 // Up to this many pairs of (sequence, query head) the join takes a workgroup to each, then one to 16, as few of them need
-// one. Measured, 1 and 16: 4,096 pairs 6.3 and 8.4 us, 8,192 9.8 and 6.5, 16,384 15.6 and 5.1, 65,536 49 and 7.5.
+// one. Measured, 1 and 16: 4,096 pairs 6.3 and 9.2 us, 8,192 9.8 and 6.3, 16,384 15.6 and 7.0, 65,536 49 and 7.5.
 constexpr int JOIN_WGS = 4096;
 template <bool E4M3, int QP, int PP, int PG>
 static void launch_paged(const PagedArgs& a, hipStream_t stream) {

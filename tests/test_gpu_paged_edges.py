@@ -54,3 +54,36 @@ def test_attention_takes_no_longer_for_what_is_behind_the_last_key(kernel, capac
     assert torch.equal(call(), expected)
     after = milliseconds(call)
     assert after < 1.3 * before, (before, after)
+
+
+@KINDS
+@pytest.mark.parametrize("hq,hkv,seqs", [(16, 8, 300), (40, 2, 110), (5, 1, 900), (16, 8, 4096)])
+def test_attention_of_few_sequences_among_free_places(kernel, dtype, hq, hkv, seqs):
+    """More pairs of sequence and head than the join takes one by one, most of them without keys, some lengths out of range."""
+    pool = Pool(8, 130, 16, hkv, False, DEV, seed=seqs)
+    used = {0: 2000, 1: 1, 2: 1500, seqs // 2: 700, seqs - 2: 2080, seqs - 1: 33}
+    lengths = [0] * seqs
+    table = pool.tables[:1].repeat(seqs, 1)
+    for i, (s, n) in enumerate(used.items()):
+        lengths[s] = n
+        table[s] = pool.tables[i]
+    pool.tables = table
+    q = queries(seqs, hq, dtype)
+    got = check(kernel, pool, q, lengths)
+    bad = list(lengths)
+    bad[3], bad[seqs // 3], bad[seqs - 3] = -1, 2081, 2 ** 31 - 1
+    again = kernel.attention_paged(q, *pool.args(), ints(bad))
+    out = torch.tensor([n != m for n, m in zip(lengths, bad)], device=DEV)
+    assert again[out].isnan().all() and torch.equal(again[~out], got[~out])
+
+
+def test_attention_of_a_long_sequence_among_many_places(kernel):
+    """The heads of a sequence of many keys are joined side by side, however many places there are besides (one after the other,
+    512 places took three times as long as 64)."""
+    pool = Pool(1, 256, 16, 8, False, DEV)
+    took = []
+    for seqs in (64, 512):
+        q, n = queries(seqs, 16, torch.float32), ints([4000] + [0] * (seqs - 1))
+        tables = pool.tables.repeat(seqs, 1)
+        took.append(milliseconds(lambda: kernel.attention_paged(q, pool.k, pool.v, tables, n)))
+    assert took[1] < 1.8 * took[0], took
