@@ -183,7 +183,12 @@ __device__ __forceinline__ uint4 bf16x8_of_e4m3(uint32_t a, uint32_t b, float sc
   return make_uint4(bf16_of_e4m3<false>(a, scale), bf16_of_e4m3<true>(a, scale), bf16_of_e4m3<false>(b, scale),
                     bf16_of_e4m3<true>(b, scale));
 }
+// What the conversion takes as a scale, of which it looks at the exponent alone: 0 is 2^-127, an infinity makes NaN.
 __device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+// The number that the byte of a scale is.
+__device__ __forceinline__ float unit_of(uint32_t byte) {
+  return byte == 255 ? __builtin_nanf("") : byte == 0 ? 0x1p-127f : __uint_as_float(byte << 23);
+}
 
 template <bool E4M3>
 __global__ void __launch_bounds__(256) cache_read_kernel(const CacheArgs a) {
@@ -300,11 +305,11 @@ __device__ __forceinline__ uint32_t byte_of(uint32_t w, int i) { return w >> (8 
 
 // One score in fp32 from the whole query: see the NaN of parts below.
 template <bool E4M3>
-__device__ __attribute__((noinline)) float whole_score(const uint8_t* k, float scale, const float* q) {
+__device__ __attribute__((noinline)) float whole_score(const uint8_t* k, float unit, const float* q) {
   float s = 0.f;
   for (int d = 0; d < D; ++d) {
     float x;
-    if constexpr (E4M3) x = __builtin_amdgcn_cvt_f32_fp8((int)k[d], 0) * scale;
+    if constexpr (E4M3) x = __builtin_amdgcn_cvt_f32_fp8((int)k[d], 0) * unit;
     else x = bf16_to_f32(reinterpret_cast<const uint16_t*>(k)[d]);
     s = fmaf(q[d], x, s);
   }
@@ -573,7 +578,7 @@ __global__ void __launch_bounds__(64 * WAVES, 2) paged_attention_kernel(const Pa
               int64_t at, sat;
               place(t, 8 * g + j, at, sat);
               if (n < nq && l == l && s[j >> 2][j & 3] != s[j >> 2][j & 3])
-                s[j >> 2][j & 3] = whole_score<E4M3>(kbase + at, E4M3 ? scale_of(ksb[sat]) : 1.f,
+                s[j >> 2][j & 3] = whole_score<E4M3>(kbase + at, E4M3 ? unit_of(ksb[sat]) : 1.f,
                                                      reinterpret_cast<const float*>(qrow));
             }
           }

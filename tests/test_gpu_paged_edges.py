@@ -1,9 +1,11 @@
 """``attention_paged`` and the paged cache on the GPU where shares of the work, scales and rows end in unusual places, against
 the definitions in 64 bits (``paged_pool``; the tolerances are derived in ``test_gpu_paged``)."""
+import math
+
 import pytest
 import torch
 
-from paged_pool import Pool
+from paged_pool import D, Pool
 from test_gpu_paged import DEV, KINDS, PAGES, check, ints, queries
 
 pytestmark = pytest.mark.gpu
@@ -87,3 +89,47 @@ def test_attention_of_a_long_sequence_among_many_places(kernel):
         tables = pool.tables.repeat(seqs, 1)
         took.append(milliseconds(lambda: kernel.attention_paged(q, pool.k, pool.v, tables, n)))
     assert took[1] < 1.8 * took[0], took
+
+
+def test_scales_that_cache_write_does_not_make(kernel):
+    """Bytes 0 .. 9 and 255 of the scales: powers of two down to 2^-127, and rows of NaN whatever their values are."""
+    numbers = torch.arange(256, dtype=torch.uint8, device=DEV).view(2, D)
+    units = torch.tensor([*range(12), 255], dtype=torch.uint8, device=DEV)
+    pool = Pool(len(units), 2, 32, 2, True, DEV, fill=False)
+    at = pool.tables[:, 0].long()
+    for pages, scales in ((pool.k, pool.ks), (pool.v, pool.vs)):
+        pages.view(torch.uint8)[at, :, 3] = numbers
+        scales.view(torch.uint8)[at, :, 3] = units[:, None]
+    k, v = kernel.cache_read(*pool.args(), ints([3] * len(units)), [1] * len(units), *pool.scales())
+    expected = numbers.view(torch.float8_e4m3fn).double() * torch.exp2(units.double() - 127)[:, None, None]
+    expected[-1] = math.nan
+    for x in (k, v):
+        assert torch.equal(x.isnan(), expected.isnan())
+        # bf16's rounding, and its numbers below 2^-126, 2^-133 apart
+        assert ((x.double() - expected).abs() <= 2.0 ** -134).logical_or(expected.isnan()).all()
+
+
+@KINDS
+@pytest.mark.parametrize("entries", [8, 64])
+@pytest.mark.parametrize("page_size", [4, 8, 64])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_attention_of_rows_whose_scale_is_nan(kernel, dtype, entries, page_size, sign):
+    """A scale of 255 is a row of NaN, however its finite values and the query would add up."""
+    pool = Pool(3, entries * 64 // page_size, page_size, 2, True, DEV)
+    lengths = [300, 45, 64]
+    q = queries(3, 8, dtype).abs() * sign
+    plain = check(kernel, pool, q, lengths)
+    for which in "kv":
+        pages, scales = (pool.k, pool.ks) if which == "k" else (pool.v, pool.vs)
+        for s, p, head in ((0, 123, 1), (1, 44, 0), (2, 0, 1)):
+            page, row = pool.tables[s, p // page_size].item(), p % page_size
+            kept = pages.view(torch.uint8)[page, head, row].clone(), scales.view(torch.uint8)[page, head, row].item()
+            pages.view(torch.uint8)[page, head, row] = 0x38  # 1
+            for byte in (255, 127):
+                scales.view(torch.uint8)[page, head, row] = byte
+                got = kernel.attention_paged(q, *pool.args(), ints(lengths), *pool.scales())
+                hit = torch.zeros_like(got, dtype=torch.bool)
+                hit[s, 4 * head:4 * head + 4] = True
+                assert torch.equal(got[~hit], plain[~hit])
+                assert got[hit].isnan().all() if byte == 255 else got[hit].isfinite().all()
+            pages.view(torch.uint8)[page, head, row], scales.view(torch.uint8)[page, head, row] = kept
