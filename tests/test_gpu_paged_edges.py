@@ -5,8 +5,8 @@ import math
 import pytest
 import torch
 
-from paged_pool import D, Pool
-from test_gpu_paged import DEV, KINDS, PAGES, check, ints, queries
+from paged_pool import E8, D, Pool
+from test_gpu_paged import DEV, KINDS, PAGES, check, ints, queries, write_and_check
 
 pytestmark = pytest.mark.gpu
 
@@ -133,3 +133,82 @@ def test_attention_of_rows_whose_scale_is_nan(kernel, dtype, entries, page_size,
                 assert torch.equal(got[~hit], plain[~hit])
                 assert got[hit].isnan().all() if byte == 255 else got[hit].isfinite().all()
             pages.view(torch.uint8)[page, head, row], scales.view(torch.uint8)[page, head, row] = kept
+
+
+def loose_scales(pool, first, between):
+    """pool's scales as slices of wider ones: `first` bytes before each head's, `between` bytes in all besides them."""
+    made = []
+    for scales in (pool.ks, pool.vs):
+        n, h, p = scales.shape
+        wide = torch.full((n, h, p + between), 255, dtype=torch.uint8, device=DEV)
+        wide[..., first:first + p] = scales.view(torch.uint8)
+        made.append(wide[..., first:first + p].view(E8))
+    pool.ks, pool.vs = made
+
+
+@KINDS
+@pytest.mark.parametrize("page_size", [8, 16, 64])
+@pytest.mark.parametrize("first,between", [(0, 1), (1, 3), (4, 8), (0, 8), (3, 20)])
+def test_scales_at_any_byte(kernel, dtype, page_size, first, between):
+    """Scales whose 8 bytes of 8 rows are not one aligned number, and (0, 8) ones that are, with others between the heads."""
+    lengths = [70, 0, 1, 500, 33]
+    for capacity in (512, 1024):
+        pool = Pool(len(lengths), capacity // page_size, page_size, 8, True, DEV, seed=page_size)
+        q = queries(len(lengths), 16, dtype)
+        plain = check(kernel, pool, q, lengths)
+        loose_scales(pool, first, between)
+        got = check(kernel, pool, q, lengths)
+        assert torch.equal(got, plain)
+    rows = torch.randn(60, 8, D, generator=torch.Generator(device=DEV).manual_seed(first), device=DEV).to(dtype)
+    at = [(0, 5 + i) for i in range(40)] + [(3, 100 + i) for i in range(20)]
+    write_and_check(kernel, pool, rows, rows.flip(0), ints([5, 0, 0, 100, 0]), [40, 0, 0, 20, 0], at)
+    k, _ = kernel.cache_read(*pool.args(), ints([5, 0, 0, 100, 0]), [40, 0, 0, 20, 0], *pool.scales())
+    assert torch.equal(k.double(), torch.cat([pool.rows("k", 0, 5, 40), pool.rows("k", 3, 100, 20)]))
+
+
+@KINDS
+@PAGES
+@pytest.mark.parametrize("heads", [9, 16, 17, 40])
+def test_cache_of_more_than_8_heads(kernel, dtype, e4m3, heads):
+    """More rows to a position than a wave has in flight."""
+    pool = Pool(3, 4, 16, heads, e4m3, DEV, "rows", seed=heads)
+    lengths, begin = [20, 0, 7], [3, 0, 60]
+    rows = torch.randn(27, 2 * heads, D, generator=torch.Generator(device=DEV).manual_seed(heads), device=DEV)
+    rows = (rows * torch.exp2(torch.arange(2 * heads, device=DEV) % 13 - 6)[:, None]).to(dtype)
+    at = [(s, b + i) if b + i < 64 else None for s, (b, n) in enumerate(zip(begin, lengths)) for i in range(n)]
+    write_and_check(kernel, pool, rows[:, :heads], rows[:, heads:], ints(begin), lengths, at)
+    k, v = kernel.cache_read(*pool.args(), ints([0, 0, 60]), [23, 0, 4], *pool.scales())
+    for got, which in ((k, "k"), (v, "v")):
+        assert torch.equal(got.double(), torch.cat([pool.rows(which, 0, 0, 23), pool.rows(which, 2, 60, 4)]))
+
+
+@KINDS
+@PAGES
+@pytest.mark.parametrize("capacity", [512, 1024])
+def test_attention_whose_last_key_is_not_finite(kernel, dtype, e4m3, capacity):
+    """The last key of a tile that ends there stands in for those behind it, which have no weight: an infinite or NaN value of
+    its reaches its own elements alone, a key of NaN its head's, a key of -infinity nothing."""
+    pool = Pool(3, capacity // 16, 16, 2, e4m3, DEV)
+    lengths = [201, 33, 1]
+    q = queries(3, 8, dtype).abs()
+    plain = check(kernel, pool, q, lengths)
+    bads = [(0x7f, math.nan)] if e4m3 else [(None, math.nan), (None, math.inf), (None, -math.inf)]
+    for s, n in enumerate(lengths):
+        page, row = pool.tables[s, (n - 1) // 16].item(), (n - 1) % 16
+        for byte, bad in bads:
+            for pages in (pool.v, pool.k):
+                place = pages.view(torch.uint8)[page, 1, row, 9:10] if e4m3 else pages[page, 1, row, 9:10]
+                kept = place.clone()
+                place.fill_(byte if e4m3 else bad)
+                got = kernel.attention_paged(q, *pool.args(), ints(lengths), *pool.scales())
+                hit = torch.zeros_like(got, dtype=torch.bool)
+                if pages is pool.v:
+                    hit[s, 4:, 9] = True
+                else:
+                    hit[s, 4:] = True
+                assert torch.equal(got[~hit], plain[~hit])
+                if pages is pool.k and bad == -math.inf and n > 1:  # no weight: as without it
+                    check(kernel, pool, q, lengths)
+                else:
+                    assert not got[hit].isfinite().any()
+                place.copy_(kept)
