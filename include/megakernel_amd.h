@@ -373,7 +373,8 @@ hipError_t mk_attention_paged(const mk_paged_cache* cache, int q_heads, const vo
  * that order, the fewest whose w add up to at least top_p of the candidates' sum (top_p >= 1: all); and of these
  * those with w >= min_p (min_p <= 0: all). The likeliest token always stays. The answer is the first token, in the
  * order of the vocabulary, at which the running sum of the candidates' w is above u times their whole sum, the last one
- * if none is. T = 0: the likeliest token. All in 64 bits: sums within 2^-42 of each other count as equal.
+ * if none is. T = 0: the likeliest token. All in 64 bits: sums within 2^-42 of each other count as equal, and a w below
+ * 2^-1000 is 0.
  *   logits     fp32, row r at logits + r * row_stride (elements, >= 0), vocab (1..2^20) of them
  *   uniforms   [rows] fp32, u in [0, 1)
  *   temperature, top_k, top_p, min_p     [rows] fp32, int32, fp32, fp32

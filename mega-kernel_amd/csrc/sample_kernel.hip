@@ -107,9 +107,12 @@ __device__ __forceinline__ Scale scale_of_row(float T, double top) {
   s.in = fabs(top * s.c) < 0x1p45 ? 1.0 : 0.0;
   return s;
 }
+// Bins from the largest logit's down to which there are weights, a factor of 2^1000: what lies lower is 0, everywhere, so that a
+// chunk whose sum is not 0 has a logit that is drawn, and no weight is too small for a double's full precision.
+constexpr double DEEPEST = 1000 * RES;
 // 2^(-k / RES) for a whole number k >= 0, to 2^-51 of itself
 __device__ __forceinline__ double bin_weight(double k) {
-  k = fmin(k, 2.0e4);  // 0 from about 11,800 on
+  if (!(k <= DEEPEST)) return 0;
   const double q = floor(k * (1.0 / RES) + 1.0 / (2 * RES));
   const int i = (int)(k - q * RES);  // its powers of 2: 2^(-2^b / 11)
   double y = i & 1 ? 0x1.e0bb8d64fdb5ap-1 : 1.0;
@@ -145,10 +148,11 @@ __device__ __forceinline__ u64 fixed_in_bin(float x, const Scale& s, double fl) 
   y = fma(y, f, A);
   return __builtin_bit_cast(u64, fma(y, f, 1 + BIG)) - __builtin_bit_cast(u64, BIG);
 }
-// 2^(t / 11) for t <= 0 to fp32's accuracy, over the doubles' range: the tail's weights, below 2^-46 of the largest
+// 2^(t / 11) for t <= 0 to fp32's accuracy: the tail's weights, below 2^-46 of the largest
 __device__ __forceinline__ double exp_tail(double t) {
-  const double p = t * (1.0 / RES), n = floor(fmax(p, -1100.0));
-  return ldexp((double)__builtin_amdgcn_exp2f((float)fmax(p - n, 0.0)), (int)n);
+  if (!(t >= -DEEPEST)) return 0;
+  const double p = t * (1.0 / RES), n = floor(p);
+  return ldexp((double)__builtin_amdgcn_exp2f((float)(p - n)), (int)n);
 }
 // the bin of floor(p) below `ref`, the tail's for all from there on
 __device__ __forceinline__ int bin_of(double ref, double fl) {
@@ -438,7 +442,7 @@ __device__ __forceinline__ int border_bin(bool by_rank, int rank, double goal) {
 // The weight of a logit of the row's bin j, in 2^-FIX of 2^(-j / 11).
 __device__ __forceinline__ u64 fixed_weight(const Scale& s, double ref, float x, int j) {
   const double p = (double)x * s.c, fl = floor(p);
-  if (j == NB - 1) return (u64)(exp_tail(p - ref + (NB - 1)) * ONE);
+  if (j == NB - 1) return (u64)ceil(exp_tail(p - ref) * (ONE / smem().et[NB - 1]));  // (0 for a weight of 0 alone)
   return fixed_in_bin(x, s, fl);
 }
 

@@ -22,6 +22,12 @@ def poisoned(kernel, *args):
     return check(kernel, *args)
 
 
+def poisoned_call(kernel, *args):
+    n = args[0].shape[0]
+    torch.full((n,), -7, dtype=torch.int32, device=DEV), torch.full((n,), math.nan, device=DEV)
+    return kernel.sample(*args)
+
+
 def apart(u, x, T=1.0):
     """The numbers of u whose share of the weights' sum is no nearer than 2^-34 of itself to a running sum."""
     w = torch.exp((x.double() - x.max().double()) / T)
@@ -139,3 +145,33 @@ def test_min_p_above_1_leaves_the_likeliest_token(kernel, vocab, equal):
                                                  torch.full_like(u, p), m)
                 assert tokens.tolist() == [at[0].item()] * 4 and logprobs.tolist() == [0.0] * 4
         check(kernel, x, u, 1.0, 0, 1.0, 1.0)
+
+
+@pytest.mark.parametrize("vocab", [300, 8192, 8193, 28373])
+@pytest.mark.parametrize("k,p,m", [(0, 1.0, 0.0), (250, 1.0, 0.0), (50, 1.0, 0.0), (8000, 0.9999999, 0.0), (0, 1.0, 1e-44)])
+def test_the_smallest_weights(kernel, vocab, k, p, m):
+    """u = 0 asks for the first candidate of any weight, which a weight of at least 2^-1000 of the largest is; a row of many
+    that are less, whose sum is more, has an answer too."""
+    steps = torch.tensor([1.0, 0.7, 3.0, 13.0, 690.0])
+    x = (-steps[:, None] * torch.arange(vocab).float().flip(0)).to(DEV)
+    near = torch.full((4, vocab), -INF, device=DEV)  # below 2^-1000, next to it and above, most of a chunk of them
+    near[:, :vocab - 40] = torch.tensor([-694.0, -693.2, -693.0, -744.0], device=DEV)[:, None]
+    near[:, vocab - 1] = 0.0
+    x = torch.cat([x, near])
+    n = len(x)
+    T = rows(1.0, n)
+    tokens, logprobs = poisoned_call(kernel, x, rows(0.0, n), T, rows(k, n, torch.int32), rows(p, n), rows(m, n))
+    for r in range(n):
+        z, order = torch.sort(x[r].double() - x[r].max().double(), descending=True, stable=True)
+        kept = z[:k] if k > 0 else z
+        if p < 1:
+            w = kept.exp().cumsum(0)
+            share = torch.tensor(p).double().item()  # top_p is single precision
+            kept = kept[:int(torch.nonzero(w >= share * w[-1] * (1 - 2.0 ** -42))[0]) + 1]
+        if m > 0:
+            kept = kept[kept >= torch.tensor(m).double().log().item()]
+        kept = kept[kept >= -1000 * math.log(2)]
+        first = order[:len(kept)].min().item()
+        assert tokens[r] == first, (r, tokens[r], first)
+        want = (x[r, first].double() - x[r].max().double()).item() - kept.exp().sum().log().item()
+        assert abs(logprobs[r].item() - want) <= 2.0 ** -24 * abs(want) + 2.0 ** -22, (r, logprobs[r], want)
