@@ -355,7 +355,7 @@ hipError_t mk_cache_read(const mk_paged_cache* cache, const int32_t* begin, cons
  *            the caller, not used after the call's work completes on `stream`
  * A table entry outside [0, num_pages) among a sequence's makes its output NaN (page 0 is read in its place);
  * entries past its last page are not looked at, nor is a row past its last key. fp32 queries: products at fp32
- * accuracy. bf16 queries: the weights are products' operands of 16 bits, everything else fp32. An infinite or NaN
+ * accuracy. bf16 queries: their products are exact, the weights' at fp32 accuracy. An infinite or NaN
  * value makes the elements of its sequence's output that it is a part of infinite or NaN; a row whose scores are all
  * -infinity is NaN. The split of the work, and so the order of a sequence's sums, goes by all the lengths; the
  * same call gives the same bits. Asynchronous on `stream`; argument errors return hipErrorInvalidValue before any

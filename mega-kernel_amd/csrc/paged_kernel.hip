@@ -332,13 +332,17 @@ __device__ __forceinline__ void store_out(uint8_t* out, int64_t at, float4 y) { 
   else *reinterpret_cast<float4*>(out + 4 * at) = y;
 }
 
-// E4M3: 8-bit pages. QP, PP: bf16 parts of a query and of a weight (1 and 2 for bf16 queries, 3 for fp32 ones).
+// A weight goes into its product in this many bf16 parts, 24 bits. (Two of them, 2^-17 of a weight lost: 64 sequences of 900 to
+// 4,095 keys 0.3% faster in bf16 pages and 2.5% in 8-bit ones, but 0.2% of bf16 outputs round to another side.)
+constexpr int PP = 3;
+
+// E4M3: 8-bit pages. QP: bf16 parts of a query (1 for bf16 queries, 3 for fp32 ones).
 // PG: 2, a tile lies in one page (8-bit pages: one look-up and one address for all scales, 22.7 us instead of 23.6 for 64
 // sequences of 256 to 1,024 keys; bf16 pages gain nothing and take 1); 1, each 8 keys of it do; 0, pages are looked up key
 // by key (13 sequences of 128 to 512 keys 10.5 us instead of 9.6, 8-bit pages of 8 keys 25.9 instead of 24.4).
 // SPLIT: the tiles of all units are shared out evenly, a unit's parts joined by paged_join_kernel; else a workgroup takes a
 // unit, a wave a run of its tiles.
-template <bool E4M3, int QP, int PP, int PG, bool SPLIT>
+template <bool E4M3, int QP, int PG, bool SPLIT>
 __global__ void __launch_bounds__(64 * WAVES, 2) paged_attention_kernel(const PagedArgs a) {
   __shared__ PagedSmem sm;
   extern __shared__ __attribute__((aligned(16))) float outs[];  // [pieces][queries of a unit][OROW]
@@ -984,14 +988,14 @@ extern "C" size_t mk_attention_paged_workspace_bytes(int q_heads, int kv_heads) 
 // Up to this many pairs of (sequence, query head) the join takes a workgroup to each, then one to 16, as few of them need
 // one. Measured, 1 and 16: 4,096 pairs 6.3 and 9.2 us, 8,192 9.8 and 6.3, 16,384 15.6 and 7.0, 65,536 49 and 7.5.
 constexpr int JOIN_WGS = 4096;
-template <bool E4M3, int QP, int PP, int PG>
+template <bool E4M3, int QP, int PG>
 static void launch_paged(const PagedArgs& a, hipStream_t stream) {
   const unsigned units = (unsigned)((int64_t)a.nseq * a.hkv * a.gt);
   const unsigned lds = 2 * WAVES * std::min(a.g, NQ) * OROW * sizeof(float);
   if (!paged_split(a.capacity)) {
-    hipLaunchKernelGGL((paged_attention_kernel<E4M3, QP, PP, PG, false>), dim3(units), dim3(64 * WAVES), lds, stream, a);
+    hipLaunchKernelGGL((paged_attention_kernel<E4M3, QP, PG, false>), dim3(units), dim3(64 * WAVES), lds, stream, a);
   } else {
-    hipLaunchKernelGGL((paged_attention_kernel<E4M3, QP, PP, PG, true>), dim3(PAGED_WGS), dim3(64 * WAVES), lds, stream, a);
+    hipLaunchKernelGGL((paged_attention_kernel<E4M3, QP, PG, true>), dim3(PAGED_WGS), dim3(64 * WAVES), lds, stream, a);
     const int pairs = a.nseq * a.hkv * a.g, take = pairs > JOIN_WGS ? 16 : 1;
     hipLaunchKernelGGL(paged_join_kernel<(QP > 1)>, dim3((pairs + take - 1) / take), dim3(256), 0, stream, a, take);
   }
@@ -1024,19 +1028,15 @@ extern "C" hipError_t mk_attention_paged(const mk_paged_cache* cache, int q_head
   // the keys of a tile that surely share a page, and scales that can be loaded 8 at a time
   int pg = a.p.ks && cache->page_size >= TK ? 2 : cache->page_size >= 8 ? 1 : 0;
   if (a.p.ks && (!aligned_to(a.p.ks, 8) || !aligned_to(a.p.vs, 8) || a.p.spage % 8 != 0 || a.p.shead % 8 != 0)) pg = 0;
-  auto launch = [&](auto e4m3, auto qp, auto pp) {
+  auto launch = [&](auto e4m3, auto qp) {
     if constexpr (e4m3.value)
-      if (pg == 2) return launch_paged<true, qp.value, pp.value, 2>(a, stream);
-    if (pg == 1) launch_paged<e4m3.value, qp.value, pp.value, 1>(a, stream);
-    else launch_paged<e4m3.value, qp.value, pp.value, 0>(a, stream);
+      if (pg == 2) return launch_paged<true, qp.value, 2>(a, stream);
+    if (pg == 1) launch_paged<e4m3.value, qp.value, 1>(a, stream);
+    else launch_paged<e4m3.value, qp.value, 0>(a, stream);
   };
-  using std::integral_constant;
-  if (a.p.ks) {
-    if (q_fp32) launch(std::true_type(), integral_constant<int, 3>(), integral_constant<int, 3>());
-    else launch(std::true_type(), integral_constant<int, 1>(), integral_constant<int, 2>());
-  } else {
-    if (q_fp32) launch(std::false_type(), integral_constant<int, 3>(), integral_constant<int, 3>());
-    else launch(std::false_type(), integral_constant<int, 1>(), integral_constant<int, 2>());
-  }
+  constexpr std::integral_constant<int, 1> bf16;
+  constexpr std::integral_constant<int, 3> fp32;
+  if (a.p.ks) q_fp32 ? launch(std::true_type(), fp32) : launch(std::true_type(), bf16);
+  else q_fp32 ? launch(std::false_type(), fp32) : launch(std::false_type(), bf16);
   return hipGetLastError();
 }

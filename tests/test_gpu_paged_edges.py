@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from paged_pool import E8, D, Pool
+from paged_pool import E8, D, Pool, attention
 from test_gpu_paged import DEV, KINDS, PAGES, check, ints, queries, write_and_check
 
 pytestmark = pytest.mark.gpu
@@ -212,3 +212,19 @@ def test_attention_whose_last_key_is_not_finite(kernel, dtype, e4m3, capacity):
                 else:
                     assert not got[hit].isfinite().any()
                 place.copy_(kept)
+
+
+@PAGES
+def test_attention_of_bf16_queries_is_rounded_once(kernel, e4m3):
+    """Scores and weights of 24 bits, a score off by about 2^-22: outputs of many keys, errors of either sign like the sum's own
+    terms, are off by about 2^-22 of themselves before they are rounded, next to steps of 2^-8 to 2^-7. So about 2^-13 of them
+    round to the other side of 64 bits' result; four times as many are allowed. (Weights of 16 bits: sixteen
+    times as many of bf16 pages.)"""
+    lengths = [2000, 1333, 900, 513] * 4
+    pool = Pool(len(lengths), 2048 // 64, 64, 8, e4m3, DEV)
+    q = queries(len(lengths), 16, torch.bfloat16)
+    got = check(kernel, pool, q, lengths)
+    exact, _ = attention(pool, q, lengths)
+    other = (got != exact.to(torch.bfloat16)).double().mean().item()
+    print(f"[paged] the other side: {other:.2e}")
+    assert other < 2.0 ** -11
