@@ -399,7 +399,7 @@ struct PickSmem {
   double wsum[SW];
   int32_t wcount[SW];
   u64 wfix[SW], wfix2[SW];
-  int first[SW], last[SW];
+  int first, last;  // of the answer's candidates
   int found, border, n, above, depth, number;
   u64 sum, key;
   uint32_t klo, khi;
@@ -649,7 +649,7 @@ __device__ __forceinline__ bool gather_bin(const Row& r, const uint8_t* codes, i
       const int at = base + i * ST + tid, k = j - sm.delta[min(at / (SC / 16), chunks - 1)];  // the chunk's bin
       if (at >= units || k < 0) continue;
       const uint32_t code = (uint32_t)(k >> 1) * 0x01010101u, w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
-      uint32_t mask = 0;  // bit 4 byte + word: a byte that is the code
+      uint32_t mask = 0;  // bit 8 byte + word: a byte that is the code
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t y = w[e] ^ code, z = ~(((y & 0x7f7f7f7fu) + 0x7f7f7f7fu) | y) & 0x80808080u;
@@ -783,7 +783,8 @@ __device__ __forceinline__ u64 border_in_bin(const Row& r, const uint8_t* codes,
   return sm.sum;
 }
 
-// The border by all filters, into sm.cut, and the chunks' sums of what is kept, into sm.csum.
+// The border by all filters, one of which has to leave something out, into sm.cut, and the chunks' sums of what is kept, into
+// sm.csum.
 __device__ __forceinline__ void deep_cut(const u64* bins, const SampleStat* stat,
                                                    const uint8_t* codes, int chunks, const float* x,
                                                    int vocab, double c, double in, double ref, uint32_t ktop, int number,
@@ -868,7 +869,6 @@ __device__ __forceinline__ void deep_cut(const u64* bins, const SampleStat* stat
   }
   if (jm < cut.bin || (jm == cut.bin && (!cut.part || xm > cut.x))) cut = {jm, true, xm, INT32_MAX};
   if (tid == 0) sm.cut = cut;
-  if (!cut.part) return;  // everything
   {  // the kept weights of the border's bin
     const int j = cut.bin, n = sm.cupto[j] - number_below(j);
     if (n <= CAP) {
@@ -1083,8 +1083,8 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
       sm.found = 2 * lane + second;
       sm.goal = fmax(goal - (second ? before + c0 : before), 0.0);  // (the sums before it may have been rounded up)
       sm.z = z;
-      sm.first[0] = INT32_MAX;
-      sm.last[0] = -1;
+      sm.first = INT32_MAX;
+      sm.last = -1;
     }
   }
   __syncthreads();
@@ -1112,9 +1112,9 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
     double all;
     // the first one whose running sum exceeds the goal, the last one if none does
     const u64 hit = __builtin_amdgcn_ballot_w64(block_upto<SW>(weight, sm.wsum, all) > goal && tid < n);
-    if (hit && lane == __ffsll(hit) - 1) atomicMin(&sm.first[0], tid);
+    if (hit && lane == __ffsll(hit) - 1) atomicMin(&sm.first, tid);
     __syncthreads();
-    if (tid == min(sm.first[0], n - 1)) {
+    if (tid == min(sm.first, n - 1)) {
       a.tokens[row] = sm.token[tid];
       if (a.logprobs) a.logprobs[row] = (float)fmin(log64(weight / z), 0.0);
     }
@@ -1156,7 +1156,7 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
   double run = __shfl_up(upto, 1);
   if (lane == 0) run = waves;
   const u64 some = __builtin_amdgcn_ballot_w64(last >= 0);
-  if (some && lane == 63 - __clzll(some)) atomicMax(&sm.last[0], last);
+  if (some && lane == 63 - __clzll(some)) atomicMax(&sm.last, last);
   // Sums in another order may differ in their last digits: a little more than the thread that has it, so that one of these has
   // it wherever the goal is below all of them.
   const bool here = mine > 0 && (run + mine) * (1 + SAME) > goal && run * (1 - SAME) <= goal;
@@ -1169,9 +1169,9 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
       if (here && s > 0 && run > goal) hit = min(hit, v0 + q);
     }
   }
-  if (hit < INT32_MAX) atomicMin(&sm.first[0], hit);
+  if (hit < INT32_MAX) atomicMin(&sm.first, hit);
   __syncthreads();
-  const int v = sm.first[0] < INT32_MAX ? sm.first[0] : sm.last[0];
+  const int v = sm.first < INT32_MAX ? sm.first : sm.last;
   if (v >= v0 && v < v0 + 8) {
     a.tokens[row] = v;
     if (a.logprobs) a.logprobs[row] = (float)fmin(log64(weights[(v - v0) * ST] / z), 0.0);
