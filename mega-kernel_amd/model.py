@@ -116,6 +116,8 @@ def sample_texts(kernel, prompts, new, eos, temperature, top_k, top_p, min_p, se
     k, v = (torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in range(2))
     packed = torch.tensor([t for p in prompts for t in p], dtype=torch.int32, device=dev)
     weights = (embed, embed, final_norm, layer_weights, cos, sin)
+    # the largest of their types where they are larger: as good as no limit, as even weights as can be
+    temperature, top_k = min(temperature, torch.finfo(torch.float32).max), min(top_k, 2 ** 31 - 1)
     settings = [torch.full((rows,), x, dtype=t, device=dev) for x, t in (
         (temperature, torch.float32), (top_k, torch.int32), (top_p, torch.float32), (min_p, torch.float32))]
     numbers = torch.rand(new, rows, generator=torch.Generator().manual_seed(seed)).to(dev)
