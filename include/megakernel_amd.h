@@ -296,8 +296,8 @@ hipError_t mk_beam_reorder(int num_layers, int rows, int beams, int max_seq_len,
  *   k_pages, v_pages   row r of K/V head h of page i at i * page_stride + h * head_stride + r * row_stride
  *                      (elements, the same for both, >= 0; multiples of 8, of 16 for 8-bit pages; row_stride at
  *                      most 2^24), 128
- *                      numbers; 16-byte aligned. [num_pages][kv_heads][page_size][128], one layer of
- *                      mk_decode_paged's pools, is the plain case
+ *                      numbers; 16-byte aligned; no number of one may be one of the other's.
+ *                      [num_pages][kv_heads][page_size][128], one layer of mk_decode_paged's pools, is the plain case
  *   k_scales, v_scales NULL: the pages are bf16. Otherwise they are e4m3 (OCP), and the number of a row is its
  *                      value times 2^(b - 127), b the byte at i * scale_page_stride + h * scale_head_stride + r
  *                      (e8m0; 255: the row is NaN, and so are its values)
@@ -338,7 +338,8 @@ hipError_t mk_cache_write(const mk_paged_cache* cache, const void* k, int64_t k_
  * Reads rows of a paged cache back: positions begin[s] .. begin[s] + lengths[s] - 1 of every sequence, one
  * sequence after the other, into k and v, bf16 [rows][kv_heads][128] (16-byte aligned; they may overlap nothing else).
  * Exact for what mk_cache_write has written: an e4m3 value times its power of two is a bf16 number (only 2^128, to
- * which magnitudes from 3.29e38 on are rounded, is an infinity). A position or table entry out of range reads as NaN. Arguments, errors and asynchrony as mk_cache_write.
+ * which magnitudes from 3.29e38 on are rounded, is an infinity). A position or table entry out of range reads as NaN.
+ * Arguments, errors and asynchrony as mk_cache_write.
  */
 hipError_t mk_cache_read(const mk_paged_cache* cache, const int32_t* begin, const int32_t* lengths, void* k, void* v,
                          hipStream_t stream);
@@ -373,8 +374,11 @@ hipError_t mk_attention_paged(const mk_paged_cache* cache, int q_heads, const vo
  * that order, the fewest whose w add up to at least top_p of the candidates' sum (top_p >= 1: all); and of these
  * those with w >= min_p (min_p <= 0: all). The likeliest token always stays. The answer is the first token, in the
  * order of the vocabulary, at which the running sum of the candidates' w is above u times their whole sum, the last one
- * if none is. T = 0: the likeliest token. All in 64 bits: sums within 2^-42 of each other count as equal, and a w below
- * 2^-1000 is 0.
+ * if none is. T = 0: the likeliest token.
+ * A w is held to 2^-36 of itself, one below 2^-46 to 2^-22, and one below 2^-1000 is 0; where top_p's or top_k's border lies
+ * among those below 2^-46, these count in whole 2^-82. Sums of them are exact or in 64 bits, and two sums within 2^-42 of each
+ * other are equal (half of 10 equal logits are 5). A top_p or u that is nearer than that to a running sum's share may fall on
+ * either side of it, the same one in every call.
  *   logits     fp32, row r at logits + r * row_stride (elements, >= 0), vocab (1..2^20) of them
  *   uniforms   [rows] fp32, u in [0, 1)
  *   temperature, top_k, top_p, min_p     [rows] fp32, int32, fp32, fp32

@@ -21,9 +21,9 @@
 //                    Lane l then holds dims 32 g .. 32 g + 31 of query n.
 // K's loads for the next 32 keys leave when the scores are made, V's when its fragments are. At 2 queries to a K/V head
 // 14 of the 16 columns are zero and the matrix cores are still idle most of the time: the read of the keys bounds it.
-// Measured, bf16 queries of 16 heads on 8, both launches: 64 sequences of 900 to 4,095 keys in bf16 pages (655 MB) 119 us,
-// 5.5 TB/s; 30,001 keys of one (123 MB) 30 us, 4.1 TB/s, of which 5 are the join; 64 of 64 to 960 in 8-bit pages (69 MB) 23 us;
-// one of 300 keys 7.7 us: launch, cold code, and lengths, table and keys one after the other. Tiles through LDS would only
+// Measured, bf16 queries of 16 heads on 8, both launches: 64 sequences of 900 to 4,095 keys in bf16 pages (655 MB) 120 us,
+// 5.5 TB/s; 30,001 keys of one (123 MB) 30 us, 4.1 TB/s, of which 5 are the join; 64 of 64 to 960 in 8-bit pages (69 MB) 23.7 us;
+// one of 300 keys 7.9 us: launch, cold code, and lengths, table and keys one after the other. Tiles through LDS would only
 // add a trip: a wave's keys are its own, and no second wave reads them.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -924,7 +924,8 @@ static int64_t rows_of(const int32_t* lengths, int num_seqs) {
 // Tables of at most 512 positions, 16 tiles to a unit, take one launch: four tiles to a wave at most. Measured, heads 16 / 8,
 // bf16 pages, lengths even over capacity / 4 .. capacity, without and with the split: capacity 512 one sequence 6.4 and
 // 8.5 us, 13 of them 9.6 and 10.7, 64 17.9 and 20.7, 256 63.0 and 65.4; capacity 1,024 one 13.2 and 8.9, 13 16.5 and 12.9,
-// 64 30.6 and 33.2, 256 128 and 135, but 64 of which one is full and the others have up to 64 keys 14.7 and 10.7.
+// 64 30.6 and 33.2, 256 128 and 135, but 64 of which one is full and the others have up to 64 keys 14.7 and 10.7; capacity 768
+// 64 23.2 and 26.7, 256 92 and 101, one full among 64 12.3 and 11.1.
 static bool paged_split(int64_t capacity) { return capacity > 512; }
 
 }  // namespace mkp

@@ -5,25 +5,29 @@
 //               order of the logits;
 //   answer      the first token of the vocabulary at which the running sum of the candidates' w exceeds u times
 //               their whole sum.
-// The answer is a whole number that a border may decide, so sums are exact ones of w rounded to 2^-37 of itself, and two
+// The answer is a whole number that a border may decide, so sums are exact ones of w rounded to 2^-36 of itself, and two
 // sums within SAME of each other count as equal: 5 of 10 equal logits reach half of them, and do not exceed it.
 //
 // Bins, 11 to a factor of 2. p = x * 11 log2(e) / T falls into bin floor(p), the same for equal logits wherever they
 // are, and within its bin w is 2^((p - floor(p)) / 11), a polynomial on [1, 1.066), kept as a whole number of 2^-36: a
 // bin's sum is a sum of whole numbers, the same in any order, and its weight that sum times 2^(bin / 11). Its number of
-// logits shares the 64 bits, so that a logit is one atomic addition in LDS.
+// logits shares the 64 bits, so that a logit is one atomic addition in LDS: 8,192 logits leave 36 bits behind the point, 12 more
+// than the logits, the numbers u and top_p themselves have. More would take a second addition for the number.
 //   sample_chunk_kernel  a workgroup takes 8,192 logits of a row from registers into 512 bins (a factor of 2^46) below
 //                        their maximum (what lies lower is a tail of its own), and lists the logits of the first bins,
 //                        up to 256 of them in all;
-//   sample_pick_kernel   a workgroup per row. Borders lie among the listed logits as a rule: it bins these, finds the
+//   sample_pick_kernel   a workgroup per row. Where its borders lie among the listed logits it bins these, finds the
 //                        bin that a border falls into, sorts that bin's logits, and sums the kept ones chunk by chunk.
 //                        Where a border lies deeper it joins the chunks' bins instead and gathers the border's bin from
-//                        the row, by its logits' bins in a byte each (narrowing it first where it holds more than 4,096). The answer is looked for among
-//                        the 8,192 logits of its chunk. Without any filter the chunks' sums are all that is needed.
+//                        the row, by its logits' bins in a byte each (narrowing it first where it holds more than 4,096). The
+//                        answer is looked for among the 8,192 logits of its chunk. Without any filter the chunks' sums are all
+//                        that is needed.
+// How deep a border lies is up to the logits: of normal ones of deviation 2 with two dozen peaks, top-p 0.9 at T 0.8 goes below
+// the lists in a third of the rows, 0.95 at T 1 in nearly all (40,000 of 151,936 tokens kept), a top-k of 50 in none.
 // The logits are read once and the chunk of the answer, or its listed logits, again. Measured on MI355X: one row of 151,936 22
-// to 27 us, 9 of them the first kernel, a chain of seven barriers through cold code, and 14 the second; with a border
-// deeper than the lists 31 to 34 us of the second kernel in one workgroup (the gather by codes, the sort, the chunks' sums).
-// 64 rows (39 MB) 56 us with such borders among them: 23 us of the first kernel, which the 64-bit
+// to 25 us, 9 of them the first kernel, a chain of seven barriers, and 13 to 15 the second; with a border deeper than the lists
+// 37 to 45, 28 and more of them the second kernel's one workgroup (the gather by codes, the sort, the chunks' sums).
+// 64 rows (39 MB) 53 to 54 us with such borders among them: 24 us of the first kernel, which the 64-bit
 // products and whole-number atomics of the weights bound (its read alone takes 8 us), and the deepest row's second.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -1040,7 +1044,8 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
       deep = cut.part && cut.bin > depth;
     }
     if (deep) {
-      deep_cut(a.bins + s0 * NB, a.stat + s0, top_k <= 0 || top_k > a.list ? a.codes + s0 * SC : nullptr, chunks, x, a.vocab, sc.c, sc.in, ref, ktop, number, whole, top_k, top_p, xm, jm);
+      deep_cut(a.bins + s0 * NB, a.stat + s0, top_k <= 0 || top_k > a.list ? a.codes + s0 * SC : nullptr, chunks, x, a.vocab,
+               sc.c, sc.in, ref, ktop, number, whole, top_k, top_p, xm, jm);
       __syncthreads();
       cut = sm.cut;
     } else if (cut.part) {  // the chunks' sums of what is kept: all of it is listed, a wave's 64 are of one chunk
