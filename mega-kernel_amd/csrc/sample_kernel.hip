@@ -446,7 +446,7 @@ __device__ __forceinline__ int border_bin(bool by_rank, int rank, double goal) {
 // The weight of a logit of the row's bin j, in 2^-FIX of 2^(-j / 11).
 __device__ __forceinline__ u64 fixed_weight(const Scale& s, double ref, float x, int j) {
   const double p = (double)x * s.c, fl = floor(p);
-  if (j == NB - 1) return (u64)ceil(exp_tail(p - ref) * (ONE / smem().et[NB - 1]));  // (0 for a weight of 0 alone)
+  if (j == NB - 1) return (u64)(exp_tail(p - ref) * (ONE / smem().et[NB - 1]));
   return fixed_in_bin(x, s, fl);
 }
 
@@ -873,8 +873,17 @@ __device__ __forceinline__ void deep_cut(const u64* bins, const SampleStat* stat
   }
   if (jm < cut.bin || (jm == cut.bin && (!cut.part || xm > cut.x))) cut = {jm, true, xm, INT32_MAX};
   if (tid == 0) sm.cut = cut;
-  {  // the kept weights of the border's bin
+  // The kept weights of the border's bin. One of the tail that is no whole number of its unit is marked, so that its chunk has a
+  // sum above 0.
+  constexpr u64 MARK = 1ull << 63;  // above all sums: 2^20 weights below 2^37
+  {
     const int j = cut.bin, n = sm.cupto[j] - number_below(j);
+    auto add = [&](float y, int v) {
+      if (!cut.keeps(j, y, v)) return;
+      const u64 f = fixed_weight(r, y, j);
+      if (f > 0) atomicAdd(&sm.part[v / SC], f);
+      else if (exp_tail((double)y * r.s.c - r.ref) > 0) atomicOr(&sm.part[v / SC], MARK);
+    };
     if (n <= CAP) {
       if (holds != j) {
         if (j == NB - 1 || !codes || !gather_bin(r, codes, chunks, j, cut.x)) {
@@ -883,16 +892,10 @@ __device__ __forceinline__ void deep_cut(const u64* bins, const SampleStat* stat
         }
         held = sm.n;
       }
-      for (int i = tid; i < held; i += ST) {
-        const float y = key_x(sm.list[i]);
-        const int v = key_v(sm.list[i]);
-        if (cut.keeps(j, y, v)) atomicAdd(&sm.part[v / SC], fixed_weight(r, y, j));
-      }
+      for (int i = tid; i < held; i += ST) add(key_x(sm.list[i]), key_v(sm.list[i]));
     } else {
       bin_range(r, j);
-      sweep(r, logit_order(cut.x), sm.khi, [&](float y, int v) {
-        if (cut.keeps(j, y, v)) atomicAdd(&sm.part[v / SC], fixed_weight(r, y, j));
-      });
+      sweep(r, logit_order(cut.x), sm.khi, add);
     }
   }
   __syncthreads();
@@ -906,7 +909,8 @@ __device__ __forceinline__ void deep_cut(const u64* bins, const SampleStat* stat
       if (j < NB - 1 && j + d < cut.bin) s += (double)(b & SUM_MASK) / ONE * (sm.et[j] * sm.scale[k]);
     }
     s = sum_over_wave(s);
-    if (lane == 0) sm.csum[k] = s + (double)sm.part[k] / ONE * sm.et[cut.bin];
+    const u64 part = sm.part[k];
+    if (lane == 0) sm.csum[k] = s + (double)(part & ~MARK) / ONE * sm.et[cut.bin] + (part & MARK ? 0x1p-1000 : 0);
   }
 }
 

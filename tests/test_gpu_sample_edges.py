@@ -175,3 +175,15 @@ def test_the_smallest_weights(kernel, vocab, k, p, m):
         assert tokens[r] == first, (r, tokens[r], first)
         want = (x[r, first].double() - x[r].max().double()).item() - kept.exp().sum().log().item()
         assert abs(logprobs[r].item() - want) <= 2.0 ** -24 * abs(want) + 2.0 ** -22, (r, logprobs[r], want)
+
+
+@pytest.mark.parametrize("vocab", [600, 20000])
+@pytest.mark.parametrize("k", [257, 500])
+def test_candidates_too_small_to_count(kernel, vocab, k):
+    """A top_k's border among weights of exp(-488): their sum is far below every u but 0."""
+    x = torch.full((4, vocab), -INF, device=DEV)
+    x[:, 5:505] = -4.88 - 0.0001 * torch.arange(500, device=DEV)
+    x[:, vocab - 1] = 0.0
+    u = torch.tensor([0.0, 1e-38, 1e-30, 2.0 ** -24], device=DEV)
+    tokens, _ = check(kernel, x, u, 0.01, k)
+    assert tokens.tolist() == [5] + [vocab - 1] * 3
