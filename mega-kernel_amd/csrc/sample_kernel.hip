@@ -152,11 +152,12 @@ __device__ __forceinline__ u64 fixed_in_bin(float x, const Scale& s, double fl) 
   y = fma(y, f, A);
   return __builtin_bit_cast(u64, fma(y, f, 1 + BIG)) - __builtin_bit_cast(u64, BIG);
 }
-// 2^(t / 11) for t <= 0 to fp32's accuracy: the tail's weights, below 2^-46 of the largest
-__device__ __forceinline__ double exp_tail(double t) {
-  if (!(t >= -DEEPEST)) return 0;
-  const double p = t * (1.0 / RES), n = floor(p);
-  return ldexp((double)__builtin_amdgcn_exp2f((float)(p - n)), (int)n);
+// 2^((p - ref) / 11) to fp32's accuracy: the tail's weights, below 2^-46 of the largest. `fl` is floor(p), a logit's bin, which alone
+// decides where weights end, as it does for chunks.
+__device__ __forceinline__ double tail_weight(double p, double fl, double ref) {
+  if (!(ref - fl <= DEEPEST)) return 0;
+  const double t = (p - ref) * (1.0 / RES), n = floor(t);
+  return ldexp((double)__builtin_amdgcn_exp2f((float)(t - n)), (int)n);
 }
 // the bin of floor(p) below `ref`, the tail's for all from there on
 __device__ __forceinline__ int bin_of(double ref, double fl) {
@@ -256,7 +257,7 @@ __global__ void __launch_bounds__(64 * W) sample_chunk_kernel(const SampleArgs a
       if (bin < NB - 1) {
         atomicAdd(&bins[bin], fixed_in_bin(f[i], s, fl) + (1ull << CNT));
       } else if (f[i] > -INFINITY) {
-        tail += exp_tail(p - out.ref);
+        tail += tail_weight(p, fl, out.ref);
         ++tc;
       }
       code |= (uint32_t)(bin >> 1) << (8 * q);
@@ -446,7 +447,7 @@ __device__ __forceinline__ int border_bin(bool by_rank, int rank, double goal) {
 // The weight of a logit of the row's bin j, in 2^-FIX of 2^(-j / 11).
 __device__ __forceinline__ u64 fixed_weight(const Scale& s, double ref, float x, int j) {
   const double p = (double)x * s.c, fl = floor(p);
-  if (j == NB - 1) return (u64)(exp_tail(p - ref) * (ONE / smem().et[NB - 1]));
+  if (j == NB - 1) return (u64)(tail_weight(p, fl, ref) * (ONE / smem().et[NB - 1]));
   return fixed_in_bin(x, s, fl);
 }
 
@@ -882,7 +883,7 @@ __device__ __forceinline__ void deep_cut(const u64* bins, const SampleStat* stat
       if (!cut.keeps(j, y, v)) return;
       const u64 f = fixed_weight(r, y, j);
       if (f > 0) atomicAdd(&sm.part[v / SC], f);
-      else if (exp_tail((double)y * r.s.c - r.ref) > 0) atomicOr(&sm.part[v / SC], MARK);
+      else if (r.ref - floor((double)y * r.s.c) <= DEEPEST) atomicOr(&sm.part[v / SC], MARK);
     };
     if (n <= CAP) {
       if (holds != j) {
@@ -1155,7 +1156,7 @@ __global__ void __launch_bounds__(ST) sample_pick_kernel(const SampleArgs a) {
     const int j = bin_of(ref, fl);
     double s = 0;
     if (f[0] > -INFINITY && cut.keeps(j, f[0], v0 + q))
-      s = j < NB - 1 ? (double)fixed_in_bin(f[0], sc, fl) / ONE * sm.et[j] : exp_tail(p - ref);
+      s = j < NB - 1 ? (double)fixed_in_bin(f[0], sc, fl) / ONE * sm.et[j] : tail_weight(p, fl, ref);
     weights[q * ST] = s;
     mine += s;
     last = s > 0 ? v0 + q : last;
